@@ -37,6 +37,10 @@ extern "C" {
 #define MI_FP8_E4M3 3 /* OCP e4m3fn (gfx950 native), max 448, per-head fp32 scales */
 #define MI_I32 4       /* index / position dtypes */
 #define MI_I64 5
+/* Microscaled KV caches: blocks of 32 consecutive elements of a (token, kv-head) row
+ * share a power-of-two scale byte s: 2^(s - 127), 255 = the block is NaN. */
+#define MI_MXFP8 6 /* e4m3fn codes, one byte an element */
+#define MI_MXFP4 7 /* e2m1 codes, two elements a byte, the even one in the low bits */
 
 /* status codes */
 #define MI_OK 0
@@ -47,10 +51,14 @@ extern "C" {
 
 #define MI_ABI_VERSION 4
 
-/* One layer of the paged KV cache. Strides are in elements. */
+/* One layer of the paged KV cache. Strides are in elements (MI_MXFP4: in bytes).
+ * A microscaled layer's scale bytes lie beside the codes, contiguous as
+ *   [max_pages][2 (K, V)][num_kv_heads][head_dim / 32][page_size]
+ * (the bytes of consecutive tokens adjacent): k_scale and v_scale are the addresses of
+ * the K and of the V bytes of page 0, 4-byte aligned, given as const float*. */
 typedef struct mi_paged_kv {
   void* data;           /* element (page 0, K, slot 0, head 0, dim 0) */
-  int32_t dtype;        /* MI_BF16, MI_F16, MI_F32 or MI_FP8_E4M3 */
+  int32_t dtype;        /* MI_BF16, MI_F16, MI_F32, MI_FP8_E4M3, MI_MXFP8 or MI_MXFP4 */
   int32_t page_size;    /* tokens per page */
   int32_t num_kv_heads;
   int32_t head_dim;     /* 64, 128 or 256 */
@@ -59,7 +67,7 @@ typedef struct mi_paged_kv {
   int64_t kv_stride;    /* from the K half of a page to its V half */
   int64_t token_stride; /* between slots of a page */
   int64_t head_stride;  /* between kv heads of a slot (head_dim elements must be contiguous) */
-  const float* k_scale; /* MI_FP8_E4M3 only: [num_kv_heads] dequantisation scales, else NULL */
+  const float* k_scale; /* MI_FP8_E4M3: [num_kv_heads] dequantisation scales; microscaled: see above; else NULL */
   const float* v_scale;
 } mi_paged_kv;
 
@@ -204,6 +212,24 @@ int mi_decode_merge(const void* q, int32_t q_dtype, int64_t q_stride_token, int6
                     int64_t out_stride_head, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Decode behind a sliding window with sinks.  No counterpart in the reference
+ * (whose wrappers call FlashInfer without a window).  As mi_decode_run, but the
+ * query at position i of its request (the last of decode's queries: kv_len - 1)
+ * sees key t only if t >= i - window_left or t < sink_tokens, besides causal's
+ * t <= i; window_left < 0: every key, as mi_decode_run.  A query that sees no
+ * key gives zeros.  Reads index arrays and workspace only: the same plan serves
+ * windowed and full layers of a step.  Pages of which every key is hidden from
+ * every query of the request are never read, and their ids may be stale.
+ * 16-bit, fp8 and microscaled caches (fp32: MI_ERR_UNSUPPORTED).
+ * ------------------------------------------------------------------------ */
+int mi_decode_run_window(const void* q, int32_t q_dtype, int64_t q_stride_token, int64_t q_stride_head,
+                         const mi_paged_kv* kv, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                         const int32_t* kv_indices, const int32_t* last_page_len, int32_t batch,
+                         int32_t num_qo_heads, int32_t causal, float sm_scale, int32_t window_left,
+                         int32_t sink_tokens, void* workspace, int64_t workspace_bytes, void* out,
+                         int64_t out_stride_token, int64_t out_stride_head, void* stream);
+
+/* ------------------------------------------------------------------------
  * Decode without a caller workspace.  No counterpart in the reference: this
  * entry point is for callers that cannot allocate device memory (code under
  * HIP graph capture, tight serving loops, harnesses that forbid hipMalloc).
@@ -236,7 +262,12 @@ int mi_decode_noalloc(const void* q, int32_t q_dtype, int64_t q_stride_token, in
  * Replaces FlashInferPrefillWrapper.set_kv_cache / FlashInferDecodeWrapper.set_kv_cache
  * (mstar/utils/flashinfer_utils.py:271-288, 467-484):
  *   cache[page[i], K, slot[i]] = k[i];  cache[page[i], V, slot[i]] = v[i]
- * cast to the cache dtype (RNE; fp8: x * (1/scale) clamped to +-448, then RNE).
+ * cast to the cache dtype (RNE; fp8: x * (1/scale) clamped to +-448, then RNE;
+ * microscaled: each block of 32 with the least exponent e at which max|x| <= T * 2^e,
+ * T = 464 (MI_MXFP8) or 7 (MI_MXFP4), at least -126 and at most 119 or 125 (every code
+ * is then finite), codes RNE(x * 2^-e), the largest beyond it, scale byte e + 127; a
+ * block of zeros 127, one that holds a NaN or an infinity 255; the
+ * layer as for mi_decode_run, and the scale bytes are written too).
  * page[i] = page_idx[i * idx_stride], slot[i] = slot_idx[i * idx_stride]
  * (idx_stride 1 for token_to_page/token_to_cache, 2 for kv_cache_locations
  * [B, 2] with slot_idx = page_idx + 1).  Tokens whose page id is outside
@@ -250,6 +281,20 @@ int mi_kv_append(const mi_paged_kv* kv, const void* k, const void* v, int32_t sr
                  int64_t v_stride_head, const int64_t* page_idx, const int64_t* slot_idx,
                  int64_t idx_stride, int32_t num_tokens, const int32_t* num_tokens_device,
                  void* stream);
+
+/* Reads whole contexts back (the inverse of the appends, any cache dtype): with
+ * kv_len_r = (npages_r - 1) * page_size + last_page_len[r] (0 without pages) and
+ * t0_r the sum of kv_len over the requests before r,
+ *   k_out[t0_r + i] = K row i of request r, v_out likewise, as out_dtype
+ * (MI_BF16, MI_F16 or MI_F32, rounded to nearest even; the cache's own 16-bit dtype
+ * is copied).  k_out, v_out: contiguous [out_tokens, num_kv_heads, head_dim],
+ * 16-byte aligned; rows from the last request's end on, or beyond out_tokens, are not
+ * written, nor those of pages outside [0, max_pages).  num_indices: elements of
+ * kv_indices.  Replaces the reference's gathers of a request's pages by torch
+ * indexing (mstar/engine/kv_store.py:330-380 moves them page by page). */
+int mi_kv_read(const mi_paged_kv* kv, const int32_t* kv_indptr, const int32_t* kv_indices,
+               const int32_t* last_page_len, int32_t batch, int32_t num_indices, void* k_out, void* v_out,
+               int32_t out_dtype, int64_t out_tokens, void* stream);
 
 /* ------------------------------------------------------------------------
  * P3 + P7 — ragged prefill plan and attention.
@@ -357,6 +402,17 @@ int mi_prefill_tiles(const void* q, int32_t q_dtype, int64_t q_stride_token, int
                      int32_t max_qo_tokens, int32_t num_qo_heads, int32_t causal, float sm_scale,
                      void* workspace, int64_t workspace_bytes, void* out, int64_t out_stride_token,
                      int64_t out_stride_head, void* stream);
+
+/* mi_prefill_run (parts 3), mi_prefill_short (1) or mi_prefill_tiles (2) behind a
+ * sliding window with sinks (see mi_decode_run_window), on the same plan.  Without
+ * causal a query also sees the keys behind it. */
+int mi_prefill_run_window(const void* q, int32_t q_dtype, int64_t q_stride_token, int64_t q_stride_head,
+                          const mi_paged_kv* kv, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                          const int32_t* kv_indices, const int32_t* last_page_len, int32_t batch,
+                          int32_t max_qo_tokens, int32_t num_qo_heads, int32_t causal, float sm_scale,
+                          int32_t window_left, int32_t sink_tokens, int32_t parts, void* workspace,
+                          int64_t workspace_bytes, void* out, int64_t out_stride_token, int64_t out_stride_head,
+                          void* stream);
 
 /* ------------------------------------------------------------------------
  * RoPE on the packed batch (the path's next row: the rotation every layer

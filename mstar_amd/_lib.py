@@ -26,6 +26,8 @@ MI_F32 = 2
 MI_FP8_E4M3 = 3
 MI_I32 = 4
 MI_I64 = 5
+MI_MXFP8 = 6
+MI_MXFP4 = 7
 
 MI_OK = 0
 MI_ERR_UNSUPPORTED = -2
@@ -153,6 +155,20 @@ SIGNATURES = {
         ctypes.c_int,
         [_P, _I32, _I64, _I64, ctypes.POINTER(MiPagedKV), _P, _P, _P, _P, _I32, _I32, _I32, _I32, _F32,
          _P, _I64, _P, _I64, _I64, _P],
+    ),
+    "mi_decode_run_window": (
+        ctypes.c_int,
+        [_P, _I32, _I64, _I64, ctypes.POINTER(MiPagedKV), _P, _P, _P, _P, _I32, _I32, _I32, _F32, _I32, _I32,
+         _P, _I64, _P, _I64, _I64, _P],
+    ),
+    "mi_prefill_run_window": (
+        ctypes.c_int,
+        [_P, _I32, _I64, _I64, ctypes.POINTER(MiPagedKV), _P, _P, _P, _P, _I32, _I32, _I32, _I32, _F32, _I32, _I32,
+         _I32, _P, _I64, _P, _I64, _I64, _P],
+    ),
+    "mi_kv_read": (
+        ctypes.c_int,
+        [ctypes.POINTER(MiPagedKV), _P, _P, _P, _I32, _I32, _P, _P, _I32, _I64, _P],
     ),
     "mi_rope_positions": (ctypes.c_int, [_P, _P, _I32, _P, _I32, _P]),
     "mi_copy_pages": (ctypes.c_int, [_P, _I64, _I32, _I64, _I64, _I64, _P, _P, _I32, _P]),
@@ -420,7 +436,13 @@ def paged_kv_desc(kv_cache_layer: torch.Tensor, k_scale: torch.Tensor | None = N
     Descriptors are kept by everything they are built and checked from
     (address, shape, strides, dtype, and the scales' address, dtype, size,
     layout and device), so a layer seen before costs one dictionary lookup.
+
+    A :class:`~mstar_amd.mx_cache.MXKVLayer` brings its own descriptor, and takes no scales.
     """
+    if not isinstance(kv_cache_layer, torch.Tensor):
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("a microscaled KV layer holds its own scales: pass no k_scale or v_scale")
+        return kv_cache_layer.desc
     key = (kv_cache_layer.data_ptr(), kv_cache_layer.shape, kv_cache_layer.stride(), kv_cache_layer.dtype,
            kv_cache_layer.device, _scale_key(k_scale), _scale_key(v_scale))
     d = _desc_cache.get(key)

@@ -46,6 +46,8 @@ HIPCC_FLAGS = [
 # kernels, which run faster under the backend's max-ILP scheduler (see that file).
 EXTRA_FLAGS = {
     "mi_prefill_d128.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
+    "mi_prefill_win_d128.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
+    "mi_prefill_mx_d128.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
 }
 
 

@@ -31,6 +31,7 @@ import torch
 
 from . import _lib
 from .kv_store import KVCacheConfig, KVRequestState, PagedAllocationManager, _host_step
+from .mx_cache import MXKVCache
 from .paged_attention import PagedDecodeWrapper, PagedPrefillWrapper
 from .rope import apply_llama31_rope_pos_ids_inplace, apply_rope_pos_ids_inplace, rope_positions
 from .trace import trace_range
@@ -111,7 +112,8 @@ class BatchedCacheManager:
         kv_scales: torch.Tensor | None = None,
     ):
         """``kv_scales`` (extension): fp32 ``[num_layers, 2, num_kv_heads]`` per-head
-        dequantisation scales of an fp8-e4m3 ``kv_cache``."""
+        dequantisation scales of an fp8-e4m3 ``kv_cache``.  ``kv_cache`` may be an
+        :class:`~mstar_amd.mx_cache.MXKVCache` (extension), which holds its own."""
         self.request_ids = request_ids
         self.active_labels = active_labels_per_request
         self.kv_cache = kv_cache
@@ -266,7 +268,8 @@ class BatchedCacheManager:
     def _plan_attention_impl(self, seq_lens, dtype, is_causal, write_store, label) -> None:
         assert self.kv_cache is not None
         if dtype is None:
-            dtype = torch.bfloat16 if self.kv_cache.dtype == torch.float8_e4m3fn else self.kv_cache.dtype
+            mx = isinstance(self.kv_cache, MXKVCache)
+            dtype = torch.bfloat16 if mx or self.kv_cache.dtype == torch.float8_e4m3fn else self.kv_cache.dtype
         cfg = self.kv_cache_config
         ps_ = cfg.page_size
         b = len(self.request_ids)
@@ -424,20 +427,20 @@ class BatchedCacheManager:
             if write_store:
                 self.alloc_manager.flush_to_store(rid, label=to_label)
         if src:
-            kv = self.kv_cache
-            page = kv[0, 0]
-            if not page.is_contiguous():
+            pools = [self.kv_cache.codes, self.kv_cache.scales] if isinstance(self.kv_cache, MXKVCache) else [self.kv_cache]
+            if not all(kv[0, 0].is_contiguous() for kv in pools):
                 raise ValueError("snapshot_all needs each page of the KV pool to be contiguous")
-            esz = kv.element_size()
             n = len(src)
             dev = self._pack.upload(np.asarray(src + dst, dtype=np.int32))
-            _lib.check(
-                _lib.lib().mi_copy_pages(
-                    kv.data_ptr(), kv.stride(0) * esz, kv.shape[0], kv.stride(1) * esz, page.numel() * esz,
-                    kv.shape[1], dev.data_ptr(), dev.data_ptr() + 4 * n, n, _lib.stream_ptr(self.device),
-                ),
-                "mi_copy_pages",
-            )
+            for kv in pools:
+                esz = kv.element_size()
+                _lib.check(
+                    _lib.lib().mi_copy_pages(
+                        kv.data_ptr(), kv.stride(0) * esz, kv.shape[0], kv.stride(1) * esz, kv[0, 0].numel() * esz,
+                        kv.shape[1], dev.data_ptr(), dev.data_ptr() + 4 * n, n, _lib.stream_ptr(self.device),
+                    ),
+                    "mi_copy_pages",
+                )
 
     # ------------------------------------------------------------ running
     def _layer_scales(self, layer_idx: int):
@@ -446,8 +449,11 @@ class BatchedCacheManager:
         return self.kv_scales[layer_idx, 0], self.kv_scales[layer_idx, 1]
 
     def run_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
-                      layer_idx: int | None = None) -> torch.Tensor:
-        """Append this step's K/V, then attend (``cache_manager.py:653-701``)."""
+                      layer_idx: int | None = None, window_left: int = -1, sink_tokens: int = 0) -> torch.Tensor:
+        """Append this step's K/V, then attend (``cache_manager.py:653-701``).
+
+        ``window_left``, ``sink_tokens`` (extension): the layer's sliding window, as
+        the wrappers' ``run``."""
         if layer_idx is None:
             layer_idx = self.layer_idx
         orig_dtype = q.dtype
@@ -460,7 +466,7 @@ class BatchedCacheManager:
         if self.auto_write_store and ps.write_store:
             for rid in self.request_ids:
                 self.alloc_manager.flush_to_store(rid, label=label, layers=layer_idx)
-        return ps.wrapper.run(q, layer, ks, vs).to(orig_dtype)
+        return ps.wrapper.run(q, layer, ks, vs, window_left=window_left, sink_tokens=sink_tokens).to(orig_dtype)
 
     # ------------------------------------------------------------ rope
     def plan_rope(self, seq_lens: list[int], pos_ids: torch.Tensor | None = None, label: str | None = None) -> None:
@@ -552,14 +558,16 @@ class BatchedCacheManager:
     def apply_rope_and_run_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                                      rotary_dim: int | None = None, interleave: bool = False, rope_scale: float = 1,
                                      rope_theta: float = 10000.0, rope_dtype=None, layer_idx: int | None = None,
-                                     keep_k: bool = True, **kwargs) -> torch.Tensor:
+                                     keep_k: bool = True, window_left: int = -1, sink_tokens: int = 0,
+                                     **kwargs) -> torch.Tensor:
         """``apply_rope(q, k, ...)`` then ``run_attention(q, k, v)`` with the rotation and the append fused.
 
         One ``mi_rope_append`` launch rotates q (and k, unless ``keep_k`` is
         False) and writes the rotated k and v to the layer's pages; the cache
         and the attention output are bit-identical to the two-call sequence.
         Dtype handling and Llama-3.1 keywords are those of ``apply_rope``; v
-        is converted to the rope dtype with q and k.
+        is converted to the rope dtype with q and k.  ``window_left`` and
+        ``sink_tokens`` are ``run_attention``'s.
         """
         if layer_idx is None:
             layer_idx = self.layer_idx
@@ -588,7 +596,7 @@ class BatchedCacheManager:
         if self.auto_write_store and ps.write_store:
             for rid in self.request_ids:
                 self.alloc_manager.flush_to_store(rid, label=label, layers=layer_idx)
-        return ps.wrapper.run(q, layer, ks, vs).to(orig_dtype)
+        return ps.wrapper.run(q, layer, ks, vs, window_left=window_left, sink_tokens=sink_tokens).to(orig_dtype)
 
     # ------------------------------------------------------------ advance
     def advance_seq_len(self, n: int | None = None, pos_id_n: int | None = None) -> None:

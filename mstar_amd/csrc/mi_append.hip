@@ -13,7 +13,8 @@
 //   any  -> f16             : via fp32, round-to-nearest-even
 //   any  -> fp8 e4m3fn      : q = e4m3fn_RNE(clamp(x * (1/scale[h]), -448, 448))
 //   f32 -> f32               : copy;  bf16/f16 -> f32 : exact widening
-#include "mi_common.h"
+//   any  -> microscaled      : mi_mx.hip
+#include "mi_internal.h"
 
 namespace mi {
 
@@ -144,14 +145,17 @@ extern "C" int mi_kv_append(const mi_paged_kv* kv, const void* k, const void* v,
   if (kv->num_kv_heads <= 0 || kv->head_dim <= 0 || kv->page_size <= 0) return MI_ERR_INVALID;
   if (kv->head_dim % 8) return MI_ERR_UNSUPPORTED;
   const int dst = kv->dtype;
-  if (dst != MI_BF16 && dst != MI_F16 && dst != MI_FP8_E4M3 && dst != MI_F32) return MI_ERR_UNSUPPORTED;
+  if (dst != MI_BF16 && dst != MI_F16 && dst != MI_FP8_E4M3 && dst != MI_F32 && !kv_is_mx(dst)) return MI_ERR_UNSUPPORTED;
   if (src_dtype != MI_BF16 && src_dtype != MI_F16 && src_dtype != MI_F32) return MI_ERR_UNSUPPORTED;
   if (dst == MI_FP8_E4M3 && (!kv->k_scale || !kv->v_scale)) return MI_ERR_INVALID;
   // 8-element vector moves need 8-element aligned rows on both sides.
-  const int sesz = src_dtype == MI_F32 ? 4 : 2, desz = dst == MI_FP8_E4M3 ? 1 : dst == MI_F32 ? 4 : 2;
+  const int sesz = src_dtype == MI_F32 ? 4 : 2, desz = kv_elem_bytes(dst);
   if ((k_stride_token | k_stride_head | v_stride_token | v_stride_head) % 8) return MI_ERR_INVALID;
   if ((kv->page_stride | kv->kv_stride | kv->token_stride | kv->head_stride) % 8) return MI_ERR_INVALID;
   if (!aligned(k, 8 * sesz) || !aligned(v, 8 * sesz) || !aligned(kv->data, 8 * desz)) return MI_ERR_INVALID;
+  if (kv_is_mx(dst))
+    return mx_append_launch(kv, k, v, src_dtype, k_stride_token, k_stride_head, v_stride_token, v_stride_head, page_idx,
+                            slot_idx, idx_stride, num_tokens, num_tokens_device, (hipStream_t)stream);
   AppendParams ap{};
   ap.k = k;
   ap.v = v;

@@ -136,6 +136,60 @@ MI_DEVICE uint32_t fp8x2_to_mt<F16>(uint32_t w, bool hi) {
             : bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
 }
 
+// ------------------------------------------------- microscaled cache formats
+// Blocks of 32 consecutive elements of a row share a power-of-two scale byte s
+// (2^(s - 127); 255: the block is NaN); e4m3fn codes (MI_MXFP8) or e2m1 codes
+// (MI_MXFP4, the even element in the low four bits).  The conversions apply the
+// scale: exact in bf16 above its subnormal range, rounded to nearest even in
+// fp16 and below.
+enum : int { kKv16 = 0, kKvFp8 = 1, kKvMx8 = 2, kKvMx4 = 3 };  // KV formats of the attention kernels
+constexpr int kMxBlock = 32;
+
+// The scale of byte i of w as a float whose exponent field is that byte.
+MI_DEVICE float mx_scale(uint32_t w, int i) {
+  return bitcast<float>((i < 3 ? w << (23 - 8 * i) : w >> 1) & 0x7f800000u);
+}
+
+// N packed words of codes -> their elements in the MFMA type, two per word.
+template <typename MT, int KVT, int N, int M>
+MI_DEVICE void mx_to_mt(const uint32_t (&w)[N], float scale, uint32_t (&out)[M]) {
+  constexpr bool B = MT::kDtype == MI_BF16;
+  if constexpr (KVT == kKvMx8) {
+    static_assert(M <= 2 * N, "two words of elements per word of codes");
+#pragma unroll
+    for (int i = 0; i < M / 2; ++i) {
+      if constexpr (B) {
+        out[2 * i] = bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, false));
+        out[2 * i + 1] = bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, true));
+      } else {
+        out[2 * i] = bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], scale, false));
+        out[2 * i + 1] = bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], scale, true));
+      }
+    }
+  } else {
+    static_assert(M <= 4 * N, "four words of elements per word of codes");
+#pragma unroll
+    for (int i = 0; i < M; ++i) {  // the byte is a literal of the instruction: constant after unrolling
+      const uint32_t c = w[i / 4];
+      if constexpr (B) {
+        switch (i & 3) {
+          case 0: out[i] = bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0)); break;
+          case 1: out[i] = bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1)); break;
+          case 2: out[i] = bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2)); break;
+          default: out[i] = bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3)); break;
+        }
+      } else {
+        switch (i & 3) {
+          case 0: out[i] = bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 0)); break;
+          case 1: out[i] = bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 1)); break;
+          case 2: out[i] = bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 2)); break;
+          default: out[i] = bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 3)); break;
+        }
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------ lane helpers
 MI_DEVICE int lane_id() { return __lane_id(); }
 

@@ -136,8 +136,22 @@ enum : int { kPhaseAttend = 1, kPhaseMerge = 2 };
 inline bool rows_aligned16(const void* base, int64_t stride_a, int64_t stride_b, int elem_bytes) {
   return ((uintptr_t)base & 15) == 0 && (stride_a * elem_bytes) % 16 == 0 && (stride_b * elem_bytes) % 16 == 0;
 }
+// Bytes that a cache's element strides count: of the element, of the codes for
+// microscaled caches (at four bits one byte holds two elements).
+inline int kv_elem_bytes(int32_t dtype) { return dtype == MI_F32 ? 4 : dtype == MI_BF16 || dtype == MI_F16 ? 2 : 1; }
+inline bool kv_is_mx(int32_t dtype) { return dtype == MI_MXFP8 || dtype == MI_MXFP4; }
+// Caches whose codes need scales beside them.
+inline bool kv_is_scaled(int32_t dtype) { return dtype == MI_FP8_E4M3 || kv_is_mx(dtype); }
+inline int kv_format(int32_t dtype) {  // of the 16-bit and scaled caches
+  return dtype == MI_FP8_E4M3 ? kKvFp8 : dtype == MI_MXFP8 ? kKvMx8 : dtype == MI_MXFP4 ? kKvMx4 : kKv16;
+}
+// The scales a cache's format needs beside it (words of four bytes for microscaled ones).
+inline bool kv_scales_ok(const mi_paged_kv* kv) {
+  if (!kv_is_scaled(kv->dtype)) return true;
+  return kv->k_scale && kv->v_scale && (((uintptr_t)kv->k_scale | (uintptr_t)kv->v_scale) & 3) == 0;
+}
 inline bool kv_aligned16(const mi_paged_kv* kv) {
-  const int esz = kv->dtype == MI_FP8_E4M3 ? 1 : kv->dtype == MI_F32 ? 4 : 2;
+  const int esz = kv_elem_bytes(kv->dtype);
   return rows_aligned16(kv->data, kv->page_stride, kv->kv_stride, esz) &&
          rows_aligned16(kv->data, kv->token_stride, kv->head_stride, esz);
 }
@@ -166,11 +180,41 @@ struct DecodeParams {
   int32_t num_kv_heads, group, page_size, causal;
   float scale_log2;
   int32_t short_rows = kShortRowsMax;  // ragged batches: requests with qo_len * group above this are not ours
+  // Windowed runs: keys below a query's position - window_left are hidden but
+  // for the first `sinks` of the request; each of the `batch` requests has
+  // `splits` places for items (window_left < 0: no window).
+  int32_t window_left = -1, sinks = 0, splits = 0, batch = 0;
 };
+
+// The 16-token tiles of a windowed request: those that hold sinks, then those
+// from `first` on to the end of its keys, one sequence of `total` tiles that
+// `items` items share evenly.  Items are no shorter than kWinItemTiles.
+constexpr int kWinItemTiles = 16;
+struct WinTiles {
+  int sinks, first, total, items;
+};
+__device__ __forceinline__ WinTiles win_tiles(int kv_len, int qo_len, int window_left, int sinks, int splits) {
+  WinTiles w;
+  w.first = max(0, kv_len - qo_len - window_left) >> 4;
+  w.sinks = min((sinks + 15) >> 4, w.first);
+  w.total = w.sinks + ((kv_len + 15) >> 4) - w.first;
+  w.items = max(1, min(splits, (w.total + kWinItemTiles - 1) / kWinItemTiles));
+  return w;
+}
 
 // fp32 KV (q, cache and output in fp32): the attend phase of a split-KV plan
 // (mi_f32.hip), and the merge with fp32 output (mi_decode.hip).
 int f32_attend_launch(const DecodeParams& dp, int head_dim, int grid, hipStream_t stream);
+// Windowed and microscaled runs (mi_decode_win.hip, mi_decode_mx.hip): the attend
+// kernel, and the merge of a windowed run's items.
+int decode_win_launch(const DecodeParams& dp, int q_dtype, int kvt, int head_dim, int grid, hipStream_t stream);
+int decode_win_merge_launch(const DecodeParams& dp, int q_dtype, int kvt, int head_dim, hipStream_t stream);
+int decode_mx_launch(const DecodeParams& dp, int q_dtype, int kvt, int head_dim, int grid, hipStream_t stream);
+// mi_kv_append into a microscaled layer (mi_mx.hip); arguments checked but for the layer's scales and alignment.
+int mx_append_launch(const mi_paged_kv* kv, const void* k, const void* v, int32_t src_dtype, int64_t k_stride_token,
+                     int64_t k_stride_head, int64_t v_stride_token, int64_t v_stride_head, const int64_t* page_idx,
+                     const int64_t* slot_idx, int64_t idx_stride, int32_t num_tokens,
+                     const int32_t* num_tokens_device, hipStream_t stream);
 int merge_launch(const DecodeParams& dp, int head_dim, int out_dtype, int batch, hipStream_t stream);
 // fp32 ragged prefill over the prefill plan's tile list, one workgroup per
 // (tile, kv-head, block of 16 or 64 rows); rows: the most (token, q-head) rows
@@ -184,7 +228,8 @@ int decode_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_token, int6
                     int32_t num_qo_heads, int32_t causal, float sm_scale, void* workspace,
                     int64_t workspace_bytes, int64_t ws_offset, void* out,
                     int64_t out_stride_token, int64_t out_stride_head, int phases, hipStream_t stream,
-                    bool ragged_pair = false, DecodeParams* merge_args = nullptr);
+                    bool ragged_pair = false, DecodeParams* merge_args = nullptr, int32_t window_left = -1,
+                    int32_t sinks = 0);
 
 // Wavefront scans and reductions on the VALU's cross-lane paths: one row_shr
 // per power of two within a 16-lane row, then two row broadcasts.  (__shfl

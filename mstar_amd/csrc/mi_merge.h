@@ -10,7 +10,8 @@ namespace mi {
 // elements as the decode kernel's did: lane l of wavefront w merges row l%16,
 // elements d = VW*(4*(l/16) + w) + j, read from the register-order partial
 // layout with 64-lane contiguous (cache-line) loads.
-template <typename MT, int D, int RUN, bool PAIR = false>
+// WIN: the items of a windowed run (win_tiles).
+template <typename MT, int D, int RUN, bool PAIR = false, bool WIN = false>
 MI_DEVICE void merge_body(const DecodeParams& p, int32_t batch, int pair) {
   static_assert(!PAIR || D == 256, "paired kv-heads form 256-element rows");
   constexpr int VW = D / 16;
@@ -20,14 +21,22 @@ MI_DEVICE void merge_body(const DecodeParams& p, int32_t batch, int pair) {
   if (pair >= batch * nkv) return;
   const int b = pair / nkv;
   const int h = pair - b * nkv;
-  const int c0 = p.chunk_indptr[b];
-  const int nb = p.chunk_indptr[b + 1] - c0;
-  if (nb == 1) return;  // written directly by the decode kernel
   int qo_start = b, qo_len = 1;
   if (p.qo_indptr) {
     qo_start = p.qo_indptr[b];
     qo_len = p.qo_indptr[b + 1] - qo_start;
   }
+  int c0, nb;
+  if constexpr (WIN) {
+    c0 = b * p.splits;
+    const int np = p.kv_indptr[b + 1] - p.kv_indptr[b];
+    const int kv_len = np > 0 ? (np - 1) * p.page_size + p.last_page_len[b] : 0;
+    nb = win_tiles(kv_len, qo_len, p.window_left, p.sinks, p.splits).items;
+  } else {
+    c0 = p.chunk_indptr[b];
+    nb = p.chunk_indptr[b + 1] - c0;
+  }
+  if (nb == 1) return;  // written directly by the decode kernel
   const int G = p.group;
   const int rows = (PAIR ? 2 : 1) * qo_len * G;
   if (qo_len * G > p.short_rows) return;  // long-query request: written by the prefill kernel

@@ -614,7 +614,7 @@ static int launch_prefill(const PrefillParams& pp, int head_dim, int grid, hipSt
 // crossing the XCDs' L2 caches by agent-scope stores or by fences, the same 64
 // tiles took 63 and 84 us of kernel against 44 + 8.)
 constexpr int kPfMergeThreads = 512;
-template <typename MT, int D>
+template <typename MT, int D, bool WIN = false>
 MI_DEVICE void prefill_merge_body(const PrefillParams& p, int first_wave, int waves) {
   constexpr int VW = D / 16, NV = D / 64, ROWS = pf_rows(D), NG = ROWS / 16, U = D > 128 ? 4 : 8;
   constexpr float kNegInf = -__builtin_inff();
@@ -625,9 +625,18 @@ MI_DEVICE void prefill_merge_body(const PrefillParams& p, int first_wave, int wa
     const int part = w & 3, rgi = (w >> 2) % NG, th = (w >> 2) / NG;
     const int h = th % nkv;
     const int4 st = p.split_tiles[th / nkv];
-    const int b = uniform(st.x), n = uniform(st.z), slot = uniform(st.w) + h * n;
+    const int b = uniform(st.x), slot = uniform(st.w) + h * uniform(st.z);
     const int qo_start = p.qo_indptr[b];
     const int rows_total = (p.qo_indptr[b + 1] - qo_start) * G;
+    int n = uniform(st.z);
+    if constexpr (WIN) {  // the pieces that the window leaves (as the kernel counted them)
+      const int row0 = uniform(st.y), qo_len = p.qo_indptr[b + 1] - qo_start;
+      const int kv_len = (p.kv_indptr[b + 1] - p.kv_indptr[b] - 1) * p.page_size + p.last_page_len[b];
+      const int max_tok = (min(row0 + ROWS, rows_total) - 1) / G;
+      const int kv_end = p.causal ? min(kv_len, kv_len - qo_len + max_tok + 1) : kv_len;
+      n = pf_win_pieces(n, pf_win(p, kv_len, qo_len, row0 / G, max_tok, kv_end).total);
+      if (n == 1) continue;  // written by the kernel itself
+    }
     const int row = uniform(st.y) + 16 * rgi + col;
     if (row >= rows_total) continue;
     float4 acc[NV];
@@ -684,10 +693,10 @@ MI_DEVICE void prefill_merge_body(const PrefillParams& p, int first_wave, int wa
   }
 }
 
-template <typename MT, int D>
+template <typename MT, int D, bool WIN = false>
 __global__ __launch_bounds__(kPfMergeThreads) void prefill_merge_kernel(PrefillParams p) {
   constexpr int WAVES = kPfMergeThreads / 64;
-  prefill_merge_body<MT, D>(p, (int)blockIdx.x * WAVES, (int)gridDim.x * WAVES);
+  prefill_merge_body<MT, D, WIN>(p, (int)blockIdx.x * WAVES, (int)gridDim.x * WAVES);
 }
 
 // Both merges of a call that runs both parts in turn: workgroups below
@@ -715,12 +724,12 @@ static void launch_both_merges(const DecodeParams& d, int batch, const PrefillPa
   }
 }
 
-template <typename MT>
+template <typename MT, bool WIN = false>
 static void launch_prefill_merge(const PrefillParams& pp, int head_dim, int grid, hipStream_t stream) {
   switch (head_dim) {
-    case 64: hipLaunchKernelGGL((prefill_merge_kernel<MT, 64>), dim3(grid), dim3(kPfMergeThreads), 0, stream, pp); break;
-    case 128: hipLaunchKernelGGL((prefill_merge_kernel<MT, 128>), dim3(grid), dim3(kPfMergeThreads), 0, stream, pp); break;
-    default: hipLaunchKernelGGL((prefill_merge_kernel<MT, 256>), dim3(grid), dim3(kPfMergeThreads), 0, stream, pp); break;
+    case 64: hipLaunchKernelGGL((prefill_merge_kernel<MT, 64, WIN>), dim3(grid), dim3(kPfMergeThreads), 0, stream, pp); break;
+    case 128: hipLaunchKernelGGL((prefill_merge_kernel<MT, 128, WIN>), dim3(grid), dim3(kPfMergeThreads), 0, stream, pp); break;
+    default: hipLaunchKernelGGL((prefill_merge_kernel<MT, 256, WIN>), dim3(grid), dim3(kPfMergeThreads), 0, stream, pp); break;
   }
 }
 
@@ -870,12 +879,25 @@ namespace mi {
 constexpr int kPhaseShort = 1;  // short-query requests: split-KV decode kernel + merge
 constexpr int kPhaseTiles = 2;  // long-query requests: MFMA prefill tiles
 
+constexpr int32_t kPfWinMax = 1 << 30;  // beyond any context; sums with a length stay in 32 bits
+
+static int launch_prefill_more(const PrefillParams& pp, bool f16, int kvt, bool win, int head_dim, int grid,
+                               hipStream_t stream) {
+  switch (head_dim) {
+    case 64: return (win ? prefill_win_d64_launch : prefill_mx_d64_launch)(pp, f16, kvt, grid, stream);
+    case 128: return (win ? prefill_win_d128_launch : prefill_mx_d128_launch)(pp, f16, kvt, grid, stream);
+    case 256: return (win ? prefill_win_d256_launch : prefill_mx_d256_launch)(pp, f16, kvt, grid, stream);
+    default: return MI_ERR_UNSUPPORTED;
+  }
+}
+
 static int prefill_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_token, int64_t q_stride_head,
                             const mi_paged_kv* kv, const int32_t* qo_indptr, const int32_t* kv_indptr,
                             const int32_t* kv_indices, const int32_t* last_page_len, int32_t batch,
                             int32_t max_qo_tokens, int32_t num_qo_heads, int32_t causal, float sm_scale,
                             void* workspace, int64_t workspace_bytes, void* out, int64_t out_stride_token,
-                            int64_t out_stride_head, int phases, void* stream) {
+                            int64_t out_stride_head, int phases, void* stream, int32_t window_left = -1,
+                            int32_t sinks = 0) {
   if (!kv || batch < 0 || max_qo_tokens < 0 || !workspace) return MI_ERR_INVALID;
   if (batch == 0) return MI_OK;
   if (!q || !out || !kv->data || !qo_indptr || !kv_indptr || !kv_indices || !last_page_len) return MI_ERR_INVALID;
@@ -883,18 +905,18 @@ static int prefill_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_tok
   if (nkv <= 0 || num_qo_heads <= 0 || num_qo_heads % nkv) return MI_ERR_INVALID;
   const int G = num_qo_heads / nkv;
   if (G > kShortRows || kv->page_size % 16 || !ok_head_dim(D)) return MI_ERR_UNSUPPORTED;
-  const bool fp8 = kv->dtype == MI_FP8_E4M3;
+  const bool fp8 = kv->dtype == MI_FP8_E4M3, mx = kv_is_mx(kv->dtype), win = window_left >= 0;
   if (q_dtype != MI_BF16 && q_dtype != MI_F16 && q_dtype != MI_F32) return MI_ERR_UNSUPPORTED;
-  if (!fp8 && kv->dtype != q_dtype) return MI_ERR_UNSUPPORTED;
-  if (fp8 && q_dtype == MI_F32) return MI_ERR_UNSUPPORTED;
-  if (fp8 && (!kv->k_scale || !kv->v_scale)) return MI_ERR_INVALID;
+  if (!fp8 && !mx && kv->dtype != q_dtype) return MI_ERR_UNSUPPORTED;
+  if ((fp8 || mx || win) && q_dtype == MI_F32) return MI_ERR_UNSUPPORTED;
+  if (!kv_scales_ok(kv)) return MI_ERR_INVALID;
   const int qesz = q_dtype == MI_F32 ? 4 : 2;
   if (!rows_aligned16(q, q_stride_token, q_stride_head, qesz) ||
       !rows_aligned16(out, out_stride_token, out_stride_head, qesz) || !kv_aligned16(kv))
     return MI_ERR_INVALID;
   // the tile loader keeps a chunk's offset within a page (K/V half, token
   // row, column) in 32 bits
-  const int64_t kvesz = fp8 ? 1 : kv->dtype == MI_F32 ? 4 : 2;
+  const int64_t kvesz = kv_elem_bytes(kv->dtype);
   if (kv->kv_stride < 0 || kv->token_stride < 0 ||
       (kv->kv_stride + (int64_t)kv->page_size * kv->token_stride) * kvesz >= (1LL << 31))
     return MI_ERR_UNSUPPORTED;
@@ -904,14 +926,14 @@ static int prefill_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_tok
   int st = MI_OK;
   const PfSplitLayout P = pf_split_of(L, batch, G, nkv, D, workspace_bytes);
   // both parts in one call: one launch merges both (both_merges_kernel)
-  const bool both = phases == (kPhaseShort | kPhaseTiles) && P.parts > 0 && q_dtype != MI_F32 &&
+  const bool both = phases == (kPhaseShort | kPhaseTiles) && P.parts > 0 && q_dtype != MI_F32 && !win &&
                     !pair_heads(nullptr, batch, nkv, G, D, true);
   DecodeParams dmerge{};
   if (phases & kPhaseShort) {
     st = decode_run_impl(q, q_dtype, q_stride_token, q_stride_head, kv, qo_indptr, kv_indptr, kv_indices,
                          last_page_len, batch, num_qo_heads, causal, sm_scale, workspace, workspace_bytes,
                          L.split, out, out_stride_token, out_stride_head, kPhaseAttend | (both ? 0 : kPhaseMerge), s,
-                         true, &dmerge);
+                         true, &dmerge, window_left, sinks);
     if (st != MI_OK) return st;
   }
   if (!(phases & kPhaseTiles)) return MI_OK;
@@ -977,12 +999,16 @@ static int prefill_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_tok
   pp.page_size = kv->page_size;
   pp.causal = causal ? 1 : 0;
   pp.scale_log2 = sm_scale * 1.4426950408889634f;
+  pp.window_left = window_left < kPfWinMax ? window_left : kPfWinMax;
+  pp.sinks = sinks < kPfWinMax ? sinks : kPfWinMax;
   // persistent grid: one workgroup per CU (each holds two wavefronts per
   // SIMD), never more than there can be units
   const int ncu = device_cu_count();
   const int64_t units = (int64_t)(P.parts > 0 ? P.max_pieces : L.max_tiles) * nkv;
   const int grid = (int)(((units < ncu ? units : (int64_t)ncu) + 7) / 8 * 8);
-  if (q_dtype == MI_BF16)
+  if (win || mx)
+    st = launch_prefill_more(pp, q_dtype == MI_F16, kv_format(kv->dtype), win, D, grid, s);
+  else if (q_dtype == MI_BF16)
     st = fp8 ? launch_prefill<BF16, true>(pp, D, grid, s) : launch_prefill<BF16, false>(pp, D, grid, s);
   else
     st = fp8 ? launch_prefill<F16, true>(pp, D, grid, s) : launch_prefill<F16, false>(pp, D, grid, s);
@@ -992,15 +1018,18 @@ static int prefill_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_tok
   if (both) {
     const int64_t waves = (int64_t)L.max_tiles * nkv * (pf_rows(D) / 16) * 4;
     const int grid2 = batch * nkv + (int)(waves < 8LL * ncu ? (waves + 3) / 4 : 2LL * ncu);
+    const bool bytes = fp8 || mx;
     if (q_dtype == MI_BF16)
-      fp8 ? launch_both_merges<BF16, true>(dmerge, batch, pp, D, grid2, s) : launch_both_merges<BF16, false>(dmerge, batch, pp, D, grid2, s);
+      bytes ? launch_both_merges<BF16, true>(dmerge, batch, pp, D, grid2, s) : launch_both_merges<BF16, false>(dmerge, batch, pp, D, grid2, s);
     else
-      fp8 ? launch_both_merges<F16, true>(dmerge, batch, pp, D, grid2, s) : launch_both_merges<F16, false>(dmerge, batch, pp, D, grid2, s);
+      bytes ? launch_both_merges<F16, true>(dmerge, batch, pp, D, grid2, s) : launch_both_merges<F16, false>(dmerge, batch, pp, D, grid2, s);
   } else if (P.parts > 0) {
     const int64_t waves = (int64_t)L.max_tiles * nkv * (pf_rows(D) / 16) * 4, per = kPfMergeThreads / 64;
     const int mgrid = (int)(waves < ncu * per ? (waves + per - 1) / per : ncu);
-    if (q_dtype == MI_BF16) launch_prefill_merge<BF16>(pp, D, mgrid, s);
-    else launch_prefill_merge<F16>(pp, D, mgrid, s);
+    if (q_dtype == MI_BF16)
+      win ? launch_prefill_merge<BF16, true>(pp, D, mgrid, s) : launch_prefill_merge<BF16>(pp, D, mgrid, s);
+    else
+      win ? launch_prefill_merge<F16, true>(pp, D, mgrid, s) : launch_prefill_merge<F16>(pp, D, mgrid, s);
   }
   MI_CHECK_LAUNCH();
   return MI_OK;
@@ -1022,3 +1051,17 @@ static int prefill_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_tok
 extern "C" int mi_prefill_run(MI_PREFILL_ARGS) { return MI_PREFILL_FWD(mi::kPhaseShort | mi::kPhaseTiles); }
 extern "C" int mi_prefill_short(MI_PREFILL_ARGS) { return MI_PREFILL_FWD(mi::kPhaseShort); }
 extern "C" int mi_prefill_tiles(MI_PREFILL_ARGS) { return MI_PREFILL_FWD(mi::kPhaseTiles); }
+
+extern "C" int mi_prefill_run_window(const void* q, int32_t q_dtype, int64_t q_stride_token, int64_t q_stride_head,
+                                     const mi_paged_kv* kv, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                     const int32_t* kv_indices, const int32_t* last_page_len, int32_t batch,
+                                     int32_t max_qo_tokens, int32_t num_qo_heads, int32_t causal, float sm_scale,
+                                     int32_t window_left, int32_t sink_tokens, int32_t parts, void* workspace,
+                                     int64_t workspace_bytes, void* out, int64_t out_stride_token,
+                                     int64_t out_stride_head, void* stream) {
+  if (sink_tokens < 0 || parts < 1 || parts > (mi::kPhaseShort | mi::kPhaseTiles)) return MI_ERR_INVALID;
+  return mi::prefill_run_impl(q, q_dtype, q_stride_token, q_stride_head, kv, qo_indptr, kv_indptr, kv_indices,
+                              last_page_len, batch, max_qo_tokens, num_qo_heads, causal, sm_scale, workspace,
+                              workspace_bytes, out, out_stride_token, out_stride_head, parts, stream, window_left,
+                              sink_tokens);
+}

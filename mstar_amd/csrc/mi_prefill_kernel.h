@@ -53,7 +53,37 @@ struct PrefillParams {
   int64_t out_stride_tok, out_stride_head;
   int32_t num_kv_heads, group, page_size, causal;
   float scale_log2;
+  int32_t window_left, sinks;  // windowed runs: as DecodeParams
 };
+
+// The 32-key steps of a tile of a windowed run: the steps that hold sinks,
+// then those from `first` on, `total` in all; step t starts at key(t).  lo:
+// where the window of the tile's first row begins, hi: of its last row.
+struct PfWin {
+  int lo, hi, sinks, first, total;
+  MI_DEVICE int key(int t) const { return kPfKeys * (t < sinks ? t : t - sinks + first); }
+  // The keys whose page a 16-key group at `key` reads: its own, or, where the
+  // window hides the whole group, the window's first (their pages may be gone).
+  MI_DEVICE int read_key(int key, int sink_tokens) const { return key + 15 < lo && key >= sink_tokens ? lo & ~15 : key; }
+  // some row of the tile has its window begin behind the step's first key, and not all of it are sinks
+  MI_DEVICE bool partial(int kb, int sink_tokens) const { return kb < hi && kb + kPfKeys > sink_tokens; }
+};
+MI_DEVICE PfWin pf_win(const PrefillParams& p, int kv_len, int qo_len, int min_tok, int max_tok, int kv_end) {
+  PfWin w;
+  w.lo = kv_len - qo_len + min_tok - p.window_left;
+  w.hi = w.lo + max_tok - min_tok;
+  // a window that begins behind the keys the tile may see (a tail of rows without keys) is empty
+  const int steps = kv_end > 0 ? (kv_end + kPfKeys - 1) / kPfKeys : 0;
+  w.first = min(max(0, w.lo) / kPfKeys, steps);
+  w.sinks = min((p.sinks + kPfKeys - 1) / kPfKeys, w.first);
+  w.total = w.sinks + steps - w.first;
+  return w;
+}
+// Pieces of a tile of a windowed run: the plan cut it for all its keys, so
+// where the window leaves few steps a piece, fewer pieces share them (the
+// others of the plan's have nothing to do).
+constexpr int kPfWinPieceSteps = 8;
+MI_DEVICE int pf_win_pieces(int n, int total) { return max(1, min(n, total / kPfWinPieceSteps)); }
 
 // A unit's tile and, for a piece of a split tile, which part of the tile's
 // key steps it covers and where its partial goes.
@@ -168,7 +198,7 @@ MI_DEVICE void pf_done(const PrefillParams& p) {
   }
 }
 
-template <typename MT, bool FP8, int D>
+template <typename MT, int KVT, int D>
 struct PrefillCfg {
   static constexpr int THREADS = 64 * pf_waves(D);
   static constexpr int ROWS = pf_rows(D);
@@ -179,8 +209,8 @@ struct PrefillCfg {
   // V rows step 8 banks so the 4 rows x 32 bytes of one transposing read do.
   static constexpr int RSK = D * 2 + 32;
   static constexpr int RSV = D * 2 + 32;
-  static constexpr int ESZ = FP8 ? 1 : 2;                  // cache element size
-  static constexpr int CPR = D * ESZ / 16;                 // 16-byte chunks per cached row
+  static constexpr int ESZ = KVT == kKv16 ? 2 : 1;         // what the cache's strides count
+  static constexpr int CPR = KVT == kKvMx4 ? D / 32 : D * ESZ / 16;  // 16-byte chunks per cached row
   static constexpr int HALF = KEYS * CPR;                  // chunks of the K (or V) half of a tile
   static constexpr int NL = (2 * HALF + THREADS - 1) / THREADS;  // loader chunks per thread
   static constexpr int STAGE = KEYS * (RSK + RSV);         // one LDS stage: K rows then V rows
@@ -188,18 +218,20 @@ struct PrefillCfg {
   static_assert((2 * HALF) % THREADS == 0 || 2 * HALF < THREADS, "loader mapping");
 };
 
-template <typename MT, bool FP8, int D>
+template <typename MT, int KVT, int D, bool WIN = false>
 __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams p) {
   static_assert(D <= 128, "head_dim 256 runs prefill_rs_kernel");
-  using C = PrefillCfg<MT, FP8, D>;
+  using C = PrefillCfg<MT, KVT, D>;
+  constexpr bool FP8 = KVT == kKvFp8, MX = KVT == kKvMx8 || KVT == kKvMx4;
   constexpr int KS = D / 32, VW = D / 16, KEYS = C::KEYS, RSK = C::RSK, RSV = C::RSV, ESZ = C::ESZ, CPR = C::CPR;
   constexpr int THREADS = C::THREADS, NL = C::NL, HALF = C::HALF, STAGE = C::STAGE;
   constexpr int RG = pf_rg(D), WROWS = 16 * RG;  // 16-row groups and rows per wavefront
-  constexpr int LCH = FP8 ? 32 : 16;  // LDS bytes per loaded chunk
+  constexpr int LCH = KVT == kKvMx4 ? 64 : KVT == kKv16 ? 16 : 32;  // LDS bytes per loaded chunk
   constexpr float kNegInf = -__builtin_inff();
   __shared__ __attribute__((aligned(16))) uint8_t lds[3 * STAGE];
   // byte offset (from the head's base) of the first row of each 16-row group of the staged tiles
   __shared__ int64_t lds_toff[2 * kPfTileCap];
+  __shared__ int64_t lds_soff[MX ? 2 * kPfTileCap : 1];  // and of its scale bytes
 
   __shared__ int s_unit, s_slot;
 
@@ -213,9 +245,9 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
   const int unit = uniform(s_unit);
   __syncthreads();
   if (unit < 0) break;
-  const PfUnit un = pf_unit(p, unit);
+  PfUnit un = pf_unit(p, unit);
   const int h = un.h, b = un.b, row0 = un.row0;
-  s_slot = un.n > 1 ? un.slot : -1;  // for the epilogue: no register is held for it
+  if constexpr (!WIN) s_slot = un.n > 1 ? un.slot : -1;  // for the epilogue: no register is held for it
 
   const int tid = threadIdx.x;
   const int lane = lane_id();
@@ -231,7 +263,7 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
 
   // ---- this lane's query rows (one per 16-row group)
   uint4 qf[RG][KS];
-  int lim[RG];
+  int lim[RG], low[RG];  // the row's last key; WIN: the first of its window
 #pragma unroll
   for (int rg = 0; rg < RG; ++rg) {
     const int n = row0 + WROWS * wave + 16 * rg + col;
@@ -239,6 +271,7 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
     const bool valid = n < rows_total;
     const int l = p.causal ? (kv_len - qo_len + tok) : (kv_len - 1);
     lim[rg] = min(l, kv_len - 1);
+    if constexpr (WIN) low[rg] = kv_len - qo_len + tok - p.window_left;
     const uint16_t* qrow = (const uint16_t*)p.q + (int64_t)(qo_start + tok) * p.q_stride_tok +
                            (int64_t)(h * G + g) * p.q_stride_head;
 #pragma unroll
@@ -250,7 +283,18 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
   const int max_tok = last_row / G, min_tok = row0 / G;
   const int kv_end = p.causal ? min(kv_len, kv_len - qo_len + max_tok + 1) : kv_len;
   const int mask_from = p.causal ? (kv_len - qo_len + min_tok + 1) : kv_len;
-  const int n_kt = kv_end > 0 ? (kv_end + KEYS - 1) / KEYS : 0;
+  int n_kt = kv_end > 0 ? (kv_end + KEYS - 1) / KEYS : 0;
+  PfWin win;
+  if constexpr (WIN) {
+    win = pf_win(p, kv_len, qo_len, min_tok, max_tok, kv_end);
+    n_kt = win.total;
+    if (un.n > 1) {
+      const int n = pf_win_pieces(un.n, n_kt);
+      un.n = un.k < n ? n : 0;
+    }
+    s_slot = un.n > 1 ? un.slot : -1;
+  }
+  auto key_of = [&](int t) { return WIN ? win.key(t) : t * KEYS; };
   // key steps of this unit: all of the tile's, or its piece's share
   const int kt0 = un.n > 1 ? un.k * n_kt / un.n : 0, kt1 = un.n > 1 ? (un.k + 1) * n_kt / un.n : n_kt;
   if (un.n == 0) continue;  // uniform; no wait for the unit's entry ahead of the loads above
@@ -267,9 +311,12 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
   // of one half starting at a multiple of 64/CPR, so they lie in one
   // 16-row group of keys and hence in one page (page_size is a multiple of
   // 16, tiles start at multiples of 32): page and slot base are scalars.
+  // (Rows of 32 bytes put 32 rows in a wavefront's load: WIDE, addresses per lane.)
+  constexpr bool WIDE = CPR < 4;
   const uint8_t* kvb = (const uint8_t*)p.kv + (int64_t)h * p.head_stride * ESZ;
   const int64_t tok_bytes = p.token_stride * ESZ;
 
+  uint32_t l_soff[NL];  // MX: offset of the chunk's scale bytes likewise
   uint32_t l_off[NL];   // per-thread byte offset within (page, first slot of its group)
   int l_grp[NL];        // first key row of the 16-row group (wave-uniform)
   int l_row[NL];        // key row within the tile
@@ -280,9 +327,11 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
     const int half = c / HALF, rem = c - half * HALF;
     const int row = rem / CPR, ch = rem - row * CPR;
     l_row[i] = row;
-    l_grp[i] = uniform(row) & ~15;
+    l_grp[i] = (WIDE ? row : uniform(row)) & ~15;
     l_v[i] = half == 1;
     l_off[i] = (uint32_t)((int64_t)half * p.kv_stride * ESZ + (int64_t)(row - (row & ~15)) * tok_bytes + 16 * ch);
+    if constexpr (MX)  // one block of 32 elements per chunk at four bits, half of one at eight
+      l_soff[i] = (uint32_t)((h * (D / kMxBlock) + (KVT == kKvMx4 ? ch : ch >> 1)) * ps + (row & 15));
   }
   const int key_cap = np * ps - 16;  // last 16-row group inside the request's pages
   const int64_t page_bytes = p.page_stride * ESZ;
@@ -294,6 +343,7 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
   constexpr int NB = 2;
   constexpr int UNR = 6;
   uint4 rr[NB][NL];
+  uint8_t rsc[MX ? NB : 1][NL];  // MX: scale bytes of the chunks
   // A tile's loads in two parts: the row-group addresses (LDS reads of the
   // table staged per unit) and the global loads, so a step can read the
   // addresses early and issue the loads later with no address arithmetic
@@ -302,23 +352,27 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
 #pragma unroll
     for (int i = 0; i < NL; ++i) pg[i] = lds_toff[2 * (t - c0) + (l_grp[i] >> 4)];
   };
-  auto load_tile_at = [&](const int64_t (&pg)[NL], uint4 (&r)[NL]) {
+  auto load_tile_at = [&](const int64_t (&pg)[NL], int t, uint4 (&r)[NL], uint8_t (&rs)[NL]) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       if (2 * HALF % THREADS == 0 || tid + i * THREADS < 2 * HALF) {
-        const uint8_t* base = kvb + uniform64(pg[i]);
+        const uint8_t* base = kvb + (WIDE ? pg[i] : uniform64(pg[i]));
         r[i] = *(const uint4*)(base + l_off[i]);
+        if constexpr (MX) {
+          const int64_t so = lds_soff[2 * (t - c0) + (l_grp[i] >> 4)];
+          rs[i] = ((const uint8_t*)(l_v[i] ? p.v_scale : p.k_scale) + (WIDE ? so : uniform64(so)))[l_soff[i]];
+        }
       }
     }
   };
-  auto load_tile = [&](int t, uint4 (&r)[NL]) {
+  auto load_tile = [&](int t, uint4 (&r)[NL], uint8_t (&rs)[NL]) {
     int64_t pg[NL];
     tile_pages(t, pg);
-    load_tile_at(pg, r);
+    load_tile_at(pg, t, r, rs);
   };
   // TAIL: the tile may reach past kv_len (only the request's last tile can),
   // so its V rows past the end are overwritten with zeros
-  auto store_tile_impl = [&](int t, const uint4 (&r)[NL], int stage, auto tail) {
+  auto store_tile_impl = [&](int t, const uint4 (&r)[NL], const uint8_t (&rs)[NL], int stage, auto tail) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int c = tid + i * THREADS;
@@ -337,14 +391,23 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
           }
           *(uint4*)dst = make_uint4(o[0], o[1], o[2], o[3]);
           *(uint4*)(dst + 16) = make_uint4(o[4], o[5], o[6], o[7]);
+        } else if constexpr (MX) {
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          uint32_t o[LCH / 4];
+          mx_to_mt<MT, KVT>(w, mx_scale(rs[i], 0), o);
+#pragma unroll
+          for (int k = 0; k < LCH / 16; ++k)
+            *(uint4*)(dst + 16 * k) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
         } else {
           *(uint4*)dst = v;
         }
         // V rows past the KV end may hold anything (unwritten slots of the last page)
         if constexpr (decltype(tail)::value) {
-          if (l_v[i] && t * KEYS + l_row[i] >= kv_len) {
-            *(uint4*)dst = make_uint4(0, 0, 0, 0);
-            if constexpr (FP8) *(uint4*)(dst + 16) = make_uint4(0, 0, 0, 0);
+          // and so may the keys between the sinks and every row's window
+          const int key = key_of(t) + l_row[i];
+          if (l_v[i] && (key >= kv_len || (WIN && key < win.lo && key >= p.sinks))) {
+#pragma unroll
+            for (int k = 0; k < LCH / 16; ++k) *(uint4*)(dst + 16 * k) = make_uint4(0, 0, 0, 0);
           }
         }
       }
@@ -352,11 +415,12 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
   };
   // Tiles before the request's last one hold no row past kv_len (kv_end <=
   // kv_len): their stores skip the tail test, chosen by a wave-uniform branch.
-  auto store_tile = [&](int t, const uint4 (&r)[NL], int stage) {
-    if (t * KEYS + KEYS > kv_len)
-      store_tile_impl(t, r, stage, std::true_type{});
+  auto store_tile = [&](int t, const uint4 (&r)[NL], const uint8_t (&rs)[NL], int stage) {
+    const int kb = key_of(t);
+    if (kb + KEYS > kv_len || (WIN && kb < win.lo && kb + KEYS > p.sinks))
+      store_tile_impl(t, r, rs, stage, std::true_type{});
     else
-      store_tile_impl(t, r, stage, std::false_type{});
+      store_tile_impl(t, r, rs, stage, std::false_type{});
   };
 
   f32x4 acc[RG][VW];
@@ -422,15 +486,16 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
   // and raises the running max when needed (a rare branch); sm_exp forms
   // the probabilities and their row sums.
   auto sm_max = [&](int t, f32x4 (&s)[RG][2]) {
-    const int kb = t * KEYS;
-    if (t >= t_mask) {  // wave-uniform: only the tiles that reach past some row's limit
+    const int kb = key_of(t);
+    if (WIN ? kb + KEYS > mask_from || win.partial(kb, p.sinks) : t >= t_mask) {  // wave-uniform: only the tiles that reach past some row's limit
 #pragma unroll
       for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
         for (int js = 0; js < 2; ++js)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (kb + 16 * js + 4 * grp + r > lim[rg]) s[rg][js][r] = kNegInf;
+            if (const int key = kb + 16 * js + 4 * grp + r; key > lim[rg] || (WIN && key < low[rg] && key >= p.sinks))
+              s[rg][js][r] = kNegInf;
     }
     // A row's max exceeds the threshold iff one of its four lanes' maxima
     // does, so the cross-lane row max is only needed on the rare branch.
@@ -520,10 +585,14 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
     const int t1 = min(kt1, c0 + kPfTileCap);
     __syncthreads();
     for (int e = tid; e < 2 * (t1 - t0); e += THREADS) {
-      const int key = min((t0 + (e >> 1)) * KEYS + 16 * (e & 1), key_cap);
+      int key = key_of(t0 + (e >> 1)) + 16 * (e & 1);
+      if constexpr (WIN) key = win.read_key(key, p.sinks);
+      key = min(key, key_cap);
       const int pidx = (int)((unsigned)key / (unsigned)ps);
       const int slot = key - pidx * ps;
-      lds_toff[e] = (int64_t)p.kv_indices[page_base + pidx] * page_bytes + (int64_t)slot * tok_bytes;
+      const int64_t page = p.kv_indices[page_base + pidx];
+      lds_toff[e] = page * page_bytes + (int64_t)slot * tok_bytes;
+      if constexpr (MX) lds_soff[e] = page * (2LL * p.num_kv_heads * (D / kMxBlock) * ps) + slot;
     }
     __syncthreads();
     const int tl = t1 - 1;
@@ -532,9 +601,9 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
     // T-2 used; the register buffer it came from then takes tile T+1+NB.
     const int n = t1 - t0;
 #pragma unroll
-    for (int u = 0; u < NB; ++u) load_tile(min(t0 + u, tl), rr[u]);
-    store_tile(t0, rr[0], 0);
-    load_tile(min(t0 + NB, tl), rr[0]);
+    for (int u = 0; u < NB; ++u) load_tile(min(t0 + u, tl), rr[u], rsc[MX ? u : 0]);
+    store_tile(t0, rr[0], rsc[0], 0);
+    load_tile(min(t0 + NB, tl), rr[0], rsc[0]);
     __syncthreads();
     f32x4 sc[RG][2];
     uint4 pbk[RG];
@@ -546,8 +615,8 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
       sm_max(t0, sc);
       sm_exp(sc, pbk);
     }
-    store_tile(min(t0 + 1, tl), rr[1], 1);
-    load_tile(min(t0 + 1 + NB, tl), rr[1]);
+    store_tile(min(t0 + 1, tl), rr[1], rsc[MX ? 1 : 0], 1);
+    load_tile(min(t0 + 1 + NB, tl), rr[1], rsc[MX ? 1 : 0]);
     __syncthreads();
     // steps 1 .. n-1
     for (int i = 1; i < n; i += UNR) {
@@ -566,10 +635,10 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
         // (c4 583 -> 580 us).
         if (grp_a) {
           __builtin_amdgcn_s_setprio(1);
-          store_tile(min(T + 1, tl), rr[(u + 2) % NB], (u + 2) % 3);
+          store_tile(min(T + 1, tl), rr[(u + 2) % NB], rsc[MX ? (u + 2) % NB : 0], (u + 2) % 3);
           sm_max(T - 1, sc);
           sm_exp(sc, pbk);
-          load_tile_at(pg4, rr[(u + 2) % NB]);
+          load_tile_at(pg4, min(T + 1 + NB, tl), rr[(u + 2) % NB], rsc[MX ? (u + 2) % NB : 0]);
           __builtin_amdgcn_s_setprio(0);
         }
         // scores of tile T first (group B's softmax waits on them), then P.V of
@@ -579,8 +648,8 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
         vfrag((u + 1) % 3, va);
         if (!grp_a) {
           __builtin_amdgcn_s_setprio(1);
-          store_tile(min(T + 1, tl), rr[(u + 2) % NB], (u + 2) % 3);
-          load_tile_at(pg4, rr[(u + 2) % NB]);
+          store_tile(min(T + 1, tl), rr[(u + 2) % NB], rsc[MX ? (u + 2) % NB : 0], (u + 2) % 3);
+          load_tile_at(pg4, min(T + 1 + NB, tl), rr[(u + 2) % NB], rsc[MX ? (u + 2) % NB : 0]);
           sm_max(T, sc);
           sm_exp(sc, pbk);
           __builtin_amdgcn_s_setprio(0);
@@ -626,5 +695,12 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
 
 // head_dim 128 launches, defined in mi_prefill_d128.hip
 int prefill_d128_launch(const PrefillParams& pp, bool f16, bool fp8, int grid, hipStream_t stream);
+// Windowed tiles and tiles over microscaled caches: mi_prefill_win_d*.hip and mi_prefill_mx_d*.hip
+int prefill_win_d64_launch(const PrefillParams& pp, bool f16, int kvt, int grid, hipStream_t stream);
+int prefill_win_d128_launch(const PrefillParams& pp, bool f16, int kvt, int grid, hipStream_t stream);
+int prefill_win_d256_launch(const PrefillParams& pp, bool f16, int kvt, int grid, hipStream_t stream);
+int prefill_mx_d64_launch(const PrefillParams& pp, bool f16, int kvt, int grid, hipStream_t stream);
+int prefill_mx_d128_launch(const PrefillParams& pp, bool f16, int kvt, int grid, hipStream_t stream);
+int prefill_mx_d256_launch(const PrefillParams& pp, bool f16, int kvt, int grid, hipStream_t stream);
 
 }  // namespace mi

@@ -1,0 +1,21 @@
+// Prefill tiles over microscaled caches at head_dim 64 (mi_prefill_kernel.h).
+#include "mi_prefill_kernel.h"
+
+namespace mi {
+
+template <typename MT>
+static int launch(const PrefillParams& pp, int kvt, int grid, hipStream_t stream) {
+  const dim3 block(64 * pf_waves(64));
+  switch (kvt) {
+    case kKvMx8: hipLaunchKernelGGL((prefill_kernel<MT, kKvMx8, 64, false>), dim3(grid), block, 0, stream, pp); break;
+    case kKvMx4: hipLaunchKernelGGL((prefill_kernel<MT, kKvMx4, 64, false>), dim3(grid), block, 0, stream, pp); break;
+    default: return MI_ERR_UNSUPPORTED;
+  }
+  return MI_OK;
+}
+
+int prefill_mx_d64_launch(const PrefillParams& pp, bool f16, int kvt, int grid, hipStream_t stream) {
+  return f16 ? launch<F16>(pp, kvt, grid, stream) : launch<BF16>(pp, kvt, grid, stream);
+}
+
+}  // namespace mi

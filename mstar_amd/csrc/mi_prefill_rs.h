@@ -29,16 +29,17 @@
 
 namespace mi {
 
-template <typename MT, bool FP8, int D>
+template <typename MT, int KVT, int D, bool WIN = false>
 __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
-  using C = PrefillCfg<MT, FP8, D>;
+  using C = PrefillCfg<MT, KVT, D>;
+  constexpr bool FP8 = KVT == kKvFp8, MX = KVT == kKvMx8 || KVT == kKvMx4;
   // 16-row groups per pair: the O-role's accumulators (RGP x D/16 f32x4) fill
   // 128 registers at either head_dim; C::ROWS = 4 pairs x 16 x RGP
   constexpr int RGP = D > 128 ? 2 : 4, PROWS = 16 * RGP;
   static_assert(C::ROWS == 4 * PROWS, "tile rows = four pairs");
   constexpr int KS = D / 32, VW = D / 16, KEYS = C::KEYS, RSK = C::RSK, RSV = C::RSV, ESZ = C::ESZ, CPR = C::CPR;
   constexpr int THREADS = C::THREADS, NL = C::NL, HALF = C::HALF;
-  constexpr int LCH = FP8 ? 32 : 16;  // LDS bytes per loaded chunk
+  constexpr int LCH = KVT == kKvMx4 ? 64 : KVT == kKv16 ? 16 : 32;  // LDS bytes per loaded chunk
   constexpr float kNegInf = -__builtin_inff();
   static_assert(THREADS == 512, "four wavefront pairs");
   static_assert(RSK == RSV, "one LDS row stride for K and V");
@@ -47,13 +48,14 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
   // segment ^ (row & 7)), so the fragment reads stay free of bank conflicts;
   // the page-offset table holds half as many tiles to leave LDS for the rings.
   // fp8 caches: a 3-stage ring of padded rows, stored from registers.
-  constexpr bool DMA = !FP8;
+  constexpr bool DMA = KVT == kKv16;
   constexpr int RS = DMA ? D * 2 : RSK;  // LDS row stride
   constexpr int KSZ = KEYS * RS, VSZ = KEYS * RS, NKS = DMA ? 4 : 3, NVS = DMA ? 4 : 3, VOFF = NKS * KSZ;
   constexpr int CAP = DMA ? kPfTileCap / 2 : kPfTileCap;  // tiles whose page offsets are staged at a time
   static_assert(!DMA || (KEYS == 32 && D * 2 == 512 && THREADS == 512), "direct loads: 4 per thread and tile");
   __shared__ __attribute__((aligned(16))) uint8_t lds[NKS * KSZ + NVS * VSZ];
   __shared__ int64_t lds_toff[2 * CAP];
+  __shared__ int64_t lds_soff[MX ? 2 * CAP : 1];  // byte offsets of the scale bytes
   // probabilities of the step (B operand layout: per pair, row group and lane
   // one uint4) and each row's rescale factor, double-buffered by step parity
   __shared__ uint4 lds_p[2][4][RGP][64];
@@ -83,9 +85,9 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
       const int unit = uniform(s_unit);
       __syncthreads();
       if (unit < 0) break;
-      const PfUnit un = pf_unit(p, unit);
+      PfUnit un = pf_unit(p, unit);
       const int h = un.h, b = un.b, row0 = un.row0;
-      s_slot = un.n > 1 ? un.slot : -1;  // for the epilogue: no register is held for it
+      if constexpr (!WIN) s_slot = un.n > 1 ? un.slot : -1;  // for the epilogue: no register is held for it
       const int qo_start = p.qo_indptr[b];
       const int qo_len = p.qo_indptr[b + 1] - qo_start;
       const int page_base = p.kv_indptr[b];
@@ -95,13 +97,14 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
 
       // R: the S-role's Q fragments (R[rg][s] for s < KS), the O-role's accumulators
       f32x4 R[RGP][VW];
-      int lim[RGP];
+      int lim[RGP], low[RGP];
 #pragma unroll
       for (int rg = 0; rg < RGP; ++rg) {
         const int n = row0 + PROWS * pr + 16 * rg + col;
         const int tok = n / G, g = n - tok * G;
         const int l = p.causal ? (kv_len - qo_len + tok) : (kv_len - 1);
         lim[rg] = min(l, kv_len - 1);
+        if constexpr (WIN) low[rg] = kv_len - qo_len + tok - p.window_left;
         if constexpr (S) {
           const bool valid = n < rows_total;
           const uint16_t* qrow = (const uint16_t*)p.q + (int64_t)(qo_start + tok) * p.q_stride_tok +
@@ -118,7 +121,18 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
       const int max_tok = last_row / G, min_tok = row0 / G;
       const int kv_end = p.causal ? min(kv_len, kv_len - qo_len + max_tok + 1) : kv_len;
       const int mask_from = p.causal ? (kv_len - qo_len + min_tok + 1) : kv_len;
-      const int n_kt = kv_end > 0 ? (kv_end + KEYS - 1) / KEYS : 0;
+      int n_kt = kv_end > 0 ? (kv_end + KEYS - 1) / KEYS : 0;
+      PfWin win;
+      if constexpr (WIN) {
+        win = pf_win(p, kv_len, qo_len, min_tok, max_tok, kv_end);
+        n_kt = win.total;
+        if (un.n > 1) {
+          const int n = pf_win_pieces(un.n, n_kt);
+          un.n = un.k < n ? n : 0;
+        }
+        s_slot = un.n > 1 ? un.slot : -1;
+      }
+      auto key_of = [&](int t) { return WIN ? win.key(t) : t * KEYS; };
       // key steps of this unit: all of the tile's, or its piece's share
       const int kt0 = un.n > 1 ? un.k * n_kt / un.n : 0, kt1 = un.n > 1 ? (un.k + 1) * n_kt / un.n : n_kt;
       if (un.n == 0) continue;  // uniform; no wait for the unit's entry ahead of the loads above
@@ -133,7 +147,7 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
       // ---- loader (as prefill_kernel): chunk c = tid + i*THREADS -> (half, row, 16-byte column)
       const uint8_t* kvb = (const uint8_t*)p.kv + (int64_t)h * p.head_stride * ESZ;
       const int64_t tok_bytes = p.token_stride * ESZ;
-      uint32_t l_off[NL];
+      uint32_t l_off[NL], l_soff[NL];
       int l_grp[NL];
       int l_row[NL];
       bool l_v[NL];
@@ -146,6 +160,7 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
         l_grp[i] = uniform(row) & ~15;
         l_v[i] = half == 1;
         l_off[i] = (uint32_t)((int64_t)half * p.kv_stride * ESZ + (int64_t)(row - (row & ~15)) * tok_bytes + 16 * ch);
+        if constexpr (MX) l_soff[i] = (uint32_t)((h * (D / kMxBlock) + (KVT == kKvMx4 ? ch : ch >> 1)) * ps + (row & 15));
       }
       const int key_cap = np * ps - 16;
       const int64_t page_bytes = p.page_stride * ESZ;
@@ -153,25 +168,29 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
       constexpr int NB = 2;
       constexpr int UNR = 6;
       uint4 rr[NB][NL];
+      uint8_t rsc[MX ? NB : 1][NL];
       auto tile_pages = [&](int t, int64_t (&pg)[NL]) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) pg[i] = lds_toff[2 * (t - c0) + (l_grp[i] >> 4)];
       };
-      auto load_tile_at = [&](const int64_t (&pg)[NL], uint4 (&r)[NL]) {
+      auto load_tile_at = [&](const int64_t (&pg)[NL], int t, uint4 (&r)[NL], uint8_t (&rs)[NL]) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
           if (2 * HALF % THREADS == 0 || tid + i * THREADS < 2 * HALF) {
             const uint8_t* base = kvb + uniform64(pg[i]);
             r[i] = *(const uint4*)(base + l_off[i]);
+            if constexpr (MX)
+              rs[i] = ((const uint8_t*)(l_v[i] ? p.v_scale : p.k_scale) +
+                       uniform64(lds_soff[2 * (t - c0) + (l_grp[i] >> 4)]))[l_soff[i]];
           }
         }
       };
-      auto load_tile = [&](int t, uint4 (&r)[NL]) {
+      auto load_tile = [&](int t, uint4 (&r)[NL], uint8_t (&rs)[NL]) {
         int64_t pg[NL];
         tile_pages(t, pg);
-        load_tile_at(pg, r);
+        load_tile_at(pg, t, r, rs);
       };
-      auto store_tile_impl = [&](int t, const uint4 (&r)[NL], int stage, auto tail) {
+      auto store_tile_impl = [&](int t, const uint4 (&r)[NL], const uint8_t (&rs)[NL], int stage, auto tail) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
           const int c = tid + i * THREADS;
@@ -190,23 +209,33 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
               }
               *(uint4*)dst = make_uint4(o[0], o[1], o[2], o[3]);
               *(uint4*)(dst + 16) = make_uint4(o[4], o[5], o[6], o[7]);
+            } else if constexpr (MX) {
+              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+              uint32_t o[LCH / 4];
+              mx_to_mt<MT, KVT>(w, mx_scale(rs[i], 0), o);
+#pragma unroll
+              for (int k = 0; k < LCH / 16; ++k)
+                *(uint4*)(dst + 16 * k) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
             } else {
               *(uint4*)dst = v;
             }
             if constexpr (decltype(tail)::value) {
-              if (l_v[i] && t * KEYS + l_row[i] >= kv_len) {
-                *(uint4*)dst = make_uint4(0, 0, 0, 0);
-                if constexpr (FP8) *(uint4*)(dst + 16) = make_uint4(0, 0, 0, 0);
+              const int key = key_of(t) + l_row[i];
+              if (l_v[i] && (key >= kv_len || (WIN && key < win.lo && key >= p.sinks))) {
+#pragma unroll
+                for (int k = 0; k < LCH / 16; ++k) *(uint4*)(dst + 16 * k) = make_uint4(0, 0, 0, 0);
               }
             }
           }
         }
       };
-      auto store_tile = [&](int t, const uint4 (&r)[NL], int stage) {
-        if (t * KEYS + KEYS > kv_len)
-          store_tile_impl(t, r, stage, std::true_type{});
+      // the step holds V rows that no row of the tile may see
+      auto hides = [&](int kb) { return kb + KEYS > kv_len || (WIN && kb < win.lo && kb + KEYS > p.sinks); };
+      auto store_tile = [&](int t, const uint4 (&r)[NL], const uint8_t (&rs)[NL], int stage) {
+        if (hides(key_of(t)))
+          store_tile_impl(t, r, rs, stage, std::true_type{});
         else
-          store_tile_impl(t, r, stage, std::false_type{});
+          store_tile_impl(t, r, rs, stage, std::false_type{});
       };
       // Direct loads: load i of wave w fills rows 2*rp, 2*rp+1 (rp = 8*(i&1) + w,
       // both in 16-row group i&1) of the tile's K (i < 2) or V (i >= 2) half;
@@ -242,7 +271,8 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
       // End of a step: this wave's loads of K of the next tile and of V of the
       // current one have landed (`newer` loads may stay in flight: 6 = V of the
       // next tile and both halves of the one after it), and V rows of tile t
-      // past kv_len are zeroed.
+      // past kv_len (WIN: and those between the sinks and every row's window)
+      // are zeroed.
       auto dma_wait = [&](int t, int vst, int newer) {
         if (newer == 6)
           asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
@@ -250,11 +280,12 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
           asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
         else
           asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (t * KEYS + KEYS > kv_len) {
+        const int kb = key_of(t);
+        if (hides(kb)) {
 #pragma unroll
           for (int i = 2; i < 4; ++i) {
-            const int rp = 8 * (i & 1) + wave;
-            if (t * KEYS + 2 * rp + (lane >> 5) >= kv_len)
+            const int rp = 8 * (i & 1) + wave, key = kb + 2 * rp + (lane >> 5);
+            if (key >= kv_len || (WIN && key < win.lo && key >= p.sinks))
               *(uint4*)(lds + VOFF + vst * VSZ + rp * 1024 + 16 * lane) = make_uint4(0, 0, 0, 0);
           }
         }
@@ -314,15 +345,16 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
               for (int js = 0; js < 2; ++js)
                 s[rg][js] = MT::mma_16x16x32(ka[c & 1][k][js], bitcast<uint4>(R[rg][KC * c + k]), s[rg][js]);
         }
-        const int kb = t * KEYS;
-        if (t >= t_mask) {
+        const int kb = key_of(t);
+        if (WIN ? kb + KEYS > mask_from || win.partial(kb, p.sinks) : t >= t_mask) {
 #pragma unroll
           for (int rg = 0; rg < RGP; ++rg)
 #pragma unroll
             for (int js = 0; js < 2; ++js)
 #pragma unroll
               for (int r = 0; r < 4; ++r)
-                if (kb + 16 * js + 4 * grp + r > lim[rg]) s[rg][js][r] = kNegInf;
+                if (const int key = kb + 16 * js + 4 * grp + r; key > lim[rg] || (WIN && key < low[rg] && key >= p.sinks))
+                  s[rg][js][r] = kNegInf;
         }
         float ml[RGP], alpha[RGP];
 #pragma unroll
@@ -438,7 +470,9 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
           const int t1 = min(kt1, c0 + CAP);
           __syncthreads();
           for (int e = tid; e < 2 * (t1 - t0); e += THREADS) {
-            const int key = min((t0 + (e >> 1)) * KEYS + 16 * (e & 1), key_cap);
+            int key = key_of(t0 + (e >> 1)) + 16 * (e & 1);
+            if constexpr (WIN) key = win.read_key(key, p.sinks);
+            key = min(key, key_cap);
             const int pidx = (int)((unsigned)key / (unsigned)ps);
             const int slot = key - pidx * ps;
             lds_toff[e] = (int64_t)p.kv_indices[page_base + pidx] * page_bytes + (int64_t)slot * tok_bytes;
@@ -495,23 +529,27 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
           const int t1 = min(kt1, c0 + kPfTileCap);
           __syncthreads();
           for (int e = tid; e < 2 * (t1 - t0); e += THREADS) {
-            const int key = min((t0 + (e >> 1)) * KEYS + 16 * (e & 1), key_cap);
+            int key = key_of(t0 + (e >> 1)) + 16 * (e & 1);
+            if constexpr (WIN) key = win.read_key(key, p.sinks);
+            key = min(key, key_cap);
             const int pidx = (int)((unsigned)key / (unsigned)ps);
             const int slot = key - pidx * ps;
-            lds_toff[e] = (int64_t)p.kv_indices[page_base + pidx] * page_bytes + (int64_t)slot * tok_bytes;
+            const int64_t page = p.kv_indices[page_base + pidx];
+            lds_toff[e] = page * page_bytes + (int64_t)slot * tok_bytes;
+            if constexpr (MX) lds_soff[e] = page * (2LL * p.num_kv_heads * (D / kMxBlock) * ps) + slot;
           }
           __syncthreads();
           const int tl = t1 - 1;
           const int n = t1 - t0;
 #pragma unroll
-          for (int u = 0; u < NB; ++u) load_tile(min(t0 + u, tl), rr[u]);
-          store_tile(t0, rr[0], 0);
-          load_tile(min(t0 + NB, tl), rr[0]);
+          for (int u = 0; u < NB; ++u) load_tile(min(t0 + u, tl), rr[u], rsc[MX ? u : 0]);
+          store_tile(t0, rr[0], rsc[0], 0);
+          load_tile(min(t0 + NB, tl), rr[0], rsc[0]);
           __syncthreads();
           // step 0: scores of tile t0
           if constexpr (S) s_step(t0, 0);
-          store_tile(min(t0 + 1, tl), rr[1 % NB], 1);
-          load_tile(min(t0 + 1 + NB, tl), rr[1 % NB]);
+          store_tile(min(t0 + 1, tl), rr[1 % NB], rsc[MX ? 1 : 0], 1);
+          load_tile(min(t0 + 1 + NB, tl), rr[1 % NB], rsc[MX ? 1 : 0]);
           __syncthreads();
           for (int i = 1; i < n; i += UNR) {
 #pragma unroll
@@ -521,11 +559,11 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
               const int T = t0 + ii;
               if constexpr (S) {
                 s_step(T, (u + 1) % 3);  // stage of tile T = ii % 3
-                store_tile(min(T + 1, tl), rr[(u + 2) % NB], (u + 2) % 3);
-                load_tile(min(T + 1 + NB, tl), rr[(u + 2) % NB]);
+                store_tile(min(T + 1, tl), rr[(u + 2) % NB], rsc[MX ? (u + 2) % NB : 0], (u + 2) % 3);
+                load_tile(min(T + 1 + NB, tl), rr[(u + 2) % NB], rsc[MX ? (u + 2) % NB : 0]);
               } else {
-                store_tile(min(T + 1, tl), rr[(u + 2) % NB], (u + 2) % 3);
-                load_tile(min(T + 1 + NB, tl), rr[(u + 2) % NB]);
+                store_tile(min(T + 1, tl), rr[(u + 2) % NB], rsc[MX ? (u + 2) % NB : 0], (u + 2) % 3);
+                load_tile(min(T + 1 + NB, tl), rr[(u + 2) % NB], rsc[MX ? (u + 2) % NB : 0]);
                 o_step(T - 1, u % 3);  // stage of tile T-1 = (ii-1) % 3
               }
               __syncthreads();

@@ -22,6 +22,11 @@ Differences from the reference, all deliberate:
   page 0 slot 0, ``flashinfer_utils.py:251-253``).
 * Optional fp8-e4m3 KV caches (``torch.float8_e4m3fn``) with per-head fp32
   ``k_scale``/``v_scale`` passed to ``set_kv_cache`` and ``run``.
+* Microscaled KV caches (:mod:`mstar_amd.mx_cache`): an ``MXKVLayer`` in the place
+  of the KV layer tensor; ``set_kv_cache`` quantises, ``run`` reads the codes.
+* ``run(window_left=, sink_tokens=)``: a sliding window with a few first tokens
+  that stay visible.  It is an argument of the run and not of the plan, so a model
+  that mixes windowed and full layers plans a step once.
 * ``rope_set_kv_cache`` (no reference counterpart) fuses the RoPE call that
   precedes ``set_kv_cache`` in every layer with the append itself.
 """
@@ -34,6 +39,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .mx_cache import MXKVLayer
 from .trace import trace_range
 
 __all__ = [
@@ -44,6 +50,7 @@ __all__ = [
 ]
 
 _MAX_GROUP = 16  # q heads per kv head handled by one MFMA tile
+_WINDOW_MAX = 1 << 30  # beyond any context
 # Ragged batches of up to _SERIAL_REQUESTS requests run their two parts one
 # after the other on one stream: the events of a fork and join cost the host
 # more than the overlap hides (us a layer, side stream -> in turn: one 512-token
@@ -172,6 +179,15 @@ def _carve(parts: list[torch.Tensor], device: torch.device) -> list[torch.Tensor
                             device=device).split([t.shape[0] for t in parts]))
 
 
+def _window(window_left: int, sink_tokens: int, dtype: torch.dtype) -> bool:
+    """Whether a run is windowed; refuses what no kernel serves."""
+    if window_left < -1 or sink_tokens < 0:
+        raise ValueError(f"window_left {window_left} must be -1 (no window) or more, sink_tokens {sink_tokens} 0 or more")
+    if window_left >= 0 and dtype == torch.float32:
+        raise ValueError("fp32 caches have no windowed attention")
+    return window_left >= 0
+
+
 def _as_device_int(t: torch.Tensor, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     if t.dtype != dtype:
         t = t.to(dtype)
@@ -224,8 +240,17 @@ def _append(kv_cache_layer: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page
 
 def _rope_set_kv_cache(wrapper, kv_cache_layer, q, k, v, pos_ids, rotary_dim, interleave, rope_scale, rope_theta,
                        k_scale, v_scale, keep_k, llama31) -> None:
-    from .rope import rope_append
+    from .rope import apply_llama31_rope_pos_ids_inplace, apply_rope_pos_ids_inplace, rope_append
 
+    if isinstance(kv_cache_layer, MXKVLayer):  # a block's scale needs its rotated values: two launches
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("a microscaled KV layer holds its own scales: pass no k_scale or v_scale")
+        k = k if keep_k else k.clone()
+        rotate = apply_llama31_rope_pos_ids_inplace if llama31 else apply_rope_pos_ids_inplace
+        rotate(q, k, pos_ids, rotary_dim=rotary_dim, interleave=interleave, rope_scale=rope_scale, rope_theta=rope_theta,
+               **(llama31 or {}))
+        wrapper.set_kv_cache(kv_cache_layer, k, v)
+        return
     page_idx, slot_ptr, idx_stride, n, n_dev = wrapper._append_target()
     rope_append(q, k, v, kv_cache_layer, pos_ids, page_idx, slot_ptr, idx_stride, n, n_dev,
                 rotary_dim=rotary_dim, interleave=interleave, rope_scale=rope_scale, rope_theta=rope_theta,
@@ -242,7 +267,8 @@ class _FusedRopeAppend:
                           llama31: dict | None = None) -> None:
         """``apply_rope_pos_ids_inplace(q, k, pos_ids, ...)`` then ``set_kv_cache(kv_cache_layer, k, v)``.
 
-        Same results bit for bit, in one kernel (``mi_rope_append``).  ``llama31``
+        Same results bit for bit, in one kernel (``mi_rope_append``; a microscaled
+        layer takes the two calls).  ``llama31``
         holds ``low_freq_factor``/``high_freq_factor``/``old_context_len`` for
         the Llama-3.1 frequencies.  q, k and v share one dtype (bf16 or fp16);
         k and v rows must be 16-byte aligned.
@@ -424,9 +450,15 @@ class PagedDecodeWrapper(_FusedRopeAppend, _PlanArrays):
         self._planned_on(_lib.stream_ptr(self.device), kv_indptr, kv_indices, last, self.kv_cache_locations)
 
     # --------------------------------------------------------------- run
-    def run(self, q: torch.Tensor, kv_cache_layer: torch.Tensor, k_scale: torch.Tensor | None = None,
-            v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-        """Paged decode attention (``flashinfer_utils.py:455-465``): q ``[n_req, Hq, D]`` -> o."""
+    def run(self, q: torch.Tensor, kv_cache_layer: torch.Tensor | MXKVLayer, k_scale: torch.Tensor | None = None,
+            v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None, window_left: int = -1,
+            sink_tokens: int = 0) -> torch.Tensor:
+        """Paged decode attention (``flashinfer_utils.py:455-465``): q ``[n_req, Hq, D]`` -> o.
+
+        With ``window_left >= 0`` a query sees its own key, the ``window_left`` keys
+        before it and the request's first ``sink_tokens`` (extension; -1: every key).
+        Pages that hold hidden keys only are not read.
+        """
         if self.dtype is None:
             raise RuntimeError("plan() must be called before run()")
         if q.dtype != self.dtype:
@@ -445,6 +477,18 @@ class PagedDecodeWrapper(_FusedRopeAppend, _PlanArrays):
         os_ = _q_strides(out, "out")
         batch = n
         stream = self._reading_stream()
+        if _window(window_left, sink_tokens, q.dtype):
+            _lib.check(
+                _lib.lib().mi_decode_run_window(
+                    q.data_ptr(), _lib.TORCH_TO_MI[q.dtype], qs[0], qs[1], desc, None, self._indptr.data_ptr(),
+                    self._indices.data_ptr(), self._last.data_ptr(), batch, self.num_qo_heads, 0,
+                    1.0 / math.sqrt(self.head_dim), min(window_left, _WINDOW_MAX), min(sink_tokens, _WINDOW_MAX),
+                    self._workspace.data_ptr(), self._workspace.numel() * self._workspace.element_size(),
+                    out.data_ptr(), os_[0], os_[1], stream,
+                ),
+                "mi_decode_run_window",
+            )
+            return out
         _lib.check(
             _lib.lib().mi_decode_run(
                 q.data_ptr(), _lib.TORCH_TO_MI[q.dtype], qs[0], qs[1], desc, None, self._indptr.data_ptr(),
@@ -457,7 +501,7 @@ class PagedDecodeWrapper(_FusedRopeAppend, _PlanArrays):
         )
         return out
 
-    def set_kv_cache(self, kv_cache_layer: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+    def set_kv_cache(self, kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.Tensor,
                      k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
         """Write one new token per request (``flashinfer_utils.py:467-484``)."""
         _append(kv_cache_layer, k, v, *self._append_target(), k_scale, v_scale)
@@ -626,9 +670,15 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
         else:
             self._run_short = self._run_tiles = True
 
-    def run(self, q: torch.Tensor, kv_cache_layer: torch.Tensor, k_scale: torch.Tensor | None = None,
-            v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-        """Ragged paged attention (``flashinfer_utils.py:258-269``): q ``[tokens, Hq, D]`` -> o."""
+    def run(self, q: torch.Tensor, kv_cache_layer: torch.Tensor | MXKVLayer, k_scale: torch.Tensor | None = None,
+            v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None, window_left: int = -1,
+            sink_tokens: int = 0) -> torch.Tensor:
+        """Ragged paged attention (``flashinfer_utils.py:258-269``): q ``[tokens, Hq, D]`` -> o.
+
+        With ``window_left >= 0`` the query at position i of its request sees no key
+        before i - ``window_left`` but the first ``sink_tokens`` (extension; -1: every
+        key); ``causal`` hides those behind i as before.
+        """
         if self.dtype is None:
             raise RuntimeError("plan() must be called before run()")
         if q.dtype != self.dtype:
@@ -654,6 +704,12 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
         # of both, the HBM-bound decode runs on a side stream, so that it overlaps
         # the compute-bound tiles.
         args[-1] = self._reading_stream()
+        if _window(window_left, sink_tokens, q.dtype):
+            parts = (1 if self._run_short else 0) | (2 if self._run_tiles else 0)
+            if parts:
+                args[14:14] = [min(window_left, _WINDOW_MAX), min(sink_tokens, _WINDOW_MAX), parts]
+                _lib.check(_lib.lib().mi_prefill_run_window(*args), "mi_prefill_run_window")
+            return out
         if self._run_tiles and self._run_short and self._serial:
             _lib.check(_lib.lib().mi_prefill_run(*args), "mi_prefill_run")
         elif self._run_tiles and self._run_short:
@@ -668,7 +724,7 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
             _lib.check(getattr(_lib.lib(), fn)(*args), fn)
         return out
 
-    def set_kv_cache(self, kv_cache_layer: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+    def set_kv_cache(self, kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.Tensor,
                      k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
         """Scatter the planned tokens' K/V into their pages (``flashinfer_utils.py:271-288``)."""
         _append(kv_cache_layer, k, v, *self._append_target(), k_scale, v_scale)
