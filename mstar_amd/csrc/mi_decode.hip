@@ -270,15 +270,24 @@ static int dispatch_d(const DecodeParams& dp, int head_dim, int grid, int batch,
 // Windows and sink counts are clamped here: beyond any context, and sums with a length stay in 32 bits.
 constexpr int32_t kWinMax = 1 << 30;
 
-// Places for items of each request of a windowed run: as many as give every CU
-// a workgroup, none shorter than kWinItemTiles, within the workspace's partials.
-static int win_splits(int batch, int nkv, int window_left, int sinks, int max_chunks) {
-  const int64_t tiles = ((int64_t)window_left + sinks) / 16 + 3;
-  int64_t n = device_cu_count() / ((int64_t)batch * nkv);
-  if (n > (tiles + kWinItemTiles - 1) / kWinItemTiles) n = (tiles + kWinItemTiles - 1) / kWinItemTiles;
+// Items of a windowed run: a request's share of the resident workgroups, none
+// shorter than kWinItemTiles, within the workspace's partials.  One request of 1028
+// keys at 4 kv heads: one item a head 13.1 us, 2 8.6, 3 7.3, 4 and more 6.5; 96 of
+// 4100 keys at 2 kv heads, 4 bits: one 58 us, 2 45 + 4 for the merge.  With more
+// (request, kv-head) pairs than workgroups no cut paid (256 requests of up to 8256 keys at 4
+// kv heads, one item 384 us, two to four 384-394 + 4); taking the longest first did
+// (455 -> 384 us), as uncut requests are as uneven as their lengths.
+constexpr int kWinItemTiles = 16;
+static void win_items(DecodeParams& dp, int heads, int slots, int max_chunks) {
+  const int tiles = win_tiles_max(dp);
+  int64_t n = slots / ((int64_t)dp.batch * heads);
   if (n > 16) n = 16;
-  if (n > max_chunks / batch) n = max_chunks / batch;
-  return n < 1 ? 1 : (int)n;
+  if (n > max_chunks / dp.batch) n = max_chunks / dp.batch;
+  if (n < 1) n = 1;
+  dp.item_tiles = (int)((tiles + n - 1) / n);
+  if (dp.item_tiles < kWinItemTiles) dp.item_tiles = kWinItemTiles;
+  dp.splits = (tiles + dp.item_tiles - 1) / dp.item_tiles;
+  dp.sorted = dp.batch <= kSortedMax && (int64_t)dp.batch * heads * dp.splits > slots;
 }
 
 int decode_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_token, int64_t q_stride_head,
@@ -313,7 +322,7 @@ int decode_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_token, int6
   // the paired kernels: 16-bit caches whose pairs' two 128-element rows are
   // adjacent (NHD pools); fp8, fp32 and other layouts run the per-head
   // kernels on the same plan
-  const bool pair_kernel = pair && !fp8 && !mx && !win && q_dtype != MI_F32 && kv->head_stride == D;
+  const bool pair_kernel = pair && !fp8 && !mx && q_dtype != MI_F32 && kv->head_stride == D;
 
   DecodeParams dp{};
   dp.q = q;
@@ -350,14 +359,20 @@ int decode_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_token, int6
     dp.window_left = window_left < kWinMax ? window_left : kWinMax;
     dp.sinks = sinks < kWinMax ? sinks : kWinMax;
     dp.batch = batch;
-    dp.splits = win_splits(batch, nkv, dp.window_left, dp.sinks, L.max_chunks);
+    const int heads = pair_kernel ? nkv / 2 : nkv;
     const int kvt = kv_format(kv->dtype);
+    win_items(dp, heads, device_cu_count() * decode_waves(kvt, pair_kernel ? 256 : D, true), L.max_chunks);
+    if (pair_kernel) {
+      dp.num_kv_heads = heads;
+      dp.head_stride = 2 * kv->head_stride;
+    }
     st = MI_OK;
     if (phases & kPhaseAttend) {
-      const int wgrid = (int)(((int64_t)batch * dp.splits + 7) / 8 * 8 * nkv);
-      st = decode_win_launch(dp, q_dtype, kvt, D, wgrid, stream);
+      const int wgrid = (int)(((int64_t)batch * dp.splits + 7) / 8 * 8 * heads);
+      st = decode_win_launch(dp, q_dtype, kvt, D, pair_kernel, wgrid, stream);
     }
-    if (st == MI_OK && (phases & kPhaseMerge) && dp.splits > 1) st = decode_win_merge_launch(dp, q_dtype, kvt, D, stream);
+    if (st == MI_OK && (phases & kPhaseMerge) && dp.splits > 1)
+      st = decode_win_merge_launch(dp, q_dtype, kvt, D, pair_kernel, batch, stream);
     if (st != MI_OK) return st;
     MI_CHECK_LAUNCH();
     return MI_OK;

@@ -27,9 +27,27 @@ struct TileScales {
   uint32_t k, v;
 };
 
-template <int N>
+// CACHED: loads that stay in the L2.  A microscaled row is 32 to 128 bytes, less than
+// the 128-byte line it lies in or the run of a token's heads: the neighbour's
+// workgroup reads the rest of the line soon (streaming loads had it fetched again:
+// B=256, 1k-32k contexts, 4 kv heads x 64-byte rows 359 -> 294 us; 64 requests at 8
+// kv heads x 128-byte rows 33 -> 31 us).
+template <bool CACHED, int N>
 MI_DEVICE void load_words(uint32_t (&dst)[N], const uint8_t* src) {
-  if constexpr (N == 1) {
+  if constexpr (CACHED && N == 1) {
+    dst[0] = *(const uint32_t*)src;
+  } else if constexpr (CACHED && N == 2) {
+    const uint2 t = *(const uint2*)src;
+    dst[0] = t.x;
+    dst[1] = t.y;
+  } else if constexpr (CACHED) {
+    static_assert(N == 4, "a microscaled row slice is at most 16 bytes");
+    const uint4 t = *(const uint4*)src;
+    dst[0] = t.x;
+    dst[1] = t.y;
+    dst[2] = t.z;
+    dst[3] = t.w;
+  } else if constexpr (N == 1) {
     dst[0] = nt_load4(src);
   } else if constexpr (N == 2) {
     const uint2 t = nt_load8(src);
@@ -47,17 +65,74 @@ MI_DEVICE void load_words(uint32_t (&dst)[N], const uint8_t* src) {
   }
 }
 
+// The request at place `rank` of a windowed batch when its requests are taken by
+// classes of tiles, an eighth of a full window each, most first: workgroups start
+// in order, so the last ones to start are short.  The workgroup's threads class
+// 256 requests at a time and count by ballots, from the index arrays alone.
+__device__ __forceinline__ int win_item(const DecodeParams& p, int rank) {
+  constexpr int kClasses = 8;
+  __shared__ int s_count[4][kClasses], s_b;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float per_tile = (float)kClasses / (float)win_tiles_max(p);
+  auto class_of = [&](int r) {
+    if (r >= p.batch) return -1;
+    const int np = p.kv_indptr[r + 1] - p.kv_indptr[r];
+    const int qo_len = p.qo_indptr ? p.qo_indptr[r + 1] - p.qo_indptr[r] : 1;
+    if (qo_len <= 0 || qo_len * p.group > p.short_rows) return kClasses - 1;  // nothing to do here
+    const int kv_len = np > 0 ? (np - 1) * p.page_size + p.last_page_len[r] : 0;
+    return kClasses - 1 - min(kClasses - 1, (int)((float)win_tiles(kv_len, qo_len, p).total * per_tile));
+  };
+  int mine[kSortedMax / 256], total[kClasses] = {};  // this wavefront's counts, all chunks of 256
+  for (int c = 0; c * 256 < p.batch; ++c) {
+    mine[c] = class_of(c * 256 + tid);
+#pragma unroll
+    for (int k = 0; k < kClasses; ++k) total[k] += __popcll(__builtin_amdgcn_ballot_w64(mine[c] == k));
+  }
+  if (lane == 0)
+#pragma unroll
+    for (int k = 0; k < kClasses; ++k) s_count[wave][k] = total[k];
+  __syncthreads();
+  // this wavefront's first place in each class: classes before it, wavefronts before it
+  int at[kClasses], sum = 0;
+#pragma unroll
+  for (int k = 0; k < kClasses; ++k)
+    for (int w = 0; w < 4; ++w) {
+      if (w == wave) at[k] = sum;
+      sum += s_count[w][k];
+    }
+  for (int c = 0; c * 256 < p.batch; ++c) {
+    int place = -1;
+#pragma unroll
+    for (int k = 0; k < kClasses; ++k) {
+      const uint64_t in = __builtin_amdgcn_ballot_w64(mine[c] == k);
+      if (mine[c] == k) place = at[k] + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+      at[k] += __popcll(in);
+    }
+    if (place == rank) s_b = c * 256 + tid;
+  }
+  __syncthreads();
+  return uniform(s_b);
+}
+
+// Wavefronts per SIMD the registers are held to.  With two, microscaled kernels
+// keep their accumulators out of the AGPRs, so that rescaling them costs no moves
+// (4 bits, head_dim 256, 96 windows of 4k: 62.5 -> 60.2 us, and a second workgroup
+// a CU); at 8 bits and head_dim 256 that spills.
+constexpr int decode_waves(int kvt, int d, bool win) {
+  return kvt == kKvMx4 || (kvt == kKvMx8 && d <= 128) || (win && d <= 128) ? 2 : 1;
+}
+
 // PAIR (D = 256): two adjacent head_dim 128 kv-heads read as one 256-element
 // row; p.num_kv_heads counts the pairs, p.group is the real group size, query
 // row col belongs to kv-head 2h + (col >= group) (see pair_heads).
 // WIN: the sliding window with its sinks (DecodeParams::window_left, sinks).  A
 // request's tiles are then those of its sinks and of its window only
-// (win_tiles), in one sequence that the request's items share evenly; the item
-// of a workgroup follows from its place, so a windowed run needs no plan of
-// its own and a model may mix windowed and full layers under one plan.
+// (win_tiles), in one sequence that its items share evenly.  Which item a
+// workgroup takes follows from its place and the lengths (win_item), so a windowed
+// run needs no plan of its own and a model may mix windowed and full layers.
 template <typename MT, int KVT, int D, bool PAIR = false, bool WIN = false>
-__global__ __launch_bounds__(256) void decode_kernel(DecodeParams p) {
-  static_assert(!PAIR || (D == 256 && !WIN), "paired kv-heads form 256-element rows");
+__global__ __launch_bounds__(256, decode_waves(KVT, D, WIN)) void decode_kernel(DecodeParams p) {
+  static_assert(!PAIR || D == 256, "paired kv-heads form 256-element rows");
   constexpr bool FP8 = KVT == kKvFp8, MX = KVT == kKvMx8 || KVT == kKvMx4;
   constexpr int KS = D / 32;  // MFMA k-steps over head_dim for S
   constexpr int VW = D / 16;  // V elements per lane per row == output d-tiles
@@ -84,11 +159,12 @@ __global__ __launch_bounds__(256) void decode_kernel(DecodeParams p) {
   const int gr = (int)blockIdx.x - gi * gsz;
   const int h = uniform(gr >> 3);
   const int item = uniform(gi * 8 + (gr & 7));
-  int b, kidx, pg0, pg1, nitems_b;
+  int b, kidx, pg0 = 0, pg1, nitems_b;
   if constexpr (WIN) {
     if (item >= p.batch * p.splits) return;
-    b = item / p.splits;
-    kidx = item - b * p.splits;
+    kidx = item / p.batch;
+    b = item - kidx * p.batch;
+    if (p.sorted) b = win_item(p, b);
   } else {
     if (item >= p.hdr[kHdrChunks]) return;  // uniform across the workgroup
     const int4 wk = p.work[item];
@@ -111,7 +187,7 @@ __global__ __launch_bounds__(256) void decode_kernel(DecodeParams p) {
   WinTiles span;
   if constexpr (WIN) {
     if (qo_len <= 0 || qo_len * G > p.short_rows) return;  // no rows, or the prefill kernel's
-    span = win_tiles(kv_len, qo_len, p.window_left, p.sinks, p.splits);
+    span = win_tiles(kv_len, qo_len, p);
     nitems_b = span.items;
     if (kidx >= nitems_b) return;
     pg1 = np;
@@ -187,14 +263,14 @@ __global__ __launch_bounds__(256) void decode_kernel(DecodeParams p) {
     const uint8_t* vb = kb + kvhalf;
     if constexpr (KVT == kKvMx4 && D == 64) {  // four elements of a row: two bytes
 #pragma unroll
-      for (int r = 0; r < 4; ++r) t.k[r][0] = __builtin_nontemporal_load((const uint16_t*)(kb + r * vrow));
+      for (int r = 0; r < 4; ++r) t.k[r][0] = *(const uint16_t*)(kb + r * vrow);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) t.v[r][0] = __builtin_nontemporal_load((const uint16_t*)(vb + r * vrow));
+      for (int r = 0; r < 4; ++r) t.v[r][0] = *(const uint16_t*)(vb + r * vrow);
     } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) load_words(t.k[r], kb + r * vrow);
+      for (int r = 0; r < 4; ++r) load_words<MX>(t.k[r], kb + r * vrow);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) load_words(t.v[r], vb + r * vrow);
+      for (int r = 0; r < 4; ++r) load_words<MX>(t.v[r], vb + r * vrow);
     }
   };
   // The scale words of a tile: the four rows' bytes are adjacent slots of one
@@ -284,7 +360,12 @@ __global__ __launch_bounds__(256) void decode_kernel(DecodeParams p) {
     }
     // ---- online softmax (row = col; the 4 lane groups share a row)
     const float mt = rows4_max(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])));
-    const float m_new = fmaxf(m_run, mt);
+    // Windowed and microscaled kernels raise the running max only past 2^8, as the
+    // prefill kernels do: probabilities stay below 2^8, harmless in fp32 sums and
+    // 16-bit P, and the rescale, which a wavefront of 16 rows ran on about 40 % of
+    // its first 64 tiles, is rare (4 bits: 368 -> 358 us, 67.3 -> 62.5).
+    constexpr bool LAZY = WIN || MX;
+    const float m_new = LAZY ? (mt > m_run + 8.f ? mt : m_run) : fmaxf(m_run, mt);
     const float m_use = m_new == kNegInf ? 0.f : m_new;
     const float alpha = fast_exp2(m_run - m_use);
     float pr[4];

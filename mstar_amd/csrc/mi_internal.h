@@ -180,35 +180,38 @@ struct DecodeParams {
   int32_t num_kv_heads, group, page_size, causal;
   float scale_log2;
   int32_t short_rows = kShortRowsMax;  // ragged batches: requests with qo_len * group above this are not ours
-  // Windowed runs: keys below a query's position - window_left are hidden but
-  // for the first `sinks` of the request; each of the `batch` requests has
-  // `splits` places for items (window_left < 0: no window).
-  int32_t window_left = -1, sinks = 0, splits = 0, batch = 0;
+  // Windowed runs: keys below a query's position - window_left are hidden but for
+  // the first `sinks` of the request; items of about item_tiles tiles, `splits`
+  // places for each of the batch's requests; sorted: longest first.
+  int32_t window_left = -1, sinks = 0, item_tiles = 0, splits = 0, batch = 0, sorted = 0;
 };
 
 // The 16-token tiles of a windowed request: those that hold sinks, then those
 // from `first` on to the end of its keys, one sequence of `total` tiles that
-// `items` items share evenly.  Items are no shorter than kWinItemTiles.
-constexpr int kWinItemTiles = 16;
+// `items` items share evenly.
 struct WinTiles {
   int sinks, first, total, items;
 };
-__device__ __forceinline__ WinTiles win_tiles(int kv_len, int qo_len, int window_left, int sinks, int splits) {
+__device__ __forceinline__ WinTiles win_tiles(int kv_len, int qo_len, const DecodeParams& p) {
   WinTiles w;
-  w.first = max(0, kv_len - qo_len - window_left) >> 4;
-  w.sinks = min((sinks + 15) >> 4, w.first);
+  w.first = max(0, kv_len - qo_len - p.window_left) >> 4;
+  w.sinks = min((p.sinks + 15) >> 4, w.first);
   w.total = w.sinks + ((kv_len + 15) >> 4) - w.first;
-  w.items = max(1, min(splits, (w.total + kWinItemTiles - 1) / kWinItemTiles));
+  w.items = max(1, min(p.splits, (w.total + p.item_tiles - 1) / p.item_tiles));
   return w;
 }
+// The most tiles a request can have (short queries).
+__host__ __device__ inline int win_tiles_max(const DecodeParams& p) { return (p.window_left + 15) / 16 + (p.sinks + 15) / 16 + 2; }
+constexpr int kSortedMax = 1024;  // requests that a windowed run sorts by length
 
 // fp32 KV (q, cache and output in fp32): the attend phase of a split-KV plan
 // (mi_f32.hip), and the merge with fp32 output (mi_decode.hip).
 int f32_attend_launch(const DecodeParams& dp, int head_dim, int grid, hipStream_t stream);
 // Windowed and microscaled runs (mi_decode_win.hip, mi_decode_mx.hip): the attend
 // kernel, and the merge of a windowed run's items.
-int decode_win_launch(const DecodeParams& dp, int q_dtype, int kvt, int head_dim, int grid, hipStream_t stream);
-int decode_win_merge_launch(const DecodeParams& dp, int q_dtype, int kvt, int head_dim, hipStream_t stream);
+int decode_win_launch(const DecodeParams& dp, int q_dtype, int kvt, int head_dim, bool pair, int grid, hipStream_t stream);
+int decode_win_merge_launch(const DecodeParams& dp, int q_dtype, int kvt, int head_dim, bool pair, int batch,
+                            hipStream_t stream);
 int decode_mx_launch(const DecodeParams& dp, int q_dtype, int kvt, int head_dim, int grid, hipStream_t stream);
 // mi_kv_append into a microscaled layer (mi_mx.hip); arguments checked but for the layer's scales and alignment.
 int mx_append_launch(const mi_paged_kv* kv, const void* k, const void* v, int32_t src_dtype, int64_t k_stride_token,

@@ -30,8 +30,7 @@ MI_DEVICE void merge_body(const DecodeParams& p, int32_t batch, int pair) {
   if constexpr (WIN) {
     c0 = b * p.splits;
     const int np = p.kv_indptr[b + 1] - p.kv_indptr[b];
-    const int kv_len = np > 0 ? (np - 1) * p.page_size + p.last_page_len[b] : 0;
-    nb = win_tiles(kv_len, qo_len, p.window_left, p.sinks, p.splits).items;
+    nb = win_tiles(np > 0 ? (np - 1) * p.page_size + p.last_page_len[b] : 0, qo_len, p).items;
   } else {
     c0 = p.chunk_indptr[b];
     nb = p.chunk_indptr[b + 1] - c0;
