@@ -58,26 +58,50 @@ struct PrefillParams {
 
 // The 32-key steps of a tile of a windowed run: the steps that hold sinks,
 // then those from `first` on, `total` in all; step t starts at key(t).  lo:
-// where the window of the tile's first row begins, hi: of its last row.
+// where the window of the tile's first row begins.  Rows differ in what they see
+// only in the steps before `whole` (sinks, and windows that begin there) and, as
+// without a window, in the last ones; the steps between need no check.
 struct PfWin {
-  int lo, hi, sinks, first, total;
+  int lo, sinks, first, total, whole;
   MI_DEVICE int key(int t) const { return kPfKeys * (t < sinks ? t : t - sinks + first); }
+  // Position in the sequence of the step that holds a key from lo on.
+  MI_DEVICE int step_of(int key) const { return max(0, key / kPfKeys - first + sinks); }
   // The keys whose page a 16-key group at `key` reads: its own, or, where the
   // window hides the whole group, the window's first (their pages may be gone).
   MI_DEVICE int read_key(int key, int sink_tokens) const { return key + 15 < lo && key >= sink_tokens ? lo & ~15 : key; }
-  // some row of the tile has its window begin behind the step's first key, and not all of it are sinks
-  MI_DEVICE bool partial(int kb, int sink_tokens) const { return kb < hi && kb + kPfKeys > sink_tokens; }
 };
 MI_DEVICE PfWin pf_win(const PrefillParams& p, int kv_len, int qo_len, int min_tok, int max_tok, int kv_end) {
   PfWin w;
   w.lo = kv_len - qo_len + min_tok - p.window_left;
-  w.hi = w.lo + max_tok - min_tok;
   // a window that begins behind the keys the tile may see (a tail of rows without keys) is empty
   const int steps = kv_end > 0 ? (kv_end + kPfKeys - 1) / kPfKeys : 0;
   w.first = min(max(0, w.lo) / kPfKeys, steps);
   w.sinks = min((p.sinks + kPfKeys - 1) / kPfKeys, w.first);
   w.total = w.sinks + steps - w.first;
+  const int hi = w.lo + max_tok - min_tok;  // where the last row's window begins
+  w.whole = hi > 0 ? w.sinks + (hi + kPfKeys - 1) / kPfKeys - w.first : 0;
   return w;
+}
+// A windowed row's view of a step: hides the scores of one lane's keys kb + 16 js +
+// 4 grp + r.  The row sees [low, low + span], and the sinks up to there.
+MI_DEVICE void pf_win_mask(f32x4 (&s)[2], int kb, int grp, int low, uint32_t span, int sink_tokens) {
+  constexpr float kNegInf = -__builtin_inff();
+  const int rel = kb + 4 * grp - low;
+  if (kb >= sink_tokens) {  // uniform
+#pragma unroll
+    for (int js = 0; js < 2; ++js)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if ((uint32_t)(rel + 16 * js + r) > span) s[js][r] = kNegInf;
+  } else {
+#pragma unroll
+    for (int js = 0; js < 2; ++js)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = rel + 16 * js + r;
+        if ((uint32_t)at > span && (at > (int)span || at + low >= sink_tokens)) s[js][r] = kNegInf;
+      }
+  }
 }
 // Pieces of a tile of a windowed run: the plan cut it for all its keys, so
 // where the window leaves few steps a piece, fewer pieces share them (the
@@ -264,6 +288,7 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
   // ---- this lane's query rows (one per 16-row group)
   uint4 qf[RG][KS];
   int lim[RG], low[RG];  // the row's last key; WIN: the first of its window
+  uint32_t span[RG];     // WIN: keys from there to the last
 #pragma unroll
   for (int rg = 0; rg < RG; ++rg) {
     const int n = row0 + WROWS * wave + 16 * rg + col;
@@ -271,7 +296,10 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
     const bool valid = n < rows_total;
     const int l = p.causal ? (kv_len - qo_len + tok) : (kv_len - 1);
     lim[rg] = min(l, kv_len - 1);
-    if constexpr (WIN) low[rg] = kv_len - qo_len + tok - p.window_left;
+    if constexpr (WIN) {
+      low[rg] = kv_len - qo_len + tok - p.window_left;
+      span[rg] = p.causal ? p.window_left : kv_len - 1 - low[rg];
+    }
     const uint16_t* qrow = (const uint16_t*)p.q + (int64_t)(qo_start + tok) * p.q_stride_tok +
                            (int64_t)(h * G + g) * p.q_stride_head;
 #pragma unroll
@@ -295,6 +323,8 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
     s_slot = un.n > 1 ? un.slot : -1;
   }
   auto key_of = [&](int t) { return WIN ? win.key(t) : t * KEYS; };
+  // WIN: the step from which V rows may lie past kv_len
+  const int t_tail = WIN ? win.step_of(kv_len) : 0;
   // key steps of this unit: all of the tile's, or its piece's share
   const int kt0 = un.n > 1 ? un.k * n_kt / un.n : 0, kt1 = un.n > 1 ? (un.k + 1) * n_kt / un.n : n_kt;
   if (un.n == 0) continue;  // uniform; no wait for the unit's entry ahead of the loads above
@@ -416,8 +446,7 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
   // Tiles before the request's last one hold no row past kv_len (kv_end <=
   // kv_len): their stores skip the tail test, chosen by a wave-uniform branch.
   auto store_tile = [&](int t, const uint4 (&r)[NL], const uint8_t (&rs)[NL], int stage) {
-    const int kb = key_of(t);
-    if (kb + KEYS > kv_len || (WIN && kb < win.lo && kb + KEYS > p.sinks))
+    if (WIN ? t < win.whole || t >= t_tail : t * KEYS + KEYS > kv_len)
       store_tile_impl(t, r, rs, stage, std::true_type{});
     else
       store_tile_impl(t, r, rs, stage, std::false_type{});
@@ -445,7 +474,7 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
   }
 
   // first tile that reaches past some row's limit: (t+1)*KEYS > mask_from
-  const int t_mask = mask_from > 0 ? mask_from / KEYS : 0;
+  const int t_mask = WIN ? win.step_of(mask_from) : mask_from > 0 ? mask_from / KEYS : 0;
 
   // One 32-key tile: S^T = K.Q^T as two 16-key sub-tiles (16x16x32 MFMAs,
   // K fragments from LDS shared by both row groups), online softmax, then
@@ -486,16 +515,20 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
   // and raises the running max when needed (a rare branch); sm_exp forms
   // the probabilities and their row sums.
   auto sm_max = [&](int t, f32x4 (&s)[RG][2]) {
-    const int kb = key_of(t);
-    if (WIN ? kb + KEYS > mask_from || win.partial(kb, p.sinks) : t >= t_mask) {  // wave-uniform: only the tiles that reach past some row's limit
+    if (t >= t_mask || (WIN && t < win.whole)) {  // wave-uniform: only the tiles that reach past some row's limit
+      const int kb = key_of(t);
 #pragma unroll
-      for (int rg = 0; rg < RG; ++rg)
+      for (int rg = 0; rg < RG; ++rg) {
+        if constexpr (WIN) {
+          pf_win_mask(s[rg], kb, grp, low[rg], span[rg], p.sinks);
+        } else {
 #pragma unroll
-        for (int js = 0; js < 2; ++js)
+          for (int js = 0; js < 2; ++js)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (const int key = kb + 16 * js + 4 * grp + r; key > lim[rg] || (WIN && key < low[rg] && key >= p.sinks))
-              s[rg][js][r] = kNegInf;
+            for (int r = 0; r < 4; ++r)
+              if (kb + 16 * js + 4 * grp + r > lim[rg]) s[rg][js][r] = kNegInf;
+        }
+      }
     }
     // A row's max exceeds the threshold iff one of its four lanes' maxima
     // does, so the cross-lane row max is only needed on the rare branch.

@@ -98,13 +98,17 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
       // R: the S-role's Q fragments (R[rg][s] for s < KS), the O-role's accumulators
       f32x4 R[RGP][VW];
       int lim[RGP], low[RGP];
+      uint32_t span[RGP];
 #pragma unroll
       for (int rg = 0; rg < RGP; ++rg) {
         const int n = row0 + PROWS * pr + 16 * rg + col;
         const int tok = n / G, g = n - tok * G;
         const int l = p.causal ? (kv_len - qo_len + tok) : (kv_len - 1);
         lim[rg] = min(l, kv_len - 1);
-        if constexpr (WIN) low[rg] = kv_len - qo_len + tok - p.window_left;
+        if constexpr (WIN) {
+          low[rg] = kv_len - qo_len + tok - p.window_left;
+          span[rg] = p.causal ? p.window_left : kv_len - 1 - low[rg];
+        }
         if constexpr (S) {
           const bool valid = n < rows_total;
           const uint16_t* qrow = (const uint16_t*)p.q + (int64_t)(qo_start + tok) * p.q_stride_tok +
@@ -133,6 +137,7 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
         s_slot = un.n > 1 ? un.slot : -1;
       }
       auto key_of = [&](int t) { return WIN ? win.key(t) : t * KEYS; };
+      const int t_tail = WIN ? win.step_of(kv_len) : 0;
       // key steps of this unit: all of the tile's, or its piece's share
       const int kt0 = un.n > 1 ? un.k * n_kt / un.n : 0, kt1 = un.n > 1 ? (un.k + 1) * n_kt / un.n : n_kt;
       if (un.n == 0) continue;  // uniform; no wait for the unit's entry ahead of the loads above
@@ -229,10 +234,10 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
           }
         }
       };
-      // the step holds V rows that no row of the tile may see
-      auto hides = [&](int kb) { return kb + KEYS > kv_len || (WIN && kb < win.lo && kb + KEYS > p.sinks); };
+      // the step may hold V rows that no row of the tile sees
+      auto hides = [&](int t) { return WIN ? t < win.whole || t >= t_tail : t * KEYS + KEYS > kv_len; };
       auto store_tile = [&](int t, const uint4 (&r)[NL], const uint8_t (&rs)[NL], int stage) {
-        if (hides(key_of(t)))
+        if (hides(t))
           store_tile_impl(t, r, rs, stage, std::true_type{});
         else
           store_tile_impl(t, r, rs, stage, std::false_type{});
@@ -280,8 +285,8 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
           asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
         else
           asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        const int kb = key_of(t);
-        if (hides(kb)) {
+        if (hides(t)) {
+          const int kb = key_of(t);
 #pragma unroll
           for (int i = 2; i < 4; ++i) {
             const int rp = 8 * (i & 1) + wave, key = kb + 2 * rp + (lane >> 5);
@@ -303,7 +308,7 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
         thr[rg] = kNegInf;
         moff[rg] = 0.f;
       }
-      const int t_mask = mask_from > 0 ? mask_from / KEYS : 0;
+      const int t_mask = WIN ? win.step_of(mask_from) : mask_from > 0 ? mask_from / KEYS : 0;
 
       // swizzled K fragment offsets (direct-load rings): 32-dim slice s of key
       // row 16*js + col sits at kbo[s & 3] + 256*(s >> 2) + 8192*js
@@ -345,16 +350,20 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
               for (int js = 0; js < 2; ++js)
                 s[rg][js] = MT::mma_16x16x32(ka[c & 1][k][js], bitcast<uint4>(R[rg][KC * c + k]), s[rg][js]);
         }
-        const int kb = key_of(t);
-        if (WIN ? kb + KEYS > mask_from || win.partial(kb, p.sinks) : t >= t_mask) {
+        if (t >= t_mask || (WIN && t < win.whole)) {
+          const int kb = key_of(t);
 #pragma unroll
-          for (int rg = 0; rg < RGP; ++rg)
+          for (int rg = 0; rg < RGP; ++rg) {
+            if constexpr (WIN) {
+              pf_win_mask(s[rg], kb, grp, low[rg], span[rg], p.sinks);
+            } else {
 #pragma unroll
-            for (int js = 0; js < 2; ++js)
+              for (int js = 0; js < 2; ++js)
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (const int key = kb + 16 * js + 4 * grp + r; key > lim[rg] || (WIN && key < low[rg] && key >= p.sinks))
-                  s[rg][js][r] = kNegInf;
+                for (int r = 0; r < 4; ++r)
+                  if (kb + 16 * js + 4 * grp + r > lim[rg]) s[rg][js][r] = kNegInf;
+            }
+          }
         }
         float ml[RGP], alpha[RGP];
 #pragma unroll
