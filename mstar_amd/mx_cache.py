@@ -41,7 +41,7 @@ class MXKVLayer:
     of NaN.  The tensors are the caller's; the layer describes them as they are now.
     """
 
-    __slots__ = ("codes", "scales", "bits", "head_dim", "desc")
+    __slots__ = ("codes", "scales", "bits", "head_dim", "desc", "device")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dim() != 5 or codes.shape[1] != 2 or scales.dim() != 5:
@@ -63,7 +63,7 @@ class MXKVLayer:
             raise ValueError("codes: rows must be contiguous and 16-byte aligned")
         if not scales.is_contiguous() or scales.data_ptr() % 4 or page_size % 4:
             raise ValueError("scales must be contiguous and 4-byte aligned")
-        self.codes, self.scales = codes, scales
+        self.codes, self.scales, self.device = codes, scales, codes.device
         d = self.desc = _lib.MiPagedKV()
         d.data = codes.data_ptr()
         d.dtype = _lib.MI_MXFP8 if self.bits == 8 else _lib.MI_MXFP4
@@ -71,10 +71,6 @@ class MXKVLayer:
         d.page_stride, d.kv_stride, d.token_stride, d.head_stride = codes.stride()[:4]
         d.k_scale = scales.data_ptr()
         d.v_scale = scales.data_ptr() + heads * scales.shape[3] * page_size
-
-    @property
-    def device(self) -> torch.device:
-        return self.codes.device
 
     @property
     def shape(self) -> torch.Size:
@@ -120,6 +116,13 @@ class MXKVCache:
         return self.codes.is_cuda
 
 
+def _index(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """A contiguous int32 vector on ``dev``."""
+    if t.dim() != 1:
+        raise ValueError("index tensors must have one dimension")
+    return t if t.dtype is torch.int32 and t.device == dev and t.is_contiguous() else t.to(dev, torch.int32).contiguous()
+
+
 def read_kv_cache(kv_cache_layer: torch.Tensor | MXKVLayer, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
                   last_page_len: torch.Tensor, total_tokens: int, dtype: torch.dtype = torch.bfloat16,
                   k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
@@ -138,24 +141,24 @@ def read_kv_cache(kv_cache_layer: torch.Tensor | MXKVLayer, kv_indptr: torch.Ten
     dev = kv_cache_layer.device
     if dev.type != "cuda":
         raise ValueError("kv_cache_layer must be on a GPU")
-    if dtype not in _OUT:
+    code = _OUT.get(dtype)
+    if code is None:
         raise ValueError(f"dtype {dtype} is not bf16, fp16 or fp32")
-    batch = kv_indptr.shape[0] - 1
-    if kv_indptr.dim() != 1 or kv_indices.dim() != 1 or batch < 0 or last_page_len.shape != (batch,):
+    indptr, indices, last = _index(kv_indptr, dev), _index(kv_indices, dev), _index(last_page_len, dev)
+    batch = indptr.shape[0] - 1
+    if batch < 0 or last.shape[0] != batch:
         raise ValueError("index tensors disagree on the number of requests")
     if total_tokens < 0:
         raise ValueError(f"total_tokens {total_tokens} is negative")
     shape = (total_tokens, desc.num_kv_heads, desc.head_dim)
     if out is None:
-        k, v = (torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
+        k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
     else:
         k, v = out
         for t in (k, v):
-            if tuple(t.shape) != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous():
+            if t.shape != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous():
                 raise ValueError(f"out must be contiguous {shape} tensors of {dtype} on {dev}")
-    indptr, indices, last = (t.to(device=dev, dtype=torch.int32).contiguous()
-                             for t in (kv_indptr, kv_indices, last_page_len))
     _lib.check(_lib.lib().mi_kv_read(desc, indptr.data_ptr(), indices.data_ptr(), last.data_ptr(), batch,
-                                     indices.shape[0], k.data_ptr(), v.data_ptr(), _OUT[dtype], total_tokens,
+                                     indices.shape[0], k.data_ptr(), v.data_ptr(), code, total_tokens,
                                      _lib.stream_ptr(dev)), "mi_kv_read")
     return k, v

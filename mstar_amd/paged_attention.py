@@ -188,12 +188,26 @@ def _window(window_left: int, sink_tokens: int, dtype: torch.dtype) -> bool:
     return window_left >= 0
 
 
+def _check_out(out: torch.Tensor, n: int, heads: int, dim: int, q: torch.Tensor) -> None:
+    if out.shape[0] < n or out.shape[1:] != (heads, dim) or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError(f"out must hold {n} rows of {(heads, dim)} in {q.dtype} on {q.device}, got {tuple(out.shape)}, {out.dtype}")
+
+
 def _as_device_int(t: torch.Tensor, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     if t.dtype != dtype:
         t = t.to(dtype)
     if t.device != device:
         t = t.to(device, non_blocking=True)
     return t.contiguous()
+
+
+def _rows(q: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """(q, address, token stride, head stride), q copied where its rows are not 16-byte aligned."""
+    (st, sh, sd), at = q.stride(), q.data_ptr()
+    if sd != 1 or st % 8 or sh % 8 or at % 16:
+        q = q.contiguous()
+        (st, sh), at = _q_strides(q, "q"), q.data_ptr()
+    return q, at, st, sh
 
 
 def _q_strides(q: torch.Tensor, name: str) -> tuple[int, int]:
@@ -204,34 +218,38 @@ def _q_strides(q: torch.Tensor, name: str) -> tuple[int, int]:
     return q.stride(0), q.stride(1)
 
 
-def _kv_src(k: torch.Tensor, name: str) -> torch.Tensor:
+def _kv_src(k: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, int]:
+    """(k, address, token stride, head stride) of k or v in a layout the append reads."""
     if k.dim() != 3:
         raise ValueError(f"{name} must be [tokens, num_kv_heads, head_dim]")
-    if k.stride(2) != 1 or k.stride(0) % 8 or k.stride(1) % 8 or k.data_ptr() % (8 * k.element_size()):
+    (st, sh, sd), at = k.stride(), k.data_ptr()
+    if sd != 1 or st % 8 or sh % 8 or at % (8 * k.element_size()):
         k = k.contiguous()
-    return k
+        (st, sh, _), at = k.stride(), k.data_ptr()
+    return k, at, st, sh
 
 
-def _append(kv_cache_layer: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_idx: torch.Tensor,
+def _append(kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.Tensor, page_idx: torch.Tensor,
             slot_idx_ptr: int, idx_stride: int, n: int, n_dev_ptr: int | None,
             k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> None:
     if n == 0:
         return
     desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
-    if k.shape[1:] != (desc.num_kv_heads, desc.head_dim) or v.shape[1:] != k.shape[1:]:
-        raise ValueError(f"k/v shape {tuple(k.shape)} does not match the cache heads/head_dim")
-    if k.shape[0] < n or v.shape[0] < n:
-        raise ValueError(f"k/v hold {k.shape[0]} tokens, {n} planned")
+    shape = k.shape
+    if shape[1:] != (desc.num_kv_heads, desc.head_dim) or v.shape[1:] != shape[1:]:
+        raise ValueError(f"k/v shape {tuple(shape)} does not match the cache heads/head_dim")
+    if shape[0] < n or v.shape[0] < n:
+        raise ValueError(f"k/v hold {shape[0]} tokens, {n} planned")
     src_dt = _lib.TORCH_TO_MI.get(k.dtype)
     if src_dt is None or src_dt == _lib.MI_FP8_E4M3:
         raise ValueError(f"unsupported k/v dtype {k.dtype}")
     if v.dtype != k.dtype:
         v = v.to(k.dtype)
-    k = _kv_src(k, "k")
-    v = _kv_src(v, "v")
+    k, k_at, k_st, k_sh = _kv_src(k, "k")
+    v, v_at, v_st, v_sh = _kv_src(v, "v")
     _lib.check(
         _lib.lib().mi_kv_append(
-            desc, k.data_ptr(), v.data_ptr(), src_dt, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            desc, k_at, v_at, src_dt, k_st, k_sh, v_st, v_sh,
             page_idx.data_ptr(), slot_idx_ptr, idx_stride, n, n_dev_ptr, _lib.stream_ptr(kv_cache_layer.device),
         ),
         "mi_kv_append",
@@ -338,6 +356,7 @@ class PagedDecodeWrapper(_FusedRopeAppend, _PlanArrays):
         self.head_dim = head_dim
         self.page_size = page_size
         self.dtype = None
+        self._sm_scale = 1.0 / math.sqrt(head_dim)
         self._workspace = workspace_buffer
         self._staging = _Staging()
         self._n_req = 0
@@ -463,42 +482,28 @@ class PagedDecodeWrapper(_FusedRopeAppend, _PlanArrays):
             raise RuntimeError("plan() must be called before run()")
         if q.dtype != self.dtype:
             q = q.to(self.dtype)
-        n = self._n_req
-        if q.dim() != 3 or q.shape[0] < n or q.shape[1] != self.num_qo_heads or q.shape[2] != self.head_dim:
-            raise ValueError(f"q shape {tuple(q.shape)} does not match the plan")
-        if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-            q = q.contiguous()
+        n, heads, dim, shape = self._n_req, self.num_qo_heads, self.head_dim, q.shape
+        if len(shape) != 3 or shape[0] < n or shape[1] != heads or shape[2] != dim:
+            raise ValueError(f"q shape {tuple(shape)} does not match the plan")
+        q, q_at, q_st, q_sh = _rows(q)
         desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
-        if desc.num_kv_heads != self.num_kv_heads or desc.head_dim != self.head_dim or desc.page_size != self.page_size:
+        if desc.num_kv_heads != self.num_kv_heads or desc.head_dim != dim or desc.page_size != self.page_size:
             raise ValueError("kv_cache_layer geometry does not match the wrapper")
         if out is None:
-            out = torch.empty(q.shape[0], self.num_qo_heads, self.head_dim, dtype=q.dtype, device=q.device)
-        qs = _q_strides(q, "q")
-        os_ = _q_strides(out, "out")
-        batch = n
-        stream = self._reading_stream()
+            out = torch.empty(shape, dtype=q.dtype, device=q.device)
+            o_st, o_sh = heads * dim, dim
+        else:
+            o_st, o_sh = _q_strides(out, "out")
+        ws = self._workspace
+        tail = (ws.data_ptr(), ws.numel() * ws.element_size(), out.data_ptr(), o_st, o_sh, self._reading_stream())
+        args = (q_at, _lib.TORCH_TO_MI[q.dtype], q_st, q_sh, desc, None, self._indptr.data_ptr(),
+                self._indices.data_ptr(), self._last.data_ptr(), n, heads, 0, self._sm_scale)
         if _window(window_left, sink_tokens, q.dtype):
-            _lib.check(
-                _lib.lib().mi_decode_run_window(
-                    q.data_ptr(), _lib.TORCH_TO_MI[q.dtype], qs[0], qs[1], desc, None, self._indptr.data_ptr(),
-                    self._indices.data_ptr(), self._last.data_ptr(), batch, self.num_qo_heads, 0,
-                    1.0 / math.sqrt(self.head_dim), min(window_left, _WINDOW_MAX), min(sink_tokens, _WINDOW_MAX),
-                    self._workspace.data_ptr(), self._workspace.numel() * self._workspace.element_size(),
-                    out.data_ptr(), os_[0], os_[1], stream,
-                ),
-                "mi_decode_run_window",
-            )
-            return out
-        _lib.check(
-            _lib.lib().mi_decode_run(
-                q.data_ptr(), _lib.TORCH_TO_MI[q.dtype], qs[0], qs[1], desc, None, self._indptr.data_ptr(),
-                self._indices.data_ptr(), self._last.data_ptr(), batch, self.num_qo_heads, 0,
-                1.0 / math.sqrt(self.head_dim), self._workspace.data_ptr(),
-                self._workspace.numel() * self._workspace.element_size(), out.data_ptr(), os_[0], os_[1],
-                stream,
-            ),
-            "mi_decode_run",
-        )
+            _check_out(out, n, heads, dim, q)
+            _lib.check(_lib.lib().mi_decode_run_window(*args, min(window_left, _WINDOW_MAX), min(sink_tokens, _WINDOW_MAX),
+                                                       *tail), "mi_decode_run_window")
+        else:
+            _lib.check(_lib.lib().mi_decode_run(*args, *tail), "mi_decode_run")
         return out
 
     def set_kv_cache(self, kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.Tensor,
@@ -545,6 +550,7 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
         self.page_size = page_size
         self.dtype = None
         self.causal = True
+        self._sm_scale = 1.0 / math.sqrt(head_dim)
         self._workspace = workspace_buffer
         self._staging = _Staging()
         # Side stream of run(): made here so that a run() under graph capture
@@ -683,45 +689,48 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
             raise RuntimeError("plan() must be called before run()")
         if q.dtype != self.dtype:
             q = q.to(self.dtype)
-        if q.dim() != 3 or q.shape[1] != self.num_qo_heads or q.shape[2] != self.head_dim:
-            raise ValueError(f"q shape {tuple(q.shape)} does not match the wrapper")
-        if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-            q = q.contiguous()
+        heads, dim, shape = self.num_qo_heads, self.head_dim, q.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+            raise ValueError(f"q shape {tuple(shape)} does not match the wrapper")
+        q, q_at, q_st, q_sh = _rows(q)
         desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
-        if desc.num_kv_heads != self.num_kv_heads or desc.head_dim != self.head_dim or desc.page_size != self.page_size:
+        if desc.num_kv_heads != self.num_kv_heads or desc.head_dim != dim or desc.page_size != self.page_size:
             raise ValueError("kv_cache_layer geometry does not match the wrapper")
         if out is None:
-            out = torch.empty(q.shape[0], self.num_qo_heads, self.head_dim, dtype=q.dtype, device=q.device)
-        qs = _q_strides(q, "q")
-        os_ = _q_strides(out, "out")
-        ws_bytes = self._workspace.numel() * self._workspace.element_size()
-        args = [q.data_ptr(), _lib.TORCH_TO_MI[q.dtype], qs[0], qs[1], desc, self._qo.data_ptr(),
+            out = torch.empty(shape, dtype=q.dtype, device=q.device)
+            o_st, o_sh = heads * dim, dim
+        else:
+            o_st, o_sh = _q_strides(out, "out")
+        ws = self._workspace
+        args = [q_at, _lib.TORCH_TO_MI[q.dtype], q_st, q_sh, desc, self._qo.data_ptr(),
                 self._indptr.data_ptr(), self._indices.data_ptr(), self._last.data_ptr(), self._plan_batch,
-                self._plan_max_tokens, self.num_qo_heads, 1 if self.causal else 0, 1.0 / math.sqrt(self.head_dim),
-                self._workspace.data_ptr(), ws_bytes, out.data_ptr(), os_[0], os_[1], None]
+                self._plan_max_tokens, heads, 1 if self.causal else 0, self._sm_scale,
+                ws.data_ptr(), ws.numel() * ws.element_size(), out.data_ptr(), o_st, o_sh, None]
         # The MFMA tiles (long-query requests) and the split-KV decode of the
         # short-query requests write disjoint rows: where the batch can hold much
         # of both, the HBM-bound decode runs on a side stream, so that it overlaps
         # the compute-bound tiles.
         args[-1] = self._reading_stream()
+        launch = _lib.lib()
+        run, short, tiles = launch.mi_prefill_run, launch.mi_prefill_short, launch.mi_prefill_tiles
         if _window(window_left, sink_tokens, q.dtype):
-            parts = (1 if self._run_short else 0) | (2 if self._run_tiles else 0)
-            if parts:
-                args[14:14] = [min(window_left, _WINDOW_MAX), min(sink_tokens, _WINDOW_MAX), parts]
-                _lib.check(_lib.lib().mi_prefill_run_window(*args), "mi_prefill_run_window")
-            return out
+            _check_out(out, self._total_tokens, heads, dim, q)
+            if shape[0] < self._total_tokens:
+                raise ValueError(f"q holds {shape[0]} tokens, {self._total_tokens} planned")
+            window = (min(window_left, _WINDOW_MAX), min(sink_tokens, _WINDOW_MAX))
+            run, short, tiles = (lambda *a, p=p: launch.mi_prefill_run_window(*a[:14], *window, p, *a[14:]) for p in (3, 1, 2))
         if self._run_tiles and self._run_short and self._serial:
-            _lib.check(_lib.lib().mi_prefill_run(*args), "mi_prefill_run")
+            _lib.check(run(*args), "mi_prefill_run")
         elif self._run_tiles and self._run_short:
             main, side = torch.cuda.current_stream(q.device), self._side
             side.wait_stream(main)
-            _lib.check(_lib.lib().mi_prefill_tiles(*args), "mi_prefill_tiles")
+            _lib.check(tiles(*args), "mi_prefill_tiles")
             args[-1] = side.cuda_stream
-            _lib.check(_lib.lib().mi_prefill_short(*args), "mi_prefill_short")
+            _lib.check(short(*args), "mi_prefill_short")
             main.wait_stream(side)
         elif self._run_tiles or self._run_short:
-            fn = "mi_prefill_tiles" if self._run_tiles else "mi_prefill_short"
-            _lib.check(getattr(_lib.lib(), fn)(*args), fn)
+            _lib.check((tiles if self._run_tiles else short)(*args),
+                       "mi_prefill_tiles" if self._run_tiles else "mi_prefill_short")
         return out
 
     def set_kv_cache(self, kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.Tensor,
