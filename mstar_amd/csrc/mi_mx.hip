@@ -275,8 +275,8 @@ constexpr int kReadUnroll = 2;
 // consecutive entries of the page list.  Where the first one's request begins in
 // the output is a sum over the requests before it, which the workgroup's threads
 // add up from the index arrays: no plan, no launch for a prefix sum.  A thread's U
-// loads of K and V are in flight together.  HBM bound: 71k tokens at 4 kv heads x 128
-// in 4 bits 29 us (184 MB, 6.3 TB/s); 2000 tokens at 8 x 128 in 8 bits 5.0 us (9.2
+// loads of K and V are in flight together.  HBM bound: 68k tokens at 4 kv heads x 128
+// in 4 bits 29 us (175 MB, 6.0 TB/s); 2000 tokens at 8 x 128 in 8 bits 5.0 us (9.2
 // with a page to a workgroup, 6.4 with four loads a thread).
 template <int CACHE, int OUT>
 __global__ __launch_bounds__(256) void read_kv_kernel(ReadParams p) {

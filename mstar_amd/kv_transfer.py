@@ -77,6 +77,8 @@ class SequenceInfo:
 
 
 def _check_pool(kv: torch.Tensor, name: str) -> None:
+    if not isinstance(kv, torch.Tensor):
+        raise ValueError(f"{name}: only tensor pools are transferred, not {type(kv).__name__} (its scales lie beside its codes)")
     if kv.dim() != 6 or kv.shape[2] != 2:
         raise ValueError(f"{name} must be [layers, pages, 2, page_size, num_kv_heads, head_dim], got {tuple(kv.shape)}")
     if kv.stride(5) != 1 or kv.stride(4) != kv.shape[5] or kv.stride(3) != kv.shape[4] * kv.shape[5]:
@@ -93,7 +95,7 @@ def transfer_info(kv: torch.Tensor) -> DeviceKVTransferInfo:
 
 def pool_desc(info: DeviceKVTransferInfo | torch.Tensor) -> _lib.MiKvPool:
     """``mi_kv_pool`` of a whole pool ``[layers, pages, 2, ps, H, D]``."""
-    if isinstance(info, torch.Tensor):
+    if isinstance(info, torch.Tensor) or not hasattr(info, "stride"):
         info = transfer_info(info)
     es = torch.empty(0, dtype=getattr(torch, info.dtype.split(".")[-1])).element_size()
     d = _lib.MiKvPool()
@@ -375,6 +377,7 @@ class CPUPagePool:
         n = len(gpu_page_indices)
         if n == 0:
             return
+        _check_pool(gpu_kv_cache, "gpu_kv_cache")  # before any page is taken
         cpu_pages = self.page_allocator.try_allocate(n)
         if cpu_pages is None:
             logger.warning("CPU page pool exhausted: cannot offload %d pages for %s/%s", n, request_id, label)
