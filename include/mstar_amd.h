@@ -267,7 +267,8 @@ int mi_decode_noalloc(const void* q, int32_t q_dtype, int64_t q_stride_token, in
  * T = 464 (MI_MXFP8) or 7 (MI_MXFP4), at least -126 and at most 119 or 125 (every code
  * is then finite), codes RNE(x * 2^-e), the largest beyond it, scale byte e + 127; a
  * block of zeros 127, one that holds a NaN or an infinity 255; the
- * layer as for mi_decode_run, and the scale bytes are written too).
+ * layer as for mi_decode_run, and the scale bytes are written too).  The tokens of a
+ * call go to different slots.
  * page[i] = page_idx[i * idx_stride], slot[i] = slot_idx[i * idx_stride]
  * (idx_stride 1 for token_to_page/token_to_cache, 2 for kv_cache_locations
  * [B, 2] with slot_idx = page_idx + 1).  Tokens whose page id is outside

@@ -277,16 +277,14 @@ constexpr int32_t kWinMax = 1 << 30;
 // (request, kv-head) pairs than workgroups no cut paid (256 requests of up to 8256 keys at 4
 // kv heads, one item 384 us, two to four 384-394 + 4); taking the longest first did
 // (455 -> 384 us), as uncut requests are as uneven as their lengths.
-constexpr int kWinItemTiles = 16;
 static void win_items(DecodeParams& dp, int heads, int slots, int max_chunks) {
   const int tiles = win_tiles_max(dp);
   int64_t n = slots / ((int64_t)dp.batch * heads);
   if (n > 16) n = 16;
   if (n > max_chunks / dp.batch) n = max_chunks / dp.batch;
   if (n < 1) n = 1;
-  dp.item_tiles = (int)((tiles + n - 1) / n);
-  if (dp.item_tiles < kWinItemTiles) dp.item_tiles = kWinItemTiles;
-  dp.splits = (tiles + dp.item_tiles - 1) / dp.item_tiles;
+  const int most = (tiles + kWinItemTiles - 1) / kWinItemTiles;
+  dp.splits = n < most ? (int)n : most;
   dp.sorted = dp.batch <= kSortedMax && (int64_t)dp.batch * heads * dp.splits > slots;
 }
 

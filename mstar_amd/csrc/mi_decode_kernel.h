@@ -66,25 +66,32 @@ MI_DEVICE void load_words(uint32_t (&dst)[N], const uint8_t* src) {
 }
 
 // The request at place `rank` of a windowed batch when its requests are taken by
-// classes of tiles, an eighth of a full window each, most first: workgroups start
+// classes of tiles, an eighth of the batch's most each, most first: workgroups start
 // in order, so the last ones to start are short.  The workgroup's threads class
 // 256 requests at a time and count by ballots, from the index arrays alone.
 __device__ __forceinline__ int win_item(const DecodeParams& p, int rank) {
   constexpr int kClasses = 8;
-  __shared__ int s_count[4][kClasses], s_b;
+  __shared__ int s_count[4][kClasses], s_most[4], s_b;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const float per_tile = (float)kClasses / (float)win_tiles_max(p);
-  auto class_of = [&](int r) {
-    if (r >= p.batch) return -1;
+  auto tiles_of = [&](int r) {
     const int np = p.kv_indptr[r + 1] - p.kv_indptr[r];
     const int qo_len = p.qo_indptr ? p.qo_indptr[r + 1] - p.qo_indptr[r] : 1;
-    if (qo_len <= 0 || qo_len * p.group > p.short_rows) return kClasses - 1;  // nothing to do here
-    const int kv_len = np > 0 ? (np - 1) * p.page_size + p.last_page_len[r] : 0;
-    return kClasses - 1 - min(kClasses - 1, (int)((float)win_tiles(kv_len, qo_len, p).total * per_tile));
+    if (qo_len <= 0 || qo_len * p.group > p.short_rows) return 0;  // nothing to do here
+    return max(0, win_tiles(np > 0 ? (np - 1) * p.page_size + p.last_page_len[r] : 0, qo_len, p).total);
   };
-  int mine[kSortedMax / 256], total[kClasses] = {};  // this wavefront's counts, all chunks of 256
+  int mine[kSortedMax / 256], most = 1;
   for (int c = 0; c * 256 < p.batch; ++c) {
-    mine[c] = class_of(c * 256 + tid);
+    mine[c] = c * 256 + tid < p.batch ? tiles_of(c * 256 + tid) : -1;
+    most = max(most, mine[c]);
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) most = max(most, __shfl_xor(most, m, kWave));
+  if (lane == 0) s_most[wave] = most;
+  __syncthreads();
+  const float per_tile = (float)kClasses / (float)max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3]));
+  int total[kClasses] = {};  // this wavefront's counts, all chunks of 256
+  for (int c = 0; c * 256 < p.batch; ++c) {
+    if (mine[c] >= 0) mine[c] = kClasses - 1 - min(kClasses - 1, (int)((float)mine[c] * per_tile));
 #pragma unroll
     for (int k = 0; k < kClasses; ++k) total[k] += __popcll(__builtin_amdgcn_ballot_w64(mine[c] == k));
   }

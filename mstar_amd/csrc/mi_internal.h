@@ -181,14 +181,16 @@ struct DecodeParams {
   float scale_log2;
   int32_t short_rows = kShortRowsMax;  // ragged batches: requests with qo_len * group above this are not ours
   // Windowed runs: keys below a query's position - window_left are hidden but for
-  // the first `sinks` of the request; items of about item_tiles tiles, `splits`
-  // places for each of the batch's requests; sorted: longest first.
-  int32_t window_left = -1, sinks = 0, item_tiles = 0, splits = 0, batch = 0, sorted = 0;
+  // the first `sinks` of the request; `splits` places for the items of each of the
+  // batch's requests; sorted: longest first.
+  int32_t window_left = -1, sinks = 0, splits = 0, batch = 0, sorted = 0;
 };
 
 // The 16-token tiles of a windowed request: those that hold sinks, then those
 // from `first` on to the end of its keys, one sequence of `total` tiles that
-// `items` items share evenly.
+// `items` items share evenly: as many as there are places, however much shorter than
+// the window the request is (a window may be wider than every context).
+constexpr int kWinItemTiles = 16;  // the fewest worth an item of their own (mi_decode.hip)
 struct WinTiles {
   int sinks, first, total, items;
 };
@@ -197,7 +199,7 @@ __device__ __forceinline__ WinTiles win_tiles(int kv_len, int qo_len, const Deco
   w.first = max(0, kv_len - qo_len - p.window_left) >> 4;
   w.sinks = min((p.sinks + 15) >> 4, w.first);
   w.total = w.sinks + ((kv_len + 15) >> 4) - w.first;
-  w.items = max(1, min(p.splits, (w.total + p.item_tiles - 1) / p.item_tiles));
+  w.items = max(1, min(p.splits, (w.total + kWinItemTiles - 1) / kWinItemTiles));
   return w;
 }
 // The most tiles a request can have (short queries).

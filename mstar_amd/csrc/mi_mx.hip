@@ -312,6 +312,7 @@ __global__ __launch_bounds__(256) void read_kv_kernel(ReadParams p) {
     const int64_t at = tokens + (int64_t)(e - first) * p.page_size;
     const int64_t left = p.out_tokens - at;
     if (left <= 0) return;
+    if (at < 0) continue;  // entries before the first request's
     int slots = e == p.kv_indptr[r + 1] - 1 ? min(p.last_page_len[r], p.page_size) : p.page_size;
     if (slots > left) slots = (int)left;
     const int64_t page = p.kv_indices[e];

@@ -248,6 +248,39 @@ def test_large_batches(gpu, batch):
     log(f"{H.check(p, q, [1] * batch, out, 300, 1, True, 'large batch'):.2f} of the bound")
 
 
+@pytest.mark.parametrize("batch", [1, 5, 300])
+def test_window_wider_than_every_context(gpu, batch):
+    """Requests are cut and ordered by their own lengths where the window is far wider, up to the largest one."""
+    r = np.random.default_rng(batch)
+    lens = r.integers(1, 5000 if batch < 10 else 400, batch).tolist()
+    p = H.make(gpu, "bf16", lens, 16, 4, 128, seed=batch)
+    q = torch.randn(batch, 16, 128, generator=torch.Generator().manual_seed(11)).to(torch.bfloat16)
+    w = PagedDecodeWrapper(workspace(gpu, 128 << 20), 16, 4, 128, 16, device=gpu)
+    w.plan(*p.index())
+    outs = [w.run(q.to(gpu), p.layer, window_left=wl, sink_tokens=sinks) for wl, sinks in
+            ((5000, 0), (1 << 20, 7), (2**31 - 1, 2**31 - 1), (0, 2**31 - 1))]
+    for out in outs:
+        H.check(p, q, [1] * batch, out, -1, 0, True, "wide window")
+
+
+def test_read_from_pages_behind_others(gpu):
+    """A list whose first request begins behind entries of none: those are not read; pages past the pool leave their rows."""
+    p = H.make(gpu, "mx4", [40, 70], 16, 2, 64, seed=12)
+    indptr, indices, last = p.index()
+    want = read_kv_cache(p.layer, indptr, indices, last, 110)
+    shifted = torch.cat([torch.tensor([-1, 10**6, 0], dtype=torch.int32), indices])
+    got = read_kv_cache(p.layer, indptr + 3, shifted, last, 110)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    bad = indices.clone()
+    bad[1], bad[4] = -5, p.layer.shape[0]
+    out = tuple(torch.full_like(x, 9.0) for x in want)
+    read_kv_cache(p.layer, indptr, bad, last, 110, out=out)
+    for a, b in zip(out, want):
+        assert (a[16:32] == 9).all() and (a[56:72] == 9).all()
+        keep = [i for i in range(110) if not (16 <= i < 32 or 56 <= i < 72)]
+        assert torch.equal(a[keep], b[keep])
+
+
 @pytest.mark.parametrize("kind", ["bf16", "mx8"])
 def test_pool_past_32_bits(gpu, kind):
     """Pages whose byte offsets pass 2^32 (and, in the scales, 2^31): append, read, decode and chunks."""
