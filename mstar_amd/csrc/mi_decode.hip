@@ -270,21 +270,20 @@ static int dispatch_d(const DecodeParams& dp, int head_dim, int grid, int batch,
 // Windows and sink counts are clamped here: beyond any context, and sums with a length stay in 32 bits.
 constexpr int32_t kWinMax = 1 << 30;
 
-// Items of a windowed run: a request's share of the resident workgroups, none
-// shorter than kWinItemTiles, within the workspace's partials.  One request of 1028
-// keys at 4 kv heads: one item a head 13.1 us, 2 8.6, 3 7.3, 4 and more 6.5; 96 of
-// 4100 keys at 2 kv heads, 4 bits: one 58 us, 2 45 + 4 for the merge.  With more
-// (request, kv-head) pairs than workgroups no cut paid (256 requests of up to 8256 keys at 4
-// kv heads, one item 384 us, two to four 384-394 + 4); taking the longest first did
-// (455 -> 384 us), as uncut requests are as uneven as their lengths.
+// Items of a windowed run: a request's share of the resident workgroups, at most
+// win_items_max of its tiles, within the workspace's partials.  One request of 1028
+// keys at 4 kv heads: one item a head 13.1 us, 2 8.6, 3 7.3, 4 and more 6.5; of 32k
+// keys: 16 items 25 us + 4.5 for the merge, 32 16 + 7; 96 requests of 4100 keys at 2 kv heads, 4 bits: one
+// 58 us, 2 45 + 4 for the merge.  With more (request, kv-head) pairs than workgroups
+// no cut paid (256 requests of up to 8256 keys at 4 kv heads, one item 384 us, two to
+// four 384-394 + 4); taking the longest first did (455 -> 384 us), as uncut requests
+// are as uneven as their lengths.
 static void win_items(DecodeParams& dp, int heads, int slots, int max_chunks) {
-  const int tiles = win_tiles_max(dp);
   int64_t n = slots / ((int64_t)dp.batch * heads);
-  if (n > 16) n = 16;
+  const int most = win_items_max(win_tiles_max(dp));
+  if (n > most) n = most;
   if (n > max_chunks / dp.batch) n = max_chunks / dp.batch;
-  if (n < 1) n = 1;
-  const int most = (tiles + kWinItemTiles - 1) / kWinItemTiles;
-  dp.splits = n < most ? (int)n : most;
+  dp.splits = n < 1 ? 1 : (int)n;
   dp.sorted = dp.batch <= kSortedMax && (int64_t)dp.batch * heads * dp.splits > slots;
 }
 

@@ -190,16 +190,21 @@ struct DecodeParams {
 // from `first` on to the end of its keys, one sequence of `total` tiles that
 // `items` items share evenly: as many as there are places, however much shorter than
 // the window the request is (a window may be wider than every context).
-constexpr int kWinItemTiles = 16;  // the fewest worth an item of their own (mi_decode.hip)
 struct WinTiles {
   int sinks, first, total, items;
 };
+// The most items that a request of so many tiles is cut into: of 16 tiles and more
+// up to 16 items, beyond them of 64 and more (mi_decode.hip, win_items).
+__host__ __device__ inline int win_items_max(int tiles) {
+  const int short_items = (tiles + 15) >> 4, long_items = (tiles + 63) >> 6;
+  return short_items < 16 ? short_items : long_items > 16 ? long_items : 16;
+}
 __device__ __forceinline__ WinTiles win_tiles(int kv_len, int qo_len, const DecodeParams& p) {
   WinTiles w;
   w.first = max(0, kv_len - qo_len - p.window_left) >> 4;
   w.sinks = min((p.sinks + 15) >> 4, w.first);
   w.total = w.sinks + ((kv_len + 15) >> 4) - w.first;
-  w.items = max(1, min(p.splits, (w.total + kWinItemTiles - 1) / kWinItemTiles));
+  w.items = max(1, min(p.splits, win_items_max(w.total)));
   return w;
 }
 // The most tiles a request can have (short queries).
