@@ -64,6 +64,14 @@ _WINDOW_MAX = 1 << 30  # beyond any context
 # 84.7 -> 78.4); at 12288 and 16384 rows 128 still gained 4-20 %, 256 lost up to 9 %
 # (a 2045-token chunk and 3 decodes 84.9 -> 92.7).
 _SERIAL_REQUESTS, _SERIAL_GRAPH_ROWS = 16, 8192
+# Behind a window both parts are shorter, and in turn is faster, or the same, until both
+# are long (us a layer, side stream -> in turn, window 2048, 4 kv heads x 128, 6000 keys
+# a decode: one 512-token chunk and 60 decodes eager 98 -> 87, captured 94 -> 88; two of
+# 1024 and 120 decodes 174 -> 155, 174 -> 155; six of 1024 and 60 258 -> 241, 246 -> 241;
+# six and 120 275 -> 280, 279 -> 281, but window 4096 485 -> 513, 508 -> 514): rows of
+# (token, q-head) and bytes that the windows span from which on the parts fork.
+_WINDOW_FORK_ROWS, _WINDOW_FORK_BYTES = 1 << 17, 3 << 28
+_KV_BITS = {_lib.MI_BF16: 16, _lib.MI_F16: 16, _lib.MI_FP8_E4M3: 8, _lib.MI_MXFP8: 8, _lib.MI_MXFP4: 4}
 
 
 def _check_heads(num_qo_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> None:
@@ -713,13 +721,16 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
         args[-1] = self._reading_stream()
         launch = _lib.lib()
         run, short, tiles = launch.mi_prefill_run, launch.mi_prefill_short, launch.mi_prefill_tiles
+        serial = self._serial
         if _window(window_left, sink_tokens, q.dtype):
             _check_out(out, self._total_tokens, heads, dim, q)
             if shape[0] < self._total_tokens:
                 raise ValueError(f"q holds {shape[0]} tokens, {self._total_tokens} planned")
             window = (min(window_left, _WINDOW_MAX), min(sink_tokens, _WINDOW_MAX))
             run, short, tiles = (lambda *a, p=p: launch.mi_prefill_run_window(*a[:14], *window, p, *a[14:]) for p in (3, 1, 2))
-        if self._run_tiles and self._run_short and self._serial:
+            spans = self._n_req * (window[0] + window[1]) * self.num_kv_heads * dim * _KV_BITS[desc.dtype] // 4  # K and V
+            serial = serial or self._total_tokens * heads < _WINDOW_FORK_ROWS or spans < _WINDOW_FORK_BYTES
+        if self._run_tiles and self._run_short and serial:
             _lib.check(run(*args), "mi_prefill_run")
         elif self._run_tiles and self._run_short:
             main, side = torch.cuda.current_stream(q.device), self._side

@@ -178,6 +178,45 @@ def test_run_attention_window(gpu):
     assert ((out.double().cpu() - ref).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_both_parts_on_two_streams(gpu, captured):
+    """A ragged batch large enough for its chunks and decodes to fork: equal to the parts in turn, eager and replayed."""
+    hq, hkv, d, ps = 16, 2, 128, 16
+    lens, new = [4300, 4200] + [3000] * 300, [4200, 4100] + [1] * 300
+    pool = sum(-(-n // ps) for n in lens)
+    qo, *idx = _index(lens, ps, pool, 31, new=new)
+    g = torch.Generator().manual_seed(31)
+    layer = torch.randn(pool, 2, ps, hkv, d, generator=g).to(torch.bfloat16).to(gpu)
+    n = sum(new)
+    q = torch.randn(n, hq, d, generator=g).to(torch.bfloat16).to(gpu)
+    kw = dict(batch_size=len(lens), max_total_tokens=n, max_num_pages=pool, use_cuda_graph=True) if captured else {}
+    w = PagedPrefillWrapper(workspace(gpu, 256 << 20), hq, hkv, d, ps, device=gpu, **kw)
+    w.plan(qo, *idx)
+    out = torch.empty_like(q)
+
+    def run():
+        return w.run(q, layer, out=out, window_left=2900, sink_tokens=5)
+
+    forked = []
+    wait = w._side.wait_stream
+    w._side.wait_stream = lambda s: (forked.append(1), wait(s))[1]
+    run()
+    assert forked, "the parts did not fork"
+    if captured:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+    for _ in range(3 if captured else 1):
+        out.fill_(7.0)
+        graph.replay() if captured else run()
+        torch.cuda.synchronize()
+        got = out.clone()
+        w._serial = True
+        assert torch.equal(got, w.run(q, layer, window_left=2900, sink_tokens=5))
+        w._serial = False
+
+
 def test_other_streams_and_two_at_once(gpu):
     """Two wrappers with workspaces of their own, planned on the default stream and run on two others at the same time."""
     ps = [H.make(gpu, kind, [3000, 40, 700, 1], 16, 4, 128, seed=i) for i, kind in enumerate(("bf16", "mx4"))]
