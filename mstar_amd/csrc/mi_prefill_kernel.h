@@ -151,19 +151,13 @@ __host__ __device__ inline void pf_dealt(int nkv, int x, int i, int& piece, int&
 // queues are empty.  Called by one wavefront; lanes 0..7 look at the 8 queues
 // at once (starting with the XCD's own), so a claim costs its own round trips
 // and not one per queue passed: read one after the other, the empty queues
-// took a workgroup 1-2 us each when it ran out of work.  pf_claim_begin asks the own
-// queue, and pf_claim_end takes the answer, which may be much later: each begun claim
-// is ended, so that a workgroup that leaves has no claim of its own on the way.
-MI_DEVICE int pf_claim_begin(const PrefillParams& p) {
-  const int y = (int)blockIdx.x & 7;  // workgroups are dispatched to the 8 XCDs round-robin
-  int i = 0x7fffffff;
-  if (lane_id() == 0) i = __hip_atomic_fetch_add(p.ctr + y * kCtrStride, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return i;
-}
-MI_DEVICE int pf_claim_end(const PrefillParams& p, int i) {
+// took a workgroup 1-2 us each when it ran out of work.
+MI_DEVICE int pf_claim(const PrefillParams& p) {
   const int lane = lane_id();
-  const int y = ((int)blockIdx.x + lane) & 7;
+  const int y = ((int)blockIdx.x + lane) & 7;  // workgroups are dispatched to the 8 XCDs round-robin
   const int len = p.hdr[kPfCuts + 1 + y] - p.hdr[kPfCuts + y];
+  int i = 0x7fffffff;
+  if (lane == 0) i = __hip_atomic_fetch_add(p.ctr + y * kCtrStride, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   int u = uniform(i < len ? i << 3 | y : -1);
   if (u >= 0) return u;
   const int taken = __hip_atomic_load(p.ctr + y * kCtrStride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -178,8 +172,6 @@ MI_DEVICE int pf_claim_end(const PrefillParams& p, int i) {
   }
   return -1;
 }
-
-MI_DEVICE int pf_claim(const PrefillParams& p) { return pf_claim_end(p, pf_claim_begin(p)); }
 
 MI_DEVICE PfUnit pf_unit(const PrefillParams& p, int claim) {
   PfUnit r;

@@ -16,11 +16,13 @@
 // reads, not the MFMAs, set the step time.  Each SIMD holds one wavefront of
 // each role for round-robin (SIMD = wave % 4) and paired (SIMD = wave / 2)
 // placement alike, so the S-role softmax runs under the O-role MFMAs.
-// Between units the S-role is done first: it claims the next unit (asked for when the
-// last one began), reads its request and fills the table of its pages while the O-role
-// writes the last unit's rows; the O-role takes what it needs of that from LDS.  Eight
-// 2048-token chunks: behind a window of 1024 320 -> 314 us, of 128 130 -> 121, whole
-// contexts 1210 -> 1206; with the O-role reading the request for itself 320 and 126.
+// Between units the S-role is done first: it claims the next unit, reads its request
+// and fills the table of its pages while the O-role writes the last unit's rows; the
+// O-role takes what it needs of that from LDS.  Eight 2048-token chunks: behind a window
+// of 1024 320 -> 314 us, of 128 130 -> 123, whole contexts 1210 -> 1206; with the O-role
+// reading the request for itself 320 and 126.  Claiming a unit earlier, when the last
+// one begins, gains 2 us at 128, and where contexts differ (2048 to 5632 tokens before
+// the chunks) loses 5 % of 1217 us: a workgroup sits on a unit that others wait for.
 // Tiles of a 16-bit cache go from memory straight into LDS (global_load_lds,
 // 16 bytes per lane, issued at the end of step T for tile T+2): the tile bytes
 // then pass through no registers and no ds_write, which had cost ~16% of the
@@ -90,11 +92,9 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
     constexpr bool S = decltype(role)::value;
     // The next unit, claimed by wavefront 0 (of the S-role).  Between two units lies a
     // barrier more, so that s_unit is read by all before it is written again.
-    int ahead = 0;
-    if (S && wave == 0) ahead = pf_claim_begin(p);
     auto next_unit = [&]() {
       if (wave == 0) {
-        const int u = pf_claim_end(p, ahead);
+        const int u = pf_claim(p);
         if (tid == 0) s_unit = u;
       }
       __syncthreads();
@@ -192,7 +192,6 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
           s_req = rq;
         }
         __syncthreads();
-        if (wave == 0) ahead = pf_claim_begin(p);
       }
       if (un.n == 0) {  // uniform
         unit = next_unit();
