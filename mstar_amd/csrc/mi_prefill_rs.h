@@ -52,7 +52,8 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
   static_assert(C::ROWS == 4 * PROWS, "tile rows = four pairs");
   constexpr int KS = D / 32, VW = D / 16, KEYS = C::KEYS, RSK = C::RSK, RSV = C::RSV, ESZ = C::ESZ, CPR = C::CPR;
   constexpr int THREADS = C::THREADS, NL = C::NL, HALF = C::HALF;
-  constexpr int LCH = KVT == kKvMx4 ? 64 : KVT == kKv16 ? 16 : 32;  // LDS bytes per loaded chunk
+  constexpr int LCH = KVT == kKv16 ? 16 : 32;  // LDS bytes per loaded chunk
+  constexpr int CHB = KVT == kKvMx4 ? 8 : 16;  // and bytes of the cache
   constexpr float kNegInf = -__builtin_inff();
   static_assert(THREADS == 512, "four wavefront pairs");
   static_assert(RSK == RSV, "one LDS row stride for K and V");
@@ -219,8 +220,8 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
         l_row[i] = row;
         l_grp[i] = uniform(row) & ~15;
         l_v[i] = half == 1;
-        l_off[i] = (uint32_t)((int64_t)half * p.kv_stride * ESZ + (int64_t)(row - (row & ~15)) * tok_bytes + 16 * ch);
-        if constexpr (MX) l_soff[i] = (uint32_t)((h * (D / kMxBlock) + (KVT == kKvMx4 ? ch : ch >> 1)) * ps + (row & 15));
+        l_off[i] = (uint32_t)((int64_t)half * p.kv_stride * ESZ + (int64_t)(row - (row & ~15)) * tok_bytes + CHB * ch);
+        if constexpr (MX) l_soff[i] = (uint32_t)((h * (D / kMxBlock) + (ch >> 1)) * ps + (row & 15));
       }
       int c0 = 0;
       constexpr int NB = 2;
@@ -236,7 +237,13 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
         for (int i = 0; i < NL; ++i) {
           if (2 * HALF % THREADS == 0 || tid + i * THREADS < 2 * HALF) {
             const uint8_t* base = kvb + uniform64(pg[i]);
-            r[i] = *(const uint4*)(base + l_off[i]);
+            if constexpr (KVT == kKvMx4) {
+              const uint2 t = *(const uint2*)(base + l_off[i]);
+              r[i].x = t.x;
+              r[i].y = t.y;
+            } else {
+              r[i] = *(const uint4*)(base + l_off[i]);
+            }
             if constexpr (MX)
               rs[i] = ((const uint8_t*)(l_v[i] ? p.v_scale : p.k_scale) +
                        uniform64(lds_soff[2 * (t - c0) + (l_grp[i] >> 4)]))[l_soff[i]];
@@ -270,7 +277,7 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
             } else if constexpr (MX) {
               const uint32_t w[4] = {v.x, v.y, v.z, v.w};
               uint32_t o[LCH / 4];
-              mx_to_mt<MT, KVT>(w, mx_scale(rs[i], 0), o);
+              mx_to_mt<MT, KVT>(w, mx_scale(rs[i], 0), o);  // at 4 bits the first two words
 #pragma unroll
               for (int k = 0; k < LCH / 16; ++k)
                 *(uint4*)(dst + 16 * k) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
