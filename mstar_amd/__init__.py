@@ -8,6 +8,7 @@ interfaces M*'s engine calls:
 * :mod:`mstar_amd.paged_attention` — ``FlashInferPrefillWrapper`` /
   ``FlashInferDecodeWrapper`` plan()/run()/set_kv_cache() surface.
 * :mod:`mstar_amd.cache_manager` — ``BatchedCacheManager`` (GPU packing).
+* :mod:`mstar_amd.mx_cache` — the microscaled KV cache, and reading contexts back.
 * :mod:`mstar_amd.kv_store` — FIFO page allocator, request state, device block table.
 """
 
