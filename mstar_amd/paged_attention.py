@@ -196,6 +196,12 @@ def _window(window_left: int, sink_tokens: int, dtype: torch.dtype) -> bool:
     return window_left >= 0
 
 
+def _check_devices(dev: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.device != dev:
+            raise ValueError(f"{name} must be on {dev}, not on {t.device}")
+
+
 def _check_out(out: torch.Tensor, n: int, heads: int, dim: int, q: torch.Tensor) -> None:
     if out.shape[0] < n or out.shape[1:] != (heads, dim) or out.dtype != q.dtype or out.device != q.device:
         raise ValueError(f"out must hold {n} rows of {(heads, dim)} in {q.dtype} on {q.device}, got {tuple(out.shape)}, {out.dtype}")
@@ -243,6 +249,8 @@ def _append(kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.
     if n == 0:
         return
     desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
+    if isinstance(kv_cache_layer, MXKVLayer):
+        _check_devices(page_idx.device, k=k, v=v, kv_cache_layer=kv_cache_layer)
     shape = k.shape
     if shape[1:] != (desc.num_kv_heads, desc.head_dim) or v.shape[1:] != shape[1:]:
         raise ValueError(f"k/v shape {tuple(shape)} does not match the cache heads/head_dim")
@@ -494,6 +502,8 @@ class PagedDecodeWrapper(_FusedRopeAppend, _PlanArrays):
         if len(shape) != 3 or shape[0] < n or shape[1] != heads or shape[2] != dim:
             raise ValueError(f"q shape {tuple(shape)} does not match the plan")
         q, q_at, q_st, q_sh = _rows(q)
+        if window_left >= 0 or isinstance(kv_cache_layer, MXKVLayer):
+            _check_devices(self.device, q=q, kv_cache_layer=kv_cache_layer)
         desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
         if desc.num_kv_heads != self.num_kv_heads or desc.head_dim != dim or desc.page_size != self.page_size:
             raise ValueError("kv_cache_layer geometry does not match the wrapper")
@@ -701,6 +711,8 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
         if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
             raise ValueError(f"q shape {tuple(shape)} does not match the wrapper")
         q, q_at, q_st, q_sh = _rows(q)
+        if window_left >= 0 or isinstance(kv_cache_layer, MXKVLayer):
+            _check_devices(self.device, q=q, kv_cache_layer=kv_cache_layer)
         desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
         if desc.num_kv_heads != self.num_kv_heads or desc.head_dim != dim or desc.page_size != self.page_size:
             raise ValueError("kv_cache_layer geometry does not match the wrapper")

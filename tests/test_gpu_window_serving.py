@@ -379,3 +379,53 @@ def test_windowed_run_checks_its_tensors(gpu):
     f.plan(torch.tensor([0, 30, 39], dtype=torch.int32), *p.index())
     with pytest.raises(ValueError):
         f.run(torch.randn(38, 8, 128, device=gpu, dtype=torch.bfloat16), p.layer, window_left=3)
+
+
+def test_tensors_of_another_device_are_refused(gpu):
+    """A tensor in host memory reaches no kernel."""
+    p = H.make(gpu, "mx8", [40, 9], 16, 2, 128, seed=13)
+    cpu = MXKVCache(1, 8, 16, 2, 128, device="cpu")[0]
+    q, k = torch.zeros(2, 8, 128, dtype=torch.bfloat16), torch.zeros(2, 2, 128, dtype=torch.bfloat16)
+    w = PagedDecodeWrapper(workspace(gpu, 32 << 20), 8, 2, 128, 16, device=gpu)
+    w.plan(*p.index())
+    f = PagedPrefillWrapper(workspace(gpu, 64 << 20), 8, 2, 128, 16, device=gpu)
+    f.plan(torch.tensor([0, 1, 2], dtype=torch.int32), *p.index())
+    pool = torch.zeros(8, 2, 16, 2, 128, dtype=torch.bfloat16)
+    for x in (w, f):
+        for bad in (lambda: x.run(q, p.layer), lambda: x.run(q.to(gpu), cpu), lambda: x.run(q.to(gpu), pool, window_left=3),
+                    lambda: x.run(q, pool.to(gpu), window_left=3), lambda: x.set_kv_cache(p.layer, k, k.to(gpu)),
+                    lambda: x.set_kv_cache(p.layer, k.to(gpu), k), lambda: x.set_kv_cache(cpu, k.to(gpu), k.to(gpu)),
+                    lambda: x.run(q.to(gpu), p.layer, out=torch.empty_like(q), window_left=3)):
+            with pytest.raises(ValueError):
+                bad()
+
+
+def test_two_graphs_share_a_workspace(gpu):
+    """A windowed and a full run captured apart on one wrapper, replayed by turns over replans with eager work between."""
+    lens, new = [900, 300, 40, 7], [260, 1, 33, 1]
+    p = H.make(gpu, "mx4", lens, 16, 4, 128, seed=14)
+    pool = p.layer.shape[0]
+    n = sum(new)
+    w = PagedPrefillWrapper(workspace(gpu, 128 << 20), 16, 4, 128, 16, batch_size=4, max_total_tokens=n, max_num_pages=pool,
+                            device=gpu, use_cuda_graph=True)
+    g = torch.Generator().manual_seed(15)
+    q = torch.randn(n, 16, 128, generator=g).to(torch.bfloat16).to(gpu)
+    qo = torch.tensor([0] + list(np.cumsum(new)), dtype=torch.int32)
+    w.plan(qo, *p.index())
+    kws, outs, graphs = ({"window_left": 70, "sink_tokens": 2}, {}), [], []
+    for kw in kws:
+        w.run(q, p.layer, **kw)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(w.run(q, p.layer, **kw))
+    for i in range(6):
+        if i % 2 == 0:
+            q.copy_(torch.randn(n, 16, 128, generator=g).to(torch.bfloat16))
+            w.plan(qo, *p.index())
+        for j in (i % 2, 1 - i % 2):
+            outs[j].zero_()
+            graphs[j].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[j], w.run(q, p.layer, **kws[j]))
+            H.check(p, q.cpu(), new, outs[j], kws[j].get("window_left", -1), kws[j].get("sink_tokens", 0), True, f"{i} {j}")
