@@ -273,8 +273,8 @@ constexpr int32_t kWinMax = 1 << 30;
 // Items of a windowed run: a request's share of the resident workgroups, at most
 // win_items_max of its tiles, within the workspace's partials.  One request of 1028
 // keys at 4 kv heads: one item a head 13.1 us, 2 8.6, 3 7.3, 4 and more 6.5; of 32k
-// keys: 16 items 25 us + 4.5 for the merge, 32 16 + 7; 96 requests of 4100 keys at 2 kv heads, 4 bits: one
-// 58 us, 2 45 + 4 for the merge.  With more (request, kv-head) pairs than workgroups
+// keys: 16 items 25 us + 4.5 for the merge, 32 16 + 7; 96 requests of 4100 keys at 2
+// kv heads, 4 bits: one 58 us, 2 45 + 4.  With more (request, kv-head) pairs than workgroups
 // no cut paid (256 requests of up to 8256 keys at 4 kv heads, one item 384 us, two to
 // four 384-394 + 4); taking the longest first did (455 -> 384 us), as uncut requests
 // are as uneven as their lengths.
@@ -285,6 +285,17 @@ static void win_items(DecodeParams& dp, int heads, int slots, int max_chunks) {
   if (n > max_chunks / dp.batch) n = max_chunks / dp.batch;
   dp.splits = n < 1 ? 1 : (int)n;
   dp.sorted = dp.batch <= kSortedMax && (int64_t)dp.batch * heads * dp.splits > slots;
+}
+
+// Whether requests that win_items cuts go whole to a workgroup of eight wavefronts:
+// without partials and merge.  Cut in two they had as many wavefronts (us, cut -> whole:
+// 60 requests at 4 kv heads x 128, windows of 250 11.7 -> 8.4, 1024 26.9 -> 22.8, 4090
+// 87 -> 83; 96 at 2 x 256 in 4 bits, 4090 47.3 -> 43.1); cut in more, short windows
+// still gain (one request, 250 keys 7.9 -> 6.2, 500 8.8 -> 7.6) and longer ones lose
+// (1024 keys 9.0 -> 9.6 at 4 x 128, 11.4 -> 15.1 at 2 x 256 in 4 bits).
+constexpr int kWinEightTiles = 40;
+static bool win_by_eight(const DecodeParams& dp) {
+  return dp.splits == 2 || (dp.splits > 2 && win_tiles_max(dp) <= kWinEightTiles);
 }
 
 int decode_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_token, int64_t q_stride_head,
@@ -363,10 +374,13 @@ int decode_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_token, int6
       dp.num_kv_heads = heads;
       dp.head_stride = 2 * kv->head_stride;
     }
+    const bool eight = !pair_kernel && win_by_eight(dp) && decode_win8_serves(kvt, D);
+    if (eight) dp.splits = 1;
     st = MI_OK;
     if (phases & kPhaseAttend) {
       const int wgrid = (int)(((int64_t)batch * dp.splits + 7) / 8 * 8 * heads);
-      st = decode_win_launch(dp, q_dtype, kvt, D, pair_kernel, wgrid, stream);
+      st = eight ? decode_win8_launch(dp, q_dtype, kvt, D, wgrid, stream)
+                 : decode_win_launch(dp, q_dtype, kvt, D, pair_kernel, wgrid, stream);
     }
     if (st == MI_OK && (phases & kPhaseMerge) && dp.splits > 1)
       st = decode_win_merge_launch(dp, q_dtype, kvt, D, pair_kernel, batch, stream);

@@ -137,8 +137,11 @@ constexpr int decode_waves(int kvt, int d, bool win) {
 // (win_tiles), in one sequence that its items share evenly.  Which item a
 // workgroup takes follows from its place and the lengths (win_item), so a windowed
 // run needs no plan of its own and a model may mix windowed and full layers.
-template <typename MT, int KVT, int D, bool PAIR = false, bool WIN = false>
-__global__ __launch_bounds__(256, decode_waves(KVT, D, WIN)) void decode_kernel(DecodeParams p) {
+// NW: wavefronts of the workgroup.  Eight (WIN, one item a request) where a request
+// would have been cut in two workgroups of four, or in few short ones: no partials and
+// no merge.
+template <typename MT, int KVT, int D, bool PAIR = false, bool WIN = false, int NW = 4>
+__global__ __launch_bounds__(64 * NW, decode_waves(KVT, D, WIN)) void decode_kernel(DecodeParams p) {
   static_assert(!PAIR || D == 256, "paired kv-heads form 256-element rows");
   constexpr bool FP8 = KVT == kKvFp8, MX = KVT == kKvMx8 || KVT == kKvMx4;
   constexpr int KS = D / 32;  // MFMA k-steps over head_dim for S
@@ -151,10 +154,10 @@ __global__ __launch_bounds__(256, decode_waves(KVT, D, WIN)) void decode_kernel(
   // LDS: during the tile loop, per-wave K staging (rows arrive as whole
   // head_dim rows and leave as MFMA A fragments); after it, the 4 waves'
   // softmax states for the in-workgroup merge.
-  constexpr int kStageBytes = 4 * 16 * KRS;
-  constexpr int kMergeBytes = 4 * (4 * NS * 64 * 16);
+  constexpr int kStageBytes = NW * 16 * KRS;
+  constexpr int kMergeBytes = NW * (4 * NS * 64 * 16);
   __shared__ __attribute__((aligned(16))) uint8_t lds[kStageBytes > kMergeBytes ? kStageBytes : kMergeBytes];
-  __shared__ float lds_m[4][kRows], lds_l[4][kRows];
+  __shared__ float lds_m[NW][kRows], lds_l[NW][kRows];
 
   const int lane = lane_id();
   const int wave = uniform((int)threadIdx.x >> 6);
@@ -171,7 +174,8 @@ __global__ __launch_bounds__(256, decode_waves(KVT, D, WIN)) void decode_kernel(
     if (item >= p.batch * p.splits) return;
     kidx = item / p.batch;
     b = item - kidx * p.batch;
-    if (p.sorted) b = win_item(p, b);
+    if constexpr (NW == 4)
+      if (p.sorted) b = win_item(p, b);
   } else {
     if (item >= p.hdr[kHdrChunks]) return;  // uniform across the workgroup
     const int4 wk = p.work[item];
@@ -205,8 +209,8 @@ __global__ __launch_bounds__(256, decode_waves(KVT, D, WIN)) void decode_kernel(
     const int item_tok1 = min(pg1 * ps, kv_len);
     item_tiles = item_tok1 > item_tok0 ? (item_tok1 - item_tok0 + 15) >> 4 : 0;
   }
-  // this wave's contiguous quarter of the item's tiles
-  const int tq = item_tiles >> 2, trem = item_tiles & 3;
+  // this wave's contiguous share of the item's tiles
+  const int tq = item_tiles / NW, trem = item_tiles % NW;
   const int my_t0 = wave * tq + min(wave, trem);
   const int ntiles = tq + (wave < trem ? 1 : 0);
   const int tok_begin = item_tok0 + 16 * my_t0;
@@ -468,10 +472,10 @@ __global__ __launch_bounds__(256, decode_waves(KVT, D, WIN)) void decode_kernel(
     run_tiles(tok_begin, ntiles);
   }
 
-  // ---- epilogue: merge the 4 waves' states (m, l, acc) in LDS.  The acc
+  // ---- epilogue: merge the waves' states (m, l, acc) in LDS.  The acc
   // register layout is the same in every wave (lane -> row col, elements
-  // d = VW*(4*grp + r) + j), so the merge is lane-local; wave w finishes the
-  // elements with r == w.
+  // d = VW*(4*grp + r) + j), so the merge is lane-local; wave w < 4 finishes
+  // the elements with r == w.
   __syncthreads();  // all waves are done with their K staging buffers
   {
     const float l_row = rows4_sum(l_run);
@@ -487,13 +491,14 @@ __global__ __launch_bounds__(256, decode_waves(KVT, D, WIN)) void decode_kernel(
         st[(r * NS + j / 4) * 64] = make_float4(acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]);
   }
   __syncthreads();
+  if (NW > 4 && wave >= 4) return;
   float M = kNegInf;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, lds_m[w][col]);
+  for (int w = 0; w < NW; ++w) M = fmaxf(M, lds_m[w][col]);
   const float M_use = M == kNegInf ? 0.f : M;
-  float sc[4], L = 0.f;
+  float sc[NW], L = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < NW; ++w) {
     sc[w] = fast_exp2(lds_m[w][col] - M_use);  // m = -inf -> 0
     L += sc[w] * lds_l[w][col];
   }
@@ -501,7 +506,7 @@ __global__ __launch_bounds__(256, decode_waves(KVT, D, WIN)) void decode_kernel(
 #pragma unroll
   for (int i = 0; i < NS; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < NW; ++w) {
     const float4* src = (const float4*)lds + (size_t)w * 4 * NS * 64 + (size_t)wave * NS * 64 + lane;
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
@@ -550,12 +555,18 @@ __global__ __launch_bounds__(256, decode_waves(KVT, D, WIN)) void decode_kernel(
 }
 
 // One launch of the kernel (grid: blocks of 8 items x kv-heads).
-template <typename MT, int KVT, bool WIN>
+template <typename MT, int KVT, bool WIN, int NW = 4>
 static int launch_decode_kernel(const DecodeParams& dp, int head_dim, int grid, hipStream_t stream) {
+  const dim3 g(grid), block(64 * NW);
   switch (head_dim) {
-    case 64: hipLaunchKernelGGL((decode_kernel<MT, KVT, 64, false, WIN>), dim3(grid), dim3(256), 0, stream, dp); break;
-    case 128: hipLaunchKernelGGL((decode_kernel<MT, KVT, 128, false, WIN>), dim3(grid), dim3(256), 0, stream, dp); break;
-    case 256: hipLaunchKernelGGL((decode_kernel<MT, KVT, 256, false, WIN>), dim3(grid), dim3(256), 0, stream, dp); break;
+    case 64: hipLaunchKernelGGL((decode_kernel<MT, KVT, 64, false, WIN, NW>), g, block, 0, stream, dp); break;
+    case 128: hipLaunchKernelGGL((decode_kernel<MT, KVT, 128, false, WIN, NW>), g, block, 0, stream, dp); break;
+    case 256:
+      if constexpr (NW == 4 || decode_waves(KVT, 256, WIN) == 2) {
+        hipLaunchKernelGGL((decode_kernel<MT, KVT, 256, false, WIN, NW>), g, block, 0, stream, dp);
+        break;
+      }
+      return MI_ERR_UNSUPPORTED;
     default: return MI_ERR_UNSUPPORTED;
   }
   return MI_OK;

@@ -217,6 +217,10 @@ int f32_attend_launch(const DecodeParams& dp, int head_dim, int grid, hipStream_
 // Windowed and microscaled runs (mi_decode_win.hip, mi_decode_mx.hip): the attend
 // kernel, and the merge of a windowed run's items.
 int decode_win_launch(const DecodeParams& dp, int q_dtype, int kvt, int head_dim, bool pair, int grid, hipStream_t stream);
+// The same by workgroups of eight wavefronts, one item a request, for the formats and
+// head_dims whose registers allow it.
+bool decode_win8_serves(int kvt, int head_dim);
+int decode_win8_launch(const DecodeParams& dp, int q_dtype, int kvt, int head_dim, int grid, hipStream_t stream);
 int decode_win_merge_launch(const DecodeParams& dp, int q_dtype, int kvt, int head_dim, bool pair, int batch,
                             hipStream_t stream);
 int decode_mx_launch(const DecodeParams& dp, int q_dtype, int kvt, int head_dim, int grid, hipStream_t stream);

@@ -302,6 +302,19 @@ def test_window_wider_than_every_context(gpu, batch):
         H.check(p, q, [1] * batch, out, -1, 0, True, "wide window")
 
 
+@pytest.mark.parametrize("kind,hkv,d", [("bf16", 4, 128), ("mx4", 2, 256), ("bf16", 2, 256), ("mx8", 4, 64), ("fp8", 2, 128)])
+@pytest.mark.parametrize("batch,wl,sinks", [(1, 2100, 3), (1, 300, 20), (3, 640, 0), (45, 900, 40), (100, 900, 0), (60, 33, 5)])
+def test_cut_and_whole_requests(gpu, kind, hkv, d, batch, wl, sinks):
+    """Requests in many items, in few, and whole to one workgroup of four or of eight wavefronts."""
+    r = np.random.default_rng(batch + wl)
+    lens = r.integers(1, 2600 if batch < 10 else 1200, batch).tolist()
+    p = H.make(gpu, kind, lens, 16, hkv, d, seed=wl)
+    q = torch.randn(batch, 4 * hkv, d, generator=torch.Generator().manual_seed(wl)).to(torch.bfloat16)
+    w = PagedDecodeWrapper(workspace(gpu, 64 << 20), 4 * hkv, hkv, d, 16, device=gpu)
+    w.plan(*p.index())
+    H.check(p, q, [1] * batch, w.run(q.to(gpu), p.layer, *p.scales, window_left=wl, sink_tokens=sinks), wl, sinks, True, kind)
+
+
 def test_read_from_pages_behind_others(gpu):
     """A list whose first request begins behind entries of none: those are not read; pages past the pool leave their rows."""
     p = H.make(gpu, "mx4", [40, 70], 16, 2, 64, seed=12)
