@@ -315,6 +315,22 @@ def test_cut_and_whole_requests(gpu, kind, hkv, d, batch, wl, sinks):
     H.check(p, q, [1] * batch, w.run(q.to(gpu), p.layer, *p.scales, window_left=wl, sink_tokens=sinks), wl, sinks, True, kind)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(16, 2, 128), (8, 1, 256), (4, 4, 64)])
+@pytest.mark.parametrize("wl,sinks", [(0, 0), (128, 4), (150, 32), (200, 0), (320, 0), (380, 0), (400, 33), (440, 0), (470, 0), (520, 64)])
+def test_short_windows_of_cut_tiles(gpu, hq, hkv, d, wl, sinks):
+    """Tiles that the plan cut for all their keys, behind windows that leave pieces to share them or do not."""
+    new, lens = [290, 37], [6000, 2600]
+    p = H.make(gpu, "bf16", lens, 16, hkv, d, seed=wl)
+    H.hide(p, new, wl, sinks)
+    q = torch.randn(sum(new), hq, d, generator=torch.Generator().manual_seed(wl)).to(torch.bfloat16)
+    w = PagedPrefillWrapper(workspace(gpu, 128 << 20), hq, hkv, d, 16, device=gpu)
+    for causal in (True, False):
+        w.plan(torch.tensor([0, 290, 327], dtype=torch.int32), *p.index(), causal=causal)
+        out = torch.full((sum(new), hq, d), 5.0, dtype=torch.bfloat16, device=gpu)
+        w.run(q.to(gpu), p.layer, out=out, window_left=wl, sink_tokens=sinks)
+        H.check(p, q, new, out, wl, sinks, causal, f"causal {causal}")
+
+
 def test_read_from_pages_behind_others(gpu):
     """A list whose first request begins behind entries of none: those are not read; pages past the pool leave their rows."""
     p = H.make(gpu, "mx4", [40, 70], 16, 2, 64, seed=12)
