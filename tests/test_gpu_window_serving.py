@@ -315,6 +315,17 @@ def test_cut_and_whole_requests(gpu, kind, hkv, d, batch, wl, sinks):
     H.check(p, q, [1] * batch, w.run(q.to(gpu), p.layer, *p.scales, window_left=wl, sink_tokens=sinks), wl, sinks, True, kind)
 
 
+@pytest.mark.parametrize("wl,sinks", [(100, 0), (700, 20)])
+def test_paired_heads_cut_in_two(gpu, wl, sinks):
+    """One kv-head pair a request: its window is cut in two items of the pair, which are merged."""
+    lens = np.random.default_rng(wl).integers(1, 1200, 128).tolist()
+    p = H.make(gpu, "bf16", lens, 16, 2, 128, seed=wl)
+    q = torch.randn(128, 14, 128, generator=torch.Generator().manual_seed(wl)).to(torch.bfloat16)
+    w = PagedDecodeWrapper(workspace(gpu, 64 << 20), 14, 2, 128, 16, device=gpu)
+    w.plan(*p.index())
+    H.check(p, q, [1] * 128, w.run(q.to(gpu), p.layer, window_left=wl, sink_tokens=sinks), wl, sinks, True, "pair")
+
+
 @pytest.mark.parametrize("hq,hkv,d", [(16, 2, 128), (8, 1, 256), (4, 4, 64)])
 @pytest.mark.parametrize("wl,sinks", [(0, 0), (128, 4), (150, 32), (200, 0), (320, 0), (380, 0), (400, 33), (440, 0), (470, 0), (520, 64)])
 def test_short_windows_of_cut_tiles(gpu, hq, hkv, d, wl, sinks):
