@@ -202,8 +202,8 @@ __global__ __launch_bounds__(64 * NW, decode_waves(KVT, D, WIN)) void decode_ker
     nitems_b = span.items;
     if (kidx >= nitems_b) return;
     pg1 = np;
-    first_tile = kidx * span.total / nitems_b;
-    item_tiles = (kidx + 1) * span.total / nitems_b - first_tile;
+    first_tile = share_begin(kidx, nitems_b, span.total);
+    item_tiles = share_begin(kidx + 1, nitems_b, span.total) - first_tile;
   } else {
     item_tok0 = pg0 * ps;
     const int item_tok1 = min(pg1 * ps, kv_len);

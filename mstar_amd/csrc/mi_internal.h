@@ -186,6 +186,13 @@ struct DecodeParams {
   int32_t window_left = -1, sinks = 0, splits = 0, batch = 0, sorted = 0;
 };
 
+// Where the k-th of n even shares of `total` begins, k * total / n for k <= n, without
+// forming the product, which passes 2^31 where a long request is cut in many.
+__host__ __device__ inline int share_begin(int k, int n, int total) {
+  const int q = total / n;
+  return k * q + k * (total - n * q) / n;
+}
+
 // The 16-token tiles of a windowed request: those that hold sinks, then those
 // from `first` on to the end of its keys, one sequence of `total` tiles that
 // `items` items share evenly: as many as there are places, however much shorter than

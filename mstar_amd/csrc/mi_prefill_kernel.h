@@ -330,7 +330,7 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
   // WIN: the step from which V rows may lie past kv_len
   const int t_tail = WIN ? win.step_of(kv_len) : 0;
   // key steps of this unit: all of the tile's, or its piece's share
-  const int kt0 = un.n > 1 ? un.k * n_kt / un.n : 0, kt1 = un.n > 1 ? (un.k + 1) * n_kt / un.n : n_kt;
+  const int kt0 = un.n > 1 ? share_begin(un.k, un.n, n_kt) : 0, kt1 = un.n > 1 ? share_begin(un.k + 1, un.n, n_kt) : n_kt;
   if (un.n == 0) continue;  // uniform; no wait for the unit's entry ahead of the loads above
 
   float kscale = 1.f, vscale = 1.f;

@@ -170,7 +170,7 @@ __global__ __launch_bounds__(512) void prefill_rs_kernel(PrefillParams p) {
       auto key_of = [&](int t) { return WIN ? win.key(t) : t * KEYS; };
       const int t_tail = WIN ? win.step_of(kv_len) : 0;
       // key steps of this unit: all of the tile's, or its piece's share
-      const int kt0 = un.n > 1 ? un.k * n_kt / un.n : 0, kt1 = un.n > 1 ? (un.k + 1) * n_kt / un.n : n_kt;
+      const int kt0 = un.n > 1 ? share_begin(un.k, un.n, n_kt) : 0, kt1 = un.n > 1 ? share_begin(un.k + 1, un.n, n_kt) : n_kt;
       // the page table of the unit's tiles (CAP of them at a time)
       const int key_cap = np * ps - 16;
       const int64_t page_bytes = p.page_stride * ESZ, tok_bytes = p.token_stride * ESZ;
