@@ -202,9 +202,15 @@ def _check_devices(dev: torch.device, **tensors) -> None:
             raise ValueError(f"{name} must be on {dev}, not on {t.device}")
 
 
-def _check_out(out: torch.Tensor, n: int, heads: int, dim: int, q: torch.Tensor) -> None:
-    if out.shape[0] < n or out.shape[1:] != (heads, dim) or out.dtype != q.dtype or out.device != q.device:
-        raise ValueError(f"out must hold {n} rows of {(heads, dim)} in {q.dtype} on {q.device}, got {tuple(out.shape)}, {out.dtype}")
+def _out_strides(out: torch.Tensor, n: int, heads: int, dim: int, q: torch.Tensor, exact: bool) -> tuple[int, int]:
+    """Strides of an ``out`` that takes n rows like q's; ``exact``: it has no more heads or elements a head than q."""
+    strides = _q_strides(out, "out")
+    rows, h, d = out.shape
+    fits = rows >= n and ((h, d) == (heads, dim) if exact else h >= heads and d >= dim)
+    if not fits or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError(f"out must hold {n} rows of {(heads, dim)} in {q.dtype} on {q.device}, got {tuple(out.shape)}, "
+                         f"{out.dtype} on {out.device}")
+    return strides
 
 
 def _as_device_int(t: torch.Tensor, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
@@ -502,7 +508,9 @@ class PagedDecodeWrapper(_FusedRopeAppend, _PlanArrays):
         if len(shape) != 3 or shape[0] < n or shape[1] != heads or shape[2] != dim:
             raise ValueError(f"q shape {tuple(shape)} does not match the plan")
         q, q_at, q_st, q_sh = _rows(q)
-        if window_left >= 0 or isinstance(kv_cache_layer, MXKVLayer):
+        windowed = _window(window_left, sink_tokens, q.dtype)
+        extension = windowed or isinstance(kv_cache_layer, MXKVLayer)
+        if extension:
             _check_devices(self.device, q=q, kv_cache_layer=kv_cache_layer)
         desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
         if desc.num_kv_heads != self.num_kv_heads or desc.head_dim != dim or desc.page_size != self.page_size:
@@ -511,13 +519,12 @@ class PagedDecodeWrapper(_FusedRopeAppend, _PlanArrays):
             out = torch.empty(shape, dtype=q.dtype, device=q.device)
             o_st, o_sh = heads * dim, dim
         else:
-            o_st, o_sh = _q_strides(out, "out")
+            o_st, o_sh = _out_strides(out, n, heads, dim, q, extension)
         ws = self._workspace
         tail = (ws.data_ptr(), ws.numel() * ws.element_size(), out.data_ptr(), o_st, o_sh, self._reading_stream())
         args = (q_at, _lib.TORCH_TO_MI[q.dtype], q_st, q_sh, desc, None, self._indptr.data_ptr(),
                 self._indices.data_ptr(), self._last.data_ptr(), n, heads, 0, self._sm_scale)
-        if _window(window_left, sink_tokens, q.dtype):
-            _check_out(out, n, heads, dim, q)
+        if windowed:
             _lib.check(_lib.lib().mi_decode_run_window(*args, min(window_left, _WINDOW_MAX), min(sink_tokens, _WINDOW_MAX),
                                                        *tail), "mi_decode_run_window")
         else:
@@ -590,6 +597,7 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
             self.token_to_page = None
             self.token_to_cache = None
         self._total_tokens = 0
+        self._counted_tokens = 0  # as read from qo_indptr: 0 where the caller stated the count
 
     def plan(
         self,
@@ -609,6 +617,7 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
         on_cpu = all(t.is_cpu for t in srcs)
         total_tokens = int(qo_indptr.numpy()[-1]) if on_cpu else int(qo_indptr[-1].item())
         self._plan(qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, total_tokens, causal, dtype)
+        self._counted_tokens = total_tokens
 
     def plan_device(self, qo_indptr: torch.Tensor, paged_kv_indptr: torch.Tensor, paged_kv_indices: torch.Tensor,
                     paged_kv_last_page_len: torch.Tensor, total_tokens: int, causal: bool = True,
@@ -626,7 +635,7 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
         self.causal = bool(causal)
         srcs = [qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len]
         on_cpu = all(t.is_cpu for t in srcs)
-        self._total_tokens = total_tokens
+        self._total_tokens, self._counted_tokens = total_tokens, 0
         if self.use_cuda_graph:
             if n_req != self.batch_size:  # captured launches bake the batch in
                 raise ValueError(f"CUDA-graph mode plans a fixed batch of {self.batch_size}, got {n_req}")
@@ -711,8 +720,13 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
         if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
             raise ValueError(f"q shape {tuple(shape)} does not match the wrapper")
         q, q_at, q_st, q_sh = _rows(q)
-        if window_left >= 0 or isinstance(kv_cache_layer, MXKVLayer):
+        windowed = _window(window_left, sink_tokens, q.dtype)
+        extension = windowed or isinstance(kv_cache_layer, MXKVLayer)
+        if extension:
             _check_devices(self.device, q=q, kv_cache_layer=kv_cache_layer)
+        tokens = self._total_tokens if extension else self._counted_tokens
+        if shape[0] < tokens:
+            raise ValueError(f"q holds {shape[0]} tokens, {tokens} planned")
         desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
         if desc.num_kv_heads != self.num_kv_heads or desc.head_dim != dim or desc.page_size != self.page_size:
             raise ValueError("kv_cache_layer geometry does not match the wrapper")
@@ -720,7 +734,7 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
             out = torch.empty(shape, dtype=q.dtype, device=q.device)
             o_st, o_sh = heads * dim, dim
         else:
-            o_st, o_sh = _q_strides(out, "out")
+            o_st, o_sh = _out_strides(out, tokens, heads, dim, q, extension)
         ws = self._workspace
         args = [q_at, _lib.TORCH_TO_MI[q.dtype], q_st, q_sh, desc, self._qo.data_ptr(),
                 self._indptr.data_ptr(), self._indices.data_ptr(), self._last.data_ptr(), self._plan_batch,
@@ -734,10 +748,7 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
         launch = _lib.lib()
         run, short, tiles = launch.mi_prefill_run, launch.mi_prefill_short, launch.mi_prefill_tiles
         serial = self._serial
-        if _window(window_left, sink_tokens, q.dtype):
-            _check_out(out, self._total_tokens, heads, dim, q)
-            if shape[0] < self._total_tokens:
-                raise ValueError(f"q holds {shape[0]} tokens, {self._total_tokens} planned")
+        if windowed:
             window = (min(window_left, _WINDOW_MAX), min(sink_tokens, _WINDOW_MAX))
             run, short, tiles = (lambda *a, p=p: launch.mi_prefill_run_window(*a[:14], *window, p, *a[14:]) for p in (3, 1, 2))
             spans = self._n_req * (window[0] + window[1]) * self.num_kv_heads * dim * _KV_BITS[desc.dtype] // 4  # K and V
