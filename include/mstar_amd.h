@@ -287,8 +287,8 @@ int mi_kv_append(const mi_paged_kv* kv, const void* k, const void* v, int32_t sr
  * kv_len_r = (npages_r - 1) * page_size + last_page_len[r] (0 without pages) and
  * t0_r the sum of kv_len over the requests before r,
  *   k_out[t0_r + i] = K row i of request r, v_out likewise, as out_dtype
- * (MI_BF16, MI_F16 or MI_F32, rounded to nearest even; the cache's own 16-bit dtype
- * is copied).  k_out, v_out: contiguous [out_tokens, num_kv_heads, head_dim],
+ * (MI_BF16, MI_F16 or MI_F32, rounded to nearest even; microscaled values past fp16's
+ * range as its largest, +-65504; the cache's own 16-bit dtype is copied).  k_out, v_out: contiguous [out_tokens, num_kv_heads, head_dim],
  * 16-byte aligned; rows from the last request's end on, or beyond out_tokens, are not
  * written, nor those of pages outside [0, max_pages).  num_indices: elements of
  * kv_indices.  Replaces the reference's gathers of a request's pages by torch

@@ -141,7 +141,7 @@ MI_DEVICE uint32_t fp8x2_to_mt<F16>(uint32_t w, bool hi) {
 // (2^(s - 127); 255: the block is NaN); e4m3fn codes (MI_MXFP8) or e2m1 codes
 // (MI_MXFP4, the even element in the low four bits).  The conversions apply the
 // scale: exact in bf16 above its subnormal range, rounded to nearest even in
-// fp16 and below.
+// fp16 (past its range: f16_saturate) and below.
 enum : int { kKv16 = 0, kKvFp8 = 1, kKvMx8 = 2, kKvMx4 = 3 };  // KV formats of the attention kernels
 constexpr int kMxBlock = 32;
 
@@ -187,6 +187,29 @@ MI_DEVICE void mx_to_mt(const uint32_t (&w)[N], float scale, uint32_t (&out)[M])
         }
       }
     }
+  }
+}
+
+// fp16 ends at 65504, and the conversions give infinities from 65520 on, also for codes
+// that finite fp16 values were rounded to (65504 itself becomes 256 * 2^8 or 4 * 2^14).  Values
+// past the range are read as its largest instead: blocks whose scale allows such
+// codes are rare, so the kernels look at the scale bytes and correct behind one branch
+// a tile (fp16 runs: 4 bits, 256 requests of 1k-32k 309 -> 310 us, 96 windows of 4k at
+// head_dim 256 48.5 -> 49.5, 4 chunks over 7k 442 -> 446; a branch a chunk cost 6 %).
+// Whether one of the scale bytes of a word lets a code pass 65504.
+template <int KVT>
+MI_DEVICE bool mx_past_f16(uint32_t scales) {
+  constexpr uint32_t kLeast = 127 + (KVT == kKvMx8 ? 8 : 14);  // bytes from here on
+  constexpr uint32_t kAdd = 0x01010101u * (256 - kLeast);      // sets a byte's top bit if its low seven bits reach kLeast - 128
+  return (((scales & 0x7f7f7f7fu) + kAdd) & scales & 0x80808080u) != 0;
+}
+// Infinities of fp16 pairs -> the largest finite value of their sign; NaNs stay.
+template <int N>
+MI_DEVICE void f16_saturate(uint32_t (&w)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t differs = ((w[i] ^ 0x7c007c00u) & 0x7fff7fffu) + 0x7fff7fffu;  // top bit of a half: it is not an infinity
+    w[i] -= (~differs & 0x80008000u) >> 15;
   }
 }
 

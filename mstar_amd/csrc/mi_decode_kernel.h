@@ -143,7 +143,7 @@ constexpr int decode_waves(int kvt, int d, bool win) {
 template <typename MT, int KVT, int D, bool PAIR = false, bool WIN = false, int NW = 4>
 __global__ __launch_bounds__(64 * NW, decode_waves(KVT, D, WIN)) void decode_kernel(DecodeParams p) {
   static_assert(!PAIR || D == 256, "paired kv-heads form 256-element rows");
-  constexpr bool FP8 = KVT == kKvFp8, MX = KVT == kKvMx8 || KVT == kKvMx4;
+  constexpr bool FP8 = KVT == kKvFp8, MX = KVT == kKvMx8 || KVT == kKvMx4, F16_MX = MX && MT::kDtype == MI_F16;
   constexpr int KS = D / 32;  // MFMA k-steps over head_dim for S
   constexpr int VW = D / 16;  // V elements per lane per row == output d-tiles
   constexpr int ESZ = KVT == kKv16 ? 2 : 1;  // of the strides (bytes of codes for microscaled caches)
@@ -301,6 +301,7 @@ __global__ __launch_bounds__(64 * NW, decode_waves(KVT, D, WIN)) void decode_ker
   float m_run = kNegInf, l_run = 0.f;
 
   auto compute_tile = [&](TileRegs<KVT, D>& t, TileScales& sc, int tb) {
+    const bool past = F16_MX && __builtin_amdgcn_ballot_w64(mx_past_f16<KVT>(sc.k) || mx_past_f16<KVT>(sc.v));
     // ---- K rows -> LDS (row 4*grp + r, elements [VW*col, +VW)) -> A fragments
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -324,6 +325,28 @@ __global__ __launch_bounds__(64 * NW, decode_waves(KVT, D, WIN)) void decode_ker
 #pragma unroll
         for (int i = 0; i < VW / 2; i += 4)
           *(uint4*)(dst + 2 * dim_of(RUN, col, 2 * i)) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+      }
+    }
+    if constexpr (F16_MX) {  // a lane corrects the elements that it stored itself
+      if (past) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          uint8_t* row = kst + (4 * grp + r) * KRS;
+          if constexpr (VW == 4) {
+            uint2* at = (uint2*)(row + 2 * dim_of(RUN, col, 0));
+            uint32_t w[2] = {at->x, at->y};
+            f16_saturate(w);
+            *at = make_uint2(w[0], w[1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VW / 2; i += 4) {
+              uint4* at = (uint4*)(row + 2 * dim_of(RUN, col, 2 * i));
+              uint32_t w[4] = {at->x, at->y, at->z, at->w};
+              f16_saturate(w);
+              *at = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
       }
     }
     // ---- S^T = K . Q^T  (A fragment: row col, elements 8*grp + 32*st .. +8)
@@ -404,6 +427,12 @@ __global__ __launch_bounds__(64 * NW, decode_waves(KVT, D, WIN)) void decode_ker
       } else {
 #pragma unroll
         for (int i = 0; i < VW / 2; ++i) vv[r][i] = t.v[r][i];
+      }
+    }
+    if constexpr (F16_MX) {
+      if (past) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f16_saturate(vv[r]);
       }
     }
 #pragma unroll

@@ -9,8 +9,8 @@
 // quarter, of a).  Codes are RNE(x 2^-e), formed by the hardware's scaled
 // conversions.  e is held to at least -126 and at most 119 (e4m3) or 125 (e2m1), the
 // highest at which every code is a finite float: a finite row reads as finite
-// values, the largest magnitudes of its type as the largest code.  Blocks of zeros
-// have e = 0.  A block with a NaN or an infinity has scale byte 255 and reads as NaN
+// values, the largest magnitudes of its type as the largest code, and as fp16's
+// largest value what is past it (f16_saturate).  Blocks of zeros have e = 0.  A block with a NaN or an infinity has scale byte 255 and reads as NaN
 // throughout.
 #include <type_traits>
 
@@ -217,7 +217,10 @@ MI_DEVICE void row8_store(const Row8<CACHE>& r, void* out, int64_t oo) {
   constexpr bool MX = CACHE == MI_MXFP8 || CACHE == MI_MXFP4;
   if constexpr (MX && OUT != MI_F32) {
     uint32_t o[4];
-    mx_to_mt<std::conditional_t<OUT == MI_BF16, BF16, F16>, CACHE == MI_MXFP8 ? kKvMx8 : kKvMx4>(r.w, r.scale, o);
+    constexpr int KVT = CACHE == MI_MXFP8 ? kKvMx8 : kKvMx4;
+    mx_to_mt<std::conditional_t<OUT == MI_BF16, BF16, F16>, KVT>(r.w, r.scale, o);
+    if constexpr (OUT == MI_F16)
+      if (mx_past_f16<KVT>(bitcast<uint32_t>(r.scale) >> 23)) f16_saturate(o);
     stream16((uint16_t*)out + oo, make_uint4(o[0], o[1], o[2], o[3]));
   } else if constexpr (CACHE == OUT && OUT != MI_F32) {  // bit patterns kept
     stream16((uint16_t*)out + oo, make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]));

@@ -406,15 +406,19 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
   };
   // TAIL: the tile may reach past kv_len (only the request's last tile can),
   // so its V rows past the end are overwritten with zeros
+  auto chunk_at = [&](int c, int stage) {
+    const int half = c / HALF, rem = c - half * HALF;
+    const int row = rem / CPR, ch = rem - row * CPR;
+    return lds + stage * STAGE + (half ? KEYS * RSK + row * RSV : row * RSK) + LCH * ch;
+  };
   auto store_tile_impl = [&](int t, const uint4 (&r)[NL], const uint8_t (&rs)[NL], int stage, auto tail) {
+    uint32_t past = 0;  // the chunks' scale bytes (fp16: mx_past_f16)
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int c = tid + i * THREADS;
       if (2 * HALF % THREADS == 0 || c < 2 * HALF) {
-        const int half = c / HALF, rem = c - half * HALF;
-        const int row = rem / CPR, ch = rem - row * CPR;
         const uint4 v = r[i];
-        uint8_t* dst = lds + stage * STAGE + (half ? KEYS * RSK + row * RSV : row * RSK) + LCH * ch;
+        uint8_t* dst = chunk_at(c, stage);
         if constexpr (FP8) {  // 16 fp8 -> 16 MFMA-type elements (32 bytes)
           const uint32_t w[4] = {v.x, v.y, v.z, v.w};
           uint32_t o[8];
@@ -429,6 +433,7 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
           const uint32_t w[4] = {v.x, v.y, v.z, v.w};
           uint32_t o[LCH / 4];
           mx_to_mt<MT, KVT>(w, mx_scale(rs[i], 0), o);
+          past |= (uint32_t)rs[i] << (8 * i);
 #pragma unroll
           for (int k = 0; k < LCH / 16; ++k)
             *(uint4*)(dst + 16 * k) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
@@ -442,6 +447,24 @@ __global__ __launch_bounds__(64 * pf_waves(D)) void prefill_kernel(PrefillParams
           if (l_v[i] && (key >= kv_len || (WIN && key < win.lo && key >= p.sinks))) {
 #pragma unroll
             for (int k = 0; k < LCH / 16; ++k) *(uint4*)(dst + 16 * k) = make_uint4(0, 0, 0, 0);
+          }
+        }
+      }
+    }
+    if constexpr (MX && MT::kDtype == MI_F16) {  // one branch a tile: a thread corrects what it stored itself
+      static_assert(NL <= 4, "the chunks' scale bytes are one word");
+      if (__builtin_amdgcn_ballot_w64(mx_past_f16<KVT>(past))) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const int c = tid + i * THREADS;
+          if (2 * HALF % THREADS == 0 || c < 2 * HALF) {
+            uint4* at = (uint4*)chunk_at(c, stage);
+#pragma unroll
+            for (int k = 0; k < LCH / 16; ++k) {
+              uint32_t w[4] = {at[k].x, at[k].y, at[k].z, at[k].w};
+              f16_saturate(w);
+              at[k] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
         }
       }

@@ -133,7 +133,7 @@ def read_kv_cache(kv_cache_layer: torch.Tensor | MXKVLayer, kv_indptr: torch.Ten
     layer's device).  ``total_tokens``, the sum of the requests' lengths, is the caller's
     knowledge (nothing is read back); rows beyond the batch's own are left as they were,
     and so are rows beyond ``total_tokens``.  Values come in ``dtype`` (bf16, fp16 or
-    fp32), rounded to nearest.  ``out``: contiguous tensors to write instead of new ones.
+    fp32), rounded to nearest; microscaled values past fp16's range are ±65504.  ``out``: contiguous tensors to write instead of new ones.
     Reads 16-bit, fp32, fp8 (with its per-head ``k_scale`` / ``v_scale``) and microscaled
     layers.
     """
