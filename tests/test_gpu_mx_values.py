@@ -1,6 +1,7 @@
-"""GPU: what microscaled codes are read as, over every code and scale.
+"""GPU: what microscaled codes are read as, over every code and scale, and blocks that are hard to quantise.
 
 * every (code, scale byte) pair of both formats, in every output type of the read;
+* ties between codes and the limits of a block's scale, at every head_dim, each of them counted;
 * magnitudes at the top of fp16's range, whose nearest codes lie past it: read back and attended
   to in fp16 as its largest value, by every kernel.
 """
@@ -52,6 +53,50 @@ def test_every_code_under_every_scale(gpu, bits, dtype):
     got = read_kv_cache(layer, *idx, n, dtype)
     for which, x in enumerate(got):
         assert _same(x, _as(M.values(kv[0][which], kv[1][which], bits), dtype)), ("K", "V")[which]
+
+
+def _ties(bits: int) -> torch.Tensor:
+    """Every code's value, every midpoint between two and the block's limits, of both signs, in 64 bits."""
+    grid, lim = (M.E4M3[:127] if bits == 8 else M.E2M1[:8]), M.LIMIT[bits]
+    t = torch.cat([grid, (grid[1:] + grid[:-1]) / 2, torch.tensor([lim, lim * (1 + 2 ** -7), lim * (1 - 2 ** -7)], dtype=torch.float64)])
+    return torch.cat([t, -t])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_append_ties_and_limits(gpu, bits, d, dtype):
+    """Each value beside the largest code, so that its block's scale is 1, and the same blocks 2^-9 as large."""
+    ties = _ties(bits)
+    ties = ties.to(dtype).double().unique()  # what the source type holds of them
+    per = 31 * (2 * d // 32)
+    n = -(-len(ties) // per)
+    flat = torch.zeros(n * per, dtype=torch.float64)
+    flat[: len(ties)] = ties
+    x = torch.empty(n * 2 * d // 32, 32, dtype=torch.float64)
+    x[:, 0] = M.LIMIT[bits] - (16 if bits == 8 else 1)  # the largest code: 448, 6
+    x[:, 1:] = flat.view(-1, 31)
+    x = torch.cat([x, x * 2.0 ** -9]).view(2 * n, 2, d)
+    k = x.to(dtype)
+    assert (k.double() == x)[:n].all()
+    assert set(ties.tolist()) <= set(k[:n].double().flatten().tolist()), "a value is not among the rows"
+    v = k.flip(0).contiguous()
+    tokens, pages = 2 * n, -(-2 * n // 16)
+    layer = MXKVCache(1, pages, 16, 2, d, bits=bits, device=gpu)[0]
+    idx = torch.tensor([0, pages], dtype=torch.int32), torch.arange(pages, dtype=torch.int32), \
+        torch.tensor([tokens - (pages - 1) * 16], dtype=torch.int32)
+    w = PagedPrefillWrapper(workspace(gpu, 64 << 20), 4, 2, d, 16, device=gpu)
+    w.plan(torch.tensor([0, tokens], dtype=torch.int32), *idx)
+    w.set_kv_cache(layer, k.to(gpu), v.to(gpu))
+    rows, scales = layer.codes.cpu(), layer.scales.cpu()
+    for which, src in enumerate((k, v)):
+        c, s = M.quantize(src, bits)
+        got_c = rows[:, which].flatten(0, 1)[:tokens]
+        got_s = scales[:, which].permute(0, 3, 1, 2).flatten(0, 1)[:tokens]
+        assert torch.equal(got_s, s), "scale bytes differ"
+        a, b = M.unpack(got_c, bits), c
+        bad = (a != b).nonzero()
+        assert len(bad) == 0, f"{len(bad)} codes differ: {src[tuple(bad[0])]} gives {a[tuple(bad[0])]}, not {b[tuple(bad[0])]}"
 
 
 TOP = {8: (63488.0, 63500.0, 65504.0, 61440.0), 4: (57344.0, 57500.0, 60000.0, 65504.0)}
