@@ -217,7 +217,9 @@ int mi_decode_merge(const void* q, int32_t q_dtype, int64_t q_stride_token, int6
  * query at position i of its request (the last of decode's queries: kv_len - 1)
  * sees key t only if t >= i - window_left or t < sink_tokens, besides causal's
  * t <= i; window_left < 0: every key, as mi_decode_run.  A query that sees no
- * key gives zeros.  Reads index arrays and workspace only: the same plan serves
+ * key gives zeros.  The K of a hidden key never counts; the V of a key that other
+ * queries of the request see counts as 0 * V, which is NaN where V is not finite
+ * (chunks: queries of the same tile).  Reads index arrays and workspace only: the same plan serves
  * windowed and full layers of a step.  Pages of which every key is hidden from
  * every query of the request are never read, and their ids may be stale.
  * 16-bit, fp8 and microscaled caches (fp32: MI_ERR_UNSUPPORTED).

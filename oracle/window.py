@@ -19,11 +19,20 @@ def visible(kv_len: int, qo_len: int, window_left: int, sinks: int, causal: bool
     return seen & (t <= i) if causal else seen
 
 
+def _product(w: torch.Tensor, v: torch.Tensor, seen: torch.Tensor) -> torch.Tensor:
+    """sum_t w_jt v_t over the keys that row j sees; the others take no part, also where v is NaN or infinite."""
+    if torch.isfinite(v).all():
+        return w @ v  # w is zero elsewhere
+    return torch.stack([w[j, see] @ v[see] for j, see in enumerate(seen)])
+
+
 def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seen: torch.Tensor,
            out_eps: float) -> tuple[torch.Tensor, torch.Tensor]:
     """(outputs, bound) of q ``[n, Hq, D]`` over k, v ``[kv_len, Hkv, D]``, both in 64 bits.
 
-    Keys that a query does not see take no part, whatever they hold.  ``bound`` is
+    Keys that a query does not see take no part, whatever they hold (the kernels
+    keep to that but for V rows that are not finite: those may make NaN the elements they
+    hold in rows that another row of their tile sees them for).  ``bound`` is
     how far from it a kernel with 32-bit sums and probabilities and outputs rounded
     to a type of half-step ``out_eps`` (``torch.finfo(t).eps / 2``) may be:
 
@@ -55,8 +64,8 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seen: torch.Tensor
         rows = see.any(1)
         w = torch.zeros_like(s)
         w[rows] = torch.softmax(s[rows], -1)
-        out[:, h] = w @ vv
-        a = w @ vv.abs()
-        small = 2.0 ** -24 * (see.double() @ vv.abs()) if out_eps == torch.finfo(torch.float16).eps / 2 else 0.0
+        out[:, h] = _product(w, vv, see)
+        a = _product(w, vv.abs(), see)
+        small = 2.0 ** -24 * _product(see.double(), vv.abs(), see) if out_eps == torch.finfo(torch.float16).eps / 2 else 0.0
         bound[:, h] = out_eps * out[:, h].abs() + (2 * out_eps + 4 * delta + 2.0 ** -16) * a + small
     return out, bound
