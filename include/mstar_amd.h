@@ -52,6 +52,9 @@ extern "C" {
 #define MI_ABI_VERSION 4
 
 /* One layer of the paged KV cache. Strides are in elements (MI_MXFP4: in bytes).
+ * Attention takes pages of at most 2^24 tokens whose token rows span less than 2^32 bytes
+ * (decode; fp32: 16 of them; ragged runs: 2^31, see there), MI_ERR_UNSUPPORTED otherwise,
+ * and requests of up to 2^30 keys.
  * A microscaled layer's scale bytes lie beside the codes, contiguous as
  *   [max_pages][2 (K, V)][num_kv_heads][head_dim / 32][page_size]
  * (the bytes of consecutive tokens adjacent): k_scale and v_scale are the addresses of

@@ -267,6 +267,8 @@ static int dispatch_d(const DecodeParams& dp, int head_dim, int grid, int batch,
   return MI_OK;
 }
 
+constexpr int32_t kPageTokensMax = 1 << 24;
+
 // Windows and sink counts are clamped here: beyond any context, and sums with a length stay in 32 bits.
 constexpr int32_t kWinMax = 1 << 30;
 
@@ -322,6 +324,12 @@ int decode_run_impl(const void* q, int32_t q_dtype, int64_t q_stride_token, int6
   if (!rows_aligned16(q, q_stride_token, q_stride_head, qesz) ||
       !rows_aligned16(out, out_stride_token, out_stride_head, qesz) || !kv_aligned16(kv))
     return MI_ERR_INVALID;
+  // decode_kernel keeps a slot's offset within a page in 32 bits, the fp32 kernel one within
+  // 16 tokens, and both the tokens of 64 pages
+  const int64_t offsets = q_dtype == MI_F32 ? 16 : kv->page_size;
+  if (kv->token_stride < 0 || kv->token_stride >= (1LL << 32) || kv->page_size > kPageTokensMax ||
+      offsets * kv->token_stride * kv_elem_bytes(kv->dtype) >= (1LL << 32))
+    return MI_ERR_UNSUPPORTED;
   // the same pairing decision as the plan's (shapes only), so the layouts agree
   const bool pair = pair_heads(qo_indptr, batch, nkv, num_qo_heads / nkv, D, ragged_pair);
   const SplitLayout L = split_layout(batch, nkv, D, workspace_bytes - ws_offset, pair);
