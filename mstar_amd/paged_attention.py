@@ -249,11 +249,9 @@ def _kv_src(k: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, int]:
     return k, at, st, sh
 
 
-def _append(kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.Tensor, page_idx: torch.Tensor,
-            slot_idx_ptr: int, idx_stride: int, n: int, n_dev_ptr: int | None,
-            k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> None:
-    if n == 0:
-        return
+def _check_append(kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.Tensor, page_idx: torch.Tensor, n: int,
+                  k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> tuple[_lib.MiPagedKV, int]:
+    """(layer descriptor, code of k's type) of an append of n tokens."""
     desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
     if isinstance(kv_cache_layer, MXKVLayer):
         _check_devices(page_idx.device, k=k, v=v, kv_cache_layer=kv_cache_layer)
@@ -265,6 +263,19 @@ def _append(kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.
     src_dt = _lib.TORCH_TO_MI.get(k.dtype)
     if src_dt is None or src_dt == _lib.MI_FP8_E4M3:
         raise ValueError(f"unsupported k/v dtype {k.dtype}")
+    return desc, src_dt
+
+
+def _append(kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.Tensor, page_idx: torch.Tensor,
+            slot_idx_ptr: int, idx_stride: int, n: int, n_dev_ptr: int | None,
+            k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> None:
+    if n:
+        desc, src_dt = _check_append(kv_cache_layer, k, v, page_idx, n, k_scale, v_scale)
+        _launch_append(kv_cache_layer, desc, src_dt, k, v, page_idx, slot_idx_ptr, idx_stride, n, n_dev_ptr)
+
+
+def _launch_append(kv_cache_layer: torch.Tensor | MXKVLayer, desc: _lib.MiPagedKV, src_dt: int, k: torch.Tensor, v: torch.Tensor,
+                   page_idx: torch.Tensor, slot_idx_ptr: int, idx_stride: int, n: int, n_dev_ptr: int | None) -> None:
     if v.dtype != k.dtype:
         v = v.to(k.dtype)
     k, k_at, k_st, k_sh = _kv_src(k, "k")
@@ -283,13 +294,14 @@ def _rope_set_kv_cache(wrapper, kv_cache_layer, q, k, v, pos_ids, rotary_dim, in
     from .rope import apply_llama31_rope_pos_ids_inplace, apply_rope_pos_ids_inplace, rope_append
 
     if isinstance(kv_cache_layer, MXKVLayer):  # a block's scale needs its rotated values: two launches
-        if k_scale is not None or v_scale is not None:
-            raise ValueError("a microscaled KV layer holds its own scales: pass no k_scale or v_scale")
+        page_idx, slot_ptr, idx_stride, n, n_dev = wrapper._append_target()
+        desc, src_dt = _check_append(kv_cache_layer, k, v, page_idx, n, k_scale, v_scale)  # before anything is rotated
         k = k if keep_k else k.clone()
         rotate = apply_llama31_rope_pos_ids_inplace if llama31 else apply_rope_pos_ids_inplace
         rotate(q, k, pos_ids, rotary_dim=rotary_dim, interleave=interleave, rope_scale=rope_scale, rope_theta=rope_theta,
                **(llama31 or {}))
-        wrapper.set_kv_cache(kv_cache_layer, k, v)
+        if n:
+            _launch_append(kv_cache_layer, desc, src_dt, k, v, page_idx, slot_ptr, idx_stride, n, n_dev)
         return
     page_idx, slot_ptr, idx_stride, n, n_dev = wrapper._append_target()
     rope_append(q, k, v, kv_cache_layer, pos_ids, page_idx, slot_ptr, idx_stride, n, n_dev,
