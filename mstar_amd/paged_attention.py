@@ -269,6 +269,7 @@ def _check_append(kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: 
 def _append(kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.Tensor, page_idx: torch.Tensor,
             slot_idx_ptr: int, idx_stride: int, n: int, n_dev_ptr: int | None,
             k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> None:
+<<<<<<< Updated upstream
     if n:
         desc, src_dt = _check_append(kv_cache_layer, k, v, page_idx, n, k_scale, v_scale)
         _launch_append(kv_cache_layer, desc, src_dt, k, v, page_idx, slot_idx_ptr, idx_stride, n, n_dev_ptr)
@@ -276,6 +277,11 @@ def _append(kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.
 
 def _launch_append(kv_cache_layer: torch.Tensor | MXKVLayer, desc: _lib.MiPagedKV, src_dt: int, k: torch.Tensor, v: torch.Tensor,
                    page_idx: torch.Tensor, slot_idx_ptr: int, idx_stride: int, n: int, n_dev_ptr: int | None) -> None:
+=======
+    if n == 0:
+        return
+    desc, src_dt = _check_append(kv_cache_layer, k, v, page_idx, n, k_scale, v_scale)
+>>>>>>> Stashed changes
     if v.dtype != k.dtype:
         v = v.to(k.dtype)
     k, k_at, k_st, k_sh = _kv_src(k, "k")
@@ -294,8 +300,13 @@ def _rope_set_kv_cache(wrapper, kv_cache_layer, q, k, v, pos_ids, rotary_dim, in
     from .rope import apply_llama31_rope_pos_ids_inplace, apply_rope_pos_ids_inplace, rope_append
 
     if isinstance(kv_cache_layer, MXKVLayer):  # a block's scale needs its rotated values: two launches
+<<<<<<< Updated upstream
         page_idx, slot_ptr, idx_stride, n, n_dev = wrapper._append_target()
         desc, src_dt = _check_append(kv_cache_layer, k, v, page_idx, n, k_scale, v_scale)  # before anything is rotated
+=======
+        page_idx, _, _, n, _ = wrapper._append_target()
+        _check_append(kv_cache_layer, k, v, page_idx, n, k_scale, v_scale)  # before anything is rotated
+>>>>>>> Stashed changes
         k = k if keep_k else k.clone()
         rotate = apply_llama31_rope_pos_ids_inplace if llama31 else apply_rope_pos_ids_inplace
         rotate(q, k, pos_ids, rotary_dim=rotary_dim, interleave=interleave, rope_scale=rope_scale, rope_theta=rope_theta,
