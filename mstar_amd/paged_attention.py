@@ -71,7 +71,7 @@ _SERIAL_REQUESTS, _SERIAL_GRAPH_ROWS = 16, 8192
 # six and 120 275 -> 280, 279 -> 281, but window 4096 485 -> 513, 508 -> 514): rows of
 # (token, q-head) and bytes that the windows span from which on the parts fork.
 _WINDOW_FORK_ROWS, _WINDOW_FORK_BYTES = 1 << 17, 3 << 28
-_KV_BITS = {_lib.MI_BF16: 16, _lib.MI_F16: 16, _lib.MI_FP8_E4M3: 8, _lib.MI_MXFP8: 8, _lib.MI_MXFP4: 4}
+_KV_BITS = {_lib.MI_BF16: 16, _lib.MI_F16: 16, _lib.MI_F32: 32, _lib.MI_FP8_E4M3: 8, _lib.MI_MXFP8: 8, _lib.MI_MXFP4: 4}
 
 
 def _check_heads(num_qo_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> None:
@@ -269,7 +269,6 @@ def _check_append(kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: 
 def _append(kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.Tensor, page_idx: torch.Tensor,
             slot_idx_ptr: int, idx_stride: int, n: int, n_dev_ptr: int | None,
             k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> None:
-<<<<<<< Updated upstream
     if n:
         desc, src_dt = _check_append(kv_cache_layer, k, v, page_idx, n, k_scale, v_scale)
         _launch_append(kv_cache_layer, desc, src_dt, k, v, page_idx, slot_idx_ptr, idx_stride, n, n_dev_ptr)
@@ -277,11 +276,6 @@ def _append(kv_cache_layer: torch.Tensor | MXKVLayer, k: torch.Tensor, v: torch.
 
 def _launch_append(kv_cache_layer: torch.Tensor | MXKVLayer, desc: _lib.MiPagedKV, src_dt: int, k: torch.Tensor, v: torch.Tensor,
                    page_idx: torch.Tensor, slot_idx_ptr: int, idx_stride: int, n: int, n_dev_ptr: int | None) -> None:
-=======
-    if n == 0:
-        return
-    desc, src_dt = _check_append(kv_cache_layer, k, v, page_idx, n, k_scale, v_scale)
->>>>>>> Stashed changes
     if v.dtype != k.dtype:
         v = v.to(k.dtype)
     k, k_at, k_st, k_sh = _kv_src(k, "k")
@@ -300,13 +294,8 @@ def _rope_set_kv_cache(wrapper, kv_cache_layer, q, k, v, pos_ids, rotary_dim, in
     from .rope import apply_llama31_rope_pos_ids_inplace, apply_rope_pos_ids_inplace, rope_append
 
     if isinstance(kv_cache_layer, MXKVLayer):  # a block's scale needs its rotated values: two launches
-<<<<<<< Updated upstream
         page_idx, slot_ptr, idx_stride, n, n_dev = wrapper._append_target()
         desc, src_dt = _check_append(kv_cache_layer, k, v, page_idx, n, k_scale, v_scale)  # before anything is rotated
-=======
-        page_idx, _, _, n, _ = wrapper._append_target()
-        _check_append(kv_cache_layer, k, v, page_idx, n, k_scale, v_scale)  # before anything is rotated
->>>>>>> Stashed changes
         k = k if keep_k else k.clone()
         rotate = apply_llama31_rope_pos_ids_inplace if llama31 else apply_rope_pos_ids_inplace
         rotate(q, k, pos_ids, rotary_dim=rotary_dim, interleave=interleave, rope_scale=rope_scale, rope_theta=rope_theta,
