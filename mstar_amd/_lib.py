@@ -442,7 +442,10 @@ def paged_kv_desc(kv_cache_layer: torch.Tensor, k_scale: torch.Tensor | None = N
     if not isinstance(kv_cache_layer, torch.Tensor):
         if k_scale is not None or v_scale is not None:
             raise ValueError("a microscaled KV layer holds its own scales: pass no k_scale or v_scale")
-        return kv_cache_layer.desc
+        desc = getattr(kv_cache_layer, "desc", None)
+        if not isinstance(desc, MiPagedKV):
+            raise ValueError(f"a KV layer is a tensor or an MXKVLayer, not {type(kv_cache_layer).__name__}")
+        return desc
     key = (kv_cache_layer.data_ptr(), kv_cache_layer.shape, kv_cache_layer.stride(), kv_cache_layer.dtype,
            kv_cache_layer.device, _scale_key(k_scale), _scale_key(v_scale))
     d = _desc_cache.get(key)
