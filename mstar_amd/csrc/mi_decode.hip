@@ -280,6 +280,9 @@ constexpr int32_t kWinMax = 1 << 30;
 // no cut paid (256 requests of up to 8256 keys at 4 kv heads, one item 384 us, two to
 // four 384-394 + 4); taking the longest first did (455 -> 384 us), as uncut requests
 // are as uneven as their lengths.
+// n is a floor: one pair more than half of the places, or all of them, has about half the
+// wavefronts (windows of 1028 keys at head_dim 128: 256 pairs 26.7 us, 260 to 264 37;
+// 512 48, 516 to 520 60 to 71), and with one item a request those stand on CUs as they come.
 static void win_items(DecodeParams& dp, int heads, int slots, int max_chunks) {
   int64_t n = slots / ((int64_t)dp.batch * heads);
   const int most = win_items_max(win_tiles_max(dp));
@@ -294,7 +297,9 @@ static void win_items(DecodeParams& dp, int heads, int slots, int max_chunks) {
 // 60 requests at 4 kv heads x 128, windows of 250 11.7 -> 8.4, 1024 26.9 -> 22.8, 4090
 // 87 -> 83; 96 at 2 x 256 in 4 bits, 4090 47.3 -> 43.1); cut in more, short windows
 // still gain (one request, 250 keys 7.9 -> 6.2, 500 8.8 -> 7.6) and longer ones lose
-// (1024 keys 9.0 -> 9.6 at 4 x 128, 11.4 -> 15.1 at 2 x 256 in 4 bits).
+// (1024 keys 9.0 -> 9.6 at 4 x 128, 11.4 -> 15.1 at 2 x 256 in 4 bits).  The rule goes by
+// the window, as the requests' lengths are on the device: short requests behind a long
+// window are cut.  Not measured: eight wavefronts where a request has one item anyway.
 constexpr int kWinEightTiles = 40;
 static bool win_by_eight(const DecodeParams& dp) {
   return dp.splits == 2 || (dp.splits > 2 && win_tiles_max(dp) <= kWinEightTiles);
