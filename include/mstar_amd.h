@@ -472,6 +472,71 @@ int mi_rope_append(void* q, int64_t q_stride_token, int64_t q_stride_head, int32
                    float high_freq_factor, float old_context_len, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Norms of q and k head by head, rotation and append in one pass.  The attention
+ * layers of the reference call these one after the other
+ * (mstar/model/components/attention.py:148-159).  For every (token, head) row x of q and k
+ *   y = x * rsqrt(mean(x^2) + eps) * weight        over its head_dim elements,
+ * then the rotation of mi_rope_apply at pos_ids, in place (k only when keep_k != 0).  With
+ * kv != NULL also the append of the rotated k and of v [num_tokens, num_kv_heads,
+ * head_dim], as mi_rope_append appends, into every cache type that mi_kv_append takes.
+ * Norm and rotation are fp32 and values are rounded once, from fp32 to q's type and to
+ * the cache's; angles are formed in 64 bits.  q, k, v: dtype (bf16 or f16), 16-byte aligned rows, strides
+ * multiples of 8; head_dim a multiple of 8 up to 512; rotary_dim a multiple of 16 (8 where
+ * interleaved).  q_weight, k_weight: head_dim values of weight_dtype (dtype or MI_F32).
+ * num_append_tokens at most num_tokens; kv == NULL: v, page_idx, slot_idx unused. */
+int mi_qk_norm_rope(void* q, int64_t q_stride_token, int64_t q_stride_head, int32_t num_qo_heads, void* k,
+                    int64_t k_stride_token, int64_t k_stride_head, int32_t num_kv_heads, const void* v,
+                    int64_t v_stride_token, int64_t v_stride_head, int32_t dtype, int32_t head_dim,
+                    const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps, int32_t keep_k,
+                    const mi_paged_kv* kv, const int64_t* page_idx, const int64_t* slot_idx, int64_t idx_stride,
+                    int32_t num_append_tokens, const int32_t* num_tokens_device, int32_t rotary_dim,
+                    const void* pos_ids, int32_t pos_dtype, int32_t num_tokens, int32_t interleave,
+                    float rope_scale, float rope_theta, int32_t llama31, float low_freq_factor,
+                    float high_freq_factor, float old_context_len, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention weights of cached tokens, accumulated.  No counterpart in the reference.
+ *   weights[page, h, slot] += sum over the request's queries i and the q heads g of kv head h
+ *                             of softmax_t(sm_scale * q[i, g] . k[t, h])
+ * for the token t of the request that lies at (page, slot), over the keys that mi_decode_run
+ * and mi_prefill_run show query i; the request's own tokens, the last qo_len of its keys, begin at zero
+ * (what their slots held does not count).  A query that sees no key adds nothing; one
+ * that meets a NaN makes the weights of every key it sees NaN.  Slots behind a request's
+ * keys are left as they were.  weights: fp32 [max_pages][num_kv_heads][page_size], contiguous, 16-byte
+ * aligned.  qo_indptr == NULL: one query a request.  max_qo_tokens bounds qo_indptr[batch],
+ * num_indices kv_indptr[batch] (what lies past them is left out).  q types, caches, head_dim, page_size and alignment as for
+ * mi_decode_run.  parts: 1 requests of at most 16 rows (qo_len x q heads a kv head), 2 the others, 3 both
+ * (qo_indptr == NULL: 1).  Page ids outside [0, max_pages) get no weights.  Requests of a call share
+ * no page.  The same call gives the same bits.  workspace: mi_attention_weights_bytes of the same sizes
+ * (ragged: qo_indptr != NULL), 16-byte aligned, scratch of this call alone.
+ * ------------------------------------------------------------------------ */
+int64_t mi_attention_weights_bytes(int32_t batch, int32_t max_qo_tokens, int32_t num_indices, int32_t page_size,
+                                   int32_t num_qo_heads, int32_t num_kv_heads, int32_t ragged, int32_t parts);
+int mi_attention_weights(const void* q, int32_t q_dtype, int64_t q_stride_token, int64_t q_stride_head,
+                         const mi_paged_kv* kv, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                         const int32_t* kv_indices, const int32_t* last_page_len, int32_t batch,
+                         int32_t max_qo_tokens, int32_t num_indices, int32_t num_qo_heads, int32_t causal,
+                         float sm_scale, int32_t parts, float* weights, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+
+/* Eviction by such weights.  For every layer l < num_layers, request and kv head whose request
+ * holds more than `keep` tokens, the first `sinks` tokens, the last `recent` and the
+ * keep - sinks - recent heaviest between them stay (ties: the lowest place; NaN below every number; recent + sinks <= keep,
+ * MI_ERR_INVALID otherwise).  Their K and V rows, a microscaled layer's scale bytes and their
+ * weights move to the request's first `keep` places, in their order; places from `keep` on are
+ * left as they were, and so are shorter requests.  kept [num_layers][batch][num_kv_heads][keep] receives the places
+ * that stayed, ascending, -1 behind a shorter request's tokens.  kv describes layer 0, layer_stride (in
+ * kv's units) and scale_layer_stride (bytes) lead to the next one's; weights and out_weights as in
+ * mi_attention_weights, weights_layer_stride elements from layer to layer.  out_weights may be weights; otherwise weights is
+ * left as it was and every request's kept weights are written.  Pages outside [0, max_pages) weigh less than
+ * any number, and what would move from or to them stays.  num_indices: elements of kv_indices.  Requests of a call share no page.  Any cache
+ * type; rows 16-byte aligned. */
+int mi_kv_evict(const mi_paged_kv* kv, int32_t num_layers, int64_t layer_stride, int64_t scale_layer_stride,
+                const float* weights, float* out_weights, int64_t weights_layer_stride, const int32_t* kv_indptr,
+                const int32_t* kv_indices, const int32_t* last_page_len, int32_t batch, int32_t num_indices,
+                int32_t keep, int32_t recent, int32_t sinks, int32_t* kept, void* stream);
+
+/* ------------------------------------------------------------------------
  * Page snapshot copies (multi-label / CFG planning).
  * mi_copy_pages replaces the per-page copies of BatchedCacheManager.snapshot_all
  * (mstar/engine/cache_manager.py:840-870): for i < num_pairs and every layer l,

@@ -196,6 +196,22 @@ SIGNATURES = {
         [_P, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _I32, _I32, ctypes.POINTER(MiPagedKV), _P, _P,
          _I64, _I32, _P, _I32, _P, _I32, _I32, _I32, _F32, _F32, _I32, _F32, _F32, _F32, _P],
     ),
+    "mi_qk_norm_rope": (
+        ctypes.c_int,
+        [_P, _I64, _I64, _I32, _P, _I64, _I64, _I32, _P, _I64, _I64, _I32, _I32, _P, _P, _I32, _F32, _I32,
+         ctypes.POINTER(MiPagedKV), _P, _P, _I64, _I32, _P, _I32, _P, _I32, _I32, _I32, _F32, _F32, _I32, _F32, _F32,
+         _F32, _P],
+    ),
+    "mi_attention_weights_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32]),
+    "mi_attention_weights": (
+        ctypes.c_int,
+        [_P, _I32, _I64, _I64, ctypes.POINTER(MiPagedKV), _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _P,
+         _P, _I64, _P],
+    ),
+    "mi_kv_evict": (
+        ctypes.c_int,
+        [ctypes.POINTER(MiPagedKV), _I32, _I64, _I64, _P, _P, _I64, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P],
+    ),
 }
 
 _lock = threading.Lock()

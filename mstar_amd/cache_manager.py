@@ -6,9 +6,12 @@ BatchedCacheManager`` (``cache_manager.py:56-881``): ``plan_attention``,
 ``plan_rope_batched_cfg``, ``snapshot_all``, ``set_layer_idx``, ``set_active_label(s)``,
 ``get_qo_indptr_buf``, ``advance_seq_len(s)``, ``set_custom_pos_advance``,
 ``flush_to_store``, plus the pre-planned-label fast path used by the CUDA-graph
-runner (``_pre_planned_labels``, ``cache_manager.py:202-217``).  One method has
+runner (``_pre_planned_labels``, ``cache_manager.py:202-217``).  Some methods have
 no reference counterpart: ``apply_rope_and_run_attention`` fuses the RoPE of
-``apply_rope`` with the K/V append of ``run_attention`` into one kernel.
+``apply_rope`` with the K/V append of ``run_attention`` into one kernel (with the
+norms of q and k before it, where a model has them; ``apply_qk_norm_rope`` is
+those without the append), and ``evict`` holds requests to a number of tokens by
+the attention they get (:mod:`mstar_amd.eviction`).
 
 What changes is how a step is packed (``_plan_attention_impl``,
 ``cache_manager.py:229-424``).  The reference walks every request in Python,
@@ -30,10 +33,12 @@ import numpy as np
 import torch
 
 from . import _lib
+from .eviction import _pool_shape, evict_kv_cache
 from .kv_store import KVCacheConfig, KVRequestState, PagedAllocationManager, _host_step
 from .mx_cache import MXKVCache
 from .paged_attention import PagedDecodeWrapper, PagedPrefillWrapper
-from .rope import apply_llama31_rope_pos_ids_inplace, apply_rope_pos_ids_inplace, rope_positions
+from .rope import (apply_llama31_rope_pos_ids_inplace, apply_qk_norm_rope_pos_ids_inplace, apply_rope_pos_ids_inplace,
+                   rope_positions)
 from .trace import trace_range
 
 _LLAMA31_KEYS = ("low_freq_factor", "high_freq_factor", "old_context_len")
@@ -110,10 +115,15 @@ class BatchedCacheManager:
         auto_write_store: bool = False,
         enable_nvtx: bool = False,
         kv_scales: torch.Tensor | None = None,
+        kv_weights: torch.Tensor | None = None,
     ):
         """``kv_scales`` (extension): fp32 ``[num_layers, 2, num_kv_heads]`` per-head
         dequantisation scales of an fp8-e4m3 ``kv_cache``.  ``kv_cache`` may be an
-        :class:`~mstar_amd.mx_cache.MXKVCache` (extension), which holds its own."""
+        :class:`~mstar_amd.mx_cache.MXKVCache` (extension), which holds its own.
+        ``kv_weights`` (extension): the pool's :func:`~mstar_amd.eviction.kv_weights`, for
+        ``accumulate=True`` and :meth:`evict`."""
+        if kv_weights is not None and tuple(kv_weights.shape) != _pool_shape(kv_cache):
+            raise ValueError(f"kv_weights {tuple(kv_weights.shape)} do not fit the pool's {_pool_shape(kv_cache)}")
         self.request_ids = request_ids
         self.active_labels = active_labels_per_request
         self.kv_cache = kv_cache
@@ -125,6 +135,7 @@ class BatchedCacheManager:
         self.enable_nvtx = enable_nvtx
         self.auto_write_store = auto_write_store
         self.kv_scales = kv_scales
+        self.kv_weights = kv_weights
         self._cuda_graph_mode = cuda_graph_plan_states is not None
         self._plan_states: dict[str, _PlanState] = cuda_graph_plan_states if cuda_graph_plan_states is not None else {}
         self._pre_planned_labels: set[str] = set()
@@ -406,17 +417,20 @@ class BatchedCacheManager:
         first ``seq_len // page_size`` pages, grows to the source length,
         takes its seq_len and position start); the page copies of all
         requests and layers go to the GPU as one ``mi_copy_pages`` launch.
+        A state that :meth:`evict` has cut no longer begins as its copies do: all
+        its pages are copied.  ``kv_weights`` are copied for every page.
         """
         assert self.kv_cache is not None
         ps_ = self.kv_cache_config.page_size
-        src, dst = [], []
+        src, dst, whole = [], [], ([], [])
         for rid in self.request_ids:
             from_state = self._get_state(rid, from_label)
             if realloc:
                 self.alloc_manager.reset_label(rid, to_label)
             to_state = self._get_state(rid, to_label)
-            start = to_state.seq_len // ps_
+            start = 0 if from_state.evicted or to_state.evicted else to_state.seq_len // ps_
             self.alloc_manager.alloc(rid, to_label, seq_len=from_state.seq_len)
+            to_state.evicted = to_state.evicted or from_state.evicted
             to_state.seq_len = from_state.seq_len
             to_state.position_id_start = from_state.position_id_start
             a, b = from_state.page_indices[start:], to_state.page_indices[start:]
@@ -424,23 +438,30 @@ class BatchedCacheManager:
                 raise ValueError(f"{rid}: {len(a)} source pages vs {len(b)} destination pages from page {start}")
             src.extend(a)
             dst.extend(b)
+            whole[0].extend(from_state.page_indices)
+            whole[1].extend(to_state.page_indices)
             if write_store:
                 self.alloc_manager.flush_to_store(rid, label=to_label)
         if src:
             pools = [self.kv_cache.codes, self.kv_cache.scales] if isinstance(self.kv_cache, MXKVCache) else [self.kv_cache]
             if not all(kv[0, 0].is_contiguous() for kv in pools):
                 raise ValueError("snapshot_all needs each page of the KV pool to be contiguous")
-            n = len(src)
-            dev = self._pack.upload(np.asarray(src + dst, dtype=np.int32))
-            for kv in pools:
-                esz = kv.element_size()
-                _lib.check(
-                    _lib.lib().mi_copy_pages(
-                        kv.data_ptr(), kv.stride(0) * esz, kv.shape[0], kv.stride(1) * esz, kv[0, 0].numel() * esz,
-                        kv.shape[1], dev.data_ptr(), dev.data_ptr() + 4 * n, n, _lib.stream_ptr(self.device),
-                    ),
-                    "mi_copy_pages",
-                )
+            self._copy_pages(pools, src, dst)
+        if self.kv_weights is not None and whole[0]:  # every token's weight changes with every step
+            self._copy_pages([self.kv_weights], *whole)
+
+    def _copy_pages(self, pools: list[torch.Tensor], src: list[int], dst: list[int]) -> None:
+        n = len(src)
+        dev = self._pack.upload(np.asarray(src + dst, dtype=np.int32))
+        for kv in pools:
+            esz = kv.element_size()
+            _lib.check(
+                _lib.lib().mi_copy_pages(
+                    kv.data_ptr(), kv.stride(0) * esz, kv.shape[0], kv.stride(1) * esz, kv[0, 0].numel() * esz,
+                    kv.shape[1], dev.data_ptr(), dev.data_ptr() + 4 * n, n, _lib.stream_ptr(self.device),
+                ),
+                "mi_copy_pages",
+            )
 
     # ------------------------------------------------------------ running
     def _layer_scales(self, layer_idx: int):
@@ -448,12 +469,25 @@ class BatchedCacheManager:
             return None, None
         return self.kv_scales[layer_idx, 0], self.kv_scales[layer_idx, 1]
 
+    def _run(self, wrapper, q, layer, layer_idx, ks, vs, window_left, sink_tokens, accumulate) -> torch.Tensor:
+        if accumulate:
+            if self.kv_weights is None:
+                raise ValueError("accumulate=True needs the manager's kv_weights")
+            if window_left >= 0:
+                raise ValueError("attention weights are accumulated over layers without a window")
+        out = wrapper.run(q, layer, ks, vs, window_left=window_left, sink_tokens=sink_tokens)
+        if accumulate:
+            wrapper.accumulate_weights(q, layer, self.kv_weights[layer_idx], ks, vs)
+        return out
+
     def run_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
-                      layer_idx: int | None = None, window_left: int = -1, sink_tokens: int = 0) -> torch.Tensor:
+                      layer_idx: int | None = None, window_left: int = -1, sink_tokens: int = 0,
+                      accumulate: bool = False) -> torch.Tensor:
         """Append this step's K/V, then attend (``cache_manager.py:653-701``).
 
         ``window_left``, ``sink_tokens`` (extension): the layer's sliding window, as
-        the wrappers' ``run``."""
+        the wrappers' ``run``.  ``accumulate`` (extension): also add the step's attention
+        to the layer's ``kv_weights``, as the wrappers' ``accumulate_weights``."""
         if layer_idx is None:
             layer_idx = self.layer_idx
         orig_dtype = q.dtype
@@ -466,7 +500,7 @@ class BatchedCacheManager:
         if self.auto_write_store and ps.write_store:
             for rid in self.request_ids:
                 self.alloc_manager.flush_to_store(rid, label=label, layers=layer_idx)
-        return ps.wrapper.run(q, layer, ks, vs, window_left=window_left, sink_tokens=sink_tokens).to(orig_dtype)
+        return self._run(ps.wrapper, q, layer, layer_idx, ks, vs, window_left, sink_tokens, accumulate).to(orig_dtype)
 
     # ------------------------------------------------------------ rope
     def plan_rope(self, seq_lens: list[int], pos_ids: torch.Tensor | None = None, label: str | None = None) -> None:
@@ -555,20 +589,50 @@ class BatchedCacheManager:
                                        rope_scale=rope_scale, rope_theta=rope_theta)
         return q.to(orig_dtype), k.to(orig_dtype)
 
+    def apply_qk_norm_rope(self, q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                           eps: float = 1e-6, rotary_dim: int | None = None, interleave: bool = False,
+                           rope_scale: float = 1, rope_theta: float = 10000.0, rope_dtype=None, **kwargs):
+        """Norms of q and k head by head, then RoPE at the planned positions, in one pass (extension).
+
+        As ``apply_rope`` of the normed rows, rounded once
+        (:func:`~mstar_amd.rope.apply_qk_norm_rope_pos_ids_inplace`); the same dtype handling
+        and Llama-3.1 keywords.  ``q_weight``, ``k_weight``: ``[head_dim]``, in the rope dtype or fp32.
+        """
+        ps = self._plan_states[self._single_active_label()]
+        assert ps.pos_ids is not None, "plan_rope() must run before apply_qk_norm_rope()"
+        orig_dtype = q.dtype
+        if rope_dtype is not None:
+            q, k = q.to(rope_dtype), k.to(rope_dtype)
+        elif torch.is_autocast_enabled("cuda"):
+            dt = torch.get_autocast_dtype("cuda")
+            q, k = q.to(dt), k.to(dt)
+        elif q.dtype == torch.float32:
+            q, k = q.to(torch.bfloat16), k.to(torch.bfloat16)
+        llama31 = {key: v for key, v in kwargs.items() if key in _LLAMA31_KEYS and v is not None}
+        apply_qk_norm_rope_pos_ids_inplace(q, k, q_weight, k_weight, ps.pos_ids, eps=eps, rotary_dim=rotary_dim,
+                                           interleave=interleave, rope_scale=rope_scale, rope_theta=rope_theta,
+                                           llama31=llama31 or None)
+        return q.to(orig_dtype), k.to(orig_dtype)
+
     def apply_rope_and_run_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                                      rotary_dim: int | None = None, interleave: bool = False, rope_scale: float = 1,
                                      rope_theta: float = 10000.0, rope_dtype=None, layer_idx: int | None = None,
                                      keep_k: bool = True, window_left: int = -1, sink_tokens: int = 0,
-                                     **kwargs) -> torch.Tensor:
+                                     q_norm_weight: torch.Tensor | None = None, k_norm_weight: torch.Tensor | None = None,
+                                     norm_eps: float = 1e-6, accumulate: bool = False, **kwargs) -> torch.Tensor:
         """``apply_rope(q, k, ...)`` then ``run_attention(q, k, v)`` with the rotation and the append fused.
 
         One ``mi_rope_append`` launch rotates q (and k, unless ``keep_k`` is
         False) and writes the rotated k and v to the layer's pages; the cache
         and the attention output are bit-identical to the two-call sequence.
         Dtype handling and Llama-3.1 keywords are those of ``apply_rope``; v
-        is converted to the rope dtype with q and k.  ``window_left`` and
-        ``sink_tokens`` are ``run_attention``'s.
+        is converted to the rope dtype with q and k.  ``window_left``,
+        ``sink_tokens`` and ``accumulate`` are ``run_attention``'s.  With ``q_norm_weight`` and
+        ``k_norm_weight`` (``[head_dim]``, in the rope dtype or fp32) q and k are first normalised head by
+        head, in the same launch (``mi_qk_norm_rope``).
         """
+        if (q_norm_weight is None) != (k_norm_weight is None):
+            raise ValueError("q_norm_weight and k_norm_weight go together")
         if layer_idx is None:
             layer_idx = self.layer_idx
         label = self._single_active_label()
@@ -590,13 +654,56 @@ class BatchedCacheManager:
             llama31 = {"low_freq_factor": 1.0, "high_freq_factor": 4.0, "old_context_len": 8192, **llama31}
         layer = self.kv_cache[layer_idx]
         ks, vs = self._layer_scales(layer_idx)
-        ps.wrapper.rope_set_kv_cache(layer, q, k, v, ps.pos_ids, rotary_dim=rotary_dim, interleave=interleave,
-                                     rope_scale=rope_scale, rope_theta=rope_theta, k_scale=ks, v_scale=vs,
-                                     keep_k=keep_k, llama31=llama31 or None)
+        rope = dict(rotary_dim=rotary_dim, interleave=interleave, rope_scale=rope_scale, rope_theta=rope_theta, k_scale=ks,
+                    v_scale=vs, keep_k=keep_k, llama31=llama31 or None)
+        if q_norm_weight is not None:
+            ps.wrapper.qk_norm_rope_set_kv_cache(layer, q, k, v, q_norm_weight, k_norm_weight, ps.pos_ids, eps=norm_eps, **rope)
+        else:
+            ps.wrapper.rope_set_kv_cache(layer, q, k, v, ps.pos_ids, **rope)
         if self.auto_write_store and ps.write_store:
             for rid in self.request_ids:
                 self.alloc_manager.flush_to_store(rid, label=label, layers=layer_idx)
-        return ps.wrapper.run(q, layer, ks, vs, window_left=window_left, sink_tokens=sink_tokens).to(orig_dtype)
+        return self._run(ps.wrapper, q, layer, layer_idx, ks, vs, window_left, sink_tokens, accumulate).to(orig_dtype)
+
+    # ------------------------------------------------------------ eviction
+    def evict(self, keep: int, recent: int = 0, sinks: int = 0) -> int:
+        """Hold every request's active label to ``keep`` tokens by ``kv_weights``, in all layers; returns the pages freed (extension).
+
+        Between steps (after ``advance_seq_len(s)``): what :func:`~mstar_amd.eviction.evict_kv_cache`
+        does, and the pages behind the kept tokens go back to the allocator's tail.  ``seq_len`` becomes ``keep`` where it was
+        more, positions go on from ``position_id_start``.  The launch is ordered on the current stream, and so
+        must be what uses the freed pages next.
+        """
+        if self.kv_weights is None:
+            raise ValueError("evict() needs the manager's kv_weights")
+        am, ps_ = self.alloc_manager, self.kv_cache_config.page_size
+        keep, recent, sinks = int(keep), int(recent), int(sinks)
+        if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
+            raise ValueError(f"keep {keep} must be positive and hold recent {recent} and sinks {sinks}")
+        cut = []
+        for rid in self.request_ids:
+            label = self.active_labels.get(rid, "main")
+            if am.get_state(rid, label).seq_len > keep:
+                am.wait_for_retrieves(rid, label)
+                cut.append(am.get_state(rid, label))
+        if not cut:
+            return 0
+        pages = [-(-st.seq_len // ps_) for st in cut]
+        n, total = len(cut), sum(pages)
+        meta = np.empty(2 * n + 1 + total, dtype=np.int32)
+        meta[0] = 0
+        meta[1:n + 1] = np.cumsum(pages)
+        meta[n + 1:2 * n + 1] = [st.seq_len - (p - 1) * ps_ for st, p in zip(cut, pages)]
+        meta[2 * n + 1:] = [page for st, p in zip(cut, pages) for page in st.page_indices[:p]]
+        dev = self._pack.upload(meta)
+        evict_kv_cache(self.kv_cache, self.kv_weights, dev[:n + 1], dev[2 * n + 1:], dev[n + 1:2 * n + 1], keep, recent, sinks)
+        need, freed = -(-keep // ps_), []
+        with am._lock:
+            for st in cut:
+                freed.extend(st.page_indices[need:])
+                st.page_indices, st.seq_len, st.evicted = st.page_indices[:need], keep, True
+            am.page_allocator.free(freed)
+        return len(freed)
 
     # ------------------------------------------------------------ advance
     def advance_seq_len(self, n: int | None = None, pos_id_n: int | None = None) -> None:

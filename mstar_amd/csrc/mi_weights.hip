@@ -1,0 +1,275 @@
+// Attention weights of cached tokens, accumulated (mi_attention_weights).
+//
+//   w[t, h] += sum over queries i and q heads g of kv head h of  exp(s_igt - lse_ig),
+//   s_igt = sm_scale q_ig . k_th,   lse_ig = log sum_t exp(s_igt)  over the keys that query i sees,
+//
+// beginning at zero for the step's own tokens (the last qo_len of a request).  The
+// sum needs every row's lse first, so the keys are gone through twice:
+//
+// * Requests of at most 16 rows (qo_len x group; decode): K is what costs, so it is read once. The first
+//   launch writes the scores (group x 4 bytes a token and kv head, beside a row of K of 64 to 512 bytes) and
+//   a log-sum-exp for each run of pages; the second joins those and sums the exponentials.
+// * Longer ones: the products are what costs, and are done twice; a launch goes by rows with the
+//   keys streaming past (lse), one by keys with the rows streaming past (sums).
+//
+// Every sum has one order, from the index arrays and shapes alone: the same call gives the same bits.
+// Work is found from the index arrays (unit_request): no plan is read, and any plan's workspace
+// stays as it is.
+#include "mi_weights_kernel.h"
+
+namespace mi {
+
+int weights_launch_16(const WeightsParams& p, int q_dtype, int head_dim, int which, dim3 grid, hipStream_t s) {
+  return q_dtype == MI_BF16  ? launch_weights_kvt<BF16, kKv16>(p, head_dim, which, grid, s)
+         : q_dtype == MI_F16 ? launch_weights_kvt<F16, kKv16>(p, head_dim, which, grid, s)
+                             : launch_weights_kvt<F32, kKv16>(p, head_dim, which, grid, s);
+}
+
+// The second launch over short queries: a unit's tokens, four to a thread.
+__global__ __launch_bounds__(256) void weights_finish_kernel(WeightsParams p) {
+  __shared__ float s_m[16][kWRows], s_l[16][kWRows], s_lse[kWRows];
+  const int tid = (int)threadIdx.x, nkv = p.num_kv_heads;
+  const int h = uniform((int)(blockIdx.x % nkv)), unit = uniform((int)(blockIdx.x / nkv));
+  const int r = uniform(unit_request(p.kv_indptr, 1, p.unit_pages, p.batch, unit));
+  if (r < 0) return;
+  const WRequest q = w_request(p, r);
+  if (q.rows <= 0 || q.rows > kWRows) return;
+  const int begin = unit_begin(p.kv_indptr, 1, p.unit_pages, r), unit_tokens = p.unit_pages * p.page_size;
+  const int tok0 = (unit - begin) * unit_tokens, tok1 = min(tok0 + unit_tokens, q.len);
+  if (tok0 >= tok1) return;
+  // the request's log-sum-exp: 16 threads a row go through its units
+  {
+    const int row = tid & 15, part = tid >> 4, units = (q.len + unit_tokens - 1) / unit_tokens;
+    float m = -kWInf, l = 0.f;
+    bool bad = false;
+    for (int u = part; u < units; u += 16) {
+      const float e = p.unit_lse[((int64_t)(begin + u) * nkv + h) * kWRows + row];
+      bad |= e != e;
+      if (e == kWInf) continue;  // saw nothing there
+      const float mn = fmaxf(m, e), mu = mn == -kWInf ? 0.f : mn;
+      l = l * fast_exp2(m - mu) + fast_exp2(e - mu);
+      m = mn;
+    }
+    s_m[part][row] = m;
+    s_l[part][row] = bad ? __builtin_nanf("") : l;
+    __syncthreads();
+    if (tid < kWRows) {
+      float M = -kWInf, L = 0.f;
+      for (int i = 0; i < 16; ++i) M = fmaxf(M, s_m[i][tid]);
+      const float Mu = M == -kWInf ? 0.f : M;
+      for (int i = 0; i < 16; ++i) L += s_l[i][tid] * fast_exp2(s_m[i][tid] - Mu);
+      s_lse[tid] = w_lse(M, L);
+    }
+    __syncthreads();
+  }
+  const int off = q.len - q.qo_len;
+  for (int t = tok0 + 4 * tid; t < tok1; t += 1024) {
+    const int64_t tile = ((int64_t)q.first * p.page_size + t) >> 4;
+    const float* src = p.scores + (tile * nkv + h) * p.score_rows * 16 + (t & 15);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int row = 0; row < q.rows; ++row) {
+      const float4 s = *(const float4*)(src + 16 * row);
+      const float e = s_lse[row];
+      sum.x += fast_exp2(s.x - e);
+      sum.y += fast_exp2(s.y - e);
+      sum.z += fast_exp2(s.z - e);
+      sum.w += fast_exp2(s.w - e);
+    }
+    const int e = (int)((unsigned)t / (unsigned)p.page_size);
+    const int64_t page = p.kv_indices[q.first + e];
+    if (page < 0 || page >= p.max_pages) continue;
+    float* w = p.weights + (page * nkv + h) * p.page_size + t - e * p.page_size;
+    const float add[4] = {sum.x, sum.y, sum.z, sum.w};
+    if (t + 4 <= min(off, tok1)) {
+      float4 old = *(float4*)w;
+      *(float4*)w = make_float4(old.x + add[0], old.y + add[1], old.z + add[2], old.w + add[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t + i < tok1) w[i] = t + i >= off ? add[i] : w[i] + add[i];
+    }
+  }
+}
+
+// Joins the key shares' log-sum-exps of a row into the first.
+__global__ __launch_bounds__(256) void weights_join_kernel(WeightsParams p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)p.num_kv_heads * p.total_rows;
+  if (i >= n) return;
+  float m = -kWInf, l = 0.f;
+  bool bad = false;
+  for (int s = 0; s < p.key_splits; ++s) {
+    const float e = p.row_lse[s * n + i];
+    bad |= e != e;
+    if (e == kWInf) continue;
+    const float mn = fmaxf(m, e), mu = mn == -kWInf ? 0.f : mn;
+    l = l * fast_exp2(m - mu) + fast_exp2(e - mu);
+    m = mn;
+  }
+  p.row_lse[i] = w_lse(m, bad ? __builtin_nanf("") : l);
+}
+
+// Adds the row shares' sums of a token to its weight.
+__global__ __launch_bounds__(256) void weights_sum_kernel(WeightsParams p) {
+  const int nkv = p.num_kv_heads;
+  const int h = uniform((int)(blockIdx.x % nkv)), unit = uniform((int)(blockIdx.x / nkv));
+  const int r = uniform(unit_request(p.kv_indptr, 1, p.key_pages, p.batch, unit));
+  if (r < 0) return;
+  const WRequest q = w_request(p, r);
+  if (q.rows <= kWRows) return;
+  const int tok0 = (unit - unit_begin(p.kv_indptr, 1, p.key_pages, r)) * p.key_pages * p.page_size;
+  const int tok1 = min(tok0 + p.key_pages * p.page_size, q.len), off = q.len - q.qo_len;
+  for (int t = tok0 + (int)threadIdx.x; t < tok1; t += 256) {
+    float total = 0.f;
+    for (int s = 0; s < p.row_splits; ++s)
+      total += p.sums[((int64_t)s * nkv + h) * p.places + (int64_t)q.first * p.page_size + t];
+    const int e = (int)((unsigned)t / (unsigned)p.page_size);
+    const int64_t page = p.kv_indices[q.first + e];
+    if (page < 0 || page >= p.max_pages) continue;
+    float* w = p.weights + (page * nkv + h) * p.page_size + t - e * p.page_size;
+    *w = t >= off ? total : *w + total;
+  }
+}
+
+// How a call is cut, from its shapes alone, and where its scratch lies.
+struct WeightsCut {
+  int32_t unit_pages, units, score_rows;                               // short
+  int32_t row_units, key_splits, key_pages, key_units, row_splits;     // long
+  int64_t scores, unit_lse, row_lse, sums, total;                      // bytes
+};
+
+static WeightsCut weights_cut(int32_t batch, int32_t max_qo_tokens, int32_t num_indices, int32_t page_size, int32_t nkv,
+                              int32_t group, bool ragged, int parts) {
+  WeightsCut c{};
+  const int64_t tokens = (int64_t)num_indices * page_size;
+  auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  auto clamp = [](int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; };
+  int64_t at = 0;
+  // Runs of pages: about 4096 workgroups, of 64 tokens (one tile a wavefront) and more.
+  c.unit_pages = (int32_t)up(clamp(up(tokens * nkv, 4096), 64, 1 << 24), page_size);
+  c.units = (int32_t)(num_indices / c.unit_pages + batch);
+  c.score_rows = ragged ? kWRows : group;
+  if (parts & 1) {
+    c.scores = at;
+    at = mi_align_up(at + 4 * tokens * nkv * c.score_rows, 256);
+    c.unit_lse = at;
+    at = mi_align_up(at + 4LL * c.units * nkv * kWRows, 256);
+  }
+  if (parts & 2) {
+    const int64_t rows = (int64_t)max_qo_tokens * group, b = batch > 0 ? batch : 1;
+    c.row_units = (int32_t)(rows / kRowBlock + b);
+    c.key_splits = (int32_t)clamp(1024 / ((int64_t)c.row_units * nkv), 1, clamp(tokens / b / 256, 1, 16));
+    c.key_pages = (int32_t)up(kKeyBlock, page_size);
+    c.key_units = (int32_t)(num_indices / c.key_pages + b);
+    c.row_splits = (int32_t)clamp(1024 / ((int64_t)c.key_units * nkv), 1, clamp(rows / b / 64, 1, 8));
+    c.row_lse = at;
+    at = mi_align_up(at + 4 * rows * nkv * c.key_splits, 256);
+    c.sums = at;
+    if (c.row_splits > 1) at = mi_align_up(at + 4 * tokens * nkv * c.row_splits, 256);
+  }
+  c.total = at;
+  return c;
+}
+
+static bool weights_shapes_ok(int32_t batch, int32_t max_qo_tokens, int32_t num_indices, int32_t page_size, int32_t hq,
+                              int32_t nkv, int32_t parts) {
+  return batch >= 0 && max_qo_tokens >= 0 && num_indices >= 0 && page_size > 0 && nkv > 0 && hq > 0 && hq % nkv == 0 &&
+         parts >= 1 && parts <= 3;
+}
+
+}  // namespace mi
+
+extern "C" int64_t mi_attention_weights_bytes(int32_t batch, int32_t max_qo_tokens, int32_t num_indices, int32_t page_size,
+                                              int32_t num_qo_heads, int32_t num_kv_heads, int32_t ragged, int32_t parts) {
+  using namespace mi;
+  if (!weights_shapes_ok(batch, max_qo_tokens, num_indices, page_size, num_qo_heads, num_kv_heads, parts)) return MI_ERR_INVALID;
+  if (!ragged) parts = 1;
+  return weights_cut(batch, max_qo_tokens, num_indices, page_size, num_kv_heads, num_qo_heads / num_kv_heads, ragged != 0, parts).total;
+}
+
+extern "C" int mi_attention_weights(const void* q, int32_t q_dtype, int64_t q_stride_token, int64_t q_stride_head,
+                                    const mi_paged_kv* kv, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                    const int32_t* kv_indices, const int32_t* last_page_len, int32_t batch,
+                                    int32_t max_qo_tokens, int32_t num_indices, int32_t num_qo_heads, int32_t causal,
+                                    float sm_scale, int32_t parts, float* weights, void* workspace, int64_t workspace_bytes,
+                                    void* stream) {
+  using namespace mi;
+  if (!kv || !weights_shapes_ok(batch, max_qo_tokens, num_indices, kv->page_size, num_qo_heads, kv->num_kv_heads, parts))
+    return MI_ERR_INVALID;
+  if (batch == 0 || max_qo_tokens == 0 || num_indices == 0) return MI_OK;
+  if (!q || !kv->data || !kv_indptr || !kv_indices || !last_page_len || !weights || !workspace) return MI_ERR_INVALID;
+  const int nkv = kv->num_kv_heads, D = kv->head_dim, group = num_qo_heads / nkv;
+  if (group > kWRows || kv->page_size % 16 || (D != 64 && D != 128 && D != 256)) return MI_ERR_UNSUPPORTED;
+  const bool scaled = kv_is_scaled(kv->dtype);
+  if (q_dtype != MI_BF16 && q_dtype != MI_F16 && q_dtype != MI_F32) return MI_ERR_UNSUPPORTED;
+  if (scaled ? q_dtype == MI_F32 : kv->dtype != q_dtype) return MI_ERR_UNSUPPORTED;
+  if (!kv_scales_ok(kv)) return MI_ERR_INVALID;
+  if (!rows_aligned16(q, q_stride_token, q_stride_head, q_dtype == MI_F32 ? 4 : 2) || !kv_aligned16(kv)) return MI_ERR_INVALID;
+  if ((uintptr_t)weights % 16 || (uintptr_t)workspace % 16) return MI_ERR_INVALID;
+  // places in the page list and rows are counted in 32 bits
+  if ((int64_t)num_indices * kv->page_size > INT32_MAX - (1 << 25) || (int64_t)max_qo_tokens * group > INT32_MAX - 65536 ||
+      kv->page_size > (1 << 24))
+    return MI_ERR_UNSUPPORTED;
+  const bool ragged = qo_indptr != nullptr;
+  if (!ragged) parts = 1;
+  const WeightsCut c = weights_cut(batch, max_qo_tokens, num_indices, kv->page_size, nkv, group, ragged, parts);
+  if (workspace_bytes < c.total) return MI_ERR_WORKSPACE;
+  WeightsParams p{};
+  p.q = q;
+  p.q_stride_tok = q_stride_token;
+  p.q_stride_head = q_stride_head;
+  p.k = (const uint8_t*)kv->data;
+  p.page_stride = kv->page_stride;
+  p.token_stride = kv->token_stride;
+  p.head_stride = kv->head_stride;
+  p.max_pages = kv->max_pages;
+  p.k_scale = kv->k_scale;
+  p.qo_indptr = qo_indptr;
+  p.kv_indptr = kv_indptr;
+  p.kv_indices = kv_indices;
+  p.last_page_len = last_page_len;
+  p.weights = weights;
+  uint8_t* ws = (uint8_t*)workspace;
+  p.scores = (float*)(ws + c.scores);
+  p.unit_lse = (float*)(ws + c.unit_lse);
+  p.row_lse = (float*)(ws + c.row_lse);
+  p.sums = (float*)(ws + c.sums);
+  p.total_rows = (int64_t)max_qo_tokens * group;
+  p.places = (int64_t)num_indices * kv->page_size;
+  p.batch = batch;
+  p.num_kv_heads = nkv;
+  p.group = group;
+  p.page_size = kv->page_size;
+  p.causal = causal ? 1 : 0;
+  p.max_tokens = max_qo_tokens;
+  p.num_indices = num_indices;
+  p.unit_pages = c.unit_pages;
+  p.score_rows = c.score_rows;
+  p.key_splits = c.key_splits;
+  p.row_splits = c.row_splits;
+  p.key_pages = c.key_pages;
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  hipStream_t s = (hipStream_t)stream;
+  const int kvt = kv_format(kv->dtype);
+  auto launch = [&](int which, int64_t blocks) {
+    if (blocks > INT32_MAX) return MI_ERR_UNSUPPORTED;
+    const dim3 grid((uint32_t)blocks);
+    return scaled ? weights_launch_scaled(p, q_dtype, kvt, D, which, grid, s) : weights_launch_16(p, q_dtype, D, which, grid, s);
+  };
+  if (parts & 1) {
+    const int st = launch(kWScores, (int64_t)c.units * nkv);
+    if (st != MI_OK) return st;
+    hipLaunchKernelGGL(weights_finish_kernel, dim3((uint32_t)(c.units * nkv)), dim3(256), 0, s, p);
+  }
+  if (parts & 2) {
+    int st = launch(kWRowsPass, (int64_t)c.row_units * nkv * c.key_splits);
+    if (st != MI_OK) return st;
+    if (c.key_splits > 1)
+      hipLaunchKernelGGL(weights_join_kernel, dim3((uint32_t)((nkv * p.total_rows + 255) / 256)), dim3(256), 0, s, p);
+    st = launch(kWColsPass, (int64_t)c.key_units * nkv * c.row_splits);
+    if (st != MI_OK) return st;
+    if (c.row_splits > 1)
+      hipLaunchKernelGGL(weights_sum_kernel, dim3((uint32_t)(c.key_units * nkv)), dim3(256), 0, s, p);
+  }
+  MI_CHECK_LAUNCH();
+  return MI_OK;
+}

@@ -1,0 +1,431 @@
+// Accumulated attention weights of cached tokens: the kernels (mi_weights.hip describes them
+// and launches them; mi_weights_*.hip hold the instantiations).
+#pragma once
+
+#include "mi_internal.h"
+
+namespace mi {
+
+// fp32 queries and caches: a step is 16 elements of a row, four to a lane, on the fp32 MFMA.
+struct F32 {
+  static constexpr int kDtype = MI_F32;
+  MI_DEVICE static f32x4 mma_16x16x32(const uint4& a, const uint4& b, f32x4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(bitcast<float>(a.x), bitcast<float>(b.x), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(bitcast<float>(a.y), bitcast<float>(b.y), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(bitcast<float>(a.z), bitcast<float>(b.z), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(bitcast<float>(a.w), bitcast<float>(b.w), c, 0, 0, 0);
+  }
+};
+
+struct WeightsParams {
+  const void* q;
+  int64_t q_stride_tok, q_stride_head;
+  const uint8_t* k;
+  int64_t page_stride, token_stride, head_stride, max_pages;  // elements (bytes of codes: microscaled)
+  const void* k_scale;
+  const int32_t *qo_indptr, *kv_indptr, *kv_indices, *last_page_len;
+  float* weights;  // [max_pages][kv head][slot]
+  float *scores, *unit_lse;  // short queries: [16-token tile of the page list][kv head][row][16], [unit][kv head][16]
+  float *row_lse, *sums;     // long ones: [split][kv head][row], [split][kv head][place in the page list]
+  int64_t total_rows, places;
+  int32_t batch, num_kv_heads, group, page_size, causal, max_tokens, num_indices;
+  int32_t unit_pages, score_rows;             // of the short path
+  int32_t key_splits, row_splits, key_pages;  // of the long one; key_pages: of a block of keys
+  float scale_log2;
+};
+
+constexpr int kWRows = 16;       // rows of a short-query request
+constexpr int kRowBlock = 128;   // rows of a workgroup of the long path's first pass
+constexpr int kKeyBlock = 128;   // keys of a workgroup of its second
+
+// The request of a unit, where request r's units begin at indptr[r] * mul / div + r: at least as many places
+// as it needs, and found from the index array alone.  -1: before the first.
+MI_DEVICE int unit_request(const int32_t* indptr, int mul, int div, int batch, int unit) {
+  int lo = 0, n = batch;  // the last r of [lo, lo + n) with begin(r) <= unit
+  const int lane = lane_id();
+  while (n > 0) {
+    const int step = (n + 63) / 64, r = lo + lane * step;
+    const bool in = lane * step < n && (int)((int64_t)indptr[r] * mul / div) + r <= unit;
+    const int count = __popcll(__builtin_amdgcn_ballot_w64(in));  // begins ascend
+    if (count == 0) return -1;
+    const int next = lo + (count - 1) * step;
+    if (step == 1) return next;
+    n = min(step, lo + n - next);
+    lo = next;
+  }
+  return -1;
+}
+MI_DEVICE int unit_begin(const int32_t* indptr, int mul, int div, int r) { return (int)((int64_t)indptr[r] * mul / div) + r; }
+
+// A request, held to the sizes that the call's scratch was made for.
+struct WRequest {
+  int first, pages, len, qo_start, qo_len, rows;
+};
+MI_DEVICE WRequest w_request(const WeightsParams& p, int r) {
+  WRequest q;
+  q.first = p.kv_indptr[r];
+  q.pages = min(p.kv_indptr[r + 1], p.num_indices) - q.first;
+  q.len = q.pages > 0 ? max(0, (q.pages - 1) * p.page_size + min(p.last_page_len[r], p.page_size)) : 0;
+  q.qo_start = p.qo_indptr ? p.qo_indptr[r] : r;
+  q.qo_len = p.qo_indptr ? min(p.qo_indptr[r + 1], p.max_tokens) - q.qo_start : 1;
+  q.rows = q.qo_len * p.group;
+  return q;
+}
+
+// How a lane holds a row of the cache: runs of RUN consecutive elements, 16 bytes each where
+// the row is long enough, run c at element c * 4 * RUN + grp * RUN (grp: which 16 lanes).  Any one order of
+// the elements serves a product, as long as q is held in the same.
+template <typename MT, int KVT, int D>
+struct KeyTile {
+  static constexpr bool F = MT::kDtype == MI_F32, MX = KVT == kKvMx8 || KVT == kKvMx4;
+  static constexpr int BITS = F ? 32 : KVT == kKv16 ? 16 : KVT == kKvMx4 ? 4 : 8;
+  static constexpr int RUN = D / 4 < 128 / BITS ? D / 4 : 128 / BITS;
+  static constexpr int NC = D / (4 * RUN), WORDS = RUN * BITS / 32;
+  static constexpr int STEP = F ? 4 : 8;                    // elements of a lane in a step
+  static constexpr int STEPS = D / (4 * STEP), PER = RUN / STEP;  // steps, and of a run
+  static constexpr int ESZ = F ? 4 : KVT == kKv16 ? 2 : 1;  // of the strides
+  static constexpr int NBLK = D / kMxBlock;
+  uint32_t w[NC][WORDS];
+  uint8_t s[MX ? NC : 1];
+
+  // The lane's row `row` of the 16 tokens at (page, slot0) of kv head h.
+  MI_DEVICE void load(const WeightsParams& p, int64_t page, int slot, int h, int grp) {
+    const uint8_t* src = p.k + (page * p.page_stride + slot * p.token_stride + h * p.head_stride) * ESZ + grp * (RUN * BITS / 8);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if constexpr (WORDS == 4) {
+        const uint4 u = *(const uint4*)(src + c * (4 * RUN * BITS / 8));
+        w[c][0] = u.x, w[c][1] = u.y, w[c][2] = u.z, w[c][3] = u.w;
+      } else {
+        const uint2 u = *(const uint2*)(src + c * (4 * RUN * BITS / 8));
+        w[c][0] = u.x, w[c][1] = u.y;
+      }
+    }
+    if constexpr (MX) {
+      const uint8_t* sc = (const uint8_t*)p.k_scale + (page * 2 * p.num_kv_heads + h) * NBLK * p.page_size + slot;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s[c] = sc[(int64_t)((c * 4 * RUN + grp * RUN) / kMxBlock) * p.page_size];
+    }
+  }
+  MI_DEVICE void fragments(uint4 (&f)[STEPS]) const {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if constexpr (KVT == kKv16) {
+        f[c] = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
+      } else {
+        uint32_t o[4 * PER];
+        if constexpr (KVT == kKvFp8) {
+#pragma unroll
+          for (int i = 0; i < 2 * PER; ++i) {
+            o[2 * i] = fp8x2_to_mt<MT>(w[c][i], false);
+            o[2 * i + 1] = fp8x2_to_mt<MT>(w[c][i], true);
+          }
+        } else {
+          mx_to_mt<MT, KVT>(w[c], bitcast<float>((uint32_t)s[c] << 23), o);
+          if constexpr (MT::kDtype == MI_F16)
+            if (mx_past_f16<KVT>(s[c])) f16_saturate(o);
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) f[c * PER + i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      }
+    }
+  }
+  // A row of q in the same order.
+  MI_DEVICE static void query(const WeightsParams& p, int64_t tok, int head, int grp, uint4 (&f)[STEPS]) {
+    const uint8_t* src = (const uint8_t*)p.q + (tok * p.q_stride_tok + head * p.q_stride_head) * (F ? 4 : 2);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) f[c * PER + i] = *(const uint4*)(src + (c * 4 * RUN + grp * RUN + i * STEP) * (F ? 4 : 2));
+  }
+};
+
+// Page of entry e of the page list, page 0 for ids out of range (whose tokens' weights are not written).
+MI_DEVICE int64_t safe_page(const WeightsParams& p, int e) {
+  const int64_t page = p.kv_indices[e];
+  return page >= 0 && page < p.max_pages ? page : 0;
+}
+
+constexpr float kWInf = __builtin_inff();
+
+// The log2 of a row's sum, from its running maximum and sum; +inf where it saw nothing, which
+// makes every exp2(s - lse) zero; NaN where a score was NaN or +inf.
+MI_DEVICE float w_lse(float m, float l) { return l > 0.f ? m + fast_log2(l) : l == 0.f ? kWInf : __builtin_nanf(""); }
+
+// ------------------------------------------------------------ short queries
+// Requests of at most 16 (query, q head) rows: HBM bound, K is read once.  A workgroup takes a unit
+// (unit_pages pages of a request, one kv head); each wavefront's tiles of 16 keys give S^T = K Q^T, whose
+// scores (log2 domain) go to scratch, and the unit's log-sum-exp of each row.
+template <typename MT, int KVT, int D>
+__global__ __launch_bounds__(256) void weights_scores_kernel(WeightsParams p) {
+  using Tile = KeyTile<MT, KVT, D>;
+  __shared__ float s_m[4][kWRows], s_l[4][kWRows];
+  const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6), nkv = p.num_kv_heads;
+  const int h = uniform((int)(blockIdx.x % nkv)), unit = uniform((int)(blockIdx.x / nkv));
+  const int r = uniform(unit_request(p.kv_indptr, 1, p.unit_pages, p.batch, unit));
+  if (r < 0) return;
+  const WRequest q = w_request(p, r);
+  if (q.rows <= 0 || q.rows > kWRows) return;
+  const int tok0 = (unit - unit_begin(p.kv_indptr, 1, p.unit_pages, r)) * p.unit_pages * p.page_size;
+  const int tok1 = min(tok0 + p.unit_pages * p.page_size, q.len);
+  if (tok0 >= tok1) return;
+  const int tiles = (tok1 - tok0 + 15) >> 4, share = tiles / 4, extra = tiles % 4;
+  const int t0 = wave * share + min(wave, extra), t1 = t0 + share + (wave < extra ? 1 : 0);
+
+  const int col = lane & 15, grp = lane >> 4;
+  const int qtok = col / p.group, g = col - qtok * p.group;
+  const bool valid = col < q.rows;
+  const int lim = p.causal ? q.len - q.qo_len + qtok : q.len - 1;
+  uint4 qf[Tile::STEPS] = {};
+  if (valid) Tile::query(p, q.qo_start + qtok, h * p.group + g, grp, qf);
+  const float sl2 = KVT == kKvFp8 ? p.scale_log2 * ((const float*)p.k_scale)[h] : p.scale_log2;
+
+  float m = -kWInf, l = 0.f;
+  auto load = [&](Tile& t, int i) {
+    const int tok = tok0 + 16 * i, e = (int)((unsigned)tok / (unsigned)p.page_size);
+    t.load(p, safe_page(p, q.first + e), tok - e * p.page_size + col, h, grp);
+  };
+  auto compute = [&](const Tile& t, int i) {
+    const int tok = tok0 + 16 * i;
+    uint4 kf[Tile::STEPS];
+    t.fragments(kf);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int st = 0; st < Tile::STEPS; ++st) acc = MT::mma_16x16x32(kf[st], qf[st], acc);
+    float s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s[j] = acc[j] * sl2;
+      if (tok + 4 * grp + j > lim) s[j] = -kWInf;
+    }
+    if (valid) {
+      const int64_t tile = ((int64_t)q.first * p.page_size + tok) >> 4;
+      *(float4*)(p.scores + ((tile * nkv + h) * p.score_rows + col) * 16 + 4 * grp) = make_float4(s[0], s[1], s[2], s[3]);
+    }
+    const float mn = fmaxf(m, fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+    const float mu = mn == -kWInf ? 0.f : mn;
+    l = l * fast_exp2(m - mu) + ((fast_exp2(s[0] - mu) + fast_exp2(s[1] - mu)) + (fast_exp2(s[2] - mu) + fast_exp2(s[3] - mu)));
+    m = mn;
+  };
+  Tile a, b;
+  if (t0 < t1) load(a, t0);
+  for (int i = t0; i < t1; i += 2) {
+    if (i + 1 < t1) load(b, i + 1);
+    compute(a, i);
+    if (i + 2 < t1) load(a, i + 2);
+    if (i + 1 < t1) compute(b, i + 1);
+  }
+  // the four groups of lanes, then the four wavefronts
+  const float mg = rows4_max(m), mgu = mg == -kWInf ? 0.f : mg;
+  l = rows4_sum(l * fast_exp2(m - mgu));
+  if (grp == 0) {
+    s_m[wave][col] = mg;
+    s_l[wave][col] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x < kWRows) {
+    float M = -kWInf, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w][col]);
+    const float Mu = M == -kWInf ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) L += s_l[w][col] * fast_exp2(s_m[w][col] - Mu);
+    p.unit_lse[((int64_t)unit * nkv + h) * kWRows + col] = w_lse(M, L);
+  }
+}
+
+// ------------------------------------------------------------ long queries
+// First pass: the log-sum-exp of every (query, q head) row.  A workgroup takes 128 rows of a
+// request and kv head, 32 to a wavefront, and a share of the keys: S^T = K Q^T with the rows' q in
+// registers, a lane's four scores all of one row.
+template <typename MT, int KVT, int D>
+__global__ __launch_bounds__(256) void weights_rows_kernel(WeightsParams p) {
+  using Tile = KeyTile<MT, KVT, D>;
+  constexpr int NB = 2;
+  const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6), nkv = p.num_kv_heads;
+  const int h = uniform((int)(blockIdx.x % nkv)), rest = uniform((int)(blockIdx.x / nkv));
+  const int split = uniform(rest % p.key_splits), unit = uniform(rest / p.key_splits);
+  const int r = uniform(unit_request(p.qo_indptr, p.group, kRowBlock, p.batch, unit));
+  if (r < 0) return;
+  const WRequest q = w_request(p, r);
+  if (q.rows <= kWRows || q.len <= 0) return;
+  const int row0 = (unit - unit_begin(p.qo_indptr, p.group, kRowBlock, r)) * kRowBlock;
+  if (row0 >= q.rows) return;
+  const int off = q.len - q.qo_len, last_row = min(row0 + kRowBlock, q.rows) - 1;
+  const int keys = p.causal ? min(q.len, off + last_row / p.group + 1) : q.len;  // seen by some row
+  const int tiles = keys > 0 ? (keys + 15) >> 4 : 0;
+  const int t0 = share_begin(split, p.key_splits, tiles), t1 = share_begin(split + 1, p.key_splits, tiles);
+  const int col = lane & 15, grp = lane >> 4;
+  const float sl2 = KVT == kKvFp8 ? p.scale_log2 * ((const float*)p.k_scale)[h] : p.scale_log2;
+  uint4 qf[NB][Tile::STEPS];
+  int lim[NB], row[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    row[n] = row0 + 32 * wave + 16 * n + col;
+    const int at = min(row[n], q.rows - 1), tok = at / p.group;
+    Tile::query(p, q.qo_start + tok, h * p.group + at - tok * p.group, grp, qf[n]);
+    lim[n] = p.causal ? off + tok : q.len - 1;
+  }
+  float m[NB], l[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) m[n] = -kWInf, l[n] = 0.f;
+  const int clear = p.causal ? off + row0 / p.group : q.len - 1;  // keys up to here are seen by every row
+  auto load = [&](Tile& t, int i) {
+    const int tok = 16 * i, e = (int)((unsigned)tok / (unsigned)p.page_size);
+    t.load(p, safe_page(p, q.first + e), tok - e * p.page_size + col, h, grp);
+  };
+  auto compute = [&](const Tile& t, int i) {
+    const int tok = 16 * i;
+    uint4 kf[Tile::STEPS];
+    t.fragments(kf);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < Tile::STEPS; ++st) acc = MT::mma_16x16x32(kf[st], qf[n][st], acc);
+      float s[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = acc[j] * sl2;
+      if (tok + 15 > clear)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (tok + 4 * grp + j > lim[n]) s[j] = -kWInf;
+      const float mn = fmaxf(m[n], fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+      const float mu = mn == -kWInf ? 0.f : mn;
+      l[n] = l[n] * fast_exp2(m[n] - mu) +
+             ((fast_exp2(s[0] - mu) + fast_exp2(s[1] - mu)) + (fast_exp2(s[2] - mu) + fast_exp2(s[3] - mu)));
+      m[n] = mn;
+    }
+  };
+  Tile a, b;
+  if (t0 < t1) load(a, t0);
+  for (int i = t0; i < t1; i += 2) {
+    if (i + 1 < t1) load(b, i + 1);
+    compute(a, i);
+    if (i + 2 < t1) load(a, i + 2);
+    if (i + 1 < t1) compute(b, i + 1);
+  }
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const float mg = rows4_max(m[n]), mgu = mg == -kWInf ? 0.f : mg;
+    const float lg = rows4_sum(l[n] * fast_exp2(m[n] - mgu));
+    if (grp == 0 && row[n] < q.rows)
+      p.row_lse[((int64_t)split * nkv + h) * p.total_rows + (int64_t)q.qo_start * p.group + row[n]] = w_lse(mg, lg);
+  }
+}
+
+// Second pass: each key's sum of exp2(s - lse) over the rows that see it.  A workgroup takes 128
+// keys of a request and kv head, 32 to a wavefront, in registers, and a share of the rows: S = Q K^T, a
+// lane's four scores all of one key.
+template <typename MT, int KVT, int D>
+__global__ __launch_bounds__(256) void weights_cols_kernel(WeightsParams p) {
+  using Tile = KeyTile<MT, KVT, D>;
+  constexpr int NB = 2;
+  const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6), nkv = p.num_kv_heads;
+  const int h = uniform((int)(blockIdx.x % nkv)), rest = uniform((int)(blockIdx.x / nkv));
+  const int split = uniform(rest % p.row_splits), unit = uniform(rest / p.row_splits);
+  const int r = uniform(unit_request(p.kv_indptr, 1, p.key_pages, p.batch, unit));
+  if (r < 0) return;
+  const WRequest q = w_request(p, r);
+  if (q.rows <= kWRows) return;
+  // the unit's pages in blocks of 128 keys: one, but for pages that hold more
+  const int tok0 = (unit - unit_begin(p.kv_indptr, 1, p.key_pages, r)) * p.key_pages * p.page_size;
+  const int tok1 = min(tok0 + p.key_pages * p.page_size, q.len);
+  const int off = q.len - q.qo_len, G = p.group;
+  const int col = lane & 15, grp = lane >> 4;
+  const float sl2 = KVT == kKvFp8 ? p.scale_log2 * ((const float*)p.k_scale)[h] : p.scale_log2;
+  const float* lse = p.row_lse + (int64_t)h * p.total_rows + (int64_t)q.qo_start * G;
+  for (int base = tok0; base < tok1; base += kKeyBlock) {
+    uint4 kf[NB][Tile::STEPS];
+    int key[NB], from[NB];  // the key, and the first row that sees it
+    float sum[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int t16 = base + 32 * wave + 16 * n;
+      key[n] = t16 + col;
+      from[n] = p.causal ? max(0, key[n] - off) * G : 0;
+      sum[n] = 0.f;
+      const int at = min(t16, tok1 - 1) & ~15, e = (int)((unsigned)at / (unsigned)p.page_size);
+      Tile t;
+      t.load(p, safe_page(p, q.first + e), at - e * p.page_size + col, h, grp);
+      t.fragments(kf[n]);
+    }
+    // rows from the first that sees the block's first key, in tiles of 16
+    const int first = p.causal ? (max(0, base - off) * G) >> 4 : 0, tiles = ((q.rows + 15) >> 4) - first;
+    const int clear = p.causal ? max(0, min(base + kKeyBlock, q.len) - 1 - off) * G : 0;  // rows from here on see every key
+    const int t0 = first + share_begin(split, p.row_splits, max(0, tiles));
+    const int t1 = first + share_begin(split + 1, p.row_splits, max(0, tiles));
+    auto load = [&](uint4 (&qf)[Tile::STEPS], float (&e)[4], int i) {
+      const int at = min(16 * i + col, q.rows - 1), tok = at / G;
+      Tile::query(p, q.qo_start + tok, h * G + at - tok * G, grp, qf);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = 16 * i + 4 * grp + j;
+        e[j] = row < q.rows ? lse[row] : kWInf;
+      }
+    };
+    auto compute = [&](const uint4 (&qf)[Tile::STEPS], const float (&e)[4], int i) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < Tile::STEPS; ++st) acc = MT::mma_16x16x32(qf[st], kf[n][st], acc);
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = fast_exp2(acc[j] * sl2 - e[j]);
+        if (16 * i < clear)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (16 * i + 4 * grp + j < from[n]) x[j] = 0.f;
+        sum[n] += (x[0] + x[1]) + (x[2] + x[3]);
+      }
+    };
+    uint4 qa[Tile::STEPS], qb[Tile::STEPS];
+    float ea[4], eb[4];
+    if (t0 < t1) load(qa, ea, t0);
+    for (int i = t0; i < t1; i += 2) {
+      if (i + 1 < t1) load(qb, eb, i + 1);
+      compute(qa, ea, i);
+      if (i + 2 < t1) load(qa, ea, i + 2);
+      if (i + 1 < t1) compute(qb, eb, i + 1);
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const float total = rows4_sum(sum[n]);
+      if (grp != 0 || key[n] >= tok1) continue;
+      if (p.row_splits > 1) {
+        p.sums[((int64_t)split * nkv + h) * p.places + (int64_t)q.first * p.page_size + key[n]] = total;
+        continue;
+      }
+      const int e = (int)((unsigned)key[n] / (unsigned)p.page_size);
+      const int64_t page = p.kv_indices[q.first + e];
+      if (page < 0 || page >= p.max_pages) continue;
+      float* w = p.weights + (page * nkv + h) * p.page_size + key[n] - e * p.page_size;
+      *w = key[n] >= off ? total : *w + total;
+    }
+  }
+}
+
+enum : int { kWScores = 0, kWRowsPass = 1, kWColsPass = 2 };
+
+template <typename MT, int KVT, int D>
+static void launch_weights_d(const WeightsParams& p, int which, dim3 grid, hipStream_t s) {
+  if (which == kWScores) hipLaunchKernelGGL((weights_scores_kernel<MT, KVT, D>), grid, dim3(256), 0, s, p);
+  else if (which == kWRowsPass) hipLaunchKernelGGL((weights_rows_kernel<MT, KVT, D>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((weights_cols_kernel<MT, KVT, D>), grid, dim3(256), 0, s, p);
+}
+
+template <typename MT, int KVT>
+static int launch_weights_kvt(const WeightsParams& p, int head_dim, int which, dim3 grid, hipStream_t s) {
+  switch (head_dim) {
+    case 64: launch_weights_d<MT, KVT, 64>(p, which, grid, s); return MI_OK;
+    case 128: launch_weights_d<MT, KVT, 128>(p, which, grid, s); return MI_OK;
+    case 256: launch_weights_d<MT, KVT, 256>(p, which, grid, s); return MI_OK;
+    default: return MI_ERR_UNSUPPORTED;
+  }
+}
+
+int weights_launch_16(const WeightsParams& p, int q_dtype, int head_dim, int which, dim3 grid, hipStream_t s);
+int weights_launch_scaled(const WeightsParams& p, int q_dtype, int kvt, int head_dim, int which, dim3 grid, hipStream_t s);
+
+}  // namespace mi

@@ -132,6 +132,7 @@ class PositionInfo:
 class KVRequestState:
     """Per-request, per-label KV state (``kv_store.py:111-127``).
 
+    ``evicted`` (extension) marks a state whose tokens are not all it was given.
     ``slot`` is this state's row in the :class:`DeviceBlockTable` (-1: none yet).
 
     Page-list contract (what the reference's code paths do): ``page_indices``
@@ -149,6 +150,7 @@ class KVRequestState:
     read_in_progress: bool = False
     is_paused: bool = False
     slot: int = -1
+    evicted: bool = False  # cut by BatchedCacheManager.evict: its pages are no longer a prefix of a copy's
     _dev_list: object = field(default=None, repr=False, compare=False)
     _dev_len: int = field(default=0, repr=False, compare=False)
     _dev_ends: tuple = field(default=(-1, -1), repr=False, compare=False)

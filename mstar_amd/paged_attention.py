@@ -28,7 +28,10 @@ Differences from the reference, all deliberate:
   that stay visible.  It is an argument of the run and not of the plan, so a model
   that mixes windowed and full layers plans a step once.
 * ``rope_set_kv_cache`` (no reference counterpart) fuses the RoPE call that
-  precedes ``set_kv_cache`` in every layer with the append itself.
+  precedes ``set_kv_cache`` in every layer with the append itself, and
+  ``qk_norm_rope_set_kv_cache`` the norms of q and k before it as well.
+* ``accumulate_weights`` (no reference counterpart): how much attention the
+  cached tokens get, for :mod:`mstar_amd.eviction`.
 """
 
 from __future__ import annotations
@@ -328,6 +331,68 @@ class _FusedRopeAppend:
         _rope_set_kv_cache(self, kv_cache_layer, q, k, v, pos_ids, rotary_dim, interleave, rope_scale, rope_theta,
                            k_scale, v_scale, keep_k, llama31)
 
+    def qk_norm_rope_set_kv_cache(self, kv_cache_layer: torch.Tensor | MXKVLayer, q: torch.Tensor, k: torch.Tensor,
+                                  v: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, pos_ids: torch.Tensor,
+                                  eps: float = 1e-6, rotary_dim: int | None = None, interleave: bool = False,
+                                  rope_scale: float = 1, rope_theta: float = 1e4, k_scale: torch.Tensor | None = None,
+                                  v_scale: torch.Tensor | None = None, keep_k: bool = True,
+                                  llama31: dict | None = None) -> None:
+        """``apply_qk_norm_rope_pos_ids_inplace(q, k, q_weight, k_weight, pos_ids, ...)``, and k and v to the cache.
+
+        One launch for every cache type (``mi_qk_norm_rope``).  The other arguments are
+        ``rope_set_kv_cache``'s; q, k and v rows must be 16-byte aligned.  The rotated k is rounded
+        once, from fp32 to the cache's type; ``keep_k=False`` leaves ``k`` as it was.
+        """
+        from .rope import qk_norm_rope_append
+
+        if self.dtype is None:
+            raise RuntimeError("plan() must be called before qk_norm_rope_set_kv_cache()")
+        qk_norm_rope_append(q, k, v, q_weight, k_weight, kv_cache_layer, pos_ids, *self._append_target(), eps=eps,
+                            rotary_dim=rotary_dim, interleave=interleave, rope_scale=rope_scale, rope_theta=rope_theta,
+                            k_scale=k_scale, v_scale=v_scale, keep_k=keep_k, llama31=llama31)
+
+
+class _Weights:
+    """``accumulate_weights``: the attention that cached tokens get (``mi_attention_weights``)."""
+
+    def accumulate_weights(self, q: torch.Tensor, kv_cache_layer: torch.Tensor | MXKVLayer, weights: torch.Tensor,
+                           k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
+        """Add to ``weights`` the probabilities that the planned step's queries give to their requests' tokens.
+
+        ``weights`` ``[max_pages, num_kv_heads, page_size]`` (fp32, contiguous; :func:`mstar_amd.eviction.kv_weights`)
+        holds one number for each kv head of each cache slot.  Summed over a request's queries and the q
+        heads of a kv head; the request's own tokens of this step begin at zero, so slots need no
+        clearing when their page gets a new owner.  Call it once a step and layer, with ``run``'s q, after the
+        append.  Sees the keys that ``run`` without a window sees.  Requests must not share pages.
+        """
+        if self.dtype is None:
+            raise RuntimeError("plan() must be called before accumulate_weights()")
+        if q.dtype != self.dtype:
+            q = q.to(self.dtype)
+        heads, dim, shape = self.num_qo_heads, self.head_dim, q.shape
+        qo, tokens, most, parts, causal = self._weights_batch()
+        if len(shape) != 3 or shape[0] < tokens or shape[1] != heads or shape[2] != dim:
+            raise ValueError(f"q shape {tuple(shape)} does not match the plan")
+        q, q_at, q_st, q_sh = _rows(q)
+        _check_devices(self.device, q=q, kv_cache_layer=kv_cache_layer, weights=weights)
+        desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
+        if desc.num_kv_heads != self.num_kv_heads or desc.head_dim != dim or desc.page_size != self.page_size:
+            raise ValueError("kv_cache_layer geometry does not match the wrapper")
+        want = (desc.max_pages, desc.num_kv_heads, desc.page_size)
+        if weights.dtype != torch.float32 or weights.shape != want or not weights.is_contiguous() or weights.data_ptr() % 16:
+            raise ValueError(f"weights must be a contiguous, 16-byte aligned float32 tensor {want}, got {tuple(weights.shape)}, "
+                             f"{weights.dtype}")
+        entries, n = self._indices.shape[0], self._n_req
+        if not parts or not n or not entries:
+            return
+        launch, ragged = _lib.lib(), qo is not None
+        nbytes = launch.mi_attention_weights_bytes(n, most, entries, self.page_size, heads, self.num_kv_heads, ragged, parts)
+        scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=self.device)
+        _lib.check(launch.mi_attention_weights(
+            q_at, _lib.TORCH_TO_MI[q.dtype], q_st, q_sh, desc, qo.data_ptr() if ragged else None, self._indptr.data_ptr(),
+            self._indices.data_ptr(), self._last.data_ptr(), n, most, entries, heads, 1 if causal else 0, self._sm_scale,
+            parts, weights.data_ptr(), scratch.data_ptr(), scratch.numel(), self._reading_stream()), "mi_attention_weights")
+
 
 class _PlanArrays:
     """The device arrays of a wrapper's plan, and the streams that read them.
@@ -361,7 +426,7 @@ class _PlanArrays:
             self._readers |= {stream}
 
 
-class PagedDecodeWrapper(_FusedRopeAppend, _PlanArrays):
+class PagedDecodeWrapper(_FusedRopeAppend, _Weights, _PlanArrays):
     """Batched paged decode attention (``flashinfer_utils.py:291-484``)."""
 
     def __init__(
@@ -554,8 +619,12 @@ class PagedDecodeWrapper(_FusedRopeAppend, _PlanArrays):
         loc = self.kv_cache_locations
         return loc, loc.data_ptr() + 8, 2, self._n_req, None
 
+    def _weights_batch(self):
+        """(qo_indptr, tokens, their bound, which requests there are: 1 short ones, 2 long ones, causal)."""
+        return None, self._n_req, self._n_req, 1, False
 
-class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
+
+class PagedPrefillWrapper(_FusedRopeAppend, _Weights, _PlanArrays):
     """Batched ragged paged prefill attention (``flashinfer_utils.py:70-288``)."""
 
     def __init__(
@@ -789,6 +858,11 @@ class PagedPrefillWrapper(_FusedRopeAppend, _PlanArrays):
         self._reading_stream()
         n_dev = self._qo.data_ptr() + 4 * self._n_req  # qo_indptr[n_req]: real count on the device
         return self.token_to_page, self.token_to_cache.data_ptr(), 1, self._total_tokens, n_dev
+
+    def _weights_batch(self):
+        # a paired plan's tiles may be requests of 9 to 16 rows, which are short ones here
+        parts = (1 if self._run_short or self._run_tiles else 0) | (2 if self._run_tiles else 0)
+        return self._qo, self._total_tokens, self._plan_max_tokens, parts, self.causal
 
 
 # Reference names (mstar/utils/flashinfer_utils.py) for drop-in use.

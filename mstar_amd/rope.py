@@ -7,6 +7,8 @@ argument names and defaults.  q ``[tokens, Hq, D]`` and k ``[tokens, Hkv, D]``
 (bf16 or fp16, last dim contiguous) are rotated in place by ``mi_rope_apply``;
 there is no CPU fallback.  ``rope_append`` fuses the rotation with the paged
 K/V append that follows it in ``run_attention`` (``mi_rope_append``).
+``apply_qk_norm_rope_pos_ids_inplace`` and ``qk_norm_rope_append`` normalise q and k head
+by head before the rotation, in the same pass (``mi_qk_norm_rope``).
 """
 
 from __future__ import annotations
@@ -121,6 +123,98 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache_laye
         ),
         "mi_rope_append",
     )
+
+
+def _norm_weight(w: torch.Tensor, name: str, x: torch.Tensor) -> int:
+    """The type code of a norm's weight; refuses what the kernel does not read."""
+    if w.dim() != 1 or w.shape[0] != x.shape[2] or not w.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector of head_dim {x.shape[2]} elements, got {tuple(w.shape)}")
+    if w.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"{name} must be {x.dtype} or float32, got {w.dtype}")
+    if w.device != x.device:
+        raise ValueError(f"{name} must be on {x.device}, not on {w.device}")
+    return _DTYPES.get(w.dtype, _lib.MI_F32)
+
+
+def _qk_norm_rope(q, k, v, q_weight, k_weight, pos_ids, eps, rotary_dim, interleave, rope_scale, rope_theta, llama31,
+                  keep_k, desc, page_idx, slot_idx_ptr, idx_stride, num_append, num_append_device_ptr) -> None:
+    _check(q, "q")
+    _check(k, "k")
+    if q.dtype != k.dtype or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.device != k.device:
+        raise ValueError("q and k must agree on dtype, device, token count and head_dim")
+    d = q.shape[2]
+    rd = d if rotary_dim is None else int(rotary_dim)
+    least = 8 if interleave else 16
+    if rd <= 0 or rd > d or rd % least or d % 8 or d > 512:
+        raise ValueError(f"rotary_dim {rd} must be a multiple of {least} and head_dim {d} one of 8 up to 512, rotary_dim <= head_dim")
+    wd = _norm_weight(q_weight, "q_weight", q)
+    if _norm_weight(k_weight, "k_weight", k) != wd:
+        raise ValueError("q_weight and k_weight must share one dtype")
+    if not eps >= 0:
+        raise ValueError(f"eps {eps} must not be negative")
+    rows = [("q", q), ("k", k)] + ([("v", v)] if v is not None else [])
+    for name, x in rows:
+        if x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16:
+            raise ValueError(f"{name}: rows must be 16-byte aligned")
+    if pos_ids.dtype not in _POS or pos_ids.dim() != 1 or pos_ids.shape[0] < q.shape[0]:
+        raise ValueError("pos_ids must be an int32/int64 vector with one position per token")
+    pos_ids = pos_ids.to(q.device).contiguous()
+    l31 = llama31 or {}
+    _lib.check(
+        _lib.lib().mi_qk_norm_rope(
+            q.data_ptr(), q.stride(0), q.stride(1), q.shape[1], k.data_ptr(), k.stride(0), k.stride(1), k.shape[1],
+            v.data_ptr() if v is not None else None, v.stride(0) if v is not None else 0, v.stride(1) if v is not None else 0,
+            _DTYPES[q.dtype], d, q_weight.data_ptr(), k_weight.data_ptr(), wd, float(eps), 1 if keep_k else 0, desc,
+            page_idx.data_ptr() if page_idx is not None else None, slot_idx_ptr, idx_stride, num_append,
+            num_append_device_ptr, rd, pos_ids.data_ptr(), _POS[pos_ids.dtype], q.shape[0], 1 if interleave else 0,
+            float(rope_scale), float(rope_theta), 1 if llama31 else 0, float(l31.get("low_freq_factor", 1.0)),
+            float(l31.get("high_freq_factor", 4.0)), float(l31.get("old_context_len", 8192.0)),
+            _lib.stream_ptr(q.device),
+        ),
+        "mi_qk_norm_rope",
+    )
+
+
+def apply_qk_norm_rope_pos_ids_inplace(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                                       pos_ids: torch.Tensor, eps: float = 1e-6, rotary_dim: int | None = None,
+                                       interleave: bool = False, rope_scale: float = 1, rope_theta: float = 1e4,
+                                       llama31: dict | None = None) -> None:
+    """Normalise every head's row of q and k, then rotate it, in place and in one pass.
+
+    A row x becomes ``x * rsqrt(mean(x^2) + eps) * weight`` (``q_weight``, ``k_weight``: ``[head_dim]``, in q's dtype
+    or fp32), rotated as :func:`apply_rope_pos_ids_inplace` rotates (with ``llama31``'s factors as
+    :func:`apply_llama31_rope_pos_ids_inplace`, ``rope_scale`` given).  fp32 throughout, rounded once; angles are formed in 64
+    bits, so far positions turn more exactly than in the calls without a norm.
+    """
+    _qk_norm_rope(q, k, None, q_weight, k_weight, pos_ids, eps, rotary_dim, interleave, rope_scale, rope_theta, llama31,
+                  True, None, None, None, 0, 0, None)
+
+
+def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                        kv_cache_layer, pos_ids: torch.Tensor, page_idx: torch.Tensor, slot_idx_ptr: int, idx_stride: int,
+                        num_append: int, num_append_device_ptr: int | None, *, eps: float = 1e-6,
+                        rotary_dim: int | None = None, interleave: bool = False, rope_scale: float = 1,
+                        rope_theta: float = 1e4, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                        keep_k: bool = True, llama31: dict | None = None) -> None:
+    """:func:`apply_qk_norm_rope_pos_ids_inplace`, and k and v to the paged cache, in one launch.
+
+    Page map and ``keep_k`` as in :func:`rope_append`; any cache type, microscaled layers among them.  k is rounded
+    once, from fp32 to the cache's type.
+    """
+    _check(q, "q")
+    _check(k, "k")
+    _check(v, "v")
+    if v.dtype != k.dtype or v.shape != k.shape or v.device != k.device:
+        raise ValueError(f"v {tuple(v.shape)}, {v.dtype} does not agree with k {tuple(k.shape)}, {k.dtype}")
+    desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
+    if kv_cache_layer.device != k.device:
+        raise ValueError(f"kv_cache_layer must be on {k.device}, not on {kv_cache_layer.device}")
+    if k.shape[1:] != (desc.num_kv_heads, desc.head_dim):
+        raise ValueError(f"k/v shape {tuple(k.shape)} does not match the cache heads/head_dim")
+    if num_append > k.shape[0]:
+        raise ValueError(f"k/v hold {k.shape[0]} tokens, {num_append} planned")
+    _qk_norm_rope(q, k, v, q_weight, k_weight, pos_ids, eps, rotary_dim, interleave, rope_scale, rope_theta, llama31,
+                  keep_k, desc, page_idx, slot_idx_ptr, idx_stride, num_append, num_append_device_ptr)
 
 
 def rope_positions(qo_indptr: torch.Tensor, position_id_start: torch.Tensor, out: torch.Tensor,

@@ -1,0 +1,238 @@
+"""GPU: eviction by weights (mi_kv_evict): places, rows, scale bytes and weights exactly as by the definition."""
+
+import numpy as np
+import pytest
+import torch
+
+from gpu_helpers import custom_batch, log
+from mstar_amd.eviction import evict_kv_cache, kv_weights
+from mstar_amd.mx_cache import MXKVCache, MXKVLayer
+from oracle import eviction as E
+
+pytestmark = pytest.mark.gpu
+
+
+def _bytes(cache):
+    return [t.view(torch.uint8) for t in ((cache.codes, cache.scales) if isinstance(cache, (MXKVLayer, MXKVCache)) else (cache,))]
+
+
+def _pool(kind, layers, pool, ps, hkv, d, gpu, seed):
+    """A pool of random bytes in the kind's layout."""
+    g = torch.Generator().manual_seed(seed)
+    if kind in ("mx8", "mx4"):
+        cache = MXKVCache(layers or 1, pool, ps, hkv, d, bits=int(kind[2]), device=gpu)
+        for t in (cache.codes, cache.scales):
+            t.copy_(torch.randint(0, 256, t.shape, dtype=torch.uint8, generator=g))
+        return cache if layers else cache[0]
+    dtype = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32, "fp8": torch.float8_e4m3fn}[kind]
+    shape = ([layers] if layers else []) + [pool, 2, ps, hkv, d]
+    esz = torch.empty(0, dtype=dtype).element_size()
+    return torch.randint(0, 256, (*shape[:-1], d * esz), dtype=torch.uint8, generator=g).view(dtype).to(gpu)
+
+
+def _expect(cache, weights, out_weights, indptr, indices, last, keep, recent, sinks, ps, layers):
+    """The definition, on copies on the CPU."""
+    kv = [t.cpu().clone() for t in _bytes(cache)]
+    old, new = weights.cpu(), out_weights.cpu().clone()
+    if not layers:
+        kv, old, new = [t[None] for t in kv], old[None], new[None]
+    hkv, n = old.shape[2], len(last)
+    kept = np.full((old.shape[0], n, hkv, keep), -1, np.int32)
+    source = [t.clone() for t in kv]
+    for r in range(n):
+        pages = indices[indptr[r]:indptr[r + 1]].astype(np.int64)
+        length = (len(pages) - 1) * ps + int(last[r]) if len(pages) else 0
+        at = np.arange(length)
+        for layer in range(old.shape[0]):
+            for h in range(hkv):
+                w = old[layer, pages[at // ps], h, at % ps].numpy() if length else np.zeros(0, np.float32)
+                places = E.kept_places(w, keep, recent, sinks)
+                m = len(places)
+                kept[layer, r, h, :m] = places
+                if not m:
+                    continue
+                to = np.arange(m)
+                new[layer, pages[to // ps], h, to % ps] = old[layer, pages[places // ps], h, places % ps]
+                for t, s in zip(kv, source):
+                    if t.shape[3] == ps:   # rows
+                        t[layer, pages[to // ps], :, to % ps, h] = s[layer, pages[places // ps], :, places % ps, h]
+                    else:                  # scale bytes, tokens last
+                        t[layer, pages[to // ps], :, h, :, to % ps] = s[layer, pages[places // ps], :, h, :, places % ps]
+    return kept if layers else kept[0], kv if layers else [t[0] for t in kv], new if layers else new[0]
+
+
+def _weights(shape, seed, ties=True):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.exp(2 * torch.randn(shape, generator=g))
+    return torch.where(torch.rand(shape, generator=g) < 0.3, (w * 2).round() / 2, w) if ties else w
+
+
+def _check(gpu, kind, layers, lens, ps, hkv, d, keep, recent, sinks, in_place, weights=None, seed=1):
+    pool = sum(-(-n // ps) for n in lens) + 4
+    _, indptr, indices, last = custom_batch(lens, ps, pool, seed)
+    cache = _pool(kind, layers, pool, ps, hkv, d, gpu, seed)
+    w = _weights(kv_weights(cache).shape, seed) if weights is None else weights(kv_weights(cache).shape)
+    on = w.to(gpu)
+    out = on if in_place else torch.full(w.shape, -7.0, device=gpu)
+    kept, kv, new = _expect(cache, w, out, indptr, indices, last, keep, recent, sinks, ps, layers)
+    log(f"{kind} layers {layers} lens {lens[:6]} keep {keep} recent {recent} sinks {sinks} in place {in_place}")
+    got = evict_kv_cache(cache, on, *(torch.as_tensor(a) for a in (indptr, indices, last)), keep=keep, recent=recent, sinks=sinks,
+                         out_weights=None if in_place else out)
+    torch.cuda.synchronize()
+    assert np.array_equal(got.cpu().numpy(), kept)
+    for a, b in zip(_bytes(cache), kv):
+        assert torch.equal(a.cpu(), b)
+    assert torch.equal(out.cpu().view(torch.int32), new.view(torch.int32))
+    if not in_place:
+        assert torch.equal(on.cpu().view(torch.int32), w.view(torch.int32))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32", "fp8", "mx8", "mx4"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_types_and_head_dims(gpu, kind, d):
+    _check(gpu, kind, 0, [1, 40, 41, 300, 0, 64], 16, 2, d, 40, 10, 3, True)
+    _check(gpu, kind, 3, [77, 500], 16, 1, d, 64, 16, 4, False)
+
+
+@pytest.mark.parametrize("lens,ps,hkv,keep,recent,sinks", [
+    ([100], 16, 1, 1, 0, 0), ([100], 16, 1, 1, 1, 0), ([100], 16, 1, 1, 0, 1),      # one token
+    ([100, 17], 16, 3, 16, 10, 6),                                                  # nothing by weight
+    ([100, 17], 16, 3, 16, 16, 0), ([100, 17], 16, 3, 16, 0, 16),
+    ([33, 34, 35, 0, 32], 32, 2, 33, 5, 5),                                         # one past the budget
+    ([1000, 999, 4], 48, 2, 500, 100, 7),
+    ([4096, 4097, 5000], 128, 1, 4096, 64, 4),
+    ([20000], 16, 2, 1000, 100, 4),
+    ([70000, 3], 16, 1, 9999, 1, 1),
+])
+def test_budgets(gpu, lens, ps, hkv, keep, recent, sinks):
+    for in_place in (True, False):
+        _check(gpu, "bf16", 0, lens, ps, hkv, 64, keep, recent, sinks, in_place)
+
+
+def _special(shape):
+    """Zeros of both signs, infinities, NaN, negative and subnormal weights."""
+    g = torch.Generator().manual_seed(3)
+    values = torch.tensor([0.0, -0.0, float("inf"), -float("inf"), float("nan"), 1e-42, -1e-42, -3.0, 2.0, 3e38])
+    return values[torch.randint(0, len(values), shape, generator=g)]
+
+
+@pytest.mark.parametrize("weights", [_special, torch.zeros, lambda s: torch.full(s, float("nan")),
+                                     lambda s: torch.arange(int(np.prod(s))).view(s).float(),
+                                     lambda s: -torch.arange(int(np.prod(s))).view(s).float()],
+                         ids=["special", "zeros", "nan", "rising", "falling"])
+def test_weights(gpu, weights):
+    for keep, recent, sinks in ((50, 5, 2), (150, 0, 0), (400, 100, 100)):
+        _check(gpu, "bf16", 0, [500, 199, 401], 16, 2, 64, keep, recent, sinks, True, weights=weights)
+
+
+def test_many_layers_and_requests(gpu):
+    _check(gpu, "fp8", 7, np.random.default_rng(1).integers(1, 300, 20).tolist(), 16, 2, 64, 100, 20, 4, True)
+    _check(gpu, "mx4", 2, np.random.default_rng(2).integers(1, 3000, 9).tolist(), 32, 3, 128, 700, 50, 4, True)
+
+
+def test_again_after_more_tokens(gpu):
+    """Evicted, grown and evicted again, on the shorter page lists that remain."""
+    ps, hkv, d, keep = 16, 2, 64, 48
+    cache = _pool("bf16", 0, 40, ps, hkv, d, gpu, 5)
+    w = _weights((40, hkv, ps), 6).to(gpu)
+    pages = np.arange(3, 30).astype(np.int32)
+    for length in (400, 48 + 90, 48 + 1, 48):
+        n = -(-length // ps)
+        idx = (np.array([0, n], np.int32), pages[:n], np.array([length - (n - 1) * ps], np.int32))
+        kept, kv, new = _expect(cache, w, w, *idx, keep, 8, 2, ps, 0)
+        got = evict_kv_cache(cache, w, *(torch.as_tensor(a).to(gpu) for a in idx), keep=keep, recent=8, sinks=2)
+        torch.cuda.synchronize()
+        assert np.array_equal(got.cpu().numpy(), kept) and torch.equal(cache.cpu().view(torch.uint8), kv[0])
+        assert torch.equal(w.cpu(), new)
+
+
+def test_other_layouts_and_a_side_stream(gpu):
+    """Heads before tokens, layers apart by more than a layer, and another stream."""
+    ps, hkv, d, pool = 16, 2, 64, 30
+    wide = _pool("bf16", 6, pool, ps, hkv, d, gpu, 5)
+    cache = wide[::2].permute(0, 1, 2, 4, 3, 5).contiguous().permute(0, 1, 2, 4, 3, 5)
+    cache = cache if cache.stride(-2) != d else cache
+    w = _weights((3, pool, hkv, ps), 6).to(gpu)
+    _, indptr, indices, last = custom_batch([200, 90], ps, pool, 3)
+    kept, kv, new = _expect(cache.contiguous(), w, w, indptr, indices, last, 50, 5, 2, ps, 3)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = evict_kv_cache(cache, w, *(torch.as_tensor(a).to(gpu) for a in (indptr, indices, last)), keep=50, recent=5, sinks=2)
+    side.synchronize()
+    assert np.array_equal(got.cpu().numpy(), kept) and torch.equal(cache.contiguous().cpu().view(torch.uint8), kv[0])
+    assert torch.equal(w.cpu(), new)
+    strided = _pool("bf16", 6, pool, ps, hkv, d, gpu, 5)
+    untouched = strided[1::2].clone()
+    w = _weights((3, pool, hkv, ps), 6).to(gpu)
+    evict_kv_cache(strided[::2], w, *(torch.as_tensor(a).to(gpu) for a in (indptr, indices, last)), keep=50, recent=5, sinks=2)
+    torch.cuda.synchronize()
+    assert torch.equal(strided[::2].contiguous().cpu().view(torch.uint8), kv[0])
+    assert torch.equal(strided[1::2].contiguous().view(torch.uint8), untouched.contiguous().view(torch.uint8))
+
+
+def test_captured_and_replayed(gpu):
+    ps, hkv, d, pool, b = 16, 2, 64, 60, 3
+    cache, w = _pool("bf16", 2, pool, ps, hkv, d, gpu, 1), torch.zeros(2, pool, hkv, ps, device=gpu)
+    indptr, indices = torch.zeros(b + 1, dtype=torch.int32, device=gpu), torch.zeros(pool, dtype=torch.int32, device=gpu)
+    last = torch.ones(b, dtype=torch.int32, device=gpu)
+    evict_kv_cache(cache, w, indptr, indices, last, keep=40, recent=5, sinks=2)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = evict_kv_cache(cache, w, indptr, indices, last, keep=40, recent=5, sinks=2)
+    for i, lens in enumerate(([300, 39, 100], [41, 40, 600], [1, 0, 2])):
+        _, ip, ix, la = custom_batch(lens, ps, pool, i)
+        cache.copy_(_pool("bf16", 2, pool, ps, hkv, d, gpu, 10 + i))
+        w.copy_(_weights(w.shape, i))
+        indptr.copy_(torch.as_tensor(ip)), indices[: len(ix)].copy_(torch.as_tensor(ix)), last.copy_(torch.as_tensor(la))
+        want = _expect(cache, w, w, ip, ix, la, 40, 5, 2, ps, 2)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(kept.cpu().numpy(), want[0]) and torch.equal(cache.cpu().view(torch.uint8), want[1][0])
+        assert torch.equal(w.cpu(), want[2])
+
+
+def test_pages_out_of_range_stay(gpu):
+    """Tokens on a page out of range weigh least; nothing is read from or written to it."""
+    ps, hkv, d, pool = 16, 1, 64, 8
+    cache = _pool("bf16", 0, pool, ps, hkv, d, gpu, 1)
+    before = cache.clone()
+    w = torch.ones(pool, hkv, ps, device=gpu)
+    for bad in (pool, -1, 2 ** 31 - 1):
+        got = evict_kv_cache(cache, w, torch.tensor([0, 4]), torch.tensor([3, bad, 5, 6]), torch.tensor([16]), keep=40)
+        torch.cuda.synchronize()
+        assert got.cpu()[0, 0].tolist() == [*range(16), *range(32, 56)]
+        assert torch.equal(cache[[0, 1, 2, 4, 7]].view(torch.uint8), before[[0, 1, 2, 4, 7]].view(torch.uint8))
+
+
+def test_nothing_to_do(gpu):
+    cache = _pool("bf16", 2, 4, 16, 1, 64, gpu, 1)
+    before, w = cache.clone(), kv_weights(cache)
+    empty = torch.zeros(0, dtype=torch.int32)
+    assert evict_kv_cache(cache, w, torch.zeros(1, dtype=torch.int32), empty, empty, keep=5).shape == (2, 0, 1, 5)
+    got = evict_kv_cache(cache, w, torch.zeros(3, dtype=torch.int32), empty, torch.ones(2, dtype=torch.int32), keep=5)
+    assert bool((got == -1).all())
+    assert torch.equal(cache.view(torch.uint8), before.view(torch.uint8))
+
+
+def test_refusals(gpu):
+    cache = _pool("bf16", 2, 8, 16, 2, 64, gpu, 1)
+    w = kv_weights(cache)
+    idx = (torch.tensor([0, 3]), torch.tensor([0, 1, 2]), torch.tensor([7]))
+
+    def call(cache=cache, w=w, idx=idx, keep=20, **kw):
+        return evict_kv_cache(cache, w, *idx, keep=keep, **kw)
+
+    before = cache.clone()
+    for bad in (lambda: call(keep=0), lambda: call(keep=-1), lambda: call(recent=-1), lambda: call(sinks=-1), lambda: call(recent=15, sinks=6),
+                lambda: call(keep=2 ** 31), lambda: call(w=w[0]), lambda: call(w=w.double()), lambda: call(w=w.cpu()), lambda: call(cache=cache[0]),
+                lambda: call(cache=cache.cpu()), lambda: call(cache=cache[0, 0]), lambda: call(out_weights=w[:1]),
+                lambda: call(out_weights=w.half()), lambda: call(idx=(idx[0], idx[1], torch.tensor([1, 2]))),
+                lambda: call(cache=object()), lambda: call(cache=cache.to(torch.float64)),
+                lambda: call(w=torch.zeros(w.numel() + 1, device=gpu)[1:].view(w.shape)),
+                lambda: call(cache=cache[..., 4:60], w=w)):
+        with pytest.raises((ValueError, RuntimeError)):
+            bad()
+    torch.cuda.synchronize()
+    assert torch.equal(cache.view(torch.uint8), before.view(torch.uint8))
