@@ -137,8 +137,9 @@ struct WeightsCut {
   int64_t scores, unit_lse, row_lse, sums, total;                      // bytes
 };
 
+// block: rows and keys of a workgroup of the long path's passes (the scratch does not depend on it).
 static WeightsCut weights_cut(int32_t batch, int32_t max_qo_tokens, int32_t num_indices, int32_t page_size, int32_t nkv,
-                              int32_t group, bool ragged, int parts) {
+                              int32_t group, bool ragged, int parts, int block) {
   WeightsCut c{};
   const int64_t tokens = (int64_t)num_indices * page_size;
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
@@ -156,11 +157,11 @@ static WeightsCut weights_cut(int32_t batch, int32_t max_qo_tokens, int32_t num_
   }
   if (parts & 2) {
     const int64_t rows = (int64_t)max_qo_tokens * group, b = batch > 0 ? batch : 1;
-    c.row_units = (int32_t)(rows / kRowBlock + b);
-    c.key_splits = (int32_t)clamp(1024 / ((int64_t)c.row_units * nkv), 1, clamp(tokens / b / 256, 1, 16));
-    c.key_pages = (int32_t)up(kKeyBlock, page_size);
+    c.row_units = (int32_t)(rows / block + b);
+    c.key_splits = (int32_t)clamp(2048 / ((rows / 256 + b) * nkv), 1, clamp(tokens / b / 256, 1, 16));
+    c.key_pages = (int32_t)up(block, page_size);
     c.key_units = (int32_t)(num_indices / c.key_pages + b);
-    c.row_splits = (int32_t)clamp(1024 / ((int64_t)c.key_units * nkv), 1, clamp(rows / b / 64, 1, 8));
+    c.row_splits = (int32_t)clamp(2048 / ((tokens / 256 + b) * nkv), 1, clamp(rows / b / 128, 1, 8));
     c.row_lse = at;
     at = mi_align_up(at + 4 * rows * nkv * c.key_splits, 256);
     c.sums = at;
@@ -183,7 +184,7 @@ extern "C" int64_t mi_attention_weights_bytes(int32_t batch, int32_t max_qo_toke
   using namespace mi;
   if (!weights_shapes_ok(batch, max_qo_tokens, num_indices, page_size, num_qo_heads, num_kv_heads, parts)) return MI_ERR_INVALID;
   if (!ragged) parts = 1;
-  return weights_cut(batch, max_qo_tokens, num_indices, page_size, num_kv_heads, num_qo_heads / num_kv_heads, ragged != 0, parts).total;
+  return weights_cut(batch, max_qo_tokens, num_indices, page_size, num_kv_heads, num_qo_heads / num_kv_heads, ragged != 0, parts, kRowBlock).total;
 }
 
 extern "C" int mi_attention_weights(const void* q, int32_t q_dtype, int64_t q_stride_token, int64_t q_stride_head,
@@ -211,7 +212,8 @@ extern "C" int mi_attention_weights(const void* q, int32_t q_dtype, int64_t q_st
     return MI_ERR_UNSUPPORTED;
   const bool ragged = qo_indptr != nullptr;
   if (!ragged) parts = 1;
-  const WeightsCut c = weights_cut(batch, max_qo_tokens, num_indices, kv->page_size, nkv, group, ragged, parts);
+  const WeightsCut c = weights_cut(batch, max_qo_tokens, num_indices, kv->page_size, nkv, group, ragged, parts,
+                                   q_dtype == MI_F32 ? kRowBlock : mma_block(D));
   if (workspace_bytes < c.total) return MI_ERR_WORKSPACE;
   WeightsParams p{};
   p.q = q;

@@ -35,8 +35,9 @@ struct WeightsParams {
 };
 
 constexpr int kWRows = 16;       // rows of a short-query request
-constexpr int kRowBlock = 128;   // rows of a workgroup of the long path's first pass
+constexpr int kRowBlock = 128;   // rows of a workgroup of the fp32 long path's first pass
 constexpr int kKeyBlock = 128;   // keys of a workgroup of its second
+typedef __attribute__((ext_vector_type(16))) float f32x16;
 
 // The request of a unit, where request r's units begin at indptr[r] * mul / div + r: at least as many places
 // as it needs, and found from the index array alone.  -1: before the first.
@@ -234,13 +235,386 @@ __global__ __launch_bounds__(256) void weights_scores_kernel(WeightsParams p) {
   }
 }
 
+// Adds a key's sum to its weight, or leaves it to weights_sum_kernel where other workgroups have the other rows.
+MI_DEVICE void w_add(const WeightsParams& p, const WRequest& q, int h, int split, int key, int off, float total) {
+  if (p.row_splits > 1) {
+    p.sums[((int64_t)split * p.num_kv_heads + h) * p.places + (int64_t)q.first * p.page_size + key] = total;
+    return;
+  }
+  const int e = (int)((unsigned)key / (unsigned)p.page_size);
+  const int64_t page = p.kv_indices[q.first + e];
+  if (page < 0 || page >= p.max_pages) return;
+  float* w = p.weights + (page * p.num_kv_heads + h) * p.page_size + key - e * p.page_size;
+  *w = key >= off ? total : *w + total;
+}
+
 // ------------------------------------------------------------ long queries
+// Both passes hold one side of the product in registers and stream the other through LDS in tiles
+// of 32, on the 32x32x16 MFMA: a tile's fragment serves all of a wavefront's columns.  VALU bound: an exponential
+// is 16 cycles of a wavefront, as long as its share of the products at head_dim 128, and each pass has one a
+// score beside an FMA and an addition.
+template <typename MT>
+MI_DEVICE f32x16 mma_32x32x16(const uint4& a, const uint4& b, f32x16 c) {
+  if constexpr (MT::kDtype == MI_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bitcast<bf16x8>(a), bitcast<bf16x8>(b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(bitcast<f16x8>(a), bitcast<f16x8>(b), c, 0, 0, 0);
+}
+// Sum and maximum of the two lanes that hold a column's rows.
+MI_DEVICE float both_sum(float x) {
+  const uint32_t u = bitcast<uint32_t>(x);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return bitcast<float>((uint32_t)a[0]) + bitcast<float>((uint32_t)a[1]);
+}
+MI_DEVICE float both_max(float x) {
+  const uint32_t u = bitcast<uint32_t>(x);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(bitcast<float>((uint32_t)a[0]), bitcast<float>((uint32_t)a[1]));
+}
+
+constexpr int kTile = 32;                                        // rows of a streamed tile
+constexpr int stationary(int d) { return d <= 128 ? 2 : 1; }     // columns / 32 that a wavefront holds
+constexpr int mma_block(int d) { return 4 * kTile * stationary(d); }
+
+// A tile in LDS: rows of D 16-bit elements, 16-byte pieces swapped about so that the 16 rows that a
+// read takes at once lie in different banks.
+template <int D>
+MI_DEVICE int tile_at(int row, int piece) {
+  return row * (2 * D) + 16 * (piece ^ (D == 64 ? (row >> 1) & 7 : row & 15));
+}
+template <int D>
+MI_DEVICE uint4 tile_fragment(const uint8_t* tile, int row, int step, int hi) {
+  return *(const uint4*)(tile + tile_at<D>(row, 2 * step + hi));
+}
+
+// Eight elements of a cached row from element 8 * piece on, in the MFMA type.
+template <typename MT, int KVT, int D>
+MI_DEVICE uint4 key_piece(const WeightsParams& p, int64_t page, int slot, int h, int piece) {
+  constexpr int BITS = KVT == kKv16 ? 16 : KVT == kKvMx4 ? 4 : 8, ESZ = KVT == kKv16 ? 2 : 1;
+  const uint8_t* src = p.k + (page * p.page_stride + slot * p.token_stride + h * p.head_stride) * ESZ + piece * BITS;
+  if constexpr (KVT == kKv16) {
+    return *(const uint4*)src;
+  } else {
+    uint32_t w[KVT == kKvMx4 ? 1 : 2], o[4];
+    if constexpr (KVT == kKvMx4) {
+      w[0] = *(const uint32_t*)src;
+    } else {
+      const uint2 u = *(const uint2*)src;
+      w[0] = u.x, w[1] = u.y;
+    }
+    if constexpr (KVT == kKvFp8) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        o[2 * i] = fp8x2_to_mt<MT>(w[i], false);
+        o[2 * i + 1] = fp8x2_to_mt<MT>(w[i], true);
+      }
+    } else {
+      constexpr int NBLK = D / kMxBlock;
+      const uint8_t s = ((const uint8_t*)p.k_scale)[((page * 2 * p.num_kv_heads + h) * NBLK + piece / 4) * (int64_t)p.page_size + slot];
+      mx_to_mt<MT, KVT>(w, bitcast<float>((uint32_t)s << 23), o);
+      if constexpr (MT::kDtype == MI_F16)
+        if (mx_past_f16<KVT>(s)) f16_saturate(o);
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// The keys of a request as a stream of tiles: what a thread loads of each, and where in the cache that lies.
+template <typename MT, int KVT, int D>
+struct KeyStream {
+  static constexpr int UNIT = KVT == kKv16 ? 8 : 16;  // elements a thread loads at once
+  static constexpr int PER_ROW = D / UNIT, NU = (kTile * PER_ROW + 255) / 256;
+  static constexpr bool MX = KVT == kKvMx8 || KVT == kKvMx4;
+  u32x4_t w[NU];  // mx4: two words
+  uint8_t s[NU];
+  int entry[NU], slot[NU];
+  int64_t page[NU];
+
+  MI_DEVICE static int unit(int u) { return (int)threadIdx.x + 256 * u; }
+  MI_DEVICE static bool active(int u) { return kTile * PER_ROW % 256 == 0 || unit(u) < kTile * PER_ROW; }
+  MI_DEVICE void begin(const WeightsParams& p, const WRequest& q, int tile) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int tok = kTile * tile + unit(u) / PER_ROW;
+      entry[u] = (int)((unsigned)tok / (unsigned)p.page_size);
+      slot[u] = tok - entry[u] * p.page_size;
+      page[u] = safe_page(p, q.first + min(entry[u], q.pages - 1));
+    }
+  }
+  // Loads the tile that `page` is of, and the pages of the next.
+  MI_DEVICE void load(const WeightsParams& p, const WRequest& q, int h) {
+    constexpr int ESZ = KVT == kKv16 ? 2 : 1;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int part = unit(u) % PER_ROW;
+      if (active(u)) {
+        const uint8_t* src = p.k + (page[u] * p.page_stride + slot[u] * p.token_stride + h * p.head_stride) * ESZ;
+        if constexpr (KVT == kKvMx4) {
+          const uint2 x = *(const uint2*)(src + 8 * part);
+          w[u] = u32x4_t{x.x, x.y, 0u, 0u};
+        } else {
+          w[u] = *(const u32x4_t*)(src + 16 * part);
+        }
+        if constexpr (MX)
+          s[u] = ((const uint8_t*)p.k_scale)[((page[u] * 2 * p.num_kv_heads + h) * (D / kMxBlock) + part / 2) * (int64_t)p.page_size + slot[u]];
+      }
+      slot[u] += kTile;
+      while (slot[u] >= p.page_size) slot[u] -= p.page_size, ++entry[u];
+      page[u] = safe_page(p, q.first + min(entry[u], q.pages - 1));
+    }
+  }
+  MI_DEVICE void store(uint8_t* tile) const {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      if (!active(u)) continue;
+      const int row = unit(u) / PER_ROW, part = unit(u) % PER_ROW;
+      if constexpr (KVT == kKv16) {
+        *(u32x4_t*)(tile + tile_at<D>(row, part)) = w[u];
+      } else {
+        uint32_t o[8];
+        if constexpr (KVT == kKvFp8) {
+          const uint32_t x[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            o[2 * i] = fp8x2_to_mt<MT>(x[i], false);
+            o[2 * i + 1] = fp8x2_to_mt<MT>(x[i], true);
+          }
+        } else {
+          const float scale = bitcast<float>((uint32_t)s[u] << 23);
+          if constexpr (KVT == kKvMx8) {
+            const uint32_t x[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+            mx_to_mt<MT, KVT>(x, scale, o);
+          } else {
+            const uint32_t x[2] = {w[u].x, w[u].y};
+            mx_to_mt<MT, KVT>(x, scale, o);
+          }
+          if constexpr (MT::kDtype == MI_F16)
+            if (mx_past_f16<KVT>(s[u])) f16_saturate(o);
+        }
+        *(uint4*)(tile + tile_at<D>(row, 2 * part)) = make_uint4(o[0], o[1], o[2], o[3]);
+        *(uint4*)(tile + tile_at<D>(row, 2 * part + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+      }
+    }
+  }
+};
+
+// First pass: the log-sum-exp of every (query, q head) row.  A workgroup takes 128 or 256 rows of a
+// request and kv head and a share of the keys: S^T = K Q^T, a lane's scores all of one row.
+template <typename MT, int KVT, int D>
+__global__ __launch_bounds__(256, 2) void weights_rows_kernel(WeightsParams p) {
+  constexpr int NS = stationary(D), STEPS = D / 16, BLOCK = mma_block(D);
+  __shared__ __attribute__((aligned(16))) uint8_t s_tile[2][kTile * 2 * D];
+  const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6), nkv = p.num_kv_heads;
+  const int h = uniform((int)(blockIdx.x % nkv)), rest = uniform((int)(blockIdx.x / nkv));
+  const int split = uniform(rest % p.key_splits), unit = uniform(rest / p.key_splits);
+  const int r = uniform(unit_request(p.qo_indptr, p.group, BLOCK, p.batch, unit));
+  if (r < 0) return;
+  const WRequest q = w_request(p, r);
+  if (q.rows <= kWRows || q.len <= 0) return;
+  const int row0 = (unit - unit_begin(p.qo_indptr, p.group, BLOCK, r)) * BLOCK;
+  if (row0 >= q.rows) return;
+  const int off = q.len - q.qo_len, last_row = min(row0 + BLOCK, q.rows) - 1;
+  const int keys = p.causal ? min(q.len, off + last_row / p.group + 1) : q.len;  // seen by some row
+  const int tiles = keys > 0 ? (keys + kTile - 1) / kTile : 0;
+  const int t0 = share_begin(split, p.key_splits, tiles), t1 = share_begin(split + 1, p.key_splits, tiles);
+  const int col = lane & 31, hi = lane >> 5;
+  float sl2 = KVT == kKvFp8 ? p.scale_log2 * ((const float*)p.k_scale)[h] : p.scale_log2;
+  const uint32_t flip = sl2 < 0.f ? 0x80008000u : 0u;  // the maximum is taken of unscaled scores: the scale's sign goes to q
+  sl2 = fabsf(sl2);
+  uint4 qf[NS][STEPS];
+  int lim[NS], row[NS];
+#pragma unroll
+  for (int n = 0; n < NS; ++n) {
+    row[n] = row0 + kTile * (NS * wave + n) + col;
+    const int at = min(row[n], q.rows - 1), tok = at / p.group;
+    const uint16_t* src = (const uint16_t*)p.q + (int64_t)(q.qo_start + tok) * p.q_stride_tok + (int64_t)(h * p.group + at - tok * p.group) * p.q_stride_head;
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      uint4 u = *(const uint4*)(src + 16 * st + 8 * hi);
+      u.x ^= flip, u.y ^= flip, u.z ^= flip, u.w ^= flip;
+      qf[n][st] = u;
+    }
+    lim[n] = p.causal ? off + tok : q.len - 1;
+  }
+  float m[NS], l[NS];
+#pragma unroll
+  for (int n = 0; n < NS; ++n) m[n] = -kWInf, l[n] = 0.f;
+  const int clear = p.causal ? off + row0 / p.group : q.len - 1;  // keys up to here are seen by every row
+  KeyStream<MT, KVT, D> keys_in;
+  if (t0 < t1) {
+    keys_in.begin(p, q, t0);
+    keys_in.load(p, q, h);
+    keys_in.store(s_tile[0]);
+    if (t0 + 1 < t1) keys_in.load(p, q, h);
+  }
+  __syncthreads();
+  for (int i = t0; i < t1; ++i) {
+    const uint8_t* tile = s_tile[(i - t0) & 1];
+    if (i + 1 < t1) keys_in.store(s_tile[(i - t0 + 1) & 1]);
+    if (i + 2 < t1) keys_in.load(p, q, h);
+    f32x16 acc[NS] = {};
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      const uint4 a = tile_fragment<D>(tile, col, st, hi);
+#pragma unroll
+      for (int n = 0; n < NS; ++n) acc[n] = mma_32x32x16<MT>(a, qf[n][st], acc[n]);
+    }
+    const int tok = kTile * i;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      if (tok + kTile - 1 > clear)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (tok + (j & 3) + 8 * (j >> 2) + 4 * hi > lim[n]) acc[n][j] = -kWInf;
+      float top = fmaxf(acc[n][0], acc[n][1]);
+#pragma unroll
+      for (int j = 2; j < 16; j += 2) top = fmaxf(top, fmaxf(acc[n][j], acc[n][j + 1]));
+      top *= sl2;
+      if (__builtin_amdgcn_ballot_w64(top > m[n] + 8.f)) {  // raised only past 2^8: harmless in an fp32 sum, and rare
+        const float mn = fmaxf(m[n], top);
+        l[n] *= mn == -kWInf ? 0.f : fast_exp2(m[n] - mn);
+        m[n] = mn;
+      }
+      const float mu = m[n] == -kWInf ? 0.f : m[n];
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j & 3] += fast_exp2(fmaf(acc[n][j], sl2, -mu));
+      l[n] += (x[0] + x[1]) + (x[2] + x[3]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int n = 0; n < NS; ++n) {
+    const float mg = both_max(m[n]), mgu = mg == -kWInf ? 0.f : mg;
+    const float lg = both_sum(l[n] * fast_exp2(m[n] - mgu));
+    if (hi == 0 && row[n] < q.rows)
+      p.row_lse[((int64_t)split * nkv + h) * p.total_rows + (int64_t)q.qo_start * p.group + row[n]] = w_lse(mg, lg);
+  }
+}
+
+// Second pass: each key's sum of exp2(s - lse) over the rows that see it.  A workgroup takes 128 or 256
+// keys of a request and kv head and a share of the rows: S = Q K^T, a lane's scores all of one key.
+template <typename MT, int KVT, int D>
+__global__ __launch_bounds__(256, 2) void weights_cols_kernel(WeightsParams p) {
+  constexpr int NS = stationary(D), STEPS = D / 16, BLOCK = mma_block(D), PIECES = D / 8, NU = kTile * PIECES / 256;
+  __shared__ __attribute__((aligned(16))) uint8_t s_tile[2][kTile * 2 * D];
+  __shared__ __attribute__((aligned(16))) float s_lse[2][kTile];
+  const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6), nkv = p.num_kv_heads, tid = (int)threadIdx.x;
+  const int h = uniform((int)(blockIdx.x % nkv)), rest = uniform((int)(blockIdx.x / nkv));
+  const int split = uniform(rest % p.row_splits), unit = uniform(rest / p.row_splits);
+  const int r = uniform(unit_request(p.kv_indptr, 1, p.key_pages, p.batch, unit));
+  if (r < 0) return;
+  const WRequest q = w_request(p, r);
+  if (q.rows <= kWRows) return;
+  // the unit's pages in blocks: one, but for pages that hold more keys
+  const int tok0 = (unit - unit_begin(p.kv_indptr, 1, p.key_pages, r)) * p.key_pages * p.page_size;
+  const int tok1 = min(tok0 + p.key_pages * p.page_size, q.len);
+  const int off = q.len - q.qo_len, G = p.group, step_tok = kTile / G, step_g = kTile % G;
+  const int col = lane & 31, hi = lane >> 5;
+  const float sl2 = KVT == kKvFp8 ? p.scale_log2 * ((const float*)p.k_scale)[h] : p.scale_log2;
+  const float* lse = p.row_lse + (int64_t)h * p.total_rows + (int64_t)q.qo_start * G;
+  for (int base = tok0; base < tok1; base += BLOCK) {
+    // rows from the first that sees the block's first key on
+    const int first = p.causal ? (max(0, base - off) * G) / kTile : 0, tiles = max(0, (q.rows + kTile - 1) / kTile - first);
+    const int clear = p.causal ? max(0, min(base + BLOCK, q.len) - 1 - off) * G : 0;  // rows from here on see every key
+    const int t0 = first + share_begin(split, p.row_splits, tiles), t1 = first + share_begin(split + 1, p.row_splits, tiles);
+    // the stream of q rows: pieces of 16 bytes, and the tile's log-sum-exps
+    u32x4_t w[NU];
+    float e = kWInf;
+    int tok[NU], g[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int at = kTile * t0 + (tid + 256 * u) / PIECES;
+      tok[u] = at / G;
+      g[u] = at - tok[u] * G;
+    }
+    int lse_row = kTile * t0 + tid;
+    auto load = [&]() {
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const int t = min(tok[u], q.qo_len - 1);  // rows past the last: of the last token, and an lse of infinity
+        w[u] = *(const u32x4_t*)((const uint16_t*)p.q + (int64_t)(q.qo_start + t) * p.q_stride_tok + (int64_t)(h * G + g[u]) * p.q_stride_head +
+                               8 * ((tid + 256 * u) % PIECES));
+        tok[u] += step_tok;
+        g[u] += step_g;
+        if (g[u] >= G) g[u] -= G, ++tok[u];
+      }
+      if (tid < kTile) e = lse_row < q.rows ? lse[lse_row] : kWInf;
+      lse_row += kTile;
+    };
+    auto store = [&](int b) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u) *(u32x4_t*)(s_tile[b] + tile_at<D>((tid + 256 * u) / PIECES, (tid + 256 * u) % PIECES)) = w[u];
+      if (tid < kTile) s_lse[b][tid] = e;
+    };
+    if (t0 < t1) load();
+    uint4 kf[NS][STEPS];
+    int key[NS], from[NS];  // the key, and the first row that sees it
+    float sum[NS];
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      key[n] = base + kTile * (NS * wave + n) + col;
+      from[n] = p.causal ? max(0, key[n] - off) * G : 0;
+      sum[n] = 0.f;
+      const int at = min(key[n], tok1 - 1), en = (int)((unsigned)at / (unsigned)p.page_size);
+      const int64_t page = safe_page(p, q.first + en);
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) kf[n][st] = key_piece<MT, KVT, D>(p, page, at - en * p.page_size, h, 2 * st + hi);
+    }
+    if (t0 < t1) {
+      store(0);
+      if (t0 + 1 < t1) load();
+    }
+    __syncthreads();
+    for (int i = t0; i < t1; ++i) {
+      const int b = (i - t0) & 1;
+      if (i + 1 < t1) store(b ^ 1);
+      if (i + 2 < t1) load();
+      f32x16 acc[NS] = {};
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) {
+        const uint4 a = tile_fragment<D>(s_tile[b], col, st, hi);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) acc[n] = mma_32x32x16<MT>(a, kf[n][st], acc[n]);
+      }
+      float le[16];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 v = *(const float4*)(&s_lse[b][8 * j + 4 * hi]);
+        le[4 * j] = v.x, le[4 * j + 1] = v.y, le[4 * j + 2] = v.z, le[4 * j + 3] = v.w;
+      }
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        if (kTile * i < clear) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float v = fast_exp2(fmaf(acc[n][j], sl2, -le[j]));
+            x[j & 3] += kTile * i + (j & 3) + 8 * (j >> 2) + 4 * hi < from[n] ? 0.f : v;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j & 3] += fast_exp2(fmaf(acc[n][j], sl2, -le[j]));
+        }
+        sum[n] += (x[0] + x[1]) + (x[2] + x[3]);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      const float total = both_sum(sum[n]);
+      if (hi != 0 || key[n] >= tok1) continue;
+      w_add(p, q, h, split, key[n], off, total);
+    }
+  }
+}
+
+// ------------------------------------------------------------ long queries, fp32
 // First pass: the log-sum-exp of every (query, q head) row.  A workgroup takes 128 rows of a
 // request and kv head, 32 to a wavefront, and a share of the keys: S^T = K Q^T with the rows' q in
 // registers, a lane's four scores all of one row.
-template <typename MT, int KVT, int D>
-__global__ __launch_bounds__(256) void weights_rows_kernel(WeightsParams p) {
-  using Tile = KeyTile<MT, KVT, D>;
+template <int D>
+__global__ __launch_bounds__(256) void weights_rows_f32_kernel(WeightsParams p) {
+  using MT = F32;
+  using Tile = KeyTile<MT, kKv16, D>;
   constexpr int NB = 2;
   const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6), nkv = p.num_kv_heads;
   const int h = uniform((int)(blockIdx.x % nkv)), rest = uniform((int)(blockIdx.x / nkv));
@@ -256,7 +630,7 @@ __global__ __launch_bounds__(256) void weights_rows_kernel(WeightsParams p) {
   const int tiles = keys > 0 ? (keys + 15) >> 4 : 0;
   const int t0 = share_begin(split, p.key_splits, tiles), t1 = share_begin(split + 1, p.key_splits, tiles);
   const int col = lane & 15, grp = lane >> 4;
-  const float sl2 = KVT == kKvFp8 ? p.scale_log2 * ((const float*)p.k_scale)[h] : p.scale_log2;
+  const float sl2 = p.scale_log2;
   uint4 qf[NB][Tile::STEPS];
   int lim[NB], row[NB];
 #pragma unroll
@@ -317,9 +691,10 @@ __global__ __launch_bounds__(256) void weights_rows_kernel(WeightsParams p) {
 // Second pass: each key's sum of exp2(s - lse) over the rows that see it.  A workgroup takes 128
 // keys of a request and kv head, 32 to a wavefront, in registers, and a share of the rows: S = Q K^T, a
 // lane's four scores all of one key.
-template <typename MT, int KVT, int D>
-__global__ __launch_bounds__(256) void weights_cols_kernel(WeightsParams p) {
-  using Tile = KeyTile<MT, KVT, D>;
+template <int D>
+__global__ __launch_bounds__(256) void weights_cols_f32_kernel(WeightsParams p) {
+  using MT = F32;
+  using Tile = KeyTile<MT, kKv16, D>;
   constexpr int NB = 2;
   const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6), nkv = p.num_kv_heads;
   const int h = uniform((int)(blockIdx.x % nkv)), rest = uniform((int)(blockIdx.x / nkv));
@@ -333,7 +708,7 @@ __global__ __launch_bounds__(256) void weights_cols_kernel(WeightsParams p) {
   const int tok1 = min(tok0 + p.key_pages * p.page_size, q.len);
   const int off = q.len - q.qo_len, G = p.group;
   const int col = lane & 15, grp = lane >> 4;
-  const float sl2 = KVT == kKvFp8 ? p.scale_log2 * ((const float*)p.k_scale)[h] : p.scale_log2;
+  const float sl2 = p.scale_log2;
   const float* lse = p.row_lse + (int64_t)h * p.total_rows + (int64_t)q.qo_start * G;
   for (int base = tok0; base < tok1; base += kKeyBlock) {
     uint4 kf[NB][Tile::STEPS];
@@ -393,15 +768,7 @@ __global__ __launch_bounds__(256) void weights_cols_kernel(WeightsParams p) {
     for (int n = 0; n < NB; ++n) {
       const float total = rows4_sum(sum[n]);
       if (grp != 0 || key[n] >= tok1) continue;
-      if (p.row_splits > 1) {
-        p.sums[((int64_t)split * nkv + h) * p.places + (int64_t)q.first * p.page_size + key[n]] = total;
-        continue;
-      }
-      const int e = (int)((unsigned)key[n] / (unsigned)p.page_size);
-      const int64_t page = p.kv_indices[q.first + e];
-      if (page < 0 || page >= p.max_pages) continue;
-      float* w = p.weights + (page * nkv + h) * p.page_size + key[n] - e * p.page_size;
-      *w = key[n] >= off ? total : *w + total;
+      w_add(p, q, h, split, key[n], off, total);
     }
   }
 }
@@ -411,8 +778,13 @@ enum : int { kWScores = 0, kWRowsPass = 1, kWColsPass = 2 };
 template <typename MT, int KVT, int D>
 static void launch_weights_d(const WeightsParams& p, int which, dim3 grid, hipStream_t s) {
   if (which == kWScores) hipLaunchKernelGGL((weights_scores_kernel<MT, KVT, D>), grid, dim3(256), 0, s, p);
-  else if (which == kWRowsPass) hipLaunchKernelGGL((weights_rows_kernel<MT, KVT, D>), grid, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((weights_cols_kernel<MT, KVT, D>), grid, dim3(256), 0, s, p);
+  else if constexpr (MT::kDtype == MI_F32) {
+    if (which == kWRowsPass) hipLaunchKernelGGL((weights_rows_f32_kernel<D>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((weights_cols_f32_kernel<D>), grid, dim3(256), 0, s, p);
+  } else {
+    if (which == kWRowsPass) hipLaunchKernelGGL((weights_rows_kernel<MT, KVT, D>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((weights_cols_kernel<MT, KVT, D>), grid, dim3(256), 0, s, p);
+  }
 }
 
 template <typename MT, int KVT>

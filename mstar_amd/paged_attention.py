@@ -54,6 +54,7 @@ __all__ = [
 
 _MAX_GROUP = 16  # q heads per kv head handled by one MFMA tile
 _WINDOW_MAX = 1 << 30  # beyond any context
+_PAIR_MIN_BATCH = 128  # smaller batches have no paired plans (mi_prefill_short_rows)
 # Ragged batches of up to _SERIAL_REQUESTS requests run their two parts one
 # after the other on one stream: the events of a fork and join cost the host
 # more than the overlap hides (us a layer, side stream -> in turn: one 512-token
@@ -861,7 +862,8 @@ class PagedPrefillWrapper(_FusedRopeAppend, _Weights, _PlanArrays):
 
     def _weights_batch(self):
         # a paired plan's tiles may be requests of 9 to 16 rows, which are short ones here
-        parts = (1 if self._run_short or self._run_tiles else 0) | (2 if self._run_tiles else 0)
+        short = self._run_short or (self._run_tiles and self._n_req >= _PAIR_MIN_BATCH)
+        parts = (1 if short else 0) | (2 if self._run_tiles else 0)
         return self._qo, self._total_tokens, self._plan_max_tokens, parts, self.causal
 
 
