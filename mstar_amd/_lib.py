@@ -262,6 +262,11 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def stream_at(index: int) -> int:
+    """:func:`stream_ptr` of the device with this index."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 _memcpy_async = None
 
 

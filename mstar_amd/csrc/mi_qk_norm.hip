@@ -7,11 +7,12 @@
 // The row's sum, the norm and the rotation are fp32, and a value is rounded once: to the
 // q / k type, and from fp32 to the cache's type.  Angles are formed in turns in 64 bits, pos *
 // f_i / (2 pi) less its nearest whole number, which is exact enough at any position (an fp32 angle is off
-// by 4e-3 rad at 65k tokens, half a step of bf16 and four of fp16); the f_i are the launch argument.
+// by 4e-3 rad at 65k tokens, half a step of bf16 and four of fp16).
 //
 // A row is head_dim / 8 lanes (rounded up to a power of two, 16-byte loads), so a wavefront
-// holds 64 / LPR rows of one token; its lanes' (cos, sin) are formed once and serve all the rows that
-// it goes through.  The other half of a rotated pair is 16 bytes of another lane of the row.
+// holds 64 / LPR rows of one token.  Its lanes form each pair's (cos, sin) once, a pair a lane, and share them
+// through LDS for all the rows that the wavefront goes through; with the weights they become two
+// factors an element, y = rs (x own + x' off), x' the pair's other element: a shuffle of 16 bytes.
 #include <cmath>
 
 #include "mi_internal.h"
@@ -32,19 +33,35 @@ struct NormRopeParams {
   const int64_t *page_idx, *slot_idx;
   int64_t idx_stride;
   const int32_t* num_tokens_device;
-  int32_t num_tokens, num_append, num_qo_heads, num_kv_heads, head_dim, page_size, rotary_dim, interleave, pos_is_64;
-  int32_t weight_f32, keep_k, rows, steps;  // rows: of a token; steps: that a wavefront goes through
+  int32_t num_tokens, num_append, num_qo_heads, num_kv_heads, head_dim, page_size, rotary_dim, pos_is_64;
+  int32_t weight_f32, keep_k, parts, part_steps, items;  // items: of a token and a part of its steps
   float eps;
-  double turns[kNormDimMax / 2];  // of pair i a position
+  // turns a position of pair i: g = 2^(i step); g / scale, or blended with g by smooth = slope g - bias
+  double step, inv_scale, slope, bias;
+  int32_t llama31;
 };
 
 enum : int { kNoCache = -1 };
 
+template <int CTRL>
+MI_DEVICE float dpp_add(float x) {
+  return x + bitcast<float>((uint32_t)__builtin_amdgcn_update_dpp(0, (int)bitcast<uint32_t>(x), CTRL, 0xf, 0xf, false));
+}
 // Sum over the LPR adjacent lanes of a row, in all of them.
 template <int LPR>
 MI_DEVICE float row_sum(float x) {
-#pragma unroll
-  for (int m = 1; m < LPR; m <<= 1) x += __shfl_xor(x, m, kWave);
+  x = dpp_add<0xb1>(x);                        // quad_perm [1,0,3,2]
+  x = dpp_add<0x4e>(x);                        // quad_perm [2,3,0,1]
+  x = dpp_add<0x141>(x);                       // row_half_mirror
+  if constexpr (LPR >= 16) x = dpp_add<0x140>(x);  // row_mirror
+  if constexpr (LPR >= 32) {
+    const auto a = __builtin_amdgcn_permlane16_swap(bitcast<uint32_t>(x), bitcast<uint32_t>(x), false, false);
+    x = bitcast<float>((uint32_t)a[0]) + bitcast<float>((uint32_t)a[1]);
+  }
+  if constexpr (LPR >= 64) {
+    const auto a = __builtin_amdgcn_permlane32_swap(bitcast<uint32_t>(x), bitcast<uint32_t>(x), false, false);
+    x = bitcast<float>((uint32_t)a[0]) + bitcast<float>((uint32_t)a[1]);
+  }
   return x;
 }
 
@@ -82,190 +99,227 @@ MI_DEVICE void norm_cache_store(uint8_t* row, float (&y)[8], const uint4& packed
   }
 }
 
-// Rows of a token: q heads, k heads and, with a cache, v heads.
+MI_DEVICE void read8(const float* src, float (&x)[8]) {
+  const float4 a = ((const float4*)src)[0], b = ((const float4*)src)[1];
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+
+// Of a step's rows: 0 q, 1 k, 2 v.
+MI_DEVICE int kind_of(int st, int nq, int nk) { return st < nq ? 0 : st < nq + nk ? 1 : 2; }
+// Element d0 of the row of head first + slot_row.
+MI_DEVICE uint16_t* norm_row(const NormRopeParams& p, int kind, int64_t t, int first, int slot_row, int d0) {
+  uint16_t* base = (uint16_t*)(kind == 0 ? p.q : kind == 1 ? p.k : const_cast<void*>(p.v));
+  const int64_t tok = kind == 0 ? p.q_stride_tok : kind == 1 ? p.k_stride_tok : p.v_stride_tok;
+  const int64_t head = kind == 0 ? p.q_stride_head : kind == 1 ? p.k_stride_head : p.v_stride_head;
+  return base + (t * tok + first * head) + (slot_row * head + d0);
+}
+
+// A token's steps: its q heads, RPW at a time, then its k heads and, with a cache, its v heads.
 template <typename MT, int DST, int LPR, bool INTERLEAVE>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRopeParams p) {
-  constexpr int RPW = kWave / LPR;
-  const int lane = lane_id(), sub = lane % LPR, slot_row = lane / LPR;
-  const int per_token = (p.rows + RPW * p.steps - 1) / (RPW * p.steps);
-  const int64_t unit = (int64_t)blockIdx.x * 4 + uniform((int)threadIdx.x >> 6);
-  const int64_t t = unit / per_token;
-  if (t >= p.num_tokens) return;
-  const int row0 = (int)(unit - t * per_token) * RPW * p.steps;
-  const int d0 = 8 * sub, hq = p.num_qo_heads, hkv = p.num_kv_heads;
+  constexpr int RPW = kWave / LPR, DIM = 8 * LPR, NP = (DIM / 2 + kWave - 1) / kWave, U = 4;
+  __shared__ __attribute__((aligned(16))) float s_w[2][DIM];             // of q, of k
+  __shared__ __attribute__((aligned(16))) float s_cos[4][DIM / 2], s_sin[4][DIM / 2];
+  const int tid = (int)threadIdx.x, lane = lane_id(), wave = uniform(tid >> 6), sub = lane % LPR, slot_row = lane / LPR;
+  const int d0 = 8 * sub, hq = p.num_qo_heads, hkv = p.num_kv_heads, half = p.rotary_dim >> 1;
   const bool in_row = d0 < p.head_dim, rot = d0 < p.rotary_dim;
-  const int half = p.rotary_dim >> 1;
-  // the lane that holds the other halves of this one's pairs, and whose elements they are
+  // the lane that holds the other halves of this one's pairs
   const int other = INTERLEAVE || !rot ? 0 : d0 < half ? half / 8 : -(half / 8);
-
-  // the token's cache row (K half, head 0)
-  int64_t page = -1, slot = 0;
-  if (DST != kNoCache && t < p.num_append) {
-    const bool real = !p.num_tokens_device || t < *p.num_tokens_device;
-    page = p.page_idx[t * p.idx_stride];
-    slot = p.slot_idx[t * p.idx_stride];
-    if (!real || page >= p.max_pages || slot < 0 || slot >= p.page_size) page = -1;
+  const int nq = (hq + RPW - 1) / RPW, nk = (hkv + RPW - 1) / RPW, total = nq + (DST == kNoCache ? 1 : 2) * nk;
+  for (int i = tid; i < 2 * DIM; i += 256) {
+    const int d = i % DIM;
+    const void* w = i < DIM ? p.q_weight : p.k_weight;
+    s_w[0][i] = d >= p.head_dim ? 0.f : p.weight_f32 ? ((const float*)w)[d] : MT::to_f32(((const uint16_t*)w)[d]);
   }
-
-  float wq[8], wk[8], wqo[8], wko[8];  // weights of this lane's elements and of the other halves
+  double turns[NP];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int i = in_row ? d0 + e : 0, j = in_row ? d0 + 8 * other + e : 0;
-    if (p.weight_f32) {
-      wq[e] = ((const float*)p.q_weight)[i], wk[e] = ((const float*)p.k_weight)[i];
-      wqo[e] = ((const float*)p.q_weight)[j], wko[e] = ((const float*)p.k_weight)[j];
-    } else {
-      wq[e] = MT::to_f32(((const uint16_t*)p.q_weight)[i]), wk[e] = MT::to_f32(((const uint16_t*)p.k_weight)[i]);
-      wqo[e] = MT::to_f32(((const uint16_t*)p.q_weight)[j]), wko[e] = MT::to_f32(((const uint16_t*)p.k_weight)[j]);
+  for (int j = 0; j < NP; ++j) {
+    const double g = exp2((double)(lane + kWave * j) * p.step);
+    double f = g * p.inv_scale;
+    if (p.llama31) {
+      const double smooth = fmin(fmax(g * p.slope - p.bias, 0.0), 1.0);
+      f = (1.0 - smooth) * f + smooth * g;
     }
+    turns[j] = f * 0.15915494309189533577;
   }
-  float c[8], s[8];  // of element e's pair; s with its sign in the element's sum
-  {
-    const double pos = p.pos_is_64 ? (double)((const int64_t*)p.pos)[t] : (double)((const int32_t*)p.pos)[t];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (INTERLEAVE && (e & 1)) continue;
-      const int pair = !rot ? 0 : INTERLEAVE ? (d0 + e) >> 1 : d0 < half ? d0 + e : d0 + e - half;
-      const double a = pos * p.turns[pair];
-      const float x = (float)(a - rint(a));
-      float sn, cs;
-      sincospif(2.f * x, &sn, &cs);
-      c[e] = cs;
-      if constexpr (INTERLEAVE) {
-        c[e + 1] = cs;
-        s[e] = -sn;
-        s[e + 1] = sn;
-      } else {
-        s[e] = d0 < half ? -sn : sn;
-      }
-    }
-  }
+  __syncthreads();
   const float inv_dim = 1.f / (float)p.head_dim;
 
-  for (int st = 0; st < p.steps; ++st) {
-    const int r = row0 + st * RPW + slot_row;
-    const bool live = r < p.rows && in_row, is_q = r < hq, is_v = r >= hq + hkv;
-    const int h = is_q ? r : is_v ? r - hq - hkv : r - hq;
-    uint16_t* src = nullptr;
-    if (live)
-      src = is_q   ? (uint16_t*)p.q + t * p.q_stride_tok + h * p.q_stride_head
-            : is_v ? (uint16_t*)p.v + t * p.v_stride_tok + h * p.v_stride_head
-                   : (uint16_t*)p.k + t * p.k_stride_tok + h * p.k_stride_head;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (live) u = *(const uint4*)(src + d0);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    float y[8], sq = 0.f;
+  for (int item = (int)blockIdx.x * 4 + wave; item < p.items; item += (int)gridDim.x * 4) {
+    const int token = p.parts == 1 ? item : (int)((unsigned)item / (unsigned)p.parts), s0 = (item - token * p.parts) * p.part_steps;
+    const int s1 = min(s0 + p.part_steps, total);
+    const int64_t t = token;
+    auto load = [&](int st) {
+      const int kind = kind_of(st, nq, nk), first = RPW * (st - (kind == 0 ? 0 : kind == 1 ? nq : nq + nk));
+      const bool live = in_row && first + slot_row < (kind == 0 ? hq : hkv);
+      return live ? *(const uint4*)norm_row(p, kind, t, first, slot_row, d0) : make_uint4(0, 0, 0, 0);
+    };
+    uint4 u[U];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      y[2 * i] = MT::to_f32((uint16_t)(w[i] & 0xffffu));
-      y[2 * i + 1] = MT::to_f32((uint16_t)(w[i] >> 16));
+    for (int i = 0; i < U; ++i)
+      if (s0 + i < s1) u[i] = load(s0 + i);
+
+    // the token's cache row (K half, head 0)
+    int64_t page = -1, slot = 0;
+    if (DST != kNoCache && s1 > nq && token < p.num_append) {
+      const bool real = !p.num_tokens_device || token < *p.num_tokens_device;
+      page = p.page_idx[t * p.idx_stride];
+      slot = p.slot_idx[t * p.idx_stride];
+      if (!real || page >= p.max_pages || slot < 0 || slot >= p.page_size) page = -1;
     }
+    // every pair's cosine and sine once, to the wavefront's part of LDS
+    if (s0 < nq + nk) {
+      const double pos = p.pos_is_64 ? (double)((const int64_t*)p.pos)[t] : (double)((const int32_t*)p.pos)[t];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sq += y[e] * y[e];
-    const float rs = rsqrtf(row_sum<LPR>(sq) * inv_dim + p.eps);
-    if constexpr (INTERLEAVE) {
-      if (!is_v) {
+      for (int j = 0; j < NP; ++j) {
+        const int pair = lane + kWave * j;
+        if (pair < half) {
+          const double a = pos * turns[j];
+          float sn, cs;
+          sincospif(2.f * (float)(a - rint(a)), &sn, &cs);
+          s_cos[wave][pair] = cs;
+          s_sin[wave][pair] = sn;
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    float own[8], off[8];  // an element's factor in its own sum, and its partner's
+    int kind = -1;
+    auto factors = [&](int which) {
+      read8(&s_w[which][d0], own);
+      read8(&s_w[which][d0 + 8 * other], off);
+      if (!rot) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] *= rs * (is_q ? wq[e] : wk[e]);
-        if (rot) {
+        for (int e = 0; e < 8; ++e) off[e] = 0.f;
+        return;
+      }
+      if constexpr (INTERLEAVE) {
+        const float4 c = *(const float4*)&s_cos[wave][d0 / 2], s = *(const float4*)&s_sin[wave][d0 / 2];
+        const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          off[e] = -own[e + 1] * sn[e / 2];
+          off[e + 1] = own[e] * sn[e / 2];
+          own[e] *= cs[e / 2];
+          own[e + 1] *= cs[e / 2];
+        }
+      } else {
+        const int at = d0 < half ? d0 : d0 - half;
+        float cs[8], sn[8];
+        read8(&s_cos[wave][at], cs);
+        read8(&s_sin[wave][at], sn);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          own[e] *= cs[e];
+          off[e] *= d0 < half ? -sn[e] : sn[e];
+        }
+      }
+    };
+    auto process = [&](const uint4& in, int st) {
+      const int now = kind_of(st, nq, nk), first = RPW * (st - (now == 0 ? 0 : now == 1 ? nq : nq + nk)), h = first + slot_row;
+      const bool live = in_row && h < (now == 0 ? hq : hkv);
+      if (now != kind && now < 2) factors(now);
+      kind = now;
+      const uint32_t w[4] = {in.x, in.y, in.z, in.w};
+      float y[8];
+      uint4 out = in;
+      if (now < 2 || DST != MT::kDtype) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          y[2 * i] = MT::to_f32((uint16_t)(w[i] & 0xffffu));
+          y[2 * i + 1] = MT::to_f32((uint16_t)(w[i] >> 16));
+        }
+      }
+      if (now < 2) {
+        float sq = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sq = fmaf(y[e], y[e], sq);
+        const float rs = rsqrtf(row_sum<LPR>(sq) * inv_dim + p.eps);
+        if constexpr (INTERLEAVE) {
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
             const float a = y[e], b = y[e + 1];
-            y[e] = a * c[e] + b * s[e];
-            y[e + 1] = b * c[e] + a * s[e + 1];
+            y[e] = rs * (a * own[e] + b * off[e]);
+            y[e + 1] = rs * (b * own[e + 1] + a * off[e + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t o = (uint32_t)__shfl((int)w[i], lane + other, kWave);
+            y[2 * i] = rs * (y[2 * i] * own[2 * i] + MT::to_f32((uint16_t)(o & 0xffffu)) * off[2 * i]);
+            y[2 * i + 1] = rs * (y[2 * i + 1] * own[2 * i + 1] + MT::to_f32((uint16_t)(o >> 16)) * off[2 * i + 1]);
           }
         }
+        out = make_uint4(MT::pack2(y[0], y[1]), MT::pack2(y[2], y[3]), MT::pack2(y[4], y[5]), MT::pack2(y[6], y[7]));
+        if (live && (now == 0 || p.keep_k)) *(uint4*)norm_row(p, now, t, first, slot_row, d0) = out;
       }
-    } else {
-      uint32_t o[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = (uint32_t)__shfl((int)w[i], lane + other, kWave);
-      if (!is_v) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint16_t b16 = (uint16_t)(e & 1 ? o[e >> 1] >> 16 : o[e >> 1] & 0xffffu);
-          const float a = y[e] * (rs * (is_q ? wq[e] : wk[e])), b = MT::to_f32(b16) * (rs * (is_q ? wqo[e] : wko[e]));
-          y[e] = rot ? a * c[e] + b * s[e] : a;
+      if constexpr (DST != kNoCache) {
+        if (now == 0 || page < 0 || !live) return;
+        constexpr int ESZ = DST == MI_F32 ? 4 : DST == MI_BF16 || DST == MI_F16 ? 2 : 1;
+        const bool is_v = now == 2;
+        uint8_t* row = p.cache + (page * p.page_stride + slot * p.token_stride + (is_v ? p.kv_stride : 0) + h * p.head_stride +
+                                  (DST == MI_MXFP4 ? d0 >> 1 : d0)) * ESZ;
+        float inv = 1.f;
+        uint8_t* scale = nullptr;
+        if constexpr (DST == MI_FP8_E4M3) inv = 1.f / ((const float*)(is_v ? p.v_scale : p.k_scale))[h];
+        if constexpr (DST == MI_MXFP8 || DST == MI_MXFP4) {
+          const int nblk = p.head_dim / kMxBlock;
+          scale = (uint8_t*)(is_v ? p.v_scale : p.k_scale) + page * (2LL * hkv * nblk * p.page_size) +
+                  (int64_t)(h * nblk + d0 / kMxBlock) * p.page_size + slot;
         }
+        norm_cache_store<MT, DST>(row, y, out, inv, scale);
       }
-    }
-    if (!live) continue;
-    uint4 out = u;
-    if (!is_v) {
-      out = make_uint4(MT::pack2(y[0], y[1]), MT::pack2(y[2], y[3]), MT::pack2(y[4], y[5]), MT::pack2(y[6], y[7]));
-      if (is_q || p.keep_k) *(uint4*)(src + d0) = out;
-    }
-    if constexpr (DST != kNoCache) {
-      if (is_q || page < 0) continue;
-      constexpr int ESZ = DST == MI_F32 ? 4 : DST == MI_BF16 || DST == MI_F16 ? 2 : 1;
-      uint8_t* row = p.cache + (page * p.page_stride + slot * p.token_stride + (is_v ? p.kv_stride : 0) + h * p.head_stride +
-                                (DST == MI_MXFP4 ? d0 >> 1 : d0)) * ESZ;
-      float inv = 1.f;
-      uint8_t* scale = nullptr;
-      if constexpr (DST == MI_FP8_E4M3) inv = 1.f / ((const float*)(is_v ? p.v_scale : p.k_scale))[h];
-      if constexpr (DST == MI_MXFP8 || DST == MI_MXFP4) {
-        const int nblk = p.head_dim / kMxBlock;
-        scale = (uint8_t*)(is_v ? p.v_scale : p.k_scale) + page * (2LL * hkv * nblk * p.page_size) +
-                (int64_t)(h * nblk + d0 / kMxBlock) * p.page_size + slot;
+    };
+    for (int s = s0; s < s1; s += U) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (s + i >= s1) break;
+        process(u[i], s + i);
+        if (s + i + U < s1) u[i] = load(s + i + U);
       }
-      norm_cache_store<MT, DST>(row, y, out, inv, scale);
     }
   }
 }
 
 template <typename MT, int DST, int LPR>
-static void launch_norm_lpr(const NormRopeParams& p, dim3 grid, hipStream_t s) {
-  if (p.interleave) hipLaunchKernelGGL((qk_norm_rope_kernel<MT, DST, LPR, true>), grid, dim3(256), 0, s, p);
+static void launch_norm_lpr(const NormRopeParams& p, bool interleave, dim3 grid, hipStream_t s) {
+  if (interleave) hipLaunchKernelGGL((qk_norm_rope_kernel<MT, DST, LPR, true>), grid, dim3(256), 0, s, p);
   else hipLaunchKernelGGL((qk_norm_rope_kernel<MT, DST, LPR, false>), grid, dim3(256), 0, s, p);
 }
 
 template <typename MT, int DST>
-static int launch_norm(NormRopeParams& p, hipStream_t s) {
-  const int lanes = p.head_dim / 8, lpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
-  const int rpw = kWave / lpr, most = (p.rows + rpw - 1) / rpw;
-  // wavefronts for every place of the chip first, then more rows to one, which its angles serve
+static int launch_norm(NormRopeParams& p, bool interleave, hipStream_t s) {
+  const int lanes = p.head_dim / 8, lpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64, rpw = kWave / lpr;
+  const int total = (p.num_qo_heads + rpw - 1) / rpw + (DST == kNoCache ? 1 : 2) * ((p.num_kv_heads + rpw - 1) / rpw);
+  // wavefronts for every place of the chip first, then more steps to one, which its angles serve
   const int64_t places = 16LL * device_cu_count();
-  int64_t steps = (int64_t)p.num_tokens * most / places;
-  p.steps = (int)(steps < 1 ? 1 : steps > most ? most : steps);
-  const int64_t units = (int64_t)p.num_tokens * ((most + p.steps - 1) / p.steps), blocks = (units + 3) / 4;
-  if (blocks > INT32_MAX) return MI_ERR_UNSUPPORTED;
-  const dim3 grid((uint32_t)blocks);
+  const int64_t want = (places + p.num_tokens - 1) / p.num_tokens;
+  p.part_steps = want >= total ? 1 : (int)((total + want - 1) / want);
+  p.parts = (total + p.part_steps - 1) / p.part_steps;
+  p.items = p.num_tokens * p.parts;  // parts > 1 only for fewer tokens than places
+  const int64_t blocks = (p.items + 3LL) / 4, most = 8LL * device_cu_count();
+  const dim3 grid((uint32_t)(blocks < most ? blocks : most));
   switch (lpr) {
-    case 8: launch_norm_lpr<MT, DST, 8>(p, grid, s); break;
-    case 16: launch_norm_lpr<MT, DST, 16>(p, grid, s); break;
-    case 32: launch_norm_lpr<MT, DST, 32>(p, grid, s); break;
-    default: launch_norm_lpr<MT, DST, 64>(p, grid, s); break;
+    case 8: launch_norm_lpr<MT, DST, 8>(p, interleave, grid, s); break;
+    case 16: launch_norm_lpr<MT, DST, 16>(p, interleave, grid, s); break;
+    case 32: launch_norm_lpr<MT, DST, 32>(p, interleave, grid, s); break;
+    default: launch_norm_lpr<MT, DST, 64>(p, interleave, grid, s); break;
   }
   return MI_OK;
 }
 
 template <typename MT>
-static int launch_norm_dst(NormRopeParams& p, int dst, hipStream_t s) {
+static int launch_norm_dst(NormRopeParams& p, int dst, bool interleave, hipStream_t s) {
   switch (dst) {
-    case kNoCache: return launch_norm<MT, kNoCache>(p, s);
-    case MI_BF16: return launch_norm<MT, MI_BF16>(p, s);
-    case MI_F16: return launch_norm<MT, MI_F16>(p, s);
-    case MI_F32: return launch_norm<MT, MI_F32>(p, s);
-    case MI_FP8_E4M3: return launch_norm<MT, MI_FP8_E4M3>(p, s);
-    case MI_MXFP8: return launch_norm<MT, MI_MXFP8>(p, s);
-    case MI_MXFP4: return launch_norm<MT, MI_MXFP4>(p, s);
+    case kNoCache: return launch_norm<MT, kNoCache>(p, interleave, s);
+    case MI_BF16: return launch_norm<MT, MI_BF16>(p, interleave, s);
+    case MI_F16: return launch_norm<MT, MI_F16>(p, interleave, s);
+    case MI_F32: return launch_norm<MT, MI_F32>(p, interleave, s);
+    case MI_FP8_E4M3: return launch_norm<MT, MI_FP8_E4M3>(p, interleave, s);
+    case MI_MXFP8: return launch_norm<MT, MI_MXFP8>(p, interleave, s);
+    case MI_MXFP4: return launch_norm<MT, MI_MXFP4>(p, interleave, s);
     default: return MI_ERR_UNSUPPORTED;
-  }
-}
-
-// Turns a position of each pair: theta^(-2i / rotary_dim) / scale / (2 pi), by one power and products.
-static void norm_turns(NormRopeParams& p, double theta, double scale, bool llama31, double low, double high, double old) {
-  const double two_pi = 6.283185307179586476925286766559;
-  const double ratio = std::pow(theta, -2.0 / p.rotary_dim);
-  double g = 1.0;
-  for (int i = 0; i < p.rotary_dim / 2; ++i, g *= ratio) {
-    double f = g / scale;
-    if (llama31) {
-      double smooth = (old * g / two_pi - low) / (high - low);
-      smooth = smooth < 0.0 ? 0.0 : smooth > 1.0 ? 1.0 : smooth;
-      f = (1.0 - smooth) * f + smooth * g;
-    }
-    p.turns[i] = f / two_pi;
   }
 }
 
@@ -286,6 +340,7 @@ extern "C" int mi_qk_norm_rope(void* q, int64_t q_stride_token, int64_t q_stride
   if (num_tokens < 0 || num_qo_heads < 0 || num_kv_heads < 0 || num_append_tokens < 0) return MI_ERR_INVALID;
   if (num_tokens == 0 || num_qo_heads + num_kv_heads == 0) return MI_OK;
   if (!pos_ids || (num_qo_heads > 0 && (!q || !q_weight)) || (num_kv_heads > 0 && (!k || !k_weight))) return MI_ERR_INVALID;
+  if (num_tokens > INT32_MAX - (1 << 20)) return MI_ERR_UNSUPPORTED;  // a grid's stride past the last one is still an int
   if (dtype != MI_BF16 && dtype != MI_F16) return MI_ERR_UNSUPPORTED;
   if (weight_dtype != dtype && weight_dtype != MI_F32) return MI_ERR_UNSUPPORTED;
   if (pos_dtype != MI_I32 && pos_dtype != MI_I64) return MI_ERR_UNSUPPORTED;
@@ -343,14 +398,17 @@ extern "C" int mi_qk_norm_rope(void* q, int64_t q_stride_token, int64_t q_stride
   p.num_kv_heads = num_kv_heads;
   p.head_dim = head_dim;
   p.rotary_dim = rotary_dim;
-  p.interleave = interleave ? 1 : 0;
   p.weight_f32 = weight_dtype == MI_F32;
   p.keep_k = keep_k ? 1 : 0;
-  p.rows = num_qo_heads + (kv ? 2 : 1) * num_kv_heads;
   p.eps = eps;
-  norm_turns(p, rope_theta, rope_scale, llama31 != 0, low_freq_factor, high_freq_factor, old_context_len);
+  const double two_pi = 6.283185307179586476925286766559, span = (double)high_freq_factor - (double)low_freq_factor;
+  p.step = -2.0 / rotary_dim * std::log2((double)rope_theta);
+  p.inv_scale = 1.0 / (double)rope_scale;
+  p.llama31 = llama31 ? 1 : 0;
+  p.slope = llama31 ? (double)old_context_len / two_pi / span : 0.0;
+  p.bias = llama31 ? (double)low_freq_factor / span : 0.0;
   hipStream_t s = (hipStream_t)stream;
-  const int st = dtype == MI_BF16 ? launch_norm_dst<BF16>(p, dst, s) : launch_norm_dst<F16>(p, dst, s);
+  const int st = dtype == MI_BF16 ? launch_norm_dst<BF16>(p, dst, interleave != 0, s) : launch_norm_dst<F16>(p, dst, interleave != 0, s);
   if (st != MI_OK) return st;
   MI_CHECK_LAUNCH();
   return MI_OK;

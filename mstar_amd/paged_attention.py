@@ -43,6 +43,7 @@ import torch
 
 from . import _lib
 from .mx_cache import MXKVLayer
+from .rope import apply_llama31_rope_pos_ids_inplace, apply_rope_pos_ids_inplace, qk_norm_rope_append, rope_append
 from .trace import trace_range
 
 __all__ = [
@@ -295,8 +296,6 @@ def _launch_append(kv_cache_layer: torch.Tensor | MXKVLayer, desc: _lib.MiPagedK
 
 def _rope_set_kv_cache(wrapper, kv_cache_layer, q, k, v, pos_ids, rotary_dim, interleave, rope_scale, rope_theta,
                        k_scale, v_scale, keep_k, llama31) -> None:
-    from .rope import apply_llama31_rope_pos_ids_inplace, apply_rope_pos_ids_inplace, rope_append
-
     if isinstance(kv_cache_layer, MXKVLayer):  # a block's scale needs its rotated values: two launches
         page_idx, slot_ptr, idx_stride, n, n_dev = wrapper._append_target()
         desc, src_dt = _check_append(kv_cache_layer, k, v, page_idx, n, k_scale, v_scale)  # before anything is rotated
@@ -344,8 +343,6 @@ class _FusedRopeAppend:
         ``rope_set_kv_cache``'s; q, k and v rows must be 16-byte aligned.  The rotated k is rounded
         once, from fp32 to the cache's type; ``keep_k=False`` leaves ``k`` as it was.
         """
-        from .rope import qk_norm_rope_append
-
         if self.dtype is None:
             raise RuntimeError("plan() must be called before qk_norm_rope_set_kv_cache()")
         qk_norm_rope_append(q, k, v, q_weight, k_weight, kv_cache_layer, pos_ids, *self._append_target(), eps=eps,

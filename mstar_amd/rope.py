@@ -125,54 +125,71 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache_laye
     )
 
 
-def _norm_weight(w: torch.Tensor, name: str, x: torch.Tensor) -> int:
+def _norm_weight(w: torch.Tensor, name: str, dtype: torch.dtype, d: int, at: int) -> int:
     """The type code of a norm's weight; refuses what the kernel does not read."""
-    if w.dim() != 1 or w.shape[0] != x.shape[2] or not w.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous vector of head_dim {x.shape[2]} elements, got {tuple(w.shape)}")
-    if w.dtype not in (x.dtype, torch.float32):
-        raise ValueError(f"{name} must be {x.dtype} or float32, got {w.dtype}")
-    if w.device != x.device:
-        raise ValueError(f"{name} must be on {x.device}, not on {w.device}")
-    return _DTYPES.get(w.dtype, _lib.MI_F32)
+    if w.shape != (d,) or not w.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector of head_dim {d} elements, got {tuple(w.shape)}")
+    wd = w.dtype
+    if wd is not dtype and wd is not torch.float32:
+        raise ValueError(f"{name} must be {dtype} or float32, got {wd}")
+    if w.get_device() != at:
+        raise ValueError(f"{name} must be on cuda:{at}, not on {w.device}")
+    return _DTYPES.get(wd, _lib.MI_F32)
+
+
+def _norm_rows(x: torch.Tensor, name: str) -> tuple[torch.Size, int, int, int]:
+    """(shape, address, token stride, head stride) of q, k or v, in rows that the kernel reads."""
+    shape = x.shape
+    if len(shape) != 3 or x.dtype not in _DTYPES or not x.is_cuda:
+        _check(x, name)
+    (st, sh, sd), ptr = x.stride(), x.data_ptr()
+    if sd != 1:
+        _check(x, name)
+    if (st | sh) % 8 or ptr % 16:
+        raise ValueError(f"{name}: rows must be 16-byte aligned")
+    return shape, ptr, st, sh
 
 
 def _qk_norm_rope(q, k, v, q_weight, k_weight, pos_ids, eps, rotary_dim, interleave, rope_scale, rope_theta, llama31,
                   keep_k, desc, page_idx, slot_idx_ptr, idx_stride, num_append, num_append_device_ptr) -> None:
-    _check(q, "q")
-    _check(k, "k")
-    if q.dtype != k.dtype or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.device != k.device:
+    # a launch is over before these checks are, in a decode step: each attribute is read once
+    (n, hq, d), q_at, q_st, q_sh = _norm_rows(q, "q")
+    (n_k, hkv, d_k), k_at, k_st, k_sh = _norm_rows(k, "k")
+    dtype, at = q.dtype, q.get_device()
+    if k.dtype is not dtype or n_k != n or d_k != d or k.get_device() != at:
         raise ValueError("q and k must agree on dtype, device, token count and head_dim")
-    d = q.shape[2]
+    v_at, v_st, v_sh, page_at = None, 0, 0, None
+    if v is not None:
+        v_shape, v_at, v_st, v_sh = _norm_rows(v, "v")
+        if v.dtype is not dtype or v_shape != (n, hkv, d) or v.get_device() != at:
+            raise ValueError(f"v {tuple(v_shape)}, {v.dtype} does not agree with k {tuple(k.shape)}, {k.dtype}")
+        page_at = page_idx.data_ptr()
     rd = d if rotary_dim is None else int(rotary_dim)
     least = 8 if interleave else 16
     if rd <= 0 or rd > d or rd % least or d % 8 or d > 512:
         raise ValueError(f"rotary_dim {rd} must be a multiple of {least} and head_dim {d} one of 8 up to 512, rotary_dim <= head_dim")
-    wd = _norm_weight(q_weight, "q_weight", q)
-    if _norm_weight(k_weight, "k_weight", k) != wd:
+    wd = _norm_weight(q_weight, "q_weight", dtype, d, at)
+    if _norm_weight(k_weight, "k_weight", dtype, d, at) != wd:
         raise ValueError("q_weight and k_weight must share one dtype")
     if not eps >= 0:
         raise ValueError(f"eps {eps} must not be negative")
-    rows = [("q", q), ("k", k)] + ([("v", v)] if v is not None else [])
-    for name, x in rows:
-        if x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16:
-            raise ValueError(f"{name}: rows must be 16-byte aligned")
-    if pos_ids.dtype not in _POS or pos_ids.dim() != 1 or pos_ids.shape[0] < q.shape[0]:
+    pos_type, pos_shape = _POS.get(pos_ids.dtype), pos_ids.shape
+    if pos_type is None or len(pos_shape) != 1 or pos_shape[0] < n:
         raise ValueError("pos_ids must be an int32/int64 vector with one position per token")
-    pos_ids = pos_ids.to(q.device).contiguous()
-    l31 = llama31 or {}
-    _lib.check(
-        _lib.lib().mi_qk_norm_rope(
-            q.data_ptr(), q.stride(0), q.stride(1), q.shape[1], k.data_ptr(), k.stride(0), k.stride(1), k.shape[1],
-            v.data_ptr() if v is not None else None, v.stride(0) if v is not None else 0, v.stride(1) if v is not None else 0,
-            _DTYPES[q.dtype], d, q_weight.data_ptr(), k_weight.data_ptr(), wd, float(eps), 1 if keep_k else 0, desc,
-            page_idx.data_ptr() if page_idx is not None else None, slot_idx_ptr, idx_stride, num_append,
-            num_append_device_ptr, rd, pos_ids.data_ptr(), _POS[pos_ids.dtype], q.shape[0], 1 if interleave else 0,
-            float(rope_scale), float(rope_theta), 1 if llama31 else 0, float(l31.get("low_freq_factor", 1.0)),
-            float(l31.get("high_freq_factor", 4.0)), float(l31.get("old_context_len", 8192.0)),
-            _lib.stream_ptr(q.device),
-        ),
-        "mi_qk_norm_rope",
-    )
+    if pos_ids.get_device() != at or not pos_ids.is_contiguous():
+        pos_ids = pos_ids.to(q.device).contiguous()
+    smooth, low, high, old = 0, 1.0, 4.0, 8192.0
+    if llama31:
+        smooth = 1
+        low, high = llama31.get("low_freq_factor", low), llama31.get("high_freq_factor", high)
+        old = llama31.get("old_context_len", old)
+    status = _lib.lib().mi_qk_norm_rope(
+        q_at, q_st, q_sh, hq, k_at, k_st, k_sh, hkv, v_at, v_st, v_sh, _DTYPES[dtype], d, q_weight.data_ptr(),
+        k_weight.data_ptr(), wd, float(eps), 1 if keep_k else 0, desc, page_at, slot_idx_ptr, idx_stride, num_append, num_append_device_ptr, rd,
+        pos_ids.data_ptr(), pos_type, n, 1 if interleave else 0, float(rope_scale), float(rope_theta), smooth, float(low),
+        float(high), float(old), _lib.stream_at(at))
+    if status:
+        _lib.check(status, "mi_qk_norm_rope")
 
 
 def apply_qk_norm_rope_pos_ids_inplace(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -201,11 +218,6 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
     Page map and ``keep_k`` as in :func:`rope_append`; any cache type, microscaled layers among them.  k is rounded
     once, from fp32 to the cache's type.
     """
-    _check(q, "q")
-    _check(k, "k")
-    _check(v, "v")
-    if v.dtype != k.dtype or v.shape != k.shape or v.device != k.device:
-        raise ValueError(f"v {tuple(v.shape)}, {v.dtype} does not agree with k {tuple(k.shape)}, {k.dtype}")
     desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
     if kv_cache_layer.device != k.device:
         raise ValueError(f"kv_cache_layer must be on {k.device}, not on {kv_cache_layer.device}")
