@@ -494,6 +494,21 @@ int mi_qk_norm_rope(void* q, int64_t q_stride_token, int64_t q_stride_head, int3
                     float rope_scale, float rope_theta, int32_t llama31, float low_freq_factor,
                     float high_freq_factor, float old_context_len, void* stream);
 
+/* The same call, its arguments in one block: what a caller from another language fills in one step. */
+typedef struct mi_qk_norm_rope_args {
+  void *q, *k;
+  const void *v, *q_weight, *k_weight, *pos_ids;
+  const mi_paged_kv* kv;
+  const int64_t *page_idx, *slot_idx;
+  const int32_t* num_tokens_device;
+  void* stream;
+  int64_t q_stride_token, q_stride_head, k_stride_token, k_stride_head, v_stride_token, v_stride_head, idx_stride;
+  int32_t num_qo_heads, num_kv_heads, dtype, head_dim, weight_dtype, keep_k, num_append_tokens, rotary_dim, pos_dtype;
+  int32_t num_tokens, interleave, llama31;
+  float eps, rope_scale, rope_theta, low_freq_factor, high_freq_factor, old_context_len;
+} mi_qk_norm_rope_args;
+int mi_qk_norm_rope_block(const mi_qk_norm_rope_args* args);
+
 /* ------------------------------------------------------------------------
  * Attention weights of cached tokens, accumulated.  No counterpart in the reference.
  *   weights[page, h, slot] += sum over the request's queries i and the q heads g of kv head h

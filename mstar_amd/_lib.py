@@ -11,6 +11,7 @@ runtime: torch tensors and these kernels then share one HIP context.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -202,6 +203,7 @@ SIGNATURES = {
          ctypes.POINTER(MiPagedKV), _P, _P, _I64, _I32, _P, _I32, _P, _I32, _I32, _I32, _F32, _F32, _I32, _F32, _F32,
          _F32, _P],
     ),
+    "mi_qk_norm_rope_block": (ctypes.c_int, [ctypes.c_char_p]),
     "mi_attention_weights_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32]),
     "mi_attention_weights": (
         ctypes.c_int,
@@ -213,6 +215,9 @@ SIGNATURES = {
         [ctypes.POINTER(MiPagedKV), _I32, _I64, _I64, _P, _P, _I64, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P],
     ),
 }
+
+# mi_qk_norm_rope_args: packing 36 values and passing one costs the host a sixth of converting them one by one
+QK_NORM_ROPE_ARGS = struct.Struct("@11P7q12i6f")
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

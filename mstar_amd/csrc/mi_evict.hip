@@ -6,13 +6,13 @@
 // request's first `keep` slots, in their order.
 //
 // Two launches.  evict_select_kernel finds, a workgroup for each (layer, request, kv head), the
-// weight of the last token that stays by a radix select over the weights' order-preserving bits
-// and lists the places that stay.  evict_move_kernel goes through that list in tiles: a tile's rows are
-// all in registers before the first of them is written.  Places ascend, so a tile's
-// sources lie at or behind its own first destination, and what it writes lies before every later tile's
-// sources: one barrier a tile keeps the move in place, and no second copy of the cache is needed.  Tiles
-// of one row are in turn, so rows are split over workgroups by head, K and V, and by pieces of the
-// row where that leaves places of the chip empty.
+// weight of the last token that stays by a radix select over the weights' order-preserving bits,
+// held in registers, and lists the places that stay.  evict_move_kernel goes through that list in tiles.  Places
+// ascend, so a tile's sources lie at or behind its own first destination, and what it writes lies before every
+// later tile's sources: a tile is written once its rows are all in registers, while the next one's are loaded, one
+// barrier a tile keeps the move in place, and no second copy of the cache is needed.  Tiles of one row are
+// in turn, so rows are split over workgroups by head, K and V, and by pieces of 128 bytes of the row where that
+// leaves places of the chip empty.  Where little is kept one launch does both (evict_small_kernel).
 #include "mi_internal.h"
 
 namespace mi {
@@ -27,8 +27,8 @@ struct EvictParams {
   int64_t weights_layer_stride;
   const int32_t *kv_indptr, *kv_indices, *last_page_len;
   int32_t* kept;
-  int32_t batch, num_indices, num_kv_heads, page_size, keep, recent, sinks;
-  int32_t row_pieces, splits, blocks;  // 16-byte pieces of a row, workgroups that share them; blocks of a row with a scale
+  int32_t batch, num_indices, num_kv_heads, page_size, page_shift, keep, recent, sinks;
+  int32_t row_pieces, splits, blocks, parts;  // 16-byte pieces of a row, workgroups that share them; blocks with a scale
 };
 
 MI_DEVICE int evict_len(const EvictParams& p, int b, int& first, int& pages) {
@@ -37,141 +37,282 @@ MI_DEVICE int evict_len(const EvictParams& p, int b, int& first, int& pages) {
   return pages > 0 ? max(0, (pages - 1) * p.page_size + min(p.last_page_len[b], p.page_size)) : 0;
 }
 
-// Bits that order as the weights do, from 1: NaN is 0, below every number, and -0 is 0.
-MI_DEVICE uint32_t weight_bits(float w) {
-  const uint32_t u = bitcast<uint32_t>(w + 0.f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0u;
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+// Bits that order as the tokens do: 0 for none, 1 for a NaN and a page out of range, then the numbers (-0 as 0), and above
+// all of those the first and last tokens, which stay whatever they weigh.
+constexpr uint32_t kNanBits = 0x7fc00000u;
+MI_DEVICE uint32_t token_bits(const EvictParams& p, uint32_t weight, int t, int len) {
+  const uint32_t u = bitcast<uint32_t>(bitcast<float>(weight) + 0.f);
+  uint32_t bits = (u & 0x7fffffffu) > 0x7f800000u ? 1u : u & 0x80000000u ? ~u : u | 0x80000000u;
+  if (t < p.sinks || t >= len - p.recent) bits = 0xffffffffu;
+  return t < len ? bits : 0u;
 }
 
-constexpr int kSelThreads = 1024, kSelBins = 2048;
+constexpr int kSelBins = 2048;
+constexpr int kSelRegs = 8;  // of a thread, each the weights of four tokens; what is past them is read again
 
-// Weights of four adjacent tokens t .. t + 3 (t a multiple of four: they lie in one page).
+struct SelectShared {
+  int hist[2][kSelBins];  // in turn: one is cleared while the other is in use
+  int sum[16], digit, left, count, heavy[16], equal[16];
+};
+
+MI_DEVICE bool evict_page_ok(const EvictParams& p, int page) { return page >= 0 && page < p.max_pages; }
+MI_DEVICE const uint4* weights_at(const EvictParams& p, const float* weights, int64_t page, int h, int slot) {
+  return (const uint4*)(weights + (page * p.num_kv_heads + h) * p.page_size + slot);
+}
+
+// Entry of a request's page list that holds token t.
+MI_DEVICE int entry_of(const EvictParams& p, int t) {
+  return p.page_shift >= 0 ? t >> p.page_shift : (int)((unsigned)t / (unsigned)p.page_size);
+}
+// Exclusive sum over a workgroup of NT threads (smem: NT / 64 ints, free again after the caller's next barrier).
+template <int NT>
+MI_DEVICE int before_mine(int v, int* smem) {
+  const int lane = lane_id(), w = uniform((int)threadIdx.x >> 6), x = wave_inclusive_sum(v);
+  if (lane == 63) smem[w] = x;
+  __syncthreads();
+  const int t = wave_inclusive_sum(lane < NT / kWave ? smem[lane] : 0);
+  return (w ? __builtin_amdgcn_readlane(t, w - 1) : 0) + x - v;
+}
+
+// Bits of four adjacent tokens t .. t + 3 (t a multiple of four: they lie in one page).
 MI_DEVICE void load_bits4(const EvictParams& p, const float* weights, int first, int h, int t, int len, uint32_t (&u)[4]) {
-  float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
-  bool ok = t < len;
-  if (ok) {
-    const int e = (int)((unsigned)t / (unsigned)p.page_size), s = t - e * p.page_size;
-    const int64_t page = p.kv_indices[first + e];
-    ok = page >= 0 && page < p.max_pages;
-    if (ok) w = *(const float4*)(weights + (page * p.num_kv_heads + h) * p.page_size + s);
+  uint4 w = make_uint4(kNanBits, kNanBits, kNanBits, kNanBits);
+  if (t < len) {
+    const int e = entry_of(p, t), page = p.kv_indices[first + e];
+    if (evict_page_ok(p, page)) w = *weights_at(p, weights, page, h, t - e * p.page_size);
   }
-  u[0] = ok ? weight_bits(w.x) : 0u;
-  u[1] = ok ? weight_bits(w.y) : 0u;
-  u[2] = ok ? weight_bits(w.z) : 0u;
-  u[3] = ok ? weight_bits(w.w) : 0u;
+  u[0] = token_bits(p, w.x, t, len), u[1] = token_bits(p, w.y, t + 1, len);
+  u[2] = token_bits(p, w.z, t + 2, len), u[3] = token_bits(p, w.w, t + 3, len);
 }
 
-// Inclusive sum over the workgroup's 1024 threads of two counts of at most 2^31 in one 64-bit word each.
-__device__ __forceinline__ void select_scan(int a, int b, int& before_a, int& before_b, int* smem) {
-  int ta, tb;
-  before_a = block_exclusive_scan_1024(a, ta, smem);
-  before_b = block_exclusive_scan_1024(b, tb, smem);
+MI_DEVICE int lanes_before(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictParams p) {
-  __shared__ int s_hist[kSelBins];
-  __shared__ int s_scan[32];
-  __shared__ int s_digit, s_left;
-  const int tid = (int)threadIdx.x;
+// The places that stay of a (layer, request, kv head), to out, and to list where it is not null (in LDS); len > keep.
+// Wavefront w has the tokens of run w, four to a lane, 256 at a time.
+template <int NT>
+__device__ __forceinline__ void evict_select(const EvictParams& p, SelectShared& s, const float* weights, int first, int h, int len,
+                                             int32_t* out, int32_t* list) {
+  const int tid = (int)threadIdx.x, lane = lane_id(), wave = uniform(tid >> 6);
+  const int rounds = (len + 4 * NT - 1) / (4 * NT), base = wave * rounds * 256;
+  const int mine = uniform(min(rounds, (len - base + 255) >> 8));  // rounds with tokens; none where it is not positive
+  uint32_t u[kSelRegs][4];
+  {
+    int page[kSelRegs];
+#pragma unroll
+    for (int i = 0; i < kSelRegs; ++i) {
+      const int t = base + 256 * i + 4 * lane;
+      page[i] = i < mine && t < len ? p.kv_indices[first + entry_of(p, t)] : -1;
+    }
+    for (int i = tid; i < 2 * kSelBins / 4; i += NT) ((int4*)s.hist)[i] = make_int4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kSelRegs; ++i) {
+      uint4 w = make_uint4(kNanBits, kNanBits, kNanBits, kNanBits);
+      const int t = base + 256 * i + 4 * lane;
+      if (evict_page_ok(p, page[i])) w = *weights_at(p, weights, page[i], h, t - entry_of(p, t) * p.page_size);
+      u[i][0] = w.x, u[i][1] = w.y, u[i][2] = w.z, u[i][3] = w.w;
+    }
+#pragma unroll
+    for (int i = 0; i < kSelRegs; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[i][j] = token_bits(p, u[i][j], base + 256 * i + 4 * lane + j, len);
+  }
+  auto visit = [&](auto&& f) {  // four tokens at a time, ascending
+#pragma unroll
+    for (int i = 0; i < kSelRegs; ++i)
+      if (i < mine) f(base + 256 * i, u[i]);
+    for (int i = kSelRegs; i < mine; ++i) {
+      uint32_t x[4];
+      load_bits4(p, weights, first, h, base + 256 * i + 4 * lane, len, x);
+      f(base + 256 * i, x);
+    }
+  };
+  int left = p.keep, count = 0;   // to take, fewer than there are; tokens that share the digits found
+  uint32_t prefix = 0, done = 0;  // digits found of the last taken token, and their mask
+  __syncthreads();
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {  // bits 21-31, 10-20, then the last ten
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t digit = pass == 2 ? 0x3ffu : 0x7ffu;
+    int* hist = s.hist[pass & 1];
+    visit([&](int, const uint32_t (&x)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((x[j] & done) == prefix) atomicAdd(&hist[(x[j] >> shift) & digit], 1);
+    });
+    __syncthreads();
+    // the digit at which the count of heavier tokens reaches `left`: thread i holds bins BINS (NT - 1 - i) and on
+    constexpr int BINS = kSelBins / NT;
+    const int* bins = hist + BINS * (NT - 1 - tid);
+    int n[BINS], sum = 0;
+#pragma unroll
+    for (int i = 0; i < BINS; ++i) sum += n[i] = bins[i];
+    int before = before_mine<NT>(sum, s.sum);
+    if (before < left && before + sum >= left) {
+#pragma unroll
+      for (int i = BINS - 1; i >= 0; --i) {
+        if (before < left && before + n[i] >= left) {
+          s.digit = BINS * (NT - 1 - tid) + i;
+          s.left = left - before;
+          s.count = n[i];
+        }
+        before += n[i];
+      }
+    }
+    if (pass == 0) {  // the third digit's
+      // every thread is past its reading of the first's: before_mine has a barrier behind it
+      for (int i = tid; i < kSelBins / 4; i += NT) ((int4*)s.hist[0])[i] = make_int4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    prefix |= (uint32_t)s.digit << shift;
+    done |= digit << shift;
+    left = s.left;
+    count = s.count;
+    if (count == left) break;  // all that share these digits stay
+    __syncthreads();
+  }
+  auto put = [&](int to, int t) {
+    if (to >= p.keep) return;  // never, where the weights do not change under the call
+    out[to] = t;
+    if (list) list[to] = t;
+  };
+  if (count == left) {  // what stays: its digits reach those found
+    int stay = 0;
+    visit([&](int, const uint32_t (&x)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) stay += __popcll(__builtin_amdgcn_ballot_w64((x[j] & done) >= prefix));
+    });
+    if (lane == 0) s.heavy[wave] = stay;
+    __syncthreads();
+    stay = 0;
+    for (int i = 0; i < wave; ++i) stay += s.heavy[i];
+    visit([&](int t, const uint32_t (&x)[4]) {
+      int to = stay;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t m = __builtin_amdgcn_ballot_w64((x[j] & done) >= prefix);
+        to += lanes_before(m);
+        stay += __popcll(m);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((x[j] & done) >= prefix) put(to++, t + 4 * lane + j);
+    });
+    return;
+  }
+  // ties: the heavier ones, and the first `left` of those that weigh the same
+  int heavy = 0, equal = 0;
+  visit([&](int, const uint32_t (&x)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      heavy += __popcll(__builtin_amdgcn_ballot_w64(x[j] > prefix));
+      equal += __popcll(__builtin_amdgcn_ballot_w64(x[j] == prefix));
+    }
+  });
+  if (lane == 0) {
+    s.heavy[wave] = heavy;
+    s.equal[wave] = equal;
+  }
+  __syncthreads();
+  heavy = equal = 0;
+  for (int i = 0; i < wave; ++i) heavy += s.heavy[i], equal += s.equal[i];
+  visit([&](int t, const uint32_t (&x)[4]) {
+    int h0 = heavy, e0 = equal;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t a = __builtin_amdgcn_ballot_w64(x[j] > prefix), b = __builtin_amdgcn_ballot_w64(x[j] == prefix);
+      h0 += lanes_before(a);
+      e0 += lanes_before(b);
+      heavy += __popcll(a);
+      equal += __popcll(b);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool a = x[j] > prefix, b = x[j] == prefix;
+      if (a || (b && e0 < left)) put(h0 + min(e0, left), t + 4 * lane + j);
+      h0 += a;
+      e0 += b;
+    }
+  });
+}
+
+template <int NT>
+__global__ __launch_bounds__(NT, NT == 256 ? 6 : 8) void evict_select_kernel(EvictParams p) {
+  __shared__ __attribute__((aligned(16))) SelectShared s;
   const int h = uniform((int)(blockIdx.x % p.num_kv_heads)), rest = uniform((int)(blockIdx.x / p.num_kv_heads));
   const int b = uniform(rest % p.batch), layer = uniform(rest / p.batch);
   int first, pages;
   const int len = evict_len(p, b, first, pages);
   int32_t* out = p.kept + (((int64_t)layer * p.batch + b) * p.num_kv_heads + h) * p.keep;
   if (len <= p.keep) {
-    for (int j = tid; j < p.keep; j += kSelThreads) out[j] = j < len ? j : -1;
+    for (int j = (int)threadIdx.x; j < p.keep; j += NT) out[j] = j < len ? j : -1;
     return;
   }
-  const float* weights = p.weights + (int64_t)layer * p.weights_layer_stride;
-  const int lo = p.sinks, hi = len - p.recent;
-  int left = p.keep - p.sinks - p.recent;  // to take of [lo, hi), at least one fewer than there are
-  uint32_t prefix = 0, done = 0;           // digits found of the last taken weight, and their mask
-  if (left > 0) {
-    for (int shift = 21; shift >= -1; shift -= 11) {  // bits 21-31, 10-20, then the last ten
-      const int sh = shift < 0 ? 0 : shift;
-      const uint32_t digit = shift < 0 ? 0x3ffu : 0x7ffu;
-      for (int i = tid; i < kSelBins; i += kSelThreads) s_hist[i] = 0;
-      __syncthreads();
-      for (int t = 4 * tid; t < len; t += 4 * kSelThreads) {
-        uint32_t u[4];
-        load_bits4(p, weights, first, h, t, len, u);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (t + i >= lo && t + i < hi && (u[i] & done) == prefix) atomicAdd(&s_hist[(u[i] >> sh) & digit], 1);
-      }
-      __syncthreads();
-      // the digit at which the count of heavier weights reaches `left`: thread i holds bins 2047 - 2i and below
-      const int n0 = s_hist[kSelBins - 1 - 2 * tid], n1 = s_hist[kSelBins - 2 - 2 * tid];
-      int total;
-      const int before = block_exclusive_scan_1024(n0 + n1, total, s_scan);
-      if (before < left && before + n0 >= left) {
-        s_digit = kSelBins - 1 - 2 * tid;
-        s_left = left - before;
-      } else if (before + n0 < left && before + n0 + n1 >= left) {
-        s_digit = kSelBins - 2 - 2 * tid;
-        s_left = left - before - n0;
-      }
-      __syncthreads();
-      prefix |= (uint32_t)s_digit << sh;
-      done |= digit << sh;
-      left = s_left;
-      __syncthreads();
-    }
-  }
-  // `left` of the tokens whose bits equal prefix stay, the first ones; none where nothing is taken by weight
-  const bool take = p.keep - p.sinks - p.recent > 0;
-  const int per_thread = 4 * ((len + 4 * kSelThreads - 1) / (4 * kSelThreads));
-  const int t0 = min(tid * per_thread, len), t1 = min(t0 + per_thread, len);
-  int heavy = 0, equal = 0;
-  for (int t = t0; t < t1; t += 4) {
-    uint32_t u[4];
-    load_bits4(p, weights, first, h, t, len, u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = t + i;
-      if (at >= t1) continue;
-      const bool mid = at >= lo && at < hi;
-      heavy += !mid || (take && u[i] > prefix);
-      equal += mid && take && u[i] == prefix;
-    }
-  }
-  int heavy_before, equal_before;
-  select_scan(heavy, equal, heavy_before, equal_before, s_scan);
-  for (int t = t0; t < t1; t += 4) {
-    uint32_t u[4];
-    load_bits4(p, weights, first, h, t, len, u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = t + i;
-      if (at >= t1) continue;
-      const bool mid = at >= lo && at < hi;
-      const bool is_heavy = !mid || (take && u[i] > prefix), is_equal = mid && take && u[i] == prefix;
-      if (is_heavy || (is_equal && equal_before < left)) {
-        const int to = heavy_before + min(equal_before, left);
-        if (to < p.keep) out[to] = at;  // always, where the weights do not change under the call
-      }
-      heavy_before += is_heavy;
-      equal_before += is_equal;
-    }
-  }
+  evict_select<NT>(p, s, p.weights + (int64_t)layer * p.weights_layer_stride, first, h, len, out, nullptr);
 }
 
-constexpr int kMoveThreads = 256, kMoveRows = 8;  // 16-byte pieces a thread has in flight
+constexpr int kSelFew = 4096;  // tokens of a request, on average, up to which 256 threads select
+constexpr int kMoveThreads = 256, kMoveRows = 8;  // 16-byte pieces a thread has in flight, of a tile
+constexpr int kMovePlaces = 256;                  // rows of a tile, at most
 
 // Where token t of a request lies: page id and slot, false where the id is out of range.
 MI_DEVICE bool evict_place(const EvictParams& p, int first, int pages, int t, int64_t& page, int& slot) {
-  const int e = (int)((unsigned)t / (unsigned)p.page_size);
+  const int e = t >= 0 ? entry_of(p, t) : pages;
   slot = t - e * p.page_size;
   page = e < pages ? p.kv_indices[first + e] : -1;
   return page >= 0 && page < p.max_pages;
 }
 
+// One value of type T a token, THREADS threads: src(page, slot) -> dst(page, slot) of the kept ones; `still`: those that stay
+// where they are as well.
+template <typename T, int THREADS, typename Src, typename Dst>
+__device__ __forceinline__ void evict_values(const EvictParams& p, int first, int pages, const int32_t* kept, int n, bool still,
+                                             Src src, Dst dst) {
+  for (int j0 = 0; j0 < n; j0 += THREADS * kMoveRows) {
+    T x[kMoveRows];
+    T* to[kMoveRows];
+#pragma unroll
+    for (int i = 0; i < kMoveRows; ++i) {
+      const int j = j0 + i * THREADS + (int)threadIdx.x, t = j < n ? kept[j] : -1;
+      int64_t page, page_to;
+      int slot, slot_to;
+      const bool move = t >= 0 && (still || t > j) && evict_place(p, first, pages, t, page, slot) &&
+                        evict_place(p, first, pages, j, page_to, slot_to);
+      x[i] = move ? *src(page, slot) : T(0);
+      to[i] = move ? dst(page_to, slot_to) : nullptr;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMoveRows; ++i)
+      if (to[i]) *to[i] = x[i];
+  }
+}
+template <int THREADS>
+__device__ __forceinline__ void evict_weights(const EvictParams& p, int layer, int h, int first, int pages, const int32_t* kept, int n) {
+  const bool still = p.weights != p.out_weights;
+  auto at = [=](int64_t page, int slot) {
+    return layer * p.weights_layer_stride + (page * p.num_kv_heads + h) * p.page_size + slot;
+  };
+  evict_values<float, THREADS>(p, first, pages, kept, n, still, [&](int64_t page, int slot) { return p.weights + at(page, slot); },
+                               [&](int64_t page, int slot) { return p.out_weights + at(page, slot); });
+}
+// line: a block of K's rows, then of V's
+template <int THREADS>
+__device__ __forceinline__ void evict_scales(const EvictParams& p, int layer, int h, int first, int pages, const int32_t* kept, int n, int line) {
+  const int v = line >= p.blocks, blk = line - v * p.blocks;
+  uint8_t* base = p.scales + (int64_t)layer * p.scale_layer_stride;
+  const int64_t row = (int64_t)(v * p.num_kv_heads + h) * p.blocks + blk, rows = 2LL * p.num_kv_heads * p.blocks;
+  auto at = [&](int64_t page, int slot) { return base + (page * rows + row) * p.page_size + slot; };
+  evict_values<uint8_t, THREADS>(p, first, pages, kept, n, false, at, at);
+}
+
 // Workgroups: (layer, request, kv head) x parts; part 0 .. 2 splits - 1: a share of the pieces of the
-// K, then of the V rows; the last: weights and scale bytes.
+// K, then of the V rows; then the weights, and the lines of scale bytes.
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p) {
-  const int tid = (int)threadIdx.x, parts = 2 * p.splits + 1;
-  const int part = uniform((int)(blockIdx.x % parts)), unit = uniform((int)(blockIdx.x / parts));
+  __shared__ int64_t s_from[4][kMovePlaces], s_to[4][kMovePlaces];
+  const int tid = (int)threadIdx.x;
+  const int part = uniform((int)(blockIdx.x % p.parts)), unit = uniform((int)(blockIdx.x / p.parts));
   const int h = uniform(unit % p.num_kv_heads), rest = uniform(unit / p.num_kv_heads);
   const int b = uniform(rest % p.batch), layer = uniform(rest / p.batch);
   int first, pages;
@@ -179,79 +320,151 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p)
   const int32_t* kept = p.kept + (int64_t)unit * p.keep;
   const bool cut = len > p.keep;
   const int n = min(len, p.keep);
-  if (part < 2 * p.splits) {
-    if (!cut) return;
-    const int v = part >= p.splits, share = part - v * p.splits;
-    const int per = p.row_pieces / p.splits;  // pieces of a row, a power of two
-    const int row = tid / per, piece = share * per + tid % per, rows = kMoveThreads / per;
-    uint8_t* base = p.cache + layer * p.layer_stride + v * p.kv_stride + h * p.head_stride + 16 * piece;
-    for (int j0 = 0; j0 < n; j0 += rows * kMoveRows) {
-      uint4 x[kMoveRows];
-      int64_t from[kMoveRows], to[kMoveRows];
-#pragma unroll
-      for (int i = 0; i < kMoveRows; ++i) {
-        const int j = j0 + i * rows + row, src = j < n ? kept[j] : -1;
-        int64_t page, page_to;
-        int slot, slot_to;
-        const bool move = src > j && evict_place(p, first, pages, src, page, slot) &&  // not there already
-                          evict_place(p, first, pages, j, page_to, slot_to);
-        from[i] = move ? page * p.page_stride + slot * p.token_stride : -1;
-        to[i] = move ? page_to * p.page_stride + slot_to * p.token_stride : -1;
-      }
-#pragma unroll
-      for (int i = 0; i < kMoveRows; ++i) x[i] = from[i] >= 0 ? *(const uint4*)(base + from[i]) : make_uint4(0, 0, 0, 0);
-      __syncthreads();  // the tile's rows are in registers
-#pragma unroll
-      for (int i = 0; i < kMoveRows; ++i)
-        if (to[i] >= 0) *(uint4*)(base + to[i]) = x[i];
-    }
+  if (part == 2 * p.splits) {
+    if (cut || p.weights != p.out_weights) evict_weights<kMoveThreads>(p, layer, h, first, pages, kept, n);
     return;
   }
-  // weights (copied for every request, moved in place or not), then scale bytes
+  if (!cut) return;
+  if (part > 2 * p.splits) {
+    evict_scales<kMoveThreads>(p, layer, h, first, pages, kept, n, part - 2 * p.splits - 1);
+    return;
+  }
+  const int v = part >= p.splits, share = part - v * p.splits;
+  const int per = p.row_pieces / p.splits;  // pieces of a row, a power of two
+  const int row = tid / per, piece = share * per + tid % per, rows = kMoveThreads / per;
+  const int steps = min(kMoveRows, kMovePlaces / rows), tile = rows * steps;
+  uint8_t* base = p.cache + layer * p.layer_stride + v * p.kv_stride + h * p.head_stride + 16 * piece;
+  const int tiles = (n + tile - 1) / tile;
+  auto places = [&](int i) {  // of tile i's rows
+    if (i >= tiles) return;
+    for (int k = tid; k < tile; k += kMoveThreads) {
+      const int j = i * tile + k, t = j < n ? kept[j] : -1;
+      int64_t page, page_to;
+      int slot, slot_to;
+      const bool move = t > j && evict_place(p, first, pages, t, page, slot) &&  // not there already
+                        evict_place(p, first, pages, j, page_to, slot_to);
+      s_from[i & 3][k] = move ? page * p.page_stride + slot * p.token_stride : -1;
+      s_to[i & 3][k] = move ? page_to * p.page_stride + slot_to * p.token_stride : -1;
+    }
+  };
+  auto load = [&](int i, u32x4_t (&x)[kMoveRows]) {
+#pragma unroll
+    for (int k = 0; k < kMoveRows; ++k) {
+      const int64_t from = k < steps && i < tiles ? s_from[i & 3][k * rows + row] : -1;
+      x[k] = from >= 0 ? *(const u32x4_t*)(base + from) : u32x4_t{0u, 0u, 0u, 0u};
+    }
+  };
+  auto store = [&](int i, const u32x4_t (&x)[kMoveRows]) {
+#pragma unroll
+    for (int k = 0; k < kMoveRows; ++k) {
+      const int64_t to = k < steps ? s_to[i & 3][k * rows + row] : -1;
+      if (to >= 0) *(u32x4_t*)(base + to) = x[k];
+    }
+  };
+  u32x4_t x[kMoveRows], y[kMoveRows];
+  places(0);
+  places(1);
+  __syncthreads();
+  load(0, x);
+  for (int i = 0; i < tiles; i += 2) {
+    places(i + 2);
+    __syncthreads();  // tile i is in registers
+    load(i + 1, y);
+    store(i, x);
+    if (i + 1 >= tiles) break;
+    places(i + 3);
+    __syncthreads();
+    load(i + 2, x);
+    store(i + 1, y);
+  }
+}
+
+// Both in one launch, a workgroup for each (layer, request, kv head): K and V rows of a tile side by side, and the
+// weights with the first.
+constexpr int kSmallThreads = 1024, kSmallKeep = 4096, kSmallPages = 1024, kSmallPlaces = 512;
+constexpr int64_t kSmallBytes = 256 << 10;  // of K and V that stay: two tiles
+__global__ __launch_bounds__(kSmallThreads) void evict_small_kernel(EvictParams p) {
+  __shared__ __attribute__((aligned(16))) SelectShared s;
+  __shared__ int32_t s_kept[kSmallKeep], s_page[kSmallPages];
+  __shared__ int64_t s_from[kSmallPlaces], s_to[kSmallPlaces];
+  const int tid = (int)threadIdx.x;
+  const int unit = (int)blockIdx.x, h = uniform(unit % p.num_kv_heads), rest = uniform(unit / p.num_kv_heads);
+  const int b = uniform(rest % p.batch), layer = uniform(rest / p.batch);
+  int first, pages;
+  const int len = evict_len(p, b, first, pages), n = min(len, p.keep);
+  const bool cut = len > p.keep;
+  int32_t* out = p.kept + (int64_t)unit * p.keep;
   const float* weights = p.weights + (int64_t)layer * p.weights_layer_stride;
   float* out_weights = p.out_weights + (int64_t)layer * p.weights_layer_stride;
-  if (cut || p.weights != p.out_weights) {
-    for (int j0 = 0; j0 < n; j0 += kMoveThreads * kMoveRows) {
-      float x[kMoveRows];
-      float* to[kMoveRows];
-#pragma unroll
-      for (int i = 0; i < kMoveRows; ++i) {
-        const int j = j0 + i * kMoveThreads + tid, src = j < n ? kept[j] : -1;
-        int64_t page, page_to;
-        int slot, slot_to;
-        const bool move = src >= 0 && evict_place(p, first, pages, src, page, slot) && evict_place(p, first, pages, j, page_to, slot_to);
-        x[i] = move ? weights[(page * p.num_kv_heads + h) * p.page_size + slot] : 0.f;
-        to[i] = move ? out_weights + (page_to * p.num_kv_heads + h) * p.page_size + slot_to : nullptr;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kMoveRows; ++i)
-        if (to[i]) *to[i] = x[i];
+  if (tid < min(pages, kSmallPages)) s_page[tid] = p.kv_indices[first + tid];
+  if (cut) {
+    evict_select<kSmallThreads>(p, s, weights, first, h, len, out, s_kept);
+  } else {
+    for (int j = tid; j < p.keep; j += kSmallThreads) {
+      s_kept[j] = j;
+      out[j] = j < len ? j : -1;
     }
+    if (p.weights == p.out_weights) return;
   }
-  if (!cut || !p.scales) return;
-  uint8_t* scales = p.scales + (int64_t)layer * p.scale_layer_stride;
-  for (int row = 0; row < 2 * p.blocks; ++row) {  // K's blocks, then V's
-    const int v = row >= p.blocks, blk = row - v * p.blocks;
-    for (int j0 = 0; j0 < n; j0 += kMoveThreads * kMoveRows) {
-      uint8_t x[kMoveRows];
-      uint8_t* to[kMoveRows];
+  __syncthreads();
+  auto place = [&](int t, int64_t& page, int& slot) {  // as evict_place
+    const int e = t >= 0 ? entry_of(p, t) : pages;
+    slot = t - e * p.page_size;
+    page = e >= pages ? -1 : e < kSmallPages ? s_page[e] : p.kv_indices[first + e];
+    return page >= 0 && page < p.max_pages;
+  };
+  constexpr int kNW = kSmallKeep / kSmallThreads;
+  float w[kNW];
+  int64_t w_to[kNW];
 #pragma unroll
-      for (int i = 0; i < kMoveRows; ++i) {
-        const int j = j0 + i * kMoveThreads + tid, src = j < n ? kept[j] : -1;
-        int64_t page, page_to;
-        int slot, slot_to;
-        const bool move = src > j && evict_place(p, first, pages, src, page, slot) && evict_place(p, first, pages, j, page_to, slot_to);
-        const int64_t line = (int64_t)(v * p.num_kv_heads + h) * p.blocks + blk, lines = 2LL * p.num_kv_heads * p.blocks;
-        x[i] = move ? scales[(page * lines + line) * p.page_size + slot] : 0;
-        to[i] = move ? scales + (page_to * lines + line) * p.page_size + slot_to : nullptr;
-      }
-      __syncthreads();
+  for (int i = 0; i < kNW; ++i) {
+    const int j = tid + i * kSmallThreads;
+    int64_t page, page_to;
+    int slot, slot_to;
+    const bool move = j < n && place(s_kept[j], page, slot) && place(j, page_to, slot_to);
+    w[i] = move ? weights[(page * p.num_kv_heads + h) * p.page_size + slot] : 0.f;
+    w_to[i] = move ? (page_to * p.num_kv_heads + h) * p.page_size + slot_to : -1;
+  }
+  auto put_weights = [&]() {
 #pragma unroll
-      for (int i = 0; i < kMoveRows; ++i)
-        if (to[i]) *to[i] = x[i];
+    for (int i = 0; i < kNW; ++i)
+      if (w_to[i] >= 0) out_weights[w_to[i]] = w[i];
+  };
+  if (!cut) {
+    put_weights();
+    return;
+  }
+  const int per = 2 * p.row_pieces, row = tid / per, rows = kSmallThreads / per;
+  const int steps = min(kMoveRows, kSmallPlaces / rows), tile = rows * steps;
+  const int v = tid % per >= p.row_pieces, piece = tid % per - v * p.row_pieces;
+  uint8_t* base = p.cache + layer * p.layer_stride + v * p.kv_stride + h * p.head_stride + 16 * piece;
+  for (int j0 = 0; j0 < n; j0 += tile) {
+    if (tid < tile) {
+      const int j = j0 + tid, src = j < n ? s_kept[j] : -1;
+      int64_t page, page_to;
+      int slot, slot_to;
+      const bool move = src > j && place(src, page, slot) && place(j, page_to, slot_to);
+      s_from[tid] = move ? page * p.page_stride + slot * p.token_stride : -1;
+      s_to[tid] = move ? page_to * p.page_stride + slot_to * p.token_stride : -1;
     }
+    __syncthreads();
+    u32x4_t x[kMoveRows];
+#pragma unroll
+    for (int k = 0; k < kMoveRows; ++k) {
+      const int64_t from = k < steps ? s_from[k * rows + row] : -1;
+      x[k] = from >= 0 ? *(const u32x4_t*)(base + from) : u32x4_t{0u, 0u, 0u, 0u};
+    }
+    __syncthreads();  // the tile's rows are in registers, and all weights
+    if (j0 == 0) put_weights();
+#pragma unroll
+    for (int k = 0; k < kMoveRows; ++k) {
+      const int64_t to = k < steps ? s_to[k * rows + row] : -1;
+      if (to >= 0) *(u32x4_t*)(base + to) = x[k];
+    }
+    __syncthreads();
   }
+  if (p.scales)
+    for (int line = 0; line < 2 * p.blocks; ++line) evict_scales<kSmallThreads>(p, layer, h, first, pages, s_kept, n, line);
 }
 
 }  // namespace mi
@@ -303,17 +516,27 @@ extern "C" int mi_kv_evict(const mi_paged_kv* kv, int32_t num_layers, int64_t la
   p.num_indices = num_indices;
   p.num_kv_heads = kv->num_kv_heads;
   p.page_size = kv->page_size;
+  p.page_shift = (kv->page_size & (kv->page_size - 1)) == 0 ? __builtin_ctz((unsigned)kv->page_size) : -1;
   p.keep = keep;
   p.recent = recent;
   p.sinks = sinks;
   p.row_pieces = (kv->dtype == MI_MXFP4 ? kv->head_dim / 2 : kv->head_dim * esz) / 16;
   const int64_t units = (int64_t)num_layers * batch * kv->num_kv_heads;
   p.splits = 1;
-  while (p.splits * 4 < p.row_pieces && 2 * units * p.splits < 4LL * device_cu_count()) p.splits *= 2;
-  if (units * (2 * p.splits + 1) > INT32_MAX) return MI_ERR_UNSUPPORTED;
+  while (p.row_pieces / p.splits >= 16 && 2 * units * p.splits < 2LL * device_cu_count()) p.splits *= 2;
+  p.parts = 2 * p.splits + 1 + (mx ? 2 * p.blocks : 0);
+  if (units * p.parts > INT32_MAX) return MI_ERR_UNSUPPORTED;
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(evict_select_kernel, dim3((uint32_t)units), dim3(kSelThreads), 0, s, p);
-  hipLaunchKernelGGL(evict_move_kernel, dim3((uint32_t)(units * (2 * p.splits + 1))), dim3(kMoveThreads), 0, s, p);
+  if (units <= device_cu_count() && keep <= kSmallKeep && 32LL * p.row_pieces * keep <= kSmallBytes) {
+    hipLaunchKernelGGL(evict_small_kernel, dim3((uint32_t)units), dim3(kSmallThreads), 0, s, p);
+  } else {
+    // a workgroup of 256 holds 8192 tokens, and eight of them share a compute unit
+    if ((int64_t)num_indices * p.page_size / batch <= kSelFew)
+      hipLaunchKernelGGL(evict_select_kernel<256>, dim3((uint32_t)units), dim3(256), 0, s, p);
+    else
+      hipLaunchKernelGGL(evict_select_kernel<1024>, dim3((uint32_t)units), dim3(1024), 0, s, p);
+    hipLaunchKernelGGL(evict_move_kernel, dim3((uint32_t)(units * p.parts)), dim3(kMoveThreads), 0, s, p);
+  }
   MI_CHECK_LAUNCH();
   return MI_OK;
 }

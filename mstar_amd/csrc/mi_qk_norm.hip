@@ -327,6 +327,87 @@ static bool rows_aligned_by8(const void* base, int64_t a, int64_t b) { return (u
 
 }  // namespace mi
 
+extern "C" int mi_qk_norm_rope_block(const mi_qk_norm_rope_args* args) {
+  using namespace mi;
+  if (!args) return MI_ERR_INVALID;
+  const mi_qk_norm_rope_args& a = *args;
+  if (a.num_tokens < 0 || a.num_qo_heads < 0 || a.num_kv_heads < 0 || a.num_append_tokens < 0) return MI_ERR_INVALID;
+  if (a.num_tokens == 0 || a.num_qo_heads + a.num_kv_heads == 0) return MI_OK;
+  if (!a.pos_ids || (a.num_qo_heads > 0 && (!a.q || !a.q_weight)) || (a.num_kv_heads > 0 && (!a.k || !a.k_weight))) return MI_ERR_INVALID;
+  if (a.num_tokens > INT32_MAX - (1 << 20)) return MI_ERR_UNSUPPORTED;  // a grid's stride past the last one is still an int
+  if (a.dtype != MI_BF16 && a.dtype != MI_F16) return MI_ERR_UNSUPPORTED;
+  if (a.weight_dtype != a.dtype && a.weight_dtype != MI_F32) return MI_ERR_UNSUPPORTED;
+  if (a.pos_dtype != MI_I32 && a.pos_dtype != MI_I64) return MI_ERR_UNSUPPORTED;
+  if (a.head_dim <= 0 || a.head_dim % 8 || a.head_dim > kNormDimMax) return MI_ERR_UNSUPPORTED;
+  // a half-split rotation pairs whole 16-byte pieces
+  if (a.rotary_dim <= 0 || a.rotary_dim > a.head_dim || a.rotary_dim % (a.interleave ? 8 : 16)) return MI_ERR_UNSUPPORTED;
+  if (!(a.rope_scale > 0.f) || !(a.rope_theta > 0.f) || !(a.eps >= 0.f)) return MI_ERR_INVALID;
+  if (a.llama31 && (!(a.high_freq_factor > a.low_freq_factor) || !(a.low_freq_factor > 0.f))) return MI_ERR_INVALID;
+  if (a.num_qo_heads > 0 && !rows_aligned_by8(a.q, a.q_stride_token, a.q_stride_head)) return MI_ERR_INVALID;
+  if (a.num_kv_heads > 0 && !rows_aligned_by8(a.k, a.k_stride_token, a.k_stride_head)) return MI_ERR_INVALID;
+  NormRopeParams p{};
+  int dst = kNoCache;
+  if (a.kv) {
+    dst = a.kv->dtype;
+    if (dst != MI_BF16 && dst != MI_F16 && dst != MI_F32 && !kv_is_scaled(dst)) return MI_ERR_UNSUPPORTED;
+    if (!a.kv->data || !a.v || !a.page_idx || !a.slot_idx || a.idx_stride <= 0 || a.kv->page_size <= 0) return MI_ERR_INVALID;
+    if (a.kv->num_kv_heads != a.num_kv_heads || a.kv->head_dim != a.head_dim || a.num_append_tokens > a.num_tokens) return MI_ERR_INVALID;
+    if (kv_is_mx(dst) && a.head_dim % kMxBlock) return MI_ERR_UNSUPPORTED;
+    if (!rows_aligned_by8(a.v, a.v_stride_token, a.v_stride_head) || !kv_scales_ok(a.kv)) return MI_ERR_INVALID;
+    const int esz = kv_elem_bytes(dst);
+    if ((a.kv->page_stride | a.kv->kv_stride | a.kv->token_stride | a.kv->head_stride) % 8 || (uintptr_t)a.kv->data % (8 * esz))
+      return MI_ERR_INVALID;
+    if (kv_is_mx(dst) && !kv_aligned16(a.kv)) return MI_ERR_INVALID;
+    p.cache = (uint8_t*)a.kv->data;
+    p.page_stride = a.kv->page_stride;
+    p.kv_stride = a.kv->kv_stride;
+    p.token_stride = a.kv->token_stride;
+    p.head_stride = a.kv->head_stride;
+    p.max_pages = a.kv->max_pages;
+    p.k_scale = (void*)a.kv->k_scale;
+    p.v_scale = (void*)a.kv->v_scale;
+    p.page_idx = a.page_idx;
+    p.slot_idx = a.slot_idx;
+    p.idx_stride = a.idx_stride;
+    p.num_tokens_device = a.num_tokens_device;
+    p.num_append = a.num_append_tokens;
+    p.page_size = a.kv->page_size;
+  }
+  p.q = a.q;
+  p.k = a.k;
+  p.v = a.v;
+  p.q_stride_tok = a.q_stride_token;
+  p.q_stride_head = a.q_stride_head;
+  p.k_stride_tok = a.k_stride_token;
+  p.k_stride_head = a.k_stride_head;
+  p.v_stride_tok = a.v_stride_token;
+  p.v_stride_head = a.v_stride_head;
+  // a side without heads reads the other's weight, and uses none of it
+  p.q_weight = a.num_qo_heads ? a.q_weight : a.k_weight;
+  p.k_weight = a.num_kv_heads ? a.k_weight : a.q_weight;
+  p.pos = a.pos_ids;
+  p.pos_is_64 = a.pos_dtype == MI_I64;
+  p.num_tokens = a.num_tokens;
+  p.num_qo_heads = a.num_qo_heads;
+  p.num_kv_heads = a.num_kv_heads;
+  p.head_dim = a.head_dim;
+  p.rotary_dim = a.rotary_dim;
+  p.weight_f32 = a.weight_dtype == MI_F32;
+  p.keep_k = a.keep_k ? 1 : 0;
+  p.eps = a.eps;
+  const double two_pi = 6.283185307179586476925286766559, span = (double)a.high_freq_factor - (double)a.low_freq_factor;
+  p.step = -2.0 / a.rotary_dim * std::log2((double)a.rope_theta);
+  p.inv_scale = 1.0 / (double)a.rope_scale;
+  p.llama31 = a.llama31 ? 1 : 0;
+  p.slope = a.llama31 ? (double)a.old_context_len / two_pi / span : 0.0;
+  p.bias = a.llama31 ? (double)a.low_freq_factor / span : 0.0;
+  hipStream_t s = (hipStream_t)a.stream;
+  const int st = a.dtype == MI_BF16 ? launch_norm_dst<BF16>(p, dst, a.interleave != 0, s) : launch_norm_dst<F16>(p, dst, a.interleave != 0, s);
+  if (st != MI_OK) return st;
+  MI_CHECK_LAUNCH();
+  return MI_OK;
+}
+
 extern "C" int mi_qk_norm_rope(void* q, int64_t q_stride_token, int64_t q_stride_head, int32_t num_qo_heads, void* k,
                                int64_t k_stride_token, int64_t k_stride_head, int32_t num_kv_heads, const void* v,
                                int64_t v_stride_token, int64_t v_stride_head, int32_t dtype, int32_t head_dim,
@@ -336,80 +417,10 @@ extern "C" int mi_qk_norm_rope(void* q, int64_t q_stride_token, int64_t q_stride
                                const void* pos_ids, int32_t pos_dtype, int32_t num_tokens, int32_t interleave,
                                float rope_scale, float rope_theta, int32_t llama31, float low_freq_factor,
                                float high_freq_factor, float old_context_len, void* stream) {
-  using namespace mi;
-  if (num_tokens < 0 || num_qo_heads < 0 || num_kv_heads < 0 || num_append_tokens < 0) return MI_ERR_INVALID;
-  if (num_tokens == 0 || num_qo_heads + num_kv_heads == 0) return MI_OK;
-  if (!pos_ids || (num_qo_heads > 0 && (!q || !q_weight)) || (num_kv_heads > 0 && (!k || !k_weight))) return MI_ERR_INVALID;
-  if (num_tokens > INT32_MAX - (1 << 20)) return MI_ERR_UNSUPPORTED;  // a grid's stride past the last one is still an int
-  if (dtype != MI_BF16 && dtype != MI_F16) return MI_ERR_UNSUPPORTED;
-  if (weight_dtype != dtype && weight_dtype != MI_F32) return MI_ERR_UNSUPPORTED;
-  if (pos_dtype != MI_I32 && pos_dtype != MI_I64) return MI_ERR_UNSUPPORTED;
-  if (head_dim <= 0 || head_dim % 8 || head_dim > kNormDimMax) return MI_ERR_UNSUPPORTED;
-  // a half-split rotation pairs whole 16-byte pieces
-  if (rotary_dim <= 0 || rotary_dim > head_dim || rotary_dim % (interleave ? 8 : 16)) return MI_ERR_UNSUPPORTED;
-  if (!(rope_scale > 0.f) || !(rope_theta > 0.f) || !(eps >= 0.f)) return MI_ERR_INVALID;
-  if (llama31 && (!(high_freq_factor > low_freq_factor) || !(low_freq_factor > 0.f))) return MI_ERR_INVALID;
-  if (num_qo_heads > 0 && !rows_aligned_by8(q, q_stride_token, q_stride_head)) return MI_ERR_INVALID;
-  if (num_kv_heads > 0 && !rows_aligned_by8(k, k_stride_token, k_stride_head)) return MI_ERR_INVALID;
-  NormRopeParams p{};
-  int dst = kNoCache;
-  if (kv) {
-    dst = kv->dtype;
-    if (dst != MI_BF16 && dst != MI_F16 && dst != MI_F32 && !kv_is_scaled(dst)) return MI_ERR_UNSUPPORTED;
-    if (!kv->data || !v || !page_idx || !slot_idx || idx_stride <= 0 || kv->page_size <= 0) return MI_ERR_INVALID;
-    if (kv->num_kv_heads != num_kv_heads || kv->head_dim != head_dim || num_append_tokens > num_tokens) return MI_ERR_INVALID;
-    if (kv_is_mx(dst) && head_dim % kMxBlock) return MI_ERR_UNSUPPORTED;
-    if (!rows_aligned_by8(v, v_stride_token, v_stride_head) || !kv_scales_ok(kv)) return MI_ERR_INVALID;
-    const int esz = kv_elem_bytes(dst);
-    if ((kv->page_stride | kv->kv_stride | kv->token_stride | kv->head_stride) % 8 || (uintptr_t)kv->data % (8 * esz))
-      return MI_ERR_INVALID;
-    if (kv_is_mx(dst) && !kv_aligned16(kv)) return MI_ERR_INVALID;
-    p.cache = (uint8_t*)kv->data;
-    p.page_stride = kv->page_stride;
-    p.kv_stride = kv->kv_stride;
-    p.token_stride = kv->token_stride;
-    p.head_stride = kv->head_stride;
-    p.max_pages = kv->max_pages;
-    p.k_scale = (void*)kv->k_scale;
-    p.v_scale = (void*)kv->v_scale;
-    p.page_idx = page_idx;
-    p.slot_idx = slot_idx;
-    p.idx_stride = idx_stride;
-    p.num_tokens_device = num_tokens_device;
-    p.num_append = num_append_tokens;
-    p.page_size = kv->page_size;
-  }
-  p.q = q;
-  p.k = k;
-  p.v = v;
-  p.q_stride_tok = q_stride_token;
-  p.q_stride_head = q_stride_head;
-  p.k_stride_tok = k_stride_token;
-  p.k_stride_head = k_stride_head;
-  p.v_stride_tok = v_stride_token;
-  p.v_stride_head = v_stride_head;
-  // a side without heads reads the other's weight, and uses none of it
-  p.q_weight = num_qo_heads ? q_weight : k_weight;
-  p.k_weight = num_kv_heads ? k_weight : q_weight;
-  p.pos = pos_ids;
-  p.pos_is_64 = pos_dtype == MI_I64;
-  p.num_tokens = num_tokens;
-  p.num_qo_heads = num_qo_heads;
-  p.num_kv_heads = num_kv_heads;
-  p.head_dim = head_dim;
-  p.rotary_dim = rotary_dim;
-  p.weight_f32 = weight_dtype == MI_F32;
-  p.keep_k = keep_k ? 1 : 0;
-  p.eps = eps;
-  const double two_pi = 6.283185307179586476925286766559, span = (double)high_freq_factor - (double)low_freq_factor;
-  p.step = -2.0 / rotary_dim * std::log2((double)rope_theta);
-  p.inv_scale = 1.0 / (double)rope_scale;
-  p.llama31 = llama31 ? 1 : 0;
-  p.slope = llama31 ? (double)old_context_len / two_pi / span : 0.0;
-  p.bias = llama31 ? (double)low_freq_factor / span : 0.0;
-  hipStream_t s = (hipStream_t)stream;
-  const int st = dtype == MI_BF16 ? launch_norm_dst<BF16>(p, dst, interleave != 0, s) : launch_norm_dst<F16>(p, dst, interleave != 0, s);
-  if (st != MI_OK) return st;
-  MI_CHECK_LAUNCH();
-  return MI_OK;
+  const mi_qk_norm_rope_args args = {
+      q, k, v, q_weight, k_weight, pos_ids, kv, page_idx, slot_idx, num_tokens_device, stream, q_stride_token, q_stride_head,
+      k_stride_token, k_stride_head, v_stride_token, v_stride_head, idx_stride, num_qo_heads, num_kv_heads, dtype, head_dim,
+      weight_dtype, keep_k, num_append_tokens, rotary_dim, pos_dtype, num_tokens, interleave, llama31, eps, rope_scale,
+      rope_theta, low_freq_factor, high_freq_factor, old_context_len};
+  return mi_qk_norm_rope_block(&args);
 }

@@ -43,7 +43,7 @@ import torch
 
 from . import _lib
 from .mx_cache import MXKVLayer
-from .rope import apply_llama31_rope_pos_ids_inplace, apply_rope_pos_ids_inplace, qk_norm_rope_append, rope_append
+from .rope import apply_llama31_rope_pos_ids_inplace, apply_rope_pos_ids_inplace, rope_append, _qk_norm_rope
 from .trace import trace_range
 
 __all__ = [
@@ -345,9 +345,8 @@ class _FusedRopeAppend:
         """
         if self.dtype is None:
             raise RuntimeError("plan() must be called before qk_norm_rope_set_kv_cache()")
-        qk_norm_rope_append(q, k, v, q_weight, k_weight, kv_cache_layer, pos_ids, *self._append_target(), eps=eps,
-                            rotary_dim=rotary_dim, interleave=interleave, rope_scale=rope_scale, rope_theta=rope_theta,
-                            k_scale=k_scale, v_scale=v_scale, keep_k=keep_k, llama31=llama31)
+        _qk_norm_rope(q, k, v, q_weight, k_weight, pos_ids, eps, rotary_dim, interleave, rope_scale, rope_theta, llama31, keep_k,
+                      kv_cache_layer, k_scale, v_scale, *self._append_target())
 
 
 class _Weights:

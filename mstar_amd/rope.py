@@ -13,6 +13,8 @@ by head before the rotation, in the same pass (``mi_qk_norm_rope``).
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -150,20 +152,27 @@ def _norm_rows(x: torch.Tensor, name: str) -> tuple[torch.Size, int, int, int]:
     return shape, ptr, st, sh
 
 
-def _qk_norm_rope(q, k, v, q_weight, k_weight, pos_ids, eps, rotary_dim, interleave, rope_scale, rope_theta, llama31,
-                  keep_k, desc, page_idx, slot_idx_ptr, idx_stride, num_append, num_append_device_ptr) -> None:
-    # a launch is over before these checks are, in a decode step: each attribute is read once
+def _qk_norm_rope(q, k, v, q_weight, k_weight, pos_ids, eps, rotary_dim, interleave, rope_scale, rope_theta, llama31, keep_k,
+                  layer=None, k_scale=None, v_scale=None, page_idx=None, slot_at=None, idx_stride=0, n_append=0, n_device_at=None):
+    # in a decode step the launch is over before these checks are: each attribute is read once
     (n, hq, d), q_at, q_st, q_sh = _norm_rows(q, "q")
     (n_k, hkv, d_k), k_at, k_st, k_sh = _norm_rows(k, "k")
     dtype, at = q.dtype, q.get_device()
     if k.dtype is not dtype or n_k != n or d_k != d or k.get_device() != at:
         raise ValueError("q and k must agree on dtype, device, token count and head_dim")
-    v_at, v_st, v_sh, page_at = None, 0, 0, None
-    if v is not None:
+    v_at = v_st = v_sh = desc_at = page_at = 0
+    if page_idx is not None:
         v_shape, v_at, v_st, v_sh = _norm_rows(v, "v")
         if v.dtype is not dtype or v_shape != (n, hkv, d) or v.get_device() != at:
             raise ValueError(f"v {tuple(v_shape)}, {v.dtype} does not agree with k {tuple(k.shape)}, {k.dtype}")
-        page_at = page_idx.data_ptr()
+        desc = _lib.paged_kv_desc(layer, k_scale, v_scale)
+        if layer.device != k.device:
+            raise ValueError(f"kv_cache_layer must be on {k.device}, not on {layer.device}")
+        if desc.num_kv_heads != hkv or desc.head_dim != d:
+            raise ValueError(f"k/v shape {tuple(k.shape)} does not match the cache heads/head_dim")
+        if n_append > n:
+            raise ValueError(f"k/v hold {n} tokens, {n_append} planned")
+        desc_at, page_at = ctypes.addressof(desc), page_idx.data_ptr()
     rd = d if rotary_dim is None else int(rotary_dim)
     least = 8 if interleave else 16
     if rd <= 0 or rd > d or rd % least or d % 8 or d > 512:
@@ -183,11 +192,10 @@ def _qk_norm_rope(q, k, v, q_weight, k_weight, pos_ids, eps, rotary_dim, interle
         smooth = 1
         low, high = llama31.get("low_freq_factor", low), llama31.get("high_freq_factor", high)
         old = llama31.get("old_context_len", old)
-    status = _lib.lib().mi_qk_norm_rope(
-        q_at, q_st, q_sh, hq, k_at, k_st, k_sh, hkv, v_at, v_st, v_sh, _DTYPES[dtype], d, q_weight.data_ptr(),
-        k_weight.data_ptr(), wd, float(eps), 1 if keep_k else 0, desc, page_at, slot_idx_ptr, idx_stride, num_append, num_append_device_ptr, rd,
-        pos_ids.data_ptr(), pos_type, n, 1 if interleave else 0, float(rope_scale), float(rope_theta), smooth, float(low),
-        float(high), float(old), _lib.stream_at(at))
+    status = _lib.lib().mi_qk_norm_rope_block(_lib.QK_NORM_ROPE_ARGS.pack(
+        q_at, k_at, v_at, q_weight.data_ptr(), k_weight.data_ptr(), pos_ids.data_ptr(), desc_at, page_at, slot_at or 0,
+        n_device_at or 0, _lib.stream_at(at), q_st, q_sh, k_st, k_sh, v_st, v_sh, idx_stride, hq, hkv, _DTYPES[dtype], d, wd,
+        1 if keep_k else 0, n_append, rd, pos_type, n, 1 if interleave else 0, smooth, eps, rope_scale, rope_theta, low, high, old))
     if status:
         _lib.check(status, "mi_qk_norm_rope")
 
@@ -203,8 +211,7 @@ def apply_qk_norm_rope_pos_ids_inplace(q: torch.Tensor, k: torch.Tensor, q_weigh
     :func:`apply_llama31_rope_pos_ids_inplace`, ``rope_scale`` given).  fp32 throughout, rounded once; angles are formed in 64
     bits, so far positions turn more exactly than in the calls without a norm.
     """
-    _qk_norm_rope(q, k, None, q_weight, k_weight, pos_ids, eps, rotary_dim, interleave, rope_scale, rope_theta, llama31,
-                  True, None, None, None, 0, 0, None)
+    _qk_norm_rope(q, k, None, q_weight, k_weight, pos_ids, eps, rotary_dim, interleave, rope_scale, rope_theta, llama31, True)
 
 
 def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -218,15 +225,10 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
     Page map and ``keep_k`` as in :func:`rope_append`; any cache type, microscaled layers among them.  k is rounded
     once, from fp32 to the cache's type.
     """
-    desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
-    if kv_cache_layer.device != k.device:
-        raise ValueError(f"kv_cache_layer must be on {k.device}, not on {kv_cache_layer.device}")
-    if k.shape[1:] != (desc.num_kv_heads, desc.head_dim):
-        raise ValueError(f"k/v shape {tuple(k.shape)} does not match the cache heads/head_dim")
-    if num_append > k.shape[0]:
-        raise ValueError(f"k/v hold {k.shape[0]} tokens, {num_append} planned")
-    _qk_norm_rope(q, k, v, q_weight, k_weight, pos_ids, eps, rotary_dim, interleave, rope_scale, rope_theta, llama31,
-                  keep_k, desc, page_idx, slot_idx_ptr, idx_stride, num_append, num_append_device_ptr)
+    if page_idx is None:
+        raise ValueError("page_idx must be a tensor of page ids")
+    _qk_norm_rope(q, k, v, q_weight, k_weight, pos_ids, eps, rotary_dim, interleave, rope_scale, rope_theta, llama31, keep_k,
+                  kv_cache_layer, k_scale, v_scale, page_idx, slot_idx_ptr, idx_stride, num_append, num_append_device_ptr)
 
 
 def rope_positions(qo_indptr: torch.Tensor, position_id_start: torch.Tensor, out: torch.Tensor,

@@ -130,6 +130,22 @@ def test_many_layers_and_requests(gpu):
     _check(gpu, "mx4", 2, np.random.default_rng(2).integers(1, 3000, 9).tolist(), 32, 3, 128, 700, 50, 4, True)
 
 
+@pytest.mark.parametrize("kind,d,lens,keep", [
+    ("mx4", 64, [9000, 5001, 5000], 5000), ("mx4", 128, [6000, 2500, 77], 2400), ("mx8", 64, [7000], 3001), ("f32", 256, [2000, 700], 513),
+    ("fp8", 256, [3000, 1300], 1029), ("f16", 128, [40000, 33333], 2111)])
+def test_many_kept(gpu, kind, d, lens, keep):
+    """Rows of 32 bytes to 1 KiB, over several tiles, more tokens than a workgroup holds at once."""
+    for layers in (0, 2):
+        _check(gpu, kind, layers, lens, 16, 2, d, keep, 100, 4, layers == 2)
+
+
+@pytest.mark.parametrize("keep", [255, 256, 511, 512, 1023, 1025])
+def test_either_side_of_what_one_launch_does(gpu, keep):
+    for lens in ([keep, keep + 1, 3 * keep, 12], [2 * keep + 5]):
+        _check(gpu, "bf16", 0, lens, 16, 2, 128, keep, 30, 4, True)
+        _check(gpu, "fp8", 2, lens, 32, 1, 128, keep, 30, 0, False)
+
+
 def test_again_after_more_tokens(gpu):
     """Evicted, grown and evicted again, on the shorter page lists that remain."""
     ps, hkv, d, keep = 16, 2, 64, 48
