@@ -523,7 +523,7 @@ int mi_qk_norm_rope_block(const mi_qk_norm_rope_args* args);
  * mi_decode_run.  parts: 1 requests of at most 16 rows (qo_len x q heads a kv head), 2 the others, 3 both
  * (qo_indptr == NULL: 1).  Page ids outside [0, max_pages) get no weights.  Requests of a call share
  * no page.  The same call gives the same bits.  workspace: mi_attention_weights_bytes of the same sizes
- * (ragged: qo_indptr != NULL), 16-byte aligned, scratch of this call alone.
+ * (ragged: qo_indptr != NULL; where that is none, NULL), 16-byte aligned, scratch of this call alone.
  * ------------------------------------------------------------------------ */
 int64_t mi_attention_weights_bytes(int32_t batch, int32_t max_qo_tokens, int32_t num_indices, int32_t page_size,
                                    int32_t num_qo_heads, int32_t num_kv_heads, int32_t ragged, int32_t parts);
@@ -533,6 +533,23 @@ int mi_attention_weights(const void* q, int32_t q_dtype, int64_t q_stride_token,
                          int32_t max_qo_tokens, int32_t num_indices, int32_t num_qo_heads, int32_t causal,
                          float sm_scale, int32_t parts, float* weights, void* workspace, int64_t workspace_bytes,
                          void* stream);
+
+/* The same call, its arguments in one block. */
+typedef struct mi_attention_weights_args {
+  const void* q;
+  const mi_paged_kv* kv;
+  const int32_t* qo_indptr;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* last_page_len;
+  float* weights;
+  void* workspace;
+  void* stream;
+  int64_t q_stride_token, q_stride_head, workspace_bytes;
+  int32_t q_dtype, batch, max_qo_tokens, num_indices, num_qo_heads, causal, parts;
+  float sm_scale;
+} mi_attention_weights_args;
+int mi_attention_weights_block(const mi_attention_weights_args* args);
 
 /* Eviction by such weights.  For every layer l < num_layers, request and kv head whose request
  * holds more than `keep` tokens, the first `sinks` tokens, the last `recent` and the
@@ -550,6 +567,21 @@ int mi_kv_evict(const mi_paged_kv* kv, int32_t num_layers, int64_t layer_stride,
                 const float* weights, float* out_weights, int64_t weights_layer_stride, const int32_t* kv_indptr,
                 const int32_t* kv_indices, const int32_t* last_page_len, int32_t batch, int32_t num_indices,
                 int32_t keep, int32_t recent, int32_t sinks, int32_t* kept, void* stream);
+
+/* The same call, its arguments in one block. */
+typedef struct mi_kv_evict_args {
+  const mi_paged_kv* kv;
+  const float* weights;
+  float* out_weights;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* last_page_len;
+  int32_t* kept;
+  void* stream;
+  int64_t layer_stride, scale_layer_stride, weights_layer_stride;
+  int32_t num_layers, batch, num_indices, keep, recent, sinks;
+} mi_kv_evict_args;
+int mi_kv_evict_block(const mi_kv_evict_args* args);
 
 /* ------------------------------------------------------------------------
  * Page snapshot copies (multi-label / CFG planning).

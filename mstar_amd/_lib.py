@@ -204,6 +204,8 @@ SIGNATURES = {
          _F32, _P],
     ),
     "mi_qk_norm_rope_block": (ctypes.c_int, [ctypes.c_char_p]),
+    "mi_attention_weights_block": (ctypes.c_int, [ctypes.c_char_p]),
+    "mi_kv_evict_block": (ctypes.c_int, [ctypes.c_char_p]),
     "mi_attention_weights_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32]),
     "mi_attention_weights": (
         ctypes.c_int,
@@ -216,8 +218,10 @@ SIGNATURES = {
     ),
 }
 
-# mi_qk_norm_rope_args: packing 36 values and passing one costs the host a sixth of converting them one by one
+# The argument blocks of mi_*_block: packing 36 values and passing one costs the host a sixth of converting each.
 QK_NORM_ROPE_ARGS = struct.Struct("@11P7q12i6f")
+ATTENTION_WEIGHTS_ARGS = struct.Struct("@9P3q7if")
+KV_EVICT_ARGS = struct.Struct("@8P3q6i")
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -469,69 +469,68 @@ __global__ __launch_bounds__(kSmallThreads) void evict_small_kernel(EvictParams 
 
 }  // namespace mi
 
-extern "C" int mi_kv_evict(const mi_paged_kv* kv, int32_t num_layers, int64_t layer_stride, int64_t scale_layer_stride,
-                           const float* weights, float* out_weights, int64_t weights_layer_stride, const int32_t* kv_indptr,
-                           const int32_t* kv_indices, const int32_t* last_page_len, int32_t batch, int32_t num_indices, int32_t keep,
-                           int32_t recent, int32_t sinks, int32_t* kept, void* stream) {
+extern "C" int mi_kv_evict_block(const mi_kv_evict_args* args) {
   using namespace mi;
-  if (!kv || num_layers < 0 || batch < 0 || num_indices < 0) return MI_ERR_INVALID;
-  if (keep <= 0 || recent < 0 || sinks < 0 || recent > keep - sinks) return MI_ERR_INVALID;
-  if (num_layers == 0 || batch == 0) return MI_OK;
-  if (!kv->data || !weights || !out_weights || !kv_indptr || !kv_indices || !last_page_len || !kept) return MI_ERR_INVALID;
-  if (kv->num_kv_heads <= 0 || kv->head_dim <= 0 || kv->page_size <= 0 || kv->max_pages < 0) return MI_ERR_INVALID;
+  if (!args) return MI_ERR_INVALID;
+  const mi_kv_evict_args& a = *args;
+  if (!a.kv || a.num_layers < 0 || a.batch < 0 || a.num_indices < 0) return MI_ERR_INVALID;
+  if (a.keep <= 0 || a.recent < 0 || a.sinks < 0 || a.recent > a.keep - a.sinks) return MI_ERR_INVALID;
+  if (a.num_layers == 0 || a.batch == 0) return MI_OK;
+  if (!a.kv->data || !a.weights || !a.out_weights || !a.kv_indptr || !a.kv_indices || !a.last_page_len || !a.kept) return MI_ERR_INVALID;
+  if (a.kv->num_kv_heads <= 0 || a.kv->head_dim <= 0 || a.kv->page_size <= 0 || a.kv->max_pages < 0) return MI_ERR_INVALID;
   // places in the page list are counted in 32 bits
-  if (kv->page_size % 4 || kv->page_size > (1 << 24) || (int64_t)num_indices * kv->page_size > INT32_MAX - (1 << 25))
+  if (a.kv->page_size % 4 || a.kv->page_size > (1 << 24) || (int64_t)a.num_indices * a.kv->page_size > INT32_MAX - (1 << 25))
     return MI_ERR_UNSUPPORTED;
-  const bool mx = kv_is_mx(kv->dtype);
-  if (!mx && kv->dtype != MI_BF16 && kv->dtype != MI_F16 && kv->dtype != MI_F32 && kv->dtype != MI_FP8_E4M3) return MI_ERR_UNSUPPORTED;
-  if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256) return MI_ERR_UNSUPPORTED;
-  const int esz = kv_elem_bytes(kv->dtype);
-  if (!kv_aligned16(kv) || (layer_stride * esz) % 16) return MI_ERR_INVALID;
-  if (((uintptr_t)weights | (uintptr_t)out_weights) % 16 || weights_layer_stride % 4) return MI_ERR_INVALID;
-  if (mx && (!kv_scales_ok(kv) || kv->head_dim % kMxBlock)) return MI_ERR_INVALID;
+  const bool mx = kv_is_mx(a.kv->dtype);
+  if (!mx && a.kv->dtype != MI_BF16 && a.kv->dtype != MI_F16 && a.kv->dtype != MI_F32 && a.kv->dtype != MI_FP8_E4M3) return MI_ERR_UNSUPPORTED;
+  if (a.kv->head_dim != 64 && a.kv->head_dim != 128 && a.kv->head_dim != 256) return MI_ERR_UNSUPPORTED;
+  const int esz = kv_elem_bytes(a.kv->dtype);
+  if (!kv_aligned16(a.kv) || (a.layer_stride * esz) % 16) return MI_ERR_INVALID;
+  if (((uintptr_t)a.weights | (uintptr_t)a.out_weights) % 16 || a.weights_layer_stride % 4) return MI_ERR_INVALID;
+  if (mx && (!kv_scales_ok(a.kv) || a.kv->head_dim % kMxBlock)) return MI_ERR_INVALID;
   EvictParams p{};
-  p.cache = (uint8_t*)kv->data;
-  p.layer_stride = layer_stride * esz;
-  p.page_stride = kv->page_stride * esz;
-  p.kv_stride = kv->kv_stride * esz;
-  p.token_stride = kv->token_stride * esz;
-  p.head_stride = kv->head_stride * esz;
-  p.max_pages = kv->max_pages;
-  p.blocks = kv->head_dim / kMxBlock;
+  p.cache = (uint8_t*)a.kv->data;
+  p.layer_stride = a.layer_stride * esz;
+  p.page_stride = a.kv->page_stride * esz;
+  p.kv_stride = a.kv->kv_stride * esz;
+  p.token_stride = a.kv->token_stride * esz;
+  p.head_stride = a.kv->head_stride * esz;
+  p.max_pages = a.kv->max_pages;
+  p.blocks = a.kv->head_dim / kMxBlock;
   if (mx) {
     // one array: V's bytes follow K's within a page
-    if ((const uint8_t*)kv->v_scale - (const uint8_t*)kv->k_scale != (int64_t)kv->num_kv_heads * p.blocks * kv->page_size)
+    if ((const uint8_t*)a.kv->v_scale - (const uint8_t*)a.kv->k_scale != (int64_t)a.kv->num_kv_heads * p.blocks * a.kv->page_size)
       return MI_ERR_INVALID;
-    p.scales = (uint8_t*)kv->k_scale;
-    p.scale_layer_stride = scale_layer_stride;
+    p.scales = (uint8_t*)a.kv->k_scale;
+    p.scale_layer_stride = a.scale_layer_stride;
   }
-  p.weights = weights;
-  p.out_weights = out_weights;
-  p.weights_layer_stride = weights_layer_stride;
-  p.kv_indptr = kv_indptr;
-  p.kv_indices = kv_indices;
-  p.last_page_len = last_page_len;
-  p.kept = kept;
-  p.batch = batch;
-  p.num_indices = num_indices;
-  p.num_kv_heads = kv->num_kv_heads;
-  p.page_size = kv->page_size;
-  p.page_shift = (kv->page_size & (kv->page_size - 1)) == 0 ? __builtin_ctz((unsigned)kv->page_size) : -1;
-  p.keep = keep;
-  p.recent = recent;
-  p.sinks = sinks;
-  p.row_pieces = (kv->dtype == MI_MXFP4 ? kv->head_dim / 2 : kv->head_dim * esz) / 16;
-  const int64_t units = (int64_t)num_layers * batch * kv->num_kv_heads;
+  p.weights = a.weights;
+  p.out_weights = a.out_weights;
+  p.weights_layer_stride = a.weights_layer_stride;
+  p.kv_indptr = a.kv_indptr;
+  p.kv_indices = a.kv_indices;
+  p.last_page_len = a.last_page_len;
+  p.kept = a.kept;
+  p.batch = a.batch;
+  p.num_indices = a.num_indices;
+  p.num_kv_heads = a.kv->num_kv_heads;
+  p.page_size = a.kv->page_size;
+  p.page_shift = (a.kv->page_size & (a.kv->page_size - 1)) == 0 ? __builtin_ctz((unsigned)a.kv->page_size) : -1;
+  p.keep = a.keep;
+  p.recent = a.recent;
+  p.sinks = a.sinks;
+  p.row_pieces = (a.kv->dtype == MI_MXFP4 ? a.kv->head_dim / 2 : a.kv->head_dim * esz) / 16;
+  const int64_t units = (int64_t)a.num_layers * a.batch * a.kv->num_kv_heads;
   p.splits = 1;
   while (p.row_pieces / p.splits >= 16 && 2 * units * p.splits < 2LL * device_cu_count()) p.splits *= 2;
   p.parts = 2 * p.splits + 1 + (mx ? 2 * p.blocks : 0);
   if (units * p.parts > INT32_MAX) return MI_ERR_UNSUPPORTED;
-  hipStream_t s = (hipStream_t)stream;
-  if (units <= device_cu_count() && keep <= kSmallKeep && 32LL * p.row_pieces * keep <= kSmallBytes) {
+  hipStream_t s = (hipStream_t)a.stream;
+  if (units <= device_cu_count() && a.keep <= kSmallKeep && 32LL * p.row_pieces * a.keep <= kSmallBytes) {
     hipLaunchKernelGGL(evict_small_kernel, dim3((uint32_t)units), dim3(kSmallThreads), 0, s, p);
   } else {
     // a workgroup of 256 holds 8192 tokens, and eight of them share a compute unit
-    if ((int64_t)num_indices * p.page_size / batch <= kSelFew)
+    if ((int64_t)a.num_indices * p.page_size / a.batch <= kSelFew)
       hipLaunchKernelGGL(evict_select_kernel<256>, dim3((uint32_t)units), dim3(256), 0, s, p);
     else
       hipLaunchKernelGGL(evict_select_kernel<1024>, dim3((uint32_t)units), dim3(1024), 0, s, p);
@@ -539,4 +538,12 @@ extern "C" int mi_kv_evict(const mi_paged_kv* kv, int32_t num_layers, int64_t la
   }
   MI_CHECK_LAUNCH();
   return MI_OK;
+}
+
+extern "C" int mi_kv_evict(const mi_paged_kv* kv, int32_t num_layers, int64_t layer_stride, int64_t scale_layer_stride,
+                           const float* weights, float* out_weights, int64_t weights_layer_stride, const int32_t* kv_indptr,
+                           const int32_t* kv_indices, const int32_t* last_page_len, int32_t batch, int32_t num_indices, int32_t keep,
+                           int32_t recent, int32_t sinks, int32_t* kept, void* stream) {
+  const mi_kv_evict_args args = {kv, weights, out_weights, kv_indptr, kv_indices, last_page_len, kept, stream, layer_stride, scale_layer_stride, weights_layer_stride, num_layers, batch, num_indices, keep, recent, sinks};
+  return mi_kv_evict_block(&args);
 }

@@ -25,29 +25,56 @@ int weights_launch_16(const WeightsParams& p, int q_dtype, int head_dim, int whi
                              : launch_weights_kvt<F32, kKv16>(p, head_dim, which, grid, s);
 }
 
-// The second launch over short queries: a unit's tokens, four to a thread.
+// The second launch over short queries: four tokens to a thread.
 __global__ __launch_bounds__(256) void weights_finish_kernel(WeightsParams p) {
   __shared__ float s_m[16][kWRows], s_l[16][kWRows], s_lse[kWRows];
   const int tid = (int)threadIdx.x, nkv = p.num_kv_heads;
   const int h = uniform((int)(blockIdx.x % nkv)), unit = uniform((int)(blockIdx.x / nkv));
-  const int r = uniform(unit_request(p.kv_indptr, 1, p.unit_pages, p.batch, unit));
+  const int r = uniform(unit_request(p.kv_indptr, 1, p.finish_pages, p.batch, unit));
   if (r < 0) return;
   const WRequest q = w_request(p, r);
   if (q.rows <= 0 || q.rows > kWRows) return;
-  const int begin = unit_begin(p.kv_indptr, 1, p.unit_pages, r), unit_tokens = p.unit_pages * p.page_size;
-  const int tok0 = (unit - begin) * unit_tokens, tok1 = min(tok0 + unit_tokens, q.len);
+  const int tok0 = (unit - unit_begin(p.kv_indptr, 1, p.finish_pages, r)) * p.finish_pages * p.page_size;
+  const int tok1 = min(tok0 + p.finish_pages * p.page_size, q.len), off = q.len - q.qo_len;
   if (tok0 >= tok1) return;
-  // the request's log-sum-exp: 16 threads a row go through its units
+  constexpr int kAhead = 8;  // rows whose scores are loaded with the token's weight, the first time ahead of the join
+  float4 s[kAhead], old;
+  float* w;
+  const float* src;
+  auto load = [&](int t) {
+    src = p.scores + (((((int64_t)q.first * p.page_size + t) >> 4) * nkv + h) * p.score_rows * 16 + (t & 15));
+    const int e = (int)((unsigned)t / (unsigned)p.page_size);
+    const int64_t page = p.kv_indices[q.first + e];
+    w = page >= 0 && page < p.max_pages ? p.weights + (page * nkv + h) * p.page_size + t - e * p.page_size : nullptr;
+#pragma unroll
+    for (int row = 0; row < kAhead; ++row)
+      if (row < q.rows) s[row] = *(const float4*)(src + 16 * row);
+    old = w ? *(const float4*)w : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  int t = tok0 + 4 * tid;
+  if (t < tok1) load(t);
+  // the request's log-sum-exp: 16 threads a row go through its units of scores
   {
-    const int row = tid & 15, part = tid >> 4, units = (q.len + unit_tokens - 1) / unit_tokens;
+    const int row = tid & 15, part = tid >> 4, tokens = p.unit_pages * p.page_size, units = (q.len + tokens - 1) / tokens;
+    const int begin = unit_begin(p.kv_indptr, 1, p.unit_pages, r);
     float m = -kWInf, l = 0.f;
     bool bad = false;
-    for (int u = part; u < units; u += 16) {
-      const float e = p.unit_lse[((int64_t)(begin + u) * nkv + h) * kWRows + row];
-      bad |= e != e;
-      if (e == kWInf) continue;  // saw nothing there
-      const float mn = fmaxf(m, e), mu = mn == -kWInf ? 0.f : mn;
-      l = l * fast_exp2(m - mu) + fast_exp2(e - mu);
+    for (int u0 = part; u0 < units; u0 += 16 * 8) {  // eight in flight
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        e[i] = u0 + 16 * i < units ? p.unit_lse[((int64_t)(begin + u0 + 16 * i) * nkv + h) * kWRows + row] : kWInf;
+      float mn = m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        bad |= e[i] != e[i];
+        if (e[i] == kWInf) e[i] = -kWInf;  // saw nothing there
+        mn = fmaxf(mn, e[i]);
+      }
+      const float mu = mn == -kWInf ? 0.f : mn;
+      l *= fast_exp2(m - mu);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) l += fast_exp2(e[i] - mu);
       m = mn;
     }
     s_m[part][row] = m;
@@ -62,32 +89,30 @@ __global__ __launch_bounds__(256) void weights_finish_kernel(WeightsParams p) {
     }
     __syncthreads();
   }
-  const int off = q.len - q.qo_len;
-  for (int t = tok0 + 4 * tid; t < tok1; t += 1024) {
-    const int64_t tile = ((int64_t)q.first * p.page_size + t) >> 4;
-    const float* src = p.scores + (tile * nkv + h) * p.score_rows * 16 + (t & 15);
+  while (t < tok1) {
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int row = 0; row < q.rows; ++row) {
-      const float4 s = *(const float4*)(src + 16 * row);
-      const float e = s_lse[row];
-      sum.x += fast_exp2(s.x - e);
-      sum.y += fast_exp2(s.y - e);
-      sum.z += fast_exp2(s.z - e);
-      sum.w += fast_exp2(s.w - e);
-    }
-    const int e = (int)((unsigned)t / (unsigned)p.page_size);
-    const int64_t page = p.kv_indices[q.first + e];
-    if (page < 0 || page >= p.max_pages) continue;
-    float* w = p.weights + (page * nkv + h) * p.page_size + t - e * p.page_size;
-    const float add[4] = {sum.x, sum.y, sum.z, sum.w};
-    if (t + 4 <= min(off, tok1)) {
-      float4 old = *(float4*)w;
-      *(float4*)w = make_float4(old.x + add[0], old.y + add[1], old.z + add[2], old.w + add[3]);
-    } else {
+    auto add = [&](const float4& x, float e) {
+      sum.x += fast_exp2(x.x - e);
+      sum.y += fast_exp2(x.y - e);
+      sum.z += fast_exp2(x.z - e);
+      sum.w += fast_exp2(x.w - e);
+    };
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (t + i < tok1) w[i] = t + i >= off ? add[i] : w[i] + add[i];
+    for (int row = 0; row < kAhead; ++row)
+      if (row < q.rows) add(s[row], s_lse[row]);
+    for (int row = kAhead; row < q.rows; ++row) add(*(const float4*)(src + 16 * row), s_lse[row]);
+    if (w) {
+      if (t + 4 <= min(off, tok1)) {
+        *(float4*)w = make_float4(old.x + sum.x, old.y + sum.y, old.z + sum.z, old.w + sum.w);
+      } else {
+        const float was[4] = {old.x, old.y, old.z, old.w}, more[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (t + i < tok1) w[i] = t + i >= off ? more[i] : was[i] + more[i];
+      }
     }
+    t += 1024;
+    if (t < tok1) load(t);
   }
 }
 
@@ -130,9 +155,13 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(WeightsParams p) {
   }
 }
 
+// Up to so many tokens in all the short requests take one launch.
+constexpr int64_t kOneTokens = 1024;
+
 // How a call is cut, from its shapes alone, and where its scratch lies.
 struct WeightsCut {
-  int32_t unit_pages, units, score_rows;                               // short
+  int32_t unit_pages, units, finish_pages, finish_units, score_rows;   // short
+  bool one;                                                            // in one launch, without scratch
   int32_t row_units, key_splits, key_pages, key_units, row_splits;     // long
   int64_t scores, unit_lse, row_lse, sums, total;                      // bytes
 };
@@ -148,8 +177,12 @@ static WeightsCut weights_cut(int32_t batch, int32_t max_qo_tokens, int32_t num_
   // Runs of pages: about 4096 workgroups, of 64 tokens (one tile a wavefront) and more.
   c.unit_pages = (int32_t)up(clamp(up(tokens * nkv, 4096), 64, 1 << 24), page_size);
   c.units = (int32_t)(num_indices / c.unit_pages + batch);
+  c.finish_pages = (int32_t)clamp(c.unit_pages, up(1024, page_size), INT32_MAX);  // as many tokens as its threads take at once
+  c.finish_units = (int32_t)(num_indices / c.finish_pages + batch);
   c.score_rows = ragged ? kWRows : group;
-  if (parts & 1) {
+  c.one = (parts & 1) && (int64_t)batch * nkv <= device_cu_count() && tokens <= kOneTokens &&
+          (tokens + kOnePad) * c.score_rows <= kOneScores;
+  if ((parts & 1) && !c.one) {
     c.scores = at;
     at = mi_align_up(at + 4 * tokens * nkv * c.score_rows, 256);
     c.unit_lse = at;
@@ -187,80 +220,82 @@ extern "C" int64_t mi_attention_weights_bytes(int32_t batch, int32_t max_qo_toke
   return weights_cut(batch, max_qo_tokens, num_indices, page_size, num_kv_heads, num_qo_heads / num_kv_heads, ragged != 0, parts, kRowBlock).total;
 }
 
-extern "C" int mi_attention_weights(const void* q, int32_t q_dtype, int64_t q_stride_token, int64_t q_stride_head,
-                                    const mi_paged_kv* kv, const int32_t* qo_indptr, const int32_t* kv_indptr,
-                                    const int32_t* kv_indices, const int32_t* last_page_len, int32_t batch,
-                                    int32_t max_qo_tokens, int32_t num_indices, int32_t num_qo_heads, int32_t causal,
-                                    float sm_scale, int32_t parts, float* weights, void* workspace, int64_t workspace_bytes,
-                                    void* stream) {
+extern "C" int mi_attention_weights_block(const mi_attention_weights_args* args) {
   using namespace mi;
-  if (!kv || !weights_shapes_ok(batch, max_qo_tokens, num_indices, kv->page_size, num_qo_heads, kv->num_kv_heads, parts))
+  if (!args) return MI_ERR_INVALID;
+  const mi_attention_weights_args& a = *args;
+  if (!a.kv || !weights_shapes_ok(a.batch, a.max_qo_tokens, a.num_indices, a.kv->page_size, a.num_qo_heads, a.kv->num_kv_heads, a.parts))
     return MI_ERR_INVALID;
-  if (batch == 0 || max_qo_tokens == 0 || num_indices == 0) return MI_OK;
-  if (!q || !kv->data || !kv_indptr || !kv_indices || !last_page_len || !weights || !workspace) return MI_ERR_INVALID;
-  const int nkv = kv->num_kv_heads, D = kv->head_dim, group = num_qo_heads / nkv;
-  if (group > kWRows || kv->page_size % 16 || (D != 64 && D != 128 && D != 256)) return MI_ERR_UNSUPPORTED;
-  const bool scaled = kv_is_scaled(kv->dtype);
-  if (q_dtype != MI_BF16 && q_dtype != MI_F16 && q_dtype != MI_F32) return MI_ERR_UNSUPPORTED;
-  if (scaled ? q_dtype == MI_F32 : kv->dtype != q_dtype) return MI_ERR_UNSUPPORTED;
-  if (!kv_scales_ok(kv)) return MI_ERR_INVALID;
-  if (!rows_aligned16(q, q_stride_token, q_stride_head, q_dtype == MI_F32 ? 4 : 2) || !kv_aligned16(kv)) return MI_ERR_INVALID;
-  if ((uintptr_t)weights % 16 || (uintptr_t)workspace % 16) return MI_ERR_INVALID;
+  if (a.batch == 0 || a.max_qo_tokens == 0 || a.num_indices == 0) return MI_OK;
+  if (!a.q || !a.kv->data || !a.kv_indptr || !a.kv_indices || !a.last_page_len || !a.weights) return MI_ERR_INVALID;
+  const int nkv = a.kv->num_kv_heads, D = a.kv->head_dim, group = a.num_qo_heads / nkv;
+  if (group > kWRows || a.kv->page_size % 16 || (D != 64 && D != 128 && D != 256)) return MI_ERR_UNSUPPORTED;
+  const bool scaled = kv_is_scaled(a.kv->dtype);
+  if (a.q_dtype != MI_BF16 && a.q_dtype != MI_F16 && a.q_dtype != MI_F32) return MI_ERR_UNSUPPORTED;
+  if (scaled ? a.q_dtype == MI_F32 : a.kv->dtype != a.q_dtype) return MI_ERR_UNSUPPORTED;
+  if (!kv_scales_ok(a.kv)) return MI_ERR_INVALID;
+  if (!rows_aligned16(a.q, a.q_stride_token, a.q_stride_head, a.q_dtype == MI_F32 ? 4 : 2) || !kv_aligned16(a.kv)) return MI_ERR_INVALID;
+  if ((uintptr_t)a.weights % 16 || (uintptr_t)a.workspace % 16) return MI_ERR_INVALID;
   // places in the page list and rows are counted in 32 bits
-  if ((int64_t)num_indices * kv->page_size > INT32_MAX - (1 << 25) || (int64_t)max_qo_tokens * group > INT32_MAX - 65536 ||
-      kv->page_size > (1 << 24))
+  if ((int64_t)a.num_indices * a.kv->page_size > INT32_MAX - (1 << 25) || (int64_t)a.max_qo_tokens * group > INT32_MAX - 65536 ||
+      a.kv->page_size > (1 << 24))
     return MI_ERR_UNSUPPORTED;
-  const bool ragged = qo_indptr != nullptr;
-  if (!ragged) parts = 1;
-  const WeightsCut c = weights_cut(batch, max_qo_tokens, num_indices, kv->page_size, nkv, group, ragged, parts,
-                                   q_dtype == MI_F32 ? kRowBlock : mma_block(D));
-  if (workspace_bytes < c.total) return MI_ERR_WORKSPACE;
+  const bool ragged = a.qo_indptr != nullptr;
+  const int parts = ragged ? a.parts : 1;
+  const WeightsCut c = weights_cut(a.batch, a.max_qo_tokens, a.num_indices, a.kv->page_size, nkv, group, ragged, parts,
+                                   a.q_dtype == MI_F32 ? kRowBlock : mma_block(D));
+  if (c.total > 0 && !a.workspace) return MI_ERR_INVALID;
+  if (a.workspace_bytes < c.total) return MI_ERR_WORKSPACE;
   WeightsParams p{};
-  p.q = q;
-  p.q_stride_tok = q_stride_token;
-  p.q_stride_head = q_stride_head;
-  p.k = (const uint8_t*)kv->data;
-  p.page_stride = kv->page_stride;
-  p.token_stride = kv->token_stride;
-  p.head_stride = kv->head_stride;
-  p.max_pages = kv->max_pages;
-  p.k_scale = kv->k_scale;
-  p.qo_indptr = qo_indptr;
-  p.kv_indptr = kv_indptr;
-  p.kv_indices = kv_indices;
-  p.last_page_len = last_page_len;
-  p.weights = weights;
-  uint8_t* ws = (uint8_t*)workspace;
+  p.q = a.q;
+  p.q_stride_tok = a.q_stride_token;
+  p.q_stride_head = a.q_stride_head;
+  p.k = (const uint8_t*)a.kv->data;
+  p.page_stride = a.kv->page_stride;
+  p.token_stride = a.kv->token_stride;
+  p.head_stride = a.kv->head_stride;
+  p.max_pages = a.kv->max_pages;
+  p.k_scale = a.kv->k_scale;
+  p.qo_indptr = a.qo_indptr;
+  p.kv_indptr = a.kv_indptr;
+  p.kv_indices = a.kv_indices;
+  p.last_page_len = a.last_page_len;
+  p.weights = a.weights;
+  uint8_t* ws = (uint8_t*)a.workspace;
   p.scores = (float*)(ws + c.scores);
   p.unit_lse = (float*)(ws + c.unit_lse);
   p.row_lse = (float*)(ws + c.row_lse);
   p.sums = (float*)(ws + c.sums);
-  p.total_rows = (int64_t)max_qo_tokens * group;
-  p.places = (int64_t)num_indices * kv->page_size;
-  p.batch = batch;
+  p.total_rows = (int64_t)a.max_qo_tokens * group;
+  p.places = (int64_t)a.num_indices * a.kv->page_size;
+  p.batch = a.batch;
   p.num_kv_heads = nkv;
   p.group = group;
-  p.page_size = kv->page_size;
-  p.causal = causal ? 1 : 0;
-  p.max_tokens = max_qo_tokens;
-  p.num_indices = num_indices;
+  p.page_size = a.kv->page_size;
+  p.causal = a.causal ? 1 : 0;
+  p.max_tokens = a.max_qo_tokens;
+  p.num_indices = a.num_indices;
   p.unit_pages = c.unit_pages;
+  p.finish_pages = c.finish_pages;
   p.score_rows = c.score_rows;
   p.key_splits = c.key_splits;
   p.row_splits = c.row_splits;
   p.key_pages = c.key_pages;
-  p.scale_log2 = sm_scale * 1.4426950408889634f;
-  hipStream_t s = (hipStream_t)stream;
-  const int kvt = kv_format(kv->dtype);
+  p.scale_log2 = a.sm_scale * 1.4426950408889634f;
+  hipStream_t s = (hipStream_t)a.stream;
+  const int kvt = kv_format(a.kv->dtype);
   auto launch = [&](int which, int64_t blocks) {
     if (blocks > INT32_MAX) return MI_ERR_UNSUPPORTED;
     const dim3 grid((uint32_t)blocks);
-    return scaled ? weights_launch_scaled(p, q_dtype, kvt, D, which, grid, s) : weights_launch_16(p, q_dtype, D, which, grid, s);
+    return scaled ? weights_launch_scaled(p, a.q_dtype, kvt, D, which, grid, s) : weights_launch_16(p, a.q_dtype, D, which, grid, s);
   };
-  if (parts & 1) {
+  if (c.one) {
+    const int st = launch(kWOne, (int64_t)a.batch * nkv);
+    if (st != MI_OK) return st;
+  } else if (parts & 1) {
     const int st = launch(kWScores, (int64_t)c.units * nkv);
     if (st != MI_OK) return st;
-    hipLaunchKernelGGL(weights_finish_kernel, dim3((uint32_t)(c.units * nkv)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(weights_finish_kernel, dim3((uint32_t)(c.finish_units * nkv)), dim3(256), 0, s, p);
   }
   if (parts & 2) {
     int st = launch(kWRowsPass, (int64_t)c.row_units * nkv * c.key_splits);
@@ -274,4 +309,14 @@ extern "C" int mi_attention_weights(const void* q, int32_t q_dtype, int64_t q_st
   }
   MI_CHECK_LAUNCH();
   return MI_OK;
+}
+
+extern "C" int mi_attention_weights(const void* q, int32_t q_dtype, int64_t q_stride_token, int64_t q_stride_head,
+                                    const mi_paged_kv* kv, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                    const int32_t* kv_indices, const int32_t* last_page_len, int32_t batch,
+                                    int32_t max_qo_tokens, int32_t num_indices, int32_t num_qo_heads, int32_t causal,
+                                    float sm_scale, int32_t parts, float* weights, void* workspace, int64_t workspace_bytes,
+                                    void* stream) {
+  const mi_attention_weights_args args = {q, kv, qo_indptr, kv_indptr, kv_indices, last_page_len, weights, workspace, stream, q_stride_token, q_stride_head, workspace_bytes, q_dtype, batch, max_qo_tokens, num_indices, num_qo_heads, causal, parts, sm_scale};
+  return mi_attention_weights_block(&args);
 }

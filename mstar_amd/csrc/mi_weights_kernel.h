@@ -29,7 +29,7 @@ struct WeightsParams {
   float *row_lse, *sums;     // long ones: [split][kv head][row], [split][kv head][place in the page list]
   int64_t total_rows, places;
   int32_t batch, num_kv_heads, group, page_size, causal, max_tokens, num_indices;
-  int32_t unit_pages, score_rows;             // of the short path
+  int32_t unit_pages, finish_pages, score_rows;  // of the short path
   int32_t key_splits, row_splits, key_pages;  // of the long one; key_pages: of a block of keys
   float scale_log2;
 };
@@ -95,7 +95,7 @@ struct KeyTile {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       if constexpr (WORDS == 4) {
-        const uint4 u = *(const uint4*)(src + c * (4 * RUN * BITS / 8));
+        const u32x4_t u = *(const u32x4_t*)(src + c * (4 * RUN * BITS / 8));
         w[c][0] = u.x, w[c][1] = u.y, w[c][2] = u.z, w[c][3] = u.w;
       } else {
         const uint2 u = *(const uint2*)(src + c * (4 * RUN * BITS / 8));
@@ -106,6 +106,21 @@ struct KeyTile {
       const uint8_t* sc = (const uint8_t*)p.k_scale + (page * 2 * p.num_kv_heads + h) * NBLK * p.page_size + slot;
 #pragma unroll
       for (int c = 0; c < NC; ++c) s[c] = sc[(int64_t)((c * 4 * RUN + grp * RUN) / kMxBlock) * p.page_size];
+    }
+  }
+  // The same from 16 rows in LDS, PITCH bytes apart.
+  template <int PITCH>
+  MI_DEVICE void read(const uint8_t* rows, int row, int grp) {
+    const uint8_t* src = rows + row * PITCH + grp * (RUN * BITS / 8);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if constexpr (WORDS == 4) {
+        const u32x4_t u = *(const u32x4_t*)(src + c * (4 * RUN * BITS / 8));
+        w[c][0] = u.x, w[c][1] = u.y, w[c][2] = u.z, w[c][3] = u.w;
+      } else {
+        const u32x2_t u = *(const u32x2_t*)(src + c * (4 * RUN * BITS / 8));
+        w[c][0] = u.x, w[c][1] = u.y;
+      }
     }
   }
   MI_DEVICE void fragments(uint4 (&f)[STEPS]) const {
@@ -141,6 +156,53 @@ struct KeyTile {
   }
 };
 
+// Sixteen rows as they are loaded: a lane has 16 bytes of every 1024, so an instruction covers
+// whole rows, and whole cache lines of them.  (Each lane loading what the MFMA wants of it, 64 bytes of a row an
+// instruction, streams K slower: 495 -> 440 us over 1.95 GB.)  They pass through LDS.
+template <typename MT, int KVT, int D>
+struct RawTile {
+  using Tile = KeyTile<MT, KVT, D>;
+  static constexpr int ROW = D * Tile::BITS / 8, PITCH = ROW + 16, N = (16 * ROW + 1023) / 1024;
+  static constexpr bool ALL = 16 * ROW % 1024 == 0;
+  u32x4_t r[N];
+  uint8_t s[Tile::MX ? Tile::NC : 1];
+
+  MI_DEVICE void load(const WeightsParams& p, int64_t page, int slot, int h, int lane) {
+    const uint8_t* src = p.k + (page * p.page_stride + slot * p.token_stride + h * p.head_stride) * Tile::ESZ;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int at = 16 * lane + 1024 * j, row = at / ROW;
+      if (!ALL && at >= 16 * ROW) continue;
+      const u32x4_t* from = (const u32x4_t*)(src + (int64_t)row * p.token_stride * Tile::ESZ + at % ROW);
+      if constexpr (ROW >= 128) r[j] = __builtin_nontemporal_load(from);
+      else r[j] = *from;  // the rest of the line is another head's
+    }
+    if constexpr (Tile::MX) {
+      const int col = lane & 15, grp = lane >> 4;
+      const uint8_t* sc = (const uint8_t*)p.k_scale + (page * 2 * p.num_kv_heads + h) * Tile::NBLK * p.page_size + slot + col;
+#pragma unroll
+      for (int c = 0; c < Tile::NC; ++c) s[c] = sc[(int64_t)((c * 4 * Tile::RUN + grp * Tile::RUN) / kMxBlock) * p.page_size];
+    }
+  }
+  // Through the wavefront's part of LDS into the MFMA's order.
+  MI_DEVICE void order(uint8_t* lds, int lane, Tile& t) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int at = 16 * lane + 1024 * j;
+      if (!ALL && at >= 16 * ROW) continue;
+      *(u32x4_t*)(lds + at / ROW * PITCH + at % ROW) = r[j];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    t.template read<PITCH>(lds, lane & 15, lane >> 4);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if constexpr (Tile::MX)
+#pragma unroll
+      for (int c = 0; c < Tile::NC; ++c) t.s[c] = s[c];
+  }
+};
+
 // Page of entry e of the page list, page 0 for ids out of range (whose tokens' weights are not written).
 MI_DEVICE int64_t safe_page(const WeightsParams& p, int e) {
   const int64_t page = p.kv_indices[e];
@@ -160,6 +222,8 @@ MI_DEVICE float w_lse(float m, float l) { return l > 0.f ? m + fast_log2(l) : l 
 template <typename MT, int KVT, int D>
 __global__ __launch_bounds__(256) void weights_scores_kernel(WeightsParams p) {
   using Tile = KeyTile<MT, KVT, D>;
+  using Raw = RawTile<MT, KVT, D>;
+  __shared__ __attribute__((aligned(16))) uint8_t s_rows[4][16 * Raw::PITCH];
   __shared__ float s_m[4][kWRows], s_l[4][kWRows];
   const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6), nkv = p.num_kv_heads;
   const int h = uniform((int)(blockIdx.x % nkv)), unit = uniform((int)(blockIdx.x / nkv));
@@ -182,12 +246,21 @@ __global__ __launch_bounds__(256) void weights_scores_kernel(WeightsParams p) {
   const float sl2 = KVT == kKvFp8 ? p.scale_log2 * ((const float*)p.k_scale)[h] : p.scale_log2;
 
   float m = -kWInf, l = 0.f;
-  auto load = [&](Tile& t, int i) {
-    const int tok = tok0 + 16 * i, e = (int)((unsigned)tok / (unsigned)p.page_size);
-    t.load(p, safe_page(p, q.first + e), tok - e * p.page_size + col, h, grp);
+  // Pages and slots of 64 tiles, one a lane: a page id loaded behind a tile's K would wait for that K.
+  int ids = 0, slots = 0, ids_first = t0 - 64;
+  auto load = [&](Raw& t, int i) {
+    if (i >= ids_first + 64) {
+      ids_first = i;
+      const int tok = tok0 + 16 * min(i + lane, t1 - 1), e = (int)((unsigned)tok / (unsigned)p.page_size);
+      ids = (int)safe_page(p, q.first + e);
+      slots = tok - e * p.page_size;
+    }
+    t.load(p, __builtin_amdgcn_readlane(ids, i - ids_first), __builtin_amdgcn_readlane(slots, i - ids_first), h, lane);
   };
-  auto compute = [&](const Tile& t, int i) {
+  auto compute = [&](const Raw& raw, int i) {
     const int tok = tok0 + 16 * i;
+    Tile t;
+    raw.order(s_rows[wave], lane, t);
     uint4 kf[Tile::STEPS];
     t.fragments(kf);
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -208,7 +281,7 @@ __global__ __launch_bounds__(256) void weights_scores_kernel(WeightsParams p) {
     l = l * fast_exp2(m - mu) + ((fast_exp2(s[0] - mu) + fast_exp2(s[1] - mu)) + (fast_exp2(s[2] - mu) + fast_exp2(s[3] - mu)));
     m = mn;
   };
-  Tile a, b;
+  Raw a, b;
   if (t0 < t1) load(a, t0);
   for (int i = t0; i < t1; i += 2) {
     if (i + 1 < t1) load(b, i + 1);
@@ -232,6 +305,106 @@ __global__ __launch_bounds__(256) void weights_scores_kernel(WeightsParams p) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) L += s_l[w][col] * fast_exp2(s_m[w][col] - Mu);
     p.unit_lse[((int64_t)unit * nkv + h) * kWRows + col] = w_lse(M, L);
+  }
+}
+
+// All of it in one launch, a workgroup for each request and kv head, where the batch's scores of a head fit its
+// LDS: tiles in turn over 16 wavefronts, scores to LDS, and behind one barrier the sums.
+constexpr int kOneScores = 32768;                      // floats
+// Half the wavefronts where a row of K and of q are 64 registers each.
+template <typename MT>
+constexpr int one_threads(int d) { return MT::kDtype == MI_F32 && d == 256 ? 512 : 1024; }
+constexpr int kOnePad = 20;                            // of a row of scores: up to 15 tokens, and 16 rows in different banks
+template <typename MT, int KVT, int D>
+__global__ __launch_bounds__(one_threads<MT>(D)) void weights_one_kernel(WeightsParams p) {
+  using Tile = KeyTile<MT, KVT, D>;
+  constexpr int NT = one_threads<MT>(D), NW = NT / kWave;
+  __shared__ __attribute__((aligned(16))) float s_scores[kOneScores];
+  __shared__ float s_m[NW][kWRows], s_l[NW][kWRows], s_lse[kWRows];
+  const int tid = (int)threadIdx.x, lane = lane_id(), wave = uniform(tid >> 6), nkv = p.num_kv_heads;
+  const int h = uniform((int)(blockIdx.x % nkv)), r = uniform((int)(blockIdx.x / nkv));
+  const WRequest q = w_request(p, r);
+  if (q.rows <= 0 || q.rows > kWRows || q.len <= 0) return;
+  const int tiles = (q.len + 15) >> 4, pitch = (q.len & ~15) + kOnePad, off = q.len - q.qo_len;
+  const int col = lane & 15, grp = lane >> 4;
+  const int qtok = col / p.group, g = col - qtok * p.group;
+  const bool valid = col < q.rows;
+  const int lim = p.causal ? off + qtok : q.len - 1;
+  uint4 qf[Tile::STEPS] = {};
+  if (valid) Tile::query(p, q.qo_start + qtok, h * p.group + g, grp, qf);
+  const float sl2 = KVT == kKvFp8 ? p.scale_log2 * ((const float*)p.k_scale)[h] : p.scale_log2;
+  float m = -kWInf, l = 0.f;
+  int ids = 0, slots = 0, round = -64;  // of 64 of the wavefront's tiles, one a lane
+  auto load = [&](Tile& t, int k) {     // its k-th tile
+    if (k >= round + 64) {
+      round = k;
+      const int tok = 16 * min(wave + NW * (k + lane), tiles - 1), e = (int)((unsigned)tok / (unsigned)p.page_size);
+      ids = (int)safe_page(p, q.first + e);
+      slots = tok - e * p.page_size;
+    }
+    t.load(p, __builtin_amdgcn_readlane(ids, k - round), __builtin_amdgcn_readlane(slots, k - round) + col, h, grp);
+  };
+  auto compute = [&](const Tile& t, int k) {
+    const int tok = 16 * (wave + NW * k);
+    uint4 kf[Tile::STEPS];
+    t.fragments(kf);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int st = 0; st < Tile::STEPS; ++st) acc = MT::mma_16x16x32(kf[st], qf[st], acc);
+    float s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s[j] = acc[j] * sl2;
+      if (tok + 4 * grp + j > lim) s[j] = -kWInf;
+    }
+    if (valid) *(float4*)(s_scores + col * pitch + tok + 4 * grp) = make_float4(s[0], s[1], s[2], s[3]);
+    const float mn = fmaxf(m, fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+    const float mu = mn == -kWInf ? 0.f : mn;
+    l = l * fast_exp2(m - mu) + ((fast_exp2(s[0] - mu) + fast_exp2(s[1] - mu)) + (fast_exp2(s[2] - mu) + fast_exp2(s[3] - mu)));
+    m = mn;
+  };
+  const int mine = wave < tiles ? (tiles - wave + NW - 1) / NW : 0;
+  Tile a, b;
+  if (mine > 0) load(a, 0);
+  for (int k = 0; k < mine; k += 2) {
+    if (k + 1 < mine) load(b, k + 1);
+    compute(a, k);
+    if (k + 2 < mine) load(a, k + 2);
+    if (k + 1 < mine) compute(b, k + 1);
+  }
+  // the thread's first token's weight, while the wavefronts meet
+  auto weight_at = [&](int t) -> float* {
+    const int e = (int)((unsigned)t / (unsigned)p.page_size);
+    const int64_t page = p.kv_indices[q.first + e];
+    return page >= 0 && page < p.max_pages ? p.weights + (page * nkv + h) * p.page_size + t - e * p.page_size : nullptr;
+  };
+  float* at = tid < q.len ? weight_at(tid) : nullptr;
+  float old = at && tid < off ? *at : 0.f;
+  const float mg = rows4_max(m), mgu = mg == -kWInf ? 0.f : mg;
+  l = rows4_sum(l * fast_exp2(m - mgu));
+  if (grp == 0) {
+    s_m[wave][col] = mg;
+    s_l[wave][col] = l;
+  }
+  __syncthreads();
+  if (tid < kWRows) {
+    float M = -kWInf, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, s_m[w][tid]);
+    const float Mu = M == -kWInf ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) L += s_l[w][tid] * fast_exp2(s_m[w][tid] - Mu);
+    s_lse[tid] = w_lse(M, L);
+  }
+  __syncthreads();
+  for (int t = tid; t < q.len; t += NT) {
+    if (t != tid) {
+      at = weight_at(t);
+      old = at && t < off ? *at : 0.f;
+    }
+    float sum = 0.f;
+    for (int row = 0; row < q.rows; ++row) sum += fast_exp2(s_scores[row * pitch + t] - s_lse[row]);
+    if (at) *at = old + sum;
   }
 }
 
@@ -773,11 +946,12 @@ __global__ __launch_bounds__(256) void weights_cols_f32_kernel(WeightsParams p) 
   }
 }
 
-enum : int { kWScores = 0, kWRowsPass = 1, kWColsPass = 2 };
+enum : int { kWScores = 0, kWRowsPass = 1, kWColsPass = 2, kWOne = 3 };
 
 template <typename MT, int KVT, int D>
 static void launch_weights_d(const WeightsParams& p, int which, dim3 grid, hipStream_t s) {
-  if (which == kWScores) hipLaunchKernelGGL((weights_scores_kernel<MT, KVT, D>), grid, dim3(256), 0, s, p);
+  if (which == kWOne) hipLaunchKernelGGL((weights_one_kernel<MT, KVT, D>), grid, dim3(one_threads<MT>(D)), 0, s, p);
+  else if (which == kWScores) hipLaunchKernelGGL((weights_scores_kernel<MT, KVT, D>), grid, dim3(256), 0, s, p);
   else if constexpr (MT::kDtype == MI_F32) {
     if (which == kWRowsPass) hipLaunchKernelGGL((weights_rows_f32_kernel<D>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((weights_cols_f32_kernel<D>), grid, dim3(256), 0, s, p);

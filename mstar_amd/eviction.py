@@ -18,6 +18,8 @@ No counterpart in the reference, whose caches only grow.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -32,7 +34,10 @@ def _pool_shape(kv_cache) -> tuple[int, ...]:
         return (len(kv_cache), *_pool_shape(kv_cache[0]))
     if not isinstance(kv_cache, (torch.Tensor, MXKVLayer)):
         raise ValueError(f"a KV cache is a tensor, an MXKVLayer or an MXKVCache, not {type(kv_cache).__name__}")
-    shape = tuple(kv_cache.shape)
+    shape = kv_cache.shape
+    if len(shape) == 5 and shape[1] == 2:
+        return (shape[0], shape[3], shape[2])
+    shape = tuple(shape)
     if len(shape) not in (5, 6) or shape[-4] != 2:
         raise ValueError(f"kv_cache must be [(num_layers,) max_pages, 2, page_size, num_kv_heads, head_dim], got {shape}")
     return (*shape[:-5], shape[-5], shape[-2], shape[-3])
@@ -76,14 +81,12 @@ def evict_kv_cache(kv_cache: torch.Tensor | MXKVLayer | MXKVCache, weights: torc
     Returns int32 ``[(num_layers,) batch, num_kv_heads, keep]``: the places in the request that stayed,
     ascending, -1 behind those of a shorter request.
     """
-    shape = _pool_shape(kv_cache)
-    dev = kv_cache.device
+    shape, dev = _pool_shape(kv_cache), kv_cache.device
     if dev.type != "cuda":
         raise ValueError("kv_cache must be on a GPU")
     for name, w in (("weights", weights), ("out_weights", out_weights)):
-        if w is None:
-            continue
-        if w.dtype != torch.float32 or tuple(w.shape) != shape or not w.is_contiguous() or w.device != dev or w.data_ptr() % 16:
+        if w is not None and (w.dtype is not torch.float32 or w.shape != shape or not w.is_contiguous() or w.get_device() != dev.index
+                              or w.data_ptr() % 16):
             raise ValueError(f"{name} must be a contiguous, 16-byte aligned float32 tensor {shape} on {dev}, got {tuple(w.shape)}, "
                              f"{w.dtype} on {w.device}")
     keep, recent, sinks = int(keep), int(recent), int(sinks)
@@ -97,16 +100,18 @@ def evict_kv_cache(kv_cache: torch.Tensor | MXKVLayer | MXKVCache, weights: torc
         raise ValueError("index tensors disagree on the number of requests")
     layers = shape[0] if len(shape) == 4 else 1
     desc, layer_stride, scale_stride = _layers(kv_cache, layers) if layers else (None, 0, 0)
-    kept = torch.empty(*shape[:-3], batch, shape[-2], keep, dtype=torch.int32, device=dev)
+    kept = torch.empty((*shape[:-3], batch, shape[-2], keep), dtype=torch.int32, device=dev)
     if kept.numel() == 0:
         return kept
     if indices.shape[0] == 0:
         return kept.fill_(-1)
     out = weights if out_weights is None else out_weights
-    _lib.check(_lib.lib().mi_kv_evict(
-        desc, layers, layer_stride, scale_stride, weights.data_ptr(), out.data_ptr(), weights.stride(0) if len(shape) == 4 else 0,
-        indptr.data_ptr(), indices.data_ptr(), last.data_ptr(), batch, indices.shape[0], keep, recent, sinks, kept.data_ptr(),
-        _lib.stream_ptr(dev)), "mi_kv_evict")
+    status = _lib.lib().mi_kv_evict_block(_lib.KV_EVICT_ARGS.pack(
+        ctypes.addressof(desc), weights.data_ptr(), out.data_ptr(), indptr.data_ptr(), indices.data_ptr(), last.data_ptr(),
+        kept.data_ptr(), _lib.stream_ptr(dev), layer_stride, scale_stride, weights.stride(0) if len(shape) == 4 else 0, layers, batch,
+        indices.shape[0], keep, recent, sinks))
+    if status:
+        _lib.check(status, "mi_kv_evict")
     return kept
 
 

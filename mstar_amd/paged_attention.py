@@ -36,6 +36,8 @@ Differences from the reference, all deliberate:
 
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 
 import numpy as np
@@ -366,29 +368,37 @@ class _Weights:
             raise RuntimeError("plan() must be called before accumulate_weights()")
         if q.dtype != self.dtype:
             q = q.to(self.dtype)
-        heads, dim, shape = self.num_qo_heads, self.head_dim, q.shape
+        heads, dim, shape, dev = self.num_qo_heads, self.head_dim, q.shape, self.device.index
         qo, tokens, most, parts, causal = self._weights_batch()
         if len(shape) != 3 or shape[0] < tokens or shape[1] != heads or shape[2] != dim:
             raise ValueError(f"q shape {tuple(shape)} does not match the plan")
         q, q_at, q_st, q_sh = _rows(q)
-        _check_devices(self.device, q=q, kv_cache_layer=kv_cache_layer, weights=weights)
+        if q.get_device() != dev or weights.get_device() != dev or kv_cache_layer.device != self.device:
+            _check_devices(self.device, q=q, kv_cache_layer=kv_cache_layer, weights=weights)
         desc = _lib.paged_kv_desc(kv_cache_layer, k_scale, v_scale)
-        if desc.num_kv_heads != self.num_kv_heads or desc.head_dim != dim or desc.page_size != self.page_size:
+        hkv, page_size = self.num_kv_heads, self.page_size
+        if desc.num_kv_heads != hkv or desc.head_dim != dim or desc.page_size != page_size:
             raise ValueError("kv_cache_layer geometry does not match the wrapper")
-        want = (desc.max_pages, desc.num_kv_heads, desc.page_size)
-        if weights.dtype != torch.float32 or weights.shape != want or not weights.is_contiguous() or weights.data_ptr() % 16:
+        want, weights_at = (desc.max_pages, hkv, page_size), weights.data_ptr()
+        if weights.dtype is not torch.float32 or weights.shape != want or not weights.is_contiguous() or weights_at % 16:
             raise ValueError(f"weights must be a contiguous, 16-byte aligned float32 tensor {want}, got {tuple(weights.shape)}, "
                              f"{weights.dtype}")
         entries, n = self._indices.shape[0], self._n_req
         if not parts or not n or not entries:
             return
-        launch, ragged = _lib.lib(), qo is not None
-        nbytes = launch.mi_attention_weights_bytes(n, most, entries, self.page_size, heads, self.num_kv_heads, ragged, parts)
-        scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=self.device)
-        _lib.check(launch.mi_attention_weights(
-            q_at, _lib.TORCH_TO_MI[q.dtype], q_st, q_sh, desc, qo.data_ptr() if ragged else None, self._indptr.data_ptr(),
-            self._indices.data_ptr(), self._last.data_ptr(), n, most, entries, heads, 1 if causal else 0, self._sm_scale,
-            parts, weights.data_ptr(), scratch.data_ptr(), scratch.numel(), self._reading_stream()), "mi_attention_weights")
+        nbytes = _weights_bytes(n, most, entries, page_size, heads, hkv, 1 if qo is not None else 0, parts)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        status = _lib.lib().mi_attention_weights_block(_lib.ATTENTION_WEIGHTS_ARGS.pack(
+            q_at, ctypes.addressof(desc), qo.data_ptr() if qo is not None else 0, self._indptr.data_ptr(), self._indices.data_ptr(),
+            self._last.data_ptr(), weights_at, scratch.data_ptr() if nbytes else 0, self._reading_stream(), q_st, q_sh, nbytes,
+            _lib.TORCH_TO_MI[q.dtype], n, most, entries, heads, 1 if causal else 0, parts, self._sm_scale))
+        if status:
+            _lib.check(status, "mi_attention_weights")
+
+
+@functools.lru_cache(maxsize=256)
+def _weights_bytes(*sizes: int) -> int:
+    return _lib.lib().mi_attention_weights_bytes(*sizes)
 
 
 class _PlanArrays:

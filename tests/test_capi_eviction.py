@@ -81,14 +81,24 @@ def test_attention_weights_arguments(L, mem):
 
 def test_attention_weights_bytes(L):
     size = L.mi_attention_weights_bytes
-    # a score of every place, kv head and row at least
-    assert size(4, 4, 100, 16, 32, 4, 0, 1) >= 4 * 1600 * 32
-    assert size(4, 4, 100, 16, 32, 4, 0, 3) == size(4, 4, 100, 16, 32, 4, 0, 1)  # one query each: all are short
+    # a score of every place, kv head and row at least, where they do not fit a workgroup
+    assert size(4, 4, 1000, 16, 32, 4, 0, 1) >= 4 * 16000 * 32
+    assert size(4, 4, 60, 16, 32, 4, 0, 1) == 0
+    for entries in (60, 1000):
+        assert size(4, 4, entries, 16, 32, 4, 0, 3) == size(4, 4, entries, 16, 32, 4, 0, 1)  # one query each: all are short
     assert size(4, 400, 100, 16, 32, 4, 1, 3) > size(4, 400, 100, 16, 32, 4, 1, 1)
     assert size(4, 400, 100, 16, 32, 4, 1, 2) >= 4 * 400 * 32
     assert size(0, 0, 0, 16, 32, 4, 1, 3) >= 0
     for bad in ((-1, 4, 4, 16, 32, 4, 1, 3), (4, 4, 4, 16, 30, 4, 1, 3), (4, 4, 4, 0, 32, 4, 1, 3), (4, 4, 4, 16, 32, 4, 1, 0)):
         assert size(*bad) == INVALID
+
+
+def test_argument_blocks(L):
+    for name, fmt in (("mi_qk_norm_rope_block", _lib.QK_NORM_ROPE_ARGS), ("mi_attention_weights_block", _lib.ATTENTION_WEIGHTS_ARGS),
+                      ("mi_kv_evict_block", _lib.KV_EVICT_ARGS)):
+        assert getattr(L, name)(None) == INVALID
+        zeros = getattr(L, name)(bytes(fmt.size))  # no tokens to rotate; no layer for the others
+        assert zeros == (0 if name == "mi_qk_norm_rope_block" else INVALID)
 
 
 def test_kv_evict_arguments(L, mem):

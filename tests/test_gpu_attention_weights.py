@@ -358,3 +358,22 @@ def test_refusals(gpu):
     with pytest.raises(RuntimeError):  # an fp16 layer under a bf16 plan
         call(q, layer.half(), weights)
     assert not bool(weights.any())
+
+
+@pytest.mark.parametrize("kind,hq,hkv,d", [("bf16", 8, 2, 128), ("f16", 8, 8, 64), ("mx4", 16, 1, 64), ("fp8", 6, 2, 256), ("mx8_f16", 3, 1, 128),
+                                           ("bf16", 2, 2, 256), ("mx4", 9, 1, 128), ("mx8", 12, 1, 64), ("fp8_f16", 5, 1, 64)])
+@pytest.mark.parametrize("lens", [[1], [1024], [1000, 8], [1024, 1], [500, 300, 100, 0, 16], [9000], [12000, 5, 0, 16]])
+def test_either_side_of_one_launch(gpu, kind, hq, hkv, d, lens):
+    """Batches whose scores fit a workgroup's LDS, and those past it, with many runs of pages to join."""
+    _run(H.make(gpu, kind, lens, 16, hkv, d, seed=hq + d), gpu, hq, None)
+
+
+@pytest.mark.parametrize("lens", [[100, 33], [9000, 20], [700, 900]])
+def test_short_fp32(gpu, lens):
+    """One query a request, either side of one launch."""
+    g = torch.Generator().manual_seed(8)
+    for d, hq, hkv in ((64, 4, 2), (128, 6, 2), (256, 5, 1)):
+        p = H.make(gpu, "bf16", lens, 16, hkv, d, seed=d)
+        x = torch.randn(p.values.shape, generator=g)
+        p.kind, p.layer, p.values = "f32", x.to(gpu), x.double()
+        _run(p, gpu, hq, None, dtype=torch.float32)
