@@ -351,7 +351,8 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p)
 #pragma unroll
     for (int k = 0; k < kMoveRows; ++k) {
       const int64_t from = k < steps && i < tiles ? s_from[i & 3][k * rows + row] : -1;
-      x[k] = from >= 0 ? *(const u32x4_t*)(base + from) : u32x4_t{0u, 0u, 0u, 0u};
+      // what is read is not read again (one request of 32k tokens in 28 layers 123 -> 108 us; such stores as well: 125)
+      x[k] = from >= 0 ? __builtin_nontemporal_load((const u32x4_t*)(base + from)) : u32x4_t{0u, 0u, 0u, 0u};
     }
   };
   auto store = [&](int i, const u32x4_t (&x)[kMoveRows]) {

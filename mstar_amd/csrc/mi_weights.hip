@@ -155,8 +155,10 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(WeightsParams p) {
   }
 }
 
-// Up to so many tokens in all the short requests take one launch.
-constexpr int64_t kOneTokens = 1024;
+// One launch for short queries up to so many tokens in all, and a request on average: a workgroup
+// streams a request alone, and a second launch costs 4 us (us a call, one / two launches: 4 requests of 100 to 400
+// tokens 6.5 / 10.3, 16 of 20 to 90 6.5 / 10.2, one of 1000 11.6 / 10.2).
+constexpr int64_t kOneTokens = 2048, kOneMean = 512;
 
 // How a call is cut, from its shapes alone, and where its scratch lies.
 struct WeightsCut {
@@ -180,7 +182,7 @@ static WeightsCut weights_cut(int32_t batch, int32_t max_qo_tokens, int32_t num_
   c.finish_pages = (int32_t)clamp(c.unit_pages, up(1024, page_size), INT32_MAX);  // as many tokens as its threads take at once
   c.finish_units = (int32_t)(num_indices / c.finish_pages + batch);
   c.score_rows = ragged ? kWRows : group;
-  c.one = (parts & 1) && (int64_t)batch * nkv <= device_cu_count() && tokens <= kOneTokens &&
+  c.one = (parts & 1) && (int64_t)batch * nkv <= device_cu_count() && tokens <= kOneTokens && tokens <= kOneMean * batch &&
           (tokens + kOnePad) * c.score_rows <= kOneScores;
   if ((parts & 1) && !c.one) {
     c.scores = at;
@@ -240,6 +242,8 @@ extern "C" int mi_attention_weights_block(const mi_attention_weights_args* args)
   if ((int64_t)a.num_indices * a.kv->page_size > INT32_MAX - (1 << 25) || (int64_t)a.max_qo_tokens * group > INT32_MAX - 65536 ||
       a.kv->page_size > (1 << 24))
     return MI_ERR_UNSUPPORTED;
+  // a wavefront's rows of a page are 32 bits apart
+  if (a.kv->token_stride < 0 || a.kv->token_stride * kv_elem_bytes(a.kv->dtype) > (INT32_MAX >> 4)) return MI_ERR_UNSUPPORTED;
   const bool ragged = a.qo_indptr != nullptr;
   const int parts = ragged ? a.parts : 1;
   const WeightsCut c = weights_cut(a.batch, a.max_qo_tokens, a.num_indices, a.kv->page_size, nkv, group, ragged, parts,

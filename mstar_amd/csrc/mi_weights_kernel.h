@@ -491,76 +491,89 @@ MI_DEVICE uint4 key_piece(const WeightsParams& p, int64_t page, int slot, int h,
 }
 
 // The keys of a request as a stream of tiles: what a thread loads of each, and where in the cache that lies.
+// A wavefront's rows of a unit are 16 or fewer that begin at a multiple of their number, so they lie in one
+// page: the page's address is scalar, and a thread's offset in it is the same for every tile.  (With both
+// computed by each thread, that was half of the loop's instructions.)
 template <typename MT, int KVT, int D>
 struct KeyStream {
   static constexpr int UNIT = KVT == kKv16 ? 8 : 16;  // elements a thread loads at once
   static constexpr int PER_ROW = D / UNIT, NU = (kTile * PER_ROW + 255) / 256;
+  static constexpr int WROWS = kWave / PER_ROW;  // rows of a wavefront's unit
   static constexpr bool MX = KVT == kKvMx8 || KVT == kKvMx4;
-  u32x4_t w[NU];  // mx4: two words
-  uint8_t s[NU];
+  static_assert(WROWS >= 1 && WROWS <= 16, "a unit lies in one page");
+  struct Tile {
+    u32x4_t w[NU];  // mx4: two words
+    uint8_t s[NU];
+  };
   int entry[NU], slot[NU];
   int64_t page[NU];
+  uint32_t at, scale_at;  // the thread's bytes from its unit's first row
 
   MI_DEVICE static int unit(int u) { return (int)threadIdx.x + 256 * u; }
   MI_DEVICE static bool active(int u) { return kTile * PER_ROW % 256 == 0 || unit(u) < kTile * PER_ROW; }
   MI_DEVICE void begin(const WeightsParams& p, const WRequest& q, int tile) {
+    constexpr int ESZ = KVT == kKv16 ? 2 : 1;
+    const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6), part = lane % PER_ROW, row = lane / PER_ROW;
+    at = (uint32_t)row * (uint32_t)(p.token_stride * ESZ) + part * (KVT == kKvMx4 ? 8 : 16);
+    scale_at = (uint32_t)(part / 2) * (uint32_t)p.page_size + row;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      const int tok = kTile * tile + unit(u) / PER_ROW;
+      const int tok = kTile * tile + WROWS * (wave + 4 * u);
       entry[u] = (int)((unsigned)tok / (unsigned)p.page_size);
       slot[u] = tok - entry[u] * p.page_size;
       page[u] = safe_page(p, q.first + min(entry[u], q.pages - 1));
     }
   }
-  // Loads the tile that `page` is of, and the pages of the next.
-  MI_DEVICE void load(const WeightsParams& p, const WRequest& q, int h) {
+  // Loads the tile that `page` is of, and the pages of the next; past a request's last, any keys of its last page.
+  MI_DEVICE void load(const WeightsParams& p, const WRequest& q, int h, Tile& t) {
     constexpr int ESZ = KVT == kKv16 ? 2 : 1;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      const int part = unit(u) % PER_ROW;
       if (active(u)) {
         const uint8_t* src = p.k + (page[u] * p.page_stride + slot[u] * p.token_stride + h * p.head_stride) * ESZ;
         if constexpr (KVT == kKvMx4) {
-          const uint2 x = *(const uint2*)(src + 8 * part);
-          w[u] = u32x4_t{x.x, x.y, 0u, 0u};
+          const uint2 x = *(const uint2*)(src + at);
+          t.w[u] = u32x4_t{x.x, x.y, 0u, 0u};
         } else {
-          w[u] = *(const u32x4_t*)(src + 16 * part);
+          t.w[u] = *(const u32x4_t*)(src + at);
         }
-        if constexpr (MX)
-          s[u] = ((const uint8_t*)p.k_scale)[((page[u] * 2 * p.num_kv_heads + h) * (D / kMxBlock) + part / 2) * (int64_t)p.page_size + slot[u]];
+        if constexpr (MX) {
+          const uint8_t* sc = (const uint8_t*)p.k_scale + (page[u] * 2 * p.num_kv_heads + h) * (D / kMxBlock) * (int64_t)p.page_size + slot[u];
+          t.s[u] = sc[scale_at];
+        }
       }
       slot[u] += kTile;
       while (slot[u] >= p.page_size) slot[u] -= p.page_size, ++entry[u];
       page[u] = safe_page(p, q.first + min(entry[u], q.pages - 1));
     }
   }
-  MI_DEVICE void store(uint8_t* tile) const {
+  MI_DEVICE static void store(const Tile& t, uint8_t* tile) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       if (!active(u)) continue;
       const int row = unit(u) / PER_ROW, part = unit(u) % PER_ROW;
       if constexpr (KVT == kKv16) {
-        *(u32x4_t*)(tile + tile_at<D>(row, part)) = w[u];
+        *(u32x4_t*)(tile + tile_at<D>(row, part)) = t.w[u];
       } else {
         uint32_t o[8];
         if constexpr (KVT == kKvFp8) {
-          const uint32_t x[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+          const uint32_t x[4] = {t.w[u].x, t.w[u].y, t.w[u].z, t.w[u].w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             o[2 * i] = fp8x2_to_mt<MT>(x[i], false);
             o[2 * i + 1] = fp8x2_to_mt<MT>(x[i], true);
           }
         } else {
-          const float scale = bitcast<float>((uint32_t)s[u] << 23);
+          const float scale = bitcast<float>((uint32_t)t.s[u] << 23);
           if constexpr (KVT == kKvMx8) {
-            const uint32_t x[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+            const uint32_t x[4] = {t.w[u].x, t.w[u].y, t.w[u].z, t.w[u].w};
             mx_to_mt<MT, KVT>(x, scale, o);
           } else {
-            const uint32_t x[2] = {w[u].x, w[u].y};
+            const uint32_t x[2] = {t.w[u].x, t.w[u].y};
             mx_to_mt<MT, KVT>(x, scale, o);
           }
           if constexpr (MT::kDtype == MI_F16)
-            if (mx_past_f16<KVT>(s[u])) f16_saturate(o);
+            if (mx_past_f16<KVT>(t.s[u])) f16_saturate(o);
         }
         *(uint4*)(tile + tile_at<D>(row, 2 * part)) = make_uint4(o[0], o[1], o[2], o[3]);
         *(uint4*)(tile + tile_at<D>(row, 2 * part + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
@@ -611,18 +624,21 @@ __global__ __launch_bounds__(256, 2) void weights_rows_kernel(WeightsParams p) {
 #pragma unroll
   for (int n = 0; n < NS; ++n) m[n] = -kWInf, l[n] = 0.f;
   const int clear = p.causal ? off + row0 / p.group : q.len - 1;  // keys up to here are seen by every row
-  KeyStream<MT, KVT, D> keys_in;
+  // One tile a barrier: with two, the registers of both leave room for two wavefronts instead of three (205 -> 232 us).
+  using Keys = KeyStream<MT, KVT, D>;
+  Keys keys_in;
+  typename Keys::Tile next;
   if (t0 < t1) {
     keys_in.begin(p, q, t0);
-    keys_in.load(p, q, h);
-    keys_in.store(s_tile[0]);
-    if (t0 + 1 < t1) keys_in.load(p, q, h);
+    keys_in.load(p, q, h, next);
+    Keys::store(next, s_tile[0]);
+    if (t0 + 1 < t1) keys_in.load(p, q, h, next);
   }
   __syncthreads();
   for (int i = t0; i < t1; ++i) {
     const uint8_t* tile = s_tile[(i - t0) & 1];
-    if (i + 1 < t1) keys_in.store(s_tile[(i - t0 + 1) & 1]);
-    if (i + 2 < t1) keys_in.load(p, q, h);
+    if (i + 1 < t1) Keys::store(next, s_tile[(i - t0 + 1) & 1]);
+    if (i + 2 < t1) keys_in.load(p, q, h, next);
     f32x16 acc[NS] = {};
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
@@ -668,8 +684,8 @@ __global__ __launch_bounds__(256, 2) void weights_rows_kernel(WeightsParams p) {
 template <typename MT, int KVT, int D>
 __global__ __launch_bounds__(256, 2) void weights_cols_kernel(WeightsParams p) {
   constexpr int NS = stationary(D), STEPS = D / 16, BLOCK = mma_block(D), PIECES = D / 8, NU = kTile * PIECES / 256;
-  __shared__ __attribute__((aligned(16))) uint8_t s_tile[2][kTile * 2 * D];
-  __shared__ __attribute__((aligned(16))) float s_lse[2][kTile];
+  __shared__ __attribute__((aligned(16))) uint8_t s_tile[4][kTile * 2 * D];
+  __shared__ __attribute__((aligned(16))) float s_lse[4][kTile];
   const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6), nkv = p.num_kv_heads, tid = (int)threadIdx.x;
   const int h = uniform((int)(blockIdx.x % nkv)), rest = uniform((int)(blockIdx.x / nkv));
   const int split = uniform(rest % p.row_splits), unit = uniform(rest / p.row_splits);
@@ -690,35 +706,52 @@ __global__ __launch_bounds__(256, 2) void weights_cols_kernel(WeightsParams p) {
     const int clear = p.causal ? max(0, min(base + BLOCK, q.len) - 1 - off) * G : 0;  // rows from here on see every key
     const int t0 = first + share_begin(split, p.row_splits, tiles), t1 = first + share_begin(split + 1, p.row_splits, tiles);
     // the stream of q rows: pieces of 16 bytes, and the tile's log-sum-exps
-    u32x4_t w[NU];
-    float e = kWInf;
+    struct Rows {
+      u32x4_t w[NU];
+      float e;
+    };
     int tok[NU], g[NU];
+    const uint16_t* src[NU];  // of row (tok, g): 32 rows on, and a token on with a group's heads back, are fixed steps
+    const int64_t step = step_tok * p.q_stride_tok + step_g * p.q_stride_head, wrap = p.q_stride_tok - G * p.q_stride_head;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int at = kTile * t0 + (tid + 256 * u) / PIECES;
       tok[u] = at / G;
       g[u] = at - tok[u] * G;
+      src[u] = (const uint16_t*)p.q + (int64_t)(q.qo_start + tok[u]) * p.q_stride_tok + (int64_t)(h * G + g[u]) * p.q_stride_head +
+               8 * ((tid + 256 * u) % PIECES);
     }
     int lse_row = kTile * t0 + tid;
-    auto load = [&]() {
+    // rows past the last are read as the last token's, which sees every key (a NaN of it is one of theirs), with an lse of infinity
+    const uint16_t* const none = (const uint16_t*)p.q + (int64_t)(q.qo_start + q.qo_len - 1) * p.q_stride_tok + (int64_t)h * G * p.q_stride_head;
+    const int end = min(q.rows, kTile * t1);
+    auto load = [&](Rows& t) {
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        const int t = min(tok[u], q.qo_len - 1);  // rows past the last: of the last token, and an lse of infinity
-        w[u] = *(const u32x4_t*)((const uint16_t*)p.q + (int64_t)(q.qo_start + t) * p.q_stride_tok + (int64_t)(h * G + g[u]) * p.q_stride_head +
-                               8 * ((tid + 256 * u) % PIECES));
+        t.w[u] = *(const u32x4_t*)(tok[u] < q.qo_len ? src[u] : none);
         tok[u] += step_tok;
         g[u] += step_g;
-        if (g[u] >= G) g[u] -= G, ++tok[u];
+        src[u] += step;
+        if (g[u] >= G) {
+          g[u] -= G;
+          ++tok[u];
+          src[u] += wrap;
+        }
       }
-      if (tid < kTile) e = lse_row < q.rows ? lse[lse_row] : kWInf;
+      t.e = lse[min(lse_row, q.rows - 1)];
+      if (lse_row >= end) t.e = kWInf;
       lse_row += kTile;
     };
-    auto store = [&](int b) {
+    auto store = [&](const Rows& t, int b) {
 #pragma unroll
-      for (int u = 0; u < NU; ++u) *(u32x4_t*)(s_tile[b] + tile_at<D>((tid + 256 * u) / PIECES, (tid + 256 * u) % PIECES)) = w[u];
-      if (tid < kTile) s_lse[b][tid] = e;
+      for (int u = 0; u < NU; ++u) *(u32x4_t*)(s_tile[b] + tile_at<D>((tid + 256 * u) / PIECES, (tid + 256 * u) % PIECES)) = t.w[u];
+      if (tid < kTile) s_lse[b][tid] = t.e;
     };
-    if (t0 < t1) load();
+    Rows ra, rb;
+    if (t0 < t1) {
+      load(ra);
+      load(rb);
+    }
     uint4 kf[NS][STEPS];
     int key[NS], from[NS];  // the key, and the first row that sees it
     float sum[NS];
@@ -732,15 +765,7 @@ __global__ __launch_bounds__(256, 2) void weights_cols_kernel(WeightsParams p) {
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) kf[n][st] = key_piece<MT, KVT, D>(p, page, at - en * p.page_size, h, 2 * st + hi);
     }
-    if (t0 < t1) {
-      store(0);
-      if (t0 + 1 < t1) load();
-    }
-    __syncthreads();
-    for (int i = t0; i < t1; ++i) {
-      const int b = (i - t0) & 1;
-      if (i + 1 < t1) store(b ^ 1);
-      if (i + 2 < t1) load();
+    auto tile_of = [&](int b, int i) {
       f32x16 acc[NS] = {};
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {
@@ -769,6 +794,22 @@ __global__ __launch_bounds__(256, 2) void weights_cols_kernel(WeightsParams p) {
         }
         sum[n] += (x[0] + x[1]) + (x[2] + x[3]);
       }
+    };
+    if (t0 < t1) {
+      store(ra, 0);
+      store(rb, 1);
+      load(ra);
+      load(rb);
+    }
+    __syncthreads();
+    // Two tiles a barrier, the next two on their way into LDS and two more into registers (211 -> 197 us).
+    for (int i = t0, b = 0; i < t1; i += 2, b ^= 2) {
+      store(ra, b ^ 2);
+      store(rb, (b ^ 2) + 1);
+      load(ra);
+      load(rb);
+      tile_of(b, i);
+      tile_of(b + 1, i + 1);
       __syncthreads();
     }
 #pragma unroll

@@ -362,7 +362,7 @@ def test_refusals(gpu):
 
 @pytest.mark.parametrize("kind,hq,hkv,d", [("bf16", 8, 2, 128), ("f16", 8, 8, 64), ("mx4", 16, 1, 64), ("fp8", 6, 2, 256), ("mx8_f16", 3, 1, 128),
                                            ("bf16", 2, 2, 256), ("mx4", 9, 1, 128), ("mx8", 12, 1, 64), ("fp8_f16", 5, 1, 64)])
-@pytest.mark.parametrize("lens", [[1], [1024], [1000, 8], [1024, 1], [500, 300, 100, 0, 16], [9000], [12000, 5, 0, 16]])
+@pytest.mark.parametrize("lens", [[1], [512], [513], [1000, 8], [1024, 1], [500, 300, 100, 0, 16], [1900, 1, 1, 1, 1], [9000], [12000, 5, 0, 16]])
 def test_either_side_of_one_launch(gpu, kind, hq, hkv, d, lens):
     """Batches whose scores fit a workgroup's LDS, and those past it, with many runs of pages to join."""
     _run(H.make(gpu, kind, lens, 16, hkv, d, seed=hq + d), gpu, hq, None)
