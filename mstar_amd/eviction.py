@@ -13,6 +13,9 @@ last ones and the heaviest of the others, head by head, and moves them together.
 Keys stay rotated to the positions they were written at, and new tokens go on from the
 request's last position: only the places in the cache change.
 
+Weights live beside one pool and stay there: tokens that arrive in it by a transfer or from host memory bring
+none, and a caller that accumulates goes on from what it writes into their slots (zeros, say).
+
 No counterpart in the reference, whose caches only grow.
 """
 

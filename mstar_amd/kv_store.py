@@ -649,12 +649,16 @@ class PagedAllocationManager:
         Same page and token ranges as the reference; all layers of all pages
         go out as one launch on the engine's transfer stream.  The producer
         must have finished writing those pages (the reference's contract,
-        ``kv_store.py:548-554``).
+        ``kv_store.py:548-554``).  A state that eviction has cut is read whole,
+        into an empty one (``reset_label``): it is no continuation of what was read before.
         """
         seq_len = seq_info.seq_len
         state = self.get_state(request_id, label)
         if state.seq_len >= seq_len:
             return
+        cut = getattr(seq_info, "evicted", False)
+        if state.seq_len and (cut or state.evicted):
+            raise ValueError(f"{request_id}: the rest of an evicted state does not follow the {state.seq_len} tokens that are here")
         ps = self.config.page_size
         first = state.seq_len // ps
         last = (seq_len - 1) // ps
@@ -673,6 +677,7 @@ class PagedAllocationManager:
             self.pending_reads[request_id].setdefault(label, []).append(future)
         state.seq_len = seq_len
         state.position_id_start = seq_info.pos_id
+        state.evicted = cut
         state.read_in_progress = future is not None
 
     def get_per_label_seq_info(self, request_id: str) -> dict:
@@ -685,7 +690,7 @@ class PagedAllocationManager:
             self.wait_for_retrieves(request_id, label)
             st = self.get_state(request_id, label)
             out[label] = SequenceInfo(seq_len=st.seq_len, pos_id=st.position_id_start,
-                                      latest_kv_transfer_info=info, page_indices=st.page_indices)
+                                      latest_kv_transfer_info=info, page_indices=st.page_indices, evicted=st.evicted)
         return out
 
     # ----- CPU offloading (kv_store.py:617-660) -----

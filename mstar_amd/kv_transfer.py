@@ -68,12 +68,16 @@ class DeviceKVTransferInfo:
 
 @dataclass
 class SequenceInfo:
-    """A producer's state of one (request, label) (``request_info.py:23-29``)."""
+    """A producer's state of one (request, label) (``request_info.py:23-29``).
+
+    ``evicted`` (extension): its tokens are not all that it was given (``KVRequestState.evicted``).
+    """
 
     seq_len: int
     pos_id: int
     latest_kv_transfer_info: Any
     page_indices: list[int] = field(default_factory=list)
+    evicted: bool = False
 
 
 def _check_pool(kv: torch.Tensor, name: str) -> None:
