@@ -377,3 +377,18 @@ def test_short_fp32(gpu, lens):
         x = torch.randn(p.values.shape, generator=g)
         p.kind, p.layer, p.values = "f32", x.to(gpu), x.double()
         _run(p, gpu, hq, None, dtype=torch.float32)
+
+
+@pytest.mark.parametrize("row", [0, 7, 49])
+def test_a_query_that_is_not_finite_reaches_what_it_sees(gpu, row):
+    """Rows past the last of a tile are read as another's: a NaN there must stay with the keys that its query sees."""
+    for ctx, n in ((40, 50), (300, 50), (0, 50)):
+        p = H.make(gpu, "bf16", [ctx + n], 16, 2, 128, seed=5)
+        q = torch.randn(n, 6, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+        q[row, 1, 3] = float("nan")  # of kv head 0
+        weights = kv_weights(p.layer)
+        _wrapper(p, gpu, 6, [n]).accumulate_weights(q.to(gpu), p.layer, weights)
+        pages = torch.as_tensor(p.kv_indices).long()
+        got = weights.cpu()[pages].permute(1, 0, 2).flatten(1)[:, :ctx + n]
+        assert bool(got[0, :ctx + row + 1].isnan().all()) and bool(got[0, ctx + row + 1:].isfinite().all())
+        assert bool(got[1].isfinite().all())

@@ -146,6 +146,12 @@ def test_either_side_of_what_one_launch_does(gpu, keep):
         _check(gpu, "fp8", 2, lens, 32, 1, 128, keep, 30, 0, False)
 
 
+def test_one_long_request_among_short_ones(gpu):
+    """More tokens than the fewer threads that short requests get hold at once."""
+    _check(gpu, "bf16", 0, [20000, 8192, 8193, 3, 700, 601, 600, 5, 40, 1], 16, 2, 128, 600, 50, 4, True)
+    _check(gpu, "f16", 3, [9000, 1, 1, 2], 32, 1, 256, 601, 0, 0, False)
+
+
 def test_again_after_more_tokens(gpu):
     """Evicted, grown and evicted again, on the shorter page lists that remain."""
     ps, hkv, d, keep = 16, 2, 64, 48
