@@ -14,7 +14,7 @@
 // in turn, so rows are split over workgroups by head, K and V, and by pieces of 128 bytes of the row where that
 // leaves places of the chip empty (pieces of 64 bytes: 123 -> 147 us for one request in 28 layers, none: 140).
 // Where little is kept, and there is a compute unit for each (layer, request, kv head), one launch does both
-// (evict_small_kernel: 8 requests x 2 heads, 256 of 300 to 700 tokens stay, 12 us against 15; with 4096 units of 256 KiB
+// (evict_small_kernel: 8 requests x 2 heads, 256 of 300 to 700 tokens stay, 11 us against 15; with 4096 units of 256 KiB
 // it took 545 against 370).
 //
 // HBM bound: 256 requests of 512 to 32768 tokens, 4 heads x 128, bf16, 2048 stay: selecting 40 us, moving 1.38 GB (in and
@@ -387,9 +387,10 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p)
 }
 
 // Both in one launch, a workgroup for each (layer, request, kv head): K and V rows of a tile side by side, and the
-// weights with the first.
-constexpr int kSmallThreads = 1024, kSmallKeep = 4096, kSmallPages = 1024, kSmallPlaces = 512;
-constexpr int64_t kSmallBytes = 256 << 10;  // of K and V that stay: two tiles
+// weights with the first.  It waits far more than it moves: 512 threads 11.0 us for 8 requests x 2 heads, 1024 12.1, 256 16.1.
+constexpr int kSmallThreads = 512, kSmallKeep = 4096, kSmallPages = 1024, kSmallPlaces = 512;
+static_assert(kSmallPlaces <= kSmallThreads, "a thread finds one place of a tile");
+constexpr int64_t kSmallBytes = 256 << 10;  // of K and V that stay: four tiles
 __global__ __launch_bounds__(kSmallThreads) void evict_small_kernel(EvictParams p) {
   __shared__ __attribute__((aligned(16))) SelectShared s;
   __shared__ int32_t s_kept[kSmallKeep], s_page[kSmallPages];
@@ -403,7 +404,7 @@ __global__ __launch_bounds__(kSmallThreads) void evict_small_kernel(EvictParams 
   int32_t* out = p.kept + (int64_t)unit * p.keep;
   const float* weights = p.weights + (int64_t)layer * p.weights_layer_stride;
   float* out_weights = p.out_weights + (int64_t)layer * p.weights_layer_stride;
-  if (tid < min(pages, kSmallPages)) s_page[tid] = p.kv_indices[first + tid];
+  for (int i = tid; i < min(pages, kSmallPages); i += kSmallThreads) s_page[i] = p.kv_indices[first + i];
   if (cut) {
     evict_select<kSmallThreads>(p, s, weights, first, h, len, out, s_kept);
   } else {
@@ -446,7 +447,7 @@ __global__ __launch_bounds__(kSmallThreads) void evict_small_kernel(EvictParams 
   const int v = tid % per >= p.row_pieces, piece = tid % per - v * p.row_pieces;
   uint8_t* base = p.cache + layer * p.layer_stride + v * p.kv_stride + h * p.head_stride + 16 * piece;
   for (int j0 = 0; j0 < n; j0 += tile) {
-    if (tid < tile) {
+    if (tid < tile) {  // at most kSmallPlaces, as many as there are threads
       const int j = j0 + tid, src = j < n ? s_kept[j] : -1;
       int64_t page, page_to;
       int slot, slot_to;

@@ -392,3 +392,29 @@ def test_a_query_that_is_not_finite_reaches_what_it_sees(gpu, row):
         got = weights.cpu()[pages].permute(1, 0, 2).flatten(1)[:, :ctx + n]
         assert bool(got[0, :ctx + row + 1].isnan().all()) and bool(got[0, ctx + row + 1:].isfinite().all())
         assert bool(got[1].isfinite().all())
+
+
+def test_one_launch_captured_and_replayed(gpu):
+    """A static page list small enough for one launch: replays equal eager calls over other lengths, requests of no keys among them."""
+    hq, hkv, d, ps, b, pool = 8, 2, 128, 16, 4, 120
+    layer = torch.randn(pool, 2, ps, hkv, d, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(gpu)
+    w = PagedDecodeWrapper(workspace(gpu, 64 << 20), hq, hkv, d, ps, batch_size=b, max_num_pages=pool, device=gpu, use_cuda_graph=True)
+    e = PagedDecodeWrapper(workspace(gpu, 64 << 20), hq, hkv, d, ps, device=gpu)
+    q, weights = torch.zeros(b, hq, d, dtype=torch.bfloat16, device=gpu), torch.zeros(pool, hkv, ps, device=gpu)
+    w.plan(*(torch.as_tensor(a) for a in custom_batch([200] * b, ps, pool, 1)[1:]))
+    w.accumulate_weights(q, layer, weights)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w.accumulate_weights(q, layer, weights)
+    for i, lens in enumerate(([1, 700, 30, 200], [1800, 1, 2, 16], [64, 0, 64, 0], [1, 700, 30, 200])):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(i)))
+        start = torch.rand(weights.shape, generator=torch.Generator().manual_seed(i)).to(gpu)
+        weights.copy_(start)
+        index = [torch.as_tensor(a) for a in custom_batch(lens, ps, pool, 5 + i)[1:]]
+        w.plan(*index)
+        graph.replay()
+        e.plan(*index)
+        e.accumulate_weights(q, layer, start)
+        torch.cuda.synchronize()
+        assert bool(((weights - start).abs() <= 2e-5 * start + 1e-6).all()), lens
