@@ -681,7 +681,7 @@ class BatchedCacheManager:
         if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
             raise ValueError(f"keep {keep} must be positive and hold recent {recent} and sinks {sinks}")
         cut = []
-        for rid in self.request_ids:
+        for rid in dict.fromkeys(self.request_ids):  # a request named twice is cut once
             label = self.active_labels.get(rid, "main")
             if am.get_state(rid, label).seq_len > keep:
                 am.wait_for_retrieves(rid, label)

@@ -425,7 +425,7 @@ MI_DEVICE void w_add(const WeightsParams& p, const WRequest& q, int h, int split
 // Both passes hold one side of the product in registers and stream the other through LDS in tiles
 // of 32, on the 32x32x16 MFMA: a tile's fragment serves all of a wavefront's columns.  An exponential
 // is 16 cycles of a wavefront, as long as its share of the products at head_dim 128, and each pass has one a
-// score beside an FMA and an addition.  No one unit bounds them: of the 212 us of the first pass over 4 chunks and 22k
+// score beside an FMA and an addition.  The two take turns (MFMA busy 35-37 % of the cycles, VALU 65-67 %), so no one unit bounds them: of the 212 us of the first pass over 4 chunks and 22k
 // keys 27 go without the exponentials, 66 without seven eighths of the products, 43 without the loads.
 template <typename MT>
 MI_DEVICE f32x16 mma_32x32x16(const uint4& a, const uint4& b, f32x16 c) {

@@ -121,6 +121,26 @@ def test_a_run_of_steps(gpu, kind):
     assert [cm._get_state(r).position_id_start for r in cm.request_ids] == [a + 1000 * i for i, a in enumerate(total)]
 
 
+def test_a_request_named_twice_is_cut_once(gpu):
+    cm = _manager(gpu, "bf16")
+    g = torch.Generator().manual_seed(9)
+    cm.plan_attention([100, 60, 20])
+    for l in range(LAYERS):
+        x = torch.randn(180, HQ + 2 * HKV, D, generator=g).to(torch.bfloat16).to(gpu)
+        cm.run_attention(*x.split([HQ, HKV, HKV], 1), layer_idx=l, accumulate=True)
+    cm.advance_seq_lens()
+    before = {(r, l): _context(cm, r, l) for r in cm.request_ids for l in range(LAYERS)}
+    cm.request_ids = ["a", "b", "a"]
+    free = cm.alloc_manager.num_free_pages
+    assert cm.evict(32, recent=8, sinks=2) == (7 - 2) + (4 - 2) and cm.alloc_manager.num_free_pages == free + 7
+    assert [cm._get_state(r).seq_len for r in "abc"] == [32, 32, 20]
+    for (r, l), (k, v, w) in before.items():
+        got = _context(cm, r, l)
+        for h in range(HKV):
+            places = torch.as_tensor(E.kept_places(w[:, h].float().numpy(), 32, 8, 2))
+            assert all(torch.equal(a[:, h], b[places, h]) for a, b in zip(got, (k, v, w)))
+
+
 @pytest.mark.parametrize("kind", ["bf16", "mx8"])
 def test_snapshot_of_a_cut_request(gpu, kind):
     """A copy of a cut request holds its rows and weights, also over a copy that was made before the cut."""
