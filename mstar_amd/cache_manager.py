@@ -431,6 +431,7 @@ class BatchedCacheManager:
             start = 0 if from_state.evicted or to_state.evicted else to_state.seq_len // ps_
             self.alloc_manager.alloc(rid, to_label, seq_len=from_state.seq_len)
             to_state.evicted = to_state.evicted or from_state.evicted
+            to_state.dropped = from_state.dropped
             to_state.seq_len = from_state.seq_len
             to_state.position_id_start = from_state.position_id_start
             a, b = from_state.page_indices[start:], to_state.page_indices[start:]
@@ -672,7 +673,8 @@ class BatchedCacheManager:
         Between steps (after ``advance_seq_len(s)``): what :func:`~mstar_amd.eviction.evict_kv_cache`
         does, and the pages behind the kept tokens go back to the allocator's tail.  ``seq_len`` becomes ``keep`` where it was
         more, positions go on from ``position_id_start``.  The launch is ordered on the current stream, and so
-        must be what uses the freed pages next.
+        must be what uses the freed pages next.  A page list that was given to a reader before (``get_per_label_seq_info``)
+        is void: it must have been read by then.
         """
         if self.kv_weights is None:
             raise ValueError("evict() needs the manager's kv_weights")
@@ -701,6 +703,7 @@ class BatchedCacheManager:
         with am._lock:
             for st in cut:
                 freed.extend(st.page_indices[need:])
+                st.dropped += st.seq_len - keep
                 st.page_indices, st.seq_len, st.evicted = st.page_indices[:need], keep, True
             am.page_allocator.free(freed)
         return len(freed)

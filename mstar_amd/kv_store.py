@@ -132,7 +132,8 @@ class PositionInfo:
 class KVRequestState:
     """Per-request, per-label KV state (``kv_store.py:111-127``).
 
-    ``evicted`` (extension) marks a state whose tokens are not all it was given.
+    ``evicted`` (extension) marks a state whose tokens are not all it was given,
+    ``dropped`` counts those that are gone.
     ``slot`` is this state's row in the :class:`DeviceBlockTable` (-1: none yet).
 
     Page-list contract (what the reference's code paths do): ``page_indices``
@@ -151,6 +152,7 @@ class KVRequestState:
     is_paused: bool = False
     slot: int = -1
     evicted: bool = False  # cut by BatchedCacheManager.evict: its pages are no longer a prefix of a copy's
+    dropped: int = 0
     _dev_list: object = field(default=None, repr=False, compare=False)
     _dev_len: int = field(default=0, repr=False, compare=False)
     _dev_ends: tuple = field(default=(-1, -1), repr=False, compare=False)
@@ -650,15 +652,21 @@ class PagedAllocationManager:
         go out as one launch on the engine's transfer stream.  The producer
         must have finished writing those pages (the reference's contract,
         ``kv_store.py:548-554``).  A state that eviction has cut is read whole,
-        into an empty one (``reset_label``): it is no continuation of what was read before.
+        into an empty one (``reset_label``): it is no continuation of what was read before,
+        whichever of the two is longer.  Nothing is read, as before, where the state here has
+        gone on from that one, or was cut here and had been given as many tokens.
         """
         seq_len = seq_info.seq_len
         state = self.get_state(request_id, label)
+        cut, dropped = getattr(seq_info, "evicted", False), getattr(seq_info, "dropped", 0)
+        if state.seq_len and (cut or state.evicted):
+            # a state is as far as another when it was given as many tokens; a cut one is known only to what was cut with it
+            as_far = state.seq_len + state.dropped >= seq_len + dropped and state.position_id_start >= seq_info.pos_id
+            if not as_far or (cut and not (state.evicted and state.dropped >= dropped)):
+                raise ValueError(f"{request_id}: an evicted state does not follow the {state.seq_len} tokens that are here")
+            return
         if state.seq_len >= seq_len:
             return
-        cut = getattr(seq_info, "evicted", False)
-        if state.seq_len and (cut or state.evicted):
-            raise ValueError(f"{request_id}: the rest of an evicted state does not follow the {state.seq_len} tokens that are here")
         ps = self.config.page_size
         first = state.seq_len // ps
         last = (seq_len - 1) // ps
@@ -677,7 +685,7 @@ class PagedAllocationManager:
             self.pending_reads[request_id].setdefault(label, []).append(future)
         state.seq_len = seq_len
         state.position_id_start = seq_info.pos_id
-        state.evicted = cut
+        state.evicted, state.dropped = cut, dropped
         state.read_in_progress = future is not None
 
     def get_per_label_seq_info(self, request_id: str) -> dict:
@@ -690,7 +698,8 @@ class PagedAllocationManager:
             self.wait_for_retrieves(request_id, label)
             st = self.get_state(request_id, label)
             out[label] = SequenceInfo(seq_len=st.seq_len, pos_id=st.position_id_start,
-                                      latest_kv_transfer_info=info, page_indices=st.page_indices, evicted=st.evicted)
+                                      latest_kv_transfer_info=info, page_indices=st.page_indices, evicted=st.evicted,
+                                      dropped=st.dropped)
         return out
 
     # ----- CPU offloading (kv_store.py:617-660) -----

@@ -70,7 +70,7 @@ class DeviceKVTransferInfo:
 class SequenceInfo:
     """A producer's state of one (request, label) (``request_info.py:23-29``).
 
-    ``evicted`` (extension): its tokens are not all that it was given (``KVRequestState.evicted``).
+    ``evicted``, ``dropped`` (extension): its tokens are not all that it was given (``KVRequestState``).
     """
 
     seq_len: int
@@ -78,6 +78,7 @@ class SequenceInfo:
     latest_kv_transfer_info: Any
     page_indices: list[int] = field(default_factory=list)
     evicted: bool = False
+    dropped: int = 0
 
 
 def _check_pool(kv: torch.Tensor, name: str) -> None:
