@@ -439,8 +439,9 @@ class BatchedCacheManager:
                 raise ValueError(f"{rid}: {len(a)} source pages vs {len(b)} destination pages from page {start}")
             src.extend(a)
             dst.extend(b)
-            whole[0].extend(from_state.page_indices)
-            whole[1].extend(to_state.page_indices)
+            need = -(-from_state.seq_len // ps_)
+            whole[0].extend(from_state.page_indices[:need])
+            whole[1].extend(to_state.page_indices[:need])
             if write_store:
                 self.alloc_manager.flush_to_store(rid, label=to_label)
         if src:
