@@ -418,36 +418,42 @@ class BatchedCacheManager:
         takes its seq_len and position start); the page copies of all
         requests and layers go to the GPU as one ``mi_copy_pages`` launch.
         A state that :meth:`evict` has cut no longer begins as its copies do: all
-        its pages are copied.  ``kv_weights`` are copied for every page.
+        its pages are copied, and pages that the copy has beyond them go back to the
+        allocator.  ``kv_weights`` are copied for every page.  States change once every
+        request's lists agree.
         """
         assert self.kv_cache is not None
-        ps_ = self.kv_cache_config.page_size
-        src, dst, whole = [], [], ([], [])
+        am, ps_ = self.alloc_manager, self.kv_cache_config.page_size
+        src, dst, whole, states = [], [], ([], []), []
         for rid in self.request_ids:
             from_state = self._get_state(rid, from_label)
             if realloc:
-                self.alloc_manager.reset_label(rid, to_label)
+                am.reset_label(rid, to_label)
             to_state = self._get_state(rid, to_label)
-            start = 0 if from_state.evicted or to_state.evicted else to_state.seq_len // ps_
-            self.alloc_manager.alloc(rid, to_label, seq_len=from_state.seq_len)
-            to_state.evicted = to_state.evicted or from_state.evicted
-            to_state.dropped = from_state.dropped
-            to_state.seq_len = from_state.seq_len
-            to_state.position_id_start = from_state.position_id_start
-            a, b = from_state.page_indices[start:], to_state.page_indices[start:]
+            cut, need = from_state.evicted or to_state.evicted, -(-from_state.seq_len // ps_)
+            am.alloc(rid, to_label, seq_len=from_state.seq_len)
+            start, end = (0, need) if cut else (to_state.seq_len // ps_, None)
+            a, b = from_state.page_indices[start:end], to_state.page_indices[start:end]
             if len(a) != len(b):
                 raise ValueError(f"{rid}: {len(a)} source pages vs {len(b)} destination pages from page {start}")
             src.extend(a)
             dst.extend(b)
-            need = -(-from_state.seq_len // ps_)
             whole[0].extend(from_state.page_indices[:need])
             whole[1].extend(to_state.page_indices[:need])
+            states.append((rid, from_state, to_state, need if cut else None))
+        pools = [self.kv_cache.codes, self.kv_cache.scales] if isinstance(self.kv_cache, MXKVCache) else [self.kv_cache]
+        if src and not all(kv[0, 0].is_contiguous() for kv in pools):
+            raise ValueError("snapshot_all needs each page of the KV pool to be contiguous")
+        for rid, from_state, to_state, need in states:
+            with am._lock:
+                if need is not None and len(to_state.page_indices) > need:
+                    am.page_allocator.free(to_state.page_indices[need:])
+                    to_state.page_indices = to_state.page_indices[:need]
+                to_state.evicted, to_state.dropped = from_state.evicted, from_state.dropped
+                to_state.seq_len, to_state.position_id_start = from_state.seq_len, from_state.position_id_start
             if write_store:
-                self.alloc_manager.flush_to_store(rid, label=to_label)
+                am.flush_to_store(rid, label=to_label)
         if src:
-            pools = [self.kv_cache.codes, self.kv_cache.scales] if isinstance(self.kv_cache, MXKVCache) else [self.kv_cache]
-            if not all(kv[0, 0].is_contiguous() for kv in pools):
-                raise ValueError("snapshot_all needs each page of the KV pool to be contiguous")
             self._copy_pages(pools, src, dst)
         if self.kv_weights is not None and whole[0]:  # every token's weight changes with every step
             self._copy_pages([self.kv_weights], *whole)
