@@ -94,16 +94,20 @@ __global__ __launch_bounds__(256) void weights_finish_kernel(WeightsParams p) {
   }
   while (t < tok1) {
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](const float4& x, float e) {
-      sum.x += fast_exp2(x.x - e);
-      sum.y += fast_exp2(x.y - e);
-      sum.z += fast_exp2(x.z - e);
-      sum.w += fast_exp2(x.w - e);
+    // the first row that sees token t + i: those before it add nothing, also where their log-sum-exp is NaN
+    auto first = [&](int i) { return p.causal ? max(0, t + i - off) * p.group : 0; };
+    const int f0 = first(0), f1 = first(1), f2 = first(2), f3 = first(3);
+    auto add = [&](const float4& x, int row) {
+      const float e = s_lse[row];
+      sum.x += row < f0 ? 0.f : fast_exp2(x.x - e);
+      sum.y += row < f1 ? 0.f : fast_exp2(x.y - e);
+      sum.z += row < f2 ? 0.f : fast_exp2(x.z - e);
+      sum.w += row < f3 ? 0.f : fast_exp2(x.w - e);
     };
 #pragma unroll
     for (int row = 0; row < kAhead; ++row)
-      if (row < q.rows) add(s[row], s_lse[row]);
-    for (int row = kAhead; row < q.rows; ++row) add(*(const float4*)(src + 16 * row), s_lse[row]);
+      if (row < q.rows) add(s[row], row);
+    for (int row = kAhead; row < q.rows; ++row) add(*(const float4*)(src + 16 * row), row);
     if (w) {
       if (t + 4 <= min(off, tok1)) {
         *(float4*)w = make_float4(old.x + sum.x, old.y + sum.y, old.z + sum.z, old.w + sum.w);

@@ -403,7 +403,9 @@ __global__ __launch_bounds__(one_threads<MT>(D)) void weights_one_kernel(Weights
       old = at && t < off ? *at : 0.f;
     }
     float sum = 0.f;
-    for (int row = 0; row < q.rows; ++row) sum += fast_exp2(s_scores[row * pitch + t] - s_lse[row]);
+    // from the first row that sees the token on: the others add nothing, also where their log-sum-exp is NaN
+    for (int row = p.causal ? max(0, t - off) * p.group : 0; row < q.rows; ++row)
+      sum += fast_exp2(s_scores[row * pitch + t] - s_lse[row]);
     if (at) *at = old + sum;
   }
 }
