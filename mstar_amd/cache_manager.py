@@ -477,6 +477,18 @@ class BatchedCacheManager:
             return None, None
         return self.kv_scales[layer_idx, 0], self.kv_scales[layer_idx, 1]
 
+    def _check_window(self, label: str, window_left: int, sink_tokens: int) -> None:
+        """Refuse a window over requests of which eviction has left less than it spans."""
+        am = self.alloc_manager
+        recent, sinks = am.evicted_to
+        if window_left <= recent and (window_left < 0 or sink_tokens <= sinks):
+            return
+        for rid in self.request_ids:
+            states = am.request_states[rid]
+            for st in [states[label]] if label in states else states.values():
+                if st.evicted:
+                    raise ValueError(f"{rid}: eviction has left fewer tokens than a window of {window_left} with {sink_tokens} sinks spans")
+
     def _run(self, wrapper, q, layer, layer_idx, ks, vs, window_left, sink_tokens, accumulate) -> torch.Tensor:
         if accumulate:
             if self.kv_weights is None:
@@ -484,6 +496,9 @@ class BatchedCacheManager:
             if window_left >= 0:
                 raise ValueError("attention weights are accumulated over layers without a window")
         out = wrapper.run(q, layer, ks, vs, window_left=window_left, sink_tokens=sink_tokens)
+        if window_left >= 0:
+            am = self.alloc_manager
+            am.windows = (max(am.windows[0], window_left), max(am.windows[1], sink_tokens))
         if accumulate:
             wrapper.accumulate_weights(q, layer, self.kv_weights[layer_idx], ks, vs)
         return out
@@ -502,6 +517,7 @@ class BatchedCacheManager:
         label = self._single_active_label()
         ps = self._plan_states[label]
         assert self.kv_cache is not None and ps.wrapper is not None
+        self._check_window(label, window_left, sink_tokens)
         layer = self.kv_cache[layer_idx]
         ks, vs = self._layer_scales(layer_idx)
         ps.wrapper.set_kv_cache(layer, k, v, ks, vs)
@@ -647,6 +663,7 @@ class BatchedCacheManager:
         ps = self._plan_states[label]
         assert ps.pos_ids is not None, "plan_rope() must run before apply_rope_and_run_attention()"
         assert self.kv_cache is not None and ps.wrapper is not None
+        self._check_window(label, window_left, sink_tokens)
         orig_dtype = q.dtype
         dt = rope_dtype
         if dt is None and torch.is_autocast_enabled("cuda"):
@@ -682,6 +699,9 @@ class BatchedCacheManager:
         more, positions go on from ``position_id_start``.  The launch is ordered on the current stream, and so
         must be what uses the freed pages next.  A page list that was given to a reader before (``get_per_label_seq_info``)
         is void: it must have been read by then.
+
+        A window counts places, so that layers with one go on as if nothing had been cut where ``recent`` is at least their
+        ``window_left`` and ``sinks`` their ``sink_tokens``; less is refused once such a layer has been run over the pool.
         """
         if self.kv_weights is None:
             raise ValueError("evict() needs the manager's kv_weights")
@@ -689,6 +709,9 @@ class BatchedCacheManager:
         keep, recent, sinks = int(keep), int(recent), int(sinks)
         if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
             raise ValueError(f"keep {keep} must be positive and hold recent {recent} and sinks {sinks}")
+        if recent < am.windows[0] or sinks < am.windows[1]:
+            raise ValueError(f"layers have been run with window_left {am.windows[0]} and sink_tokens {am.windows[1]}: recent {recent} and "
+                             f"sinks {sinks} must be at least as many")
         cut = []
         for rid in dict.fromkeys(self.request_ids):  # a request named twice is cut once
             label = self.active_labels.get(rid, "main")
@@ -712,6 +735,7 @@ class BatchedCacheManager:
                 freed.extend(st.page_indices[need:])
                 st.dropped += st.seq_len - keep
                 st.page_indices, st.seq_len, st.evicted = st.page_indices[:need], keep, True
+            am.evicted_to = (min(am.evicted_to[0], recent), min(am.evicted_to[1], sinks))
             am.page_allocator.free(freed)
         return len(freed)
 

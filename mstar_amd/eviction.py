@@ -74,7 +74,8 @@ def evict_kv_cache(kv_cache: torch.Tensor | MXKVLayer | MXKVCache, weights: torc
     last ``recent`` and the heaviest of the others by ``weights`` (ties: the lowest place; NaN counts less than any number),
     ``keep`` in all.  Their K, V and weights move to the request's first ``keep`` places, in their order; places
     behind them are left as they were.  Shorter requests are left as they are.  The caller goes on with
-    ``min(length, keep)`` tokens a request, and may free the pages behind them.
+    ``min(length, keep)`` tokens a request, and may free the pages behind them.  Windowed runs count places: they
+    go on as if nothing had been cut where ``recent`` is at least ``window_left`` and ``sinks`` at least ``sink_tokens``.
 
     ``kv_cache``: one layer, or a pool of layers (``[num_layers, ...]`` or an ``MXKVCache``) whose ``weights`` (:func:`kv_weights`)
     have the same leading dimension.  The index tensors are those a wrapper plans with; CPU ones are

@@ -30,6 +30,7 @@ from __future__ import annotations
 
 import collections
 import enum
+import math
 import threading
 from dataclasses import dataclass, field
 from typing import Any
@@ -429,6 +430,10 @@ class PagedAllocationManager:
         # Bumped whenever a state object is created or a request removed, so
         # callers can keep lists of state objects between steps.
         self.state_generation = 0
+        # A window counts places, so eviction must leave what it spans: the largest (window_left, sink_tokens) that a layer
+        # was run with, and the least (recent, sinks) that an eviction has left (BatchedCacheManager).
+        self.windows: tuple[int, int] = (-1, 0)
+        self.evicted_to: tuple[float, float] = (math.inf, math.inf)
         if device is None and kv_cache is not None and kv_cache.is_cuda:
             device = kv_cache.device
         self.block_table: DeviceBlockTable | None = None
