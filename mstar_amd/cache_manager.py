@@ -477,8 +477,13 @@ class BatchedCacheManager:
             return None, None
         return self.kv_scales[layer_idx, 0], self.kv_scales[layer_idx, 1]
 
-    def _check_window(self, label: str, window_left: int, sink_tokens: int) -> None:
-        """Refuse a window over requests of which eviction has left less than it spans."""
+    def _check_run(self, label: str, window_left: int, sink_tokens: int, accumulate: bool) -> None:
+        """Before anything is rotated or appended: refuse weights that cannot be accumulated, and a window over requests of
+        which eviction has left less than it spans."""
+        if accumulate and self.kv_weights is None:
+            raise ValueError("accumulate=True needs the manager's kv_weights")
+        if accumulate and window_left >= 0:
+            raise ValueError("attention weights are accumulated over layers without a window")
         am = self.alloc_manager
         recent, sinks = am.evicted_to
         if window_left <= recent and (window_left < 0 or sink_tokens <= sinks):
@@ -490,11 +495,6 @@ class BatchedCacheManager:
                     raise ValueError(f"{rid}: eviction has left fewer tokens than a window of {window_left} with {sink_tokens} sinks spans")
 
     def _run(self, wrapper, q, layer, layer_idx, ks, vs, window_left, sink_tokens, accumulate) -> torch.Tensor:
-        if accumulate:
-            if self.kv_weights is None:
-                raise ValueError("accumulate=True needs the manager's kv_weights")
-            if window_left >= 0:
-                raise ValueError("attention weights are accumulated over layers without a window")
         out = wrapper.run(q, layer, ks, vs, window_left=window_left, sink_tokens=sink_tokens)
         if window_left >= 0:
             am = self.alloc_manager
@@ -517,7 +517,7 @@ class BatchedCacheManager:
         label = self._single_active_label()
         ps = self._plan_states[label]
         assert self.kv_cache is not None and ps.wrapper is not None
-        self._check_window(label, window_left, sink_tokens)
+        self._check_run(label, window_left, sink_tokens, accumulate)
         layer = self.kv_cache[layer_idx]
         ks, vs = self._layer_scales(layer_idx)
         ps.wrapper.set_kv_cache(layer, k, v, ks, vs)
@@ -663,7 +663,7 @@ class BatchedCacheManager:
         ps = self._plan_states[label]
         assert ps.pos_ids is not None, "plan_rope() must run before apply_rope_and_run_attention()"
         assert self.kv_cache is not None and ps.wrapper is not None
-        self._check_window(label, window_left, sink_tokens)
+        self._check_run(label, window_left, sink_tokens, accumulate)
         orig_dtype = q.dtype
         dt = rope_dtype
         if dt is None and torch.is_autocast_enabled("cuda"):
