@@ -608,6 +608,9 @@ __global__ __launch_bounds__(256, 2) void weights_rows_kernel(WeightsParams p) {
   float sl2 = KVT == kKvFp8 ? p.scale_log2 * ((const float*)p.k_scale)[h] : p.scale_log2;
   const uint32_t flip = sl2 < 0.f ? 0x80008000u : 0u;  // the maximum is taken of unscaled scores: the scale's sign goes to q
   sl2 = fabsf(sl2);
+  // Hidden scores are -inf before the scale, which zero would make NaN: then the products are scaled first, in every tile.
+  const bool zero = sl2 == 0.f;
+  if (zero) sl2 = 1.f;
   uint4 qf[NS][STEPS];
   int lim[NS], row[NS];
 #pragma unroll
@@ -626,7 +629,7 @@ __global__ __launch_bounds__(256, 2) void weights_rows_kernel(WeightsParams p) {
   float m[NS], l[NS];
 #pragma unroll
   for (int n = 0; n < NS; ++n) m[n] = -kWInf, l[n] = 0.f;
-  const int clear = p.causal ? off + row0 / p.group : q.len - 1;  // keys up to here are seen by every row
+  const int clear = zero ? -1 : p.causal ? off + row0 / p.group : q.len - 1;  // keys up to here are seen by every row
   // One tile a barrier: with two, the registers of both leave room for two wavefronts instead of three (205 -> 232 us).
   using Keys = KeyStream<MT, KVT, D>;
   Keys keys_in;
@@ -652,10 +655,14 @@ __global__ __launch_bounds__(256, 2) void weights_rows_kernel(WeightsParams p) {
     const int tok = kTile * i;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-      if (tok + kTile - 1 > clear)
+      if (tok + kTile - 1 > clear) {
+        if (zero)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[n][j] *= 0.f;
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (tok + (j & 3) + 8 * (j >> 2) + 4 * hi > lim[n]) acc[n][j] = -kWInf;
+      }
       float top = fmaxf(acc[n][0], acc[n][1]);
 #pragma unroll
       for (int j = 2; j < 16; j += 2) top = fmaxf(top, fmaxf(acc[n][j], acc[n][j + 1]));
