@@ -57,7 +57,7 @@ __all__ = [
 
 _MAX_GROUP = 16  # q heads per kv head handled by one MFMA tile
 _WINDOW_MAX = 1 << 30  # beyond any context
-_PAIR_MIN_BATCH = 128  # smaller batches have no paired plans (mi_prefill_short_rows)
+_WEIGHTS_SHORT_ROWS = 16  # of (query, q head): requests of mi_attention_weights' part 1
 # Ragged batches of up to _SERIAL_REQUESTS requests run their two parts one
 # after the other on one stream: the events of a fork and join cost the host
 # more than the overlap hides (us a layer, side stream -> in turn: one 512-token
@@ -788,8 +788,14 @@ class PagedPrefillWrapper(_FusedRopeAppend, _Weights, _PlanArrays):
             rows = np.diff(qo_indptr.numpy().astype(np.int64, copy=False)) * (self.num_qo_heads // self.num_kv_heads)
             self._run_short = bool(((rows > 0) & (rows <= short)).any())
             self._run_tiles = bool((rows > short).any())
+            few, many = self._run_short, self._run_tiles
+            if short != _WEIGHTS_SHORT_ROWS:  # a paired plan's tiles may be requests of 9 to 16 rows
+                few = bool(((rows > 0) & (rows <= _WEIGHTS_SHORT_ROWS)).any())
+                many = bool((rows > _WEIGHTS_SHORT_ROWS).any())
+            self._weights_parts = (1 if few else 0) | (2 if many else 0)
         else:
             self._run_short = self._run_tiles = True
+            self._weights_parts = 3
 
     def run(self, q: torch.Tensor, kv_cache_layer: torch.Tensor | MXKVLayer, k_scale: torch.Tensor | None = None,
             v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None, window_left: int = -1,
@@ -867,10 +873,7 @@ class PagedPrefillWrapper(_FusedRopeAppend, _Weights, _PlanArrays):
         return self.token_to_page, self.token_to_cache.data_ptr(), 1, self._total_tokens, n_dev
 
     def _weights_batch(self):
-        # a paired plan's tiles may be requests of 9 to 16 rows, which are short ones here
-        short = self._run_short or (self._run_tiles and self._n_req >= _PAIR_MIN_BATCH)
-        parts = (1 if short else 0) | (2 if self._run_tiles else 0)
-        return self._qo, self._total_tokens, self._plan_max_tokens, parts, self.causal
+        return self._qo, self._total_tokens, self._plan_max_tokens, self._weights_parts, self.causal
 
 
 # Reference names (mstar/utils/flashinfer_utils.py) for drop-in use.
