@@ -121,7 +121,7 @@ class BatchedCacheManager:
         dequantisation scales of an fp8-e4m3 ``kv_cache``.  ``kv_cache`` may be an
         :class:`~mstar_amd.mx_cache.MXKVCache` (extension), which holds its own.
         ``kv_weights`` (extension): the pool's :func:`~mstar_amd.eviction.kv_weights`, for
-        ``accumulate=True`` and :meth:`evict`."""
+        ``accumulate=True`` and :meth:`evict`; ``alloc_manager`` zeroes them for tokens that it reads or reloads."""
         if kv_weights is not None and tuple(kv_weights.shape) != _pool_shape(kv_cache):
             raise ValueError(f"kv_weights {tuple(kv_weights.shape)} do not fit the pool's {_pool_shape(kv_cache)}")
         self.request_ids = request_ids
@@ -146,6 +146,16 @@ class BatchedCacheManager:
         self._states_cache: dict = {}
         if alloc_manager.block_table is None:
             raise ValueError("the allocation manager needs a device (block table) for GPU packing")
+
+    @property
+    def kv_weights(self) -> torch.Tensor | None:
+        return self._kv_weights
+
+    @kv_weights.setter
+    def kv_weights(self, weights: torch.Tensor | None) -> None:
+        self._kv_weights = weights
+        if weights is not None:
+            self.alloc_manager.kv_weights = weights
 
     # ------------------------------------------------------------ labels
     def _get_state(self, request_id: str, label: str | None = None) -> KVRequestState:

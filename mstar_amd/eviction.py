@@ -14,7 +14,8 @@ Keys stay rotated to the positions they were written at, and new tokens go on fr
 request's last position: only the places in the cache change.
 
 Weights live beside one pool and stay there: tokens that arrive in it by a transfer or from host memory bring
-none, and a caller that accumulates goes on from what it writes into their slots (zeros, say).
+none.  Where a ``BatchedCacheManager`` has the pool's weights, the allocation manager zeroes those tokens' slots as it
+queues the copies; a caller that has kept weights writes them behind that, and one that moves pages itself zeroes them.
 
 No counterpart in the reference, whose caches only grow.
 """

@@ -434,6 +434,8 @@ class PagedAllocationManager:
         # was run with, and the least (recent, sinks) that an eviction has left (BatchedCacheManager).
         self.windows: tuple[int, int] = (-1, 0)
         self.evicted_to: tuple[float, float] = (math.inf, math.inf)
+        # The pool's attention weights, known from the first BatchedCacheManager that has them.
+        self.kv_weights: torch.Tensor | None = None
         if device is None and kv_cache is not None and kv_cache.is_cuda:
             device = kv_cache.device
         self.block_table: DeviceBlockTable | None = None
@@ -604,6 +606,19 @@ class PagedAllocationManager:
             del self.pending_reads[request_id]
             self.state_generation += 1
 
+    def _clear_weights(self, pages: list[int], first_slot: int = 0) -> None:
+        """Zero the weights of tokens about to arrive in ``pages``, in the first of them from ``first_slot`` on: what the
+        pages' last owners left is not theirs.  Ordered on the current stream."""
+        w = self.kv_weights
+        if w is None or not pages:
+            return
+        if first_slot:
+            w[:, pages[0], :, first_slot:] = 0
+            pages = pages[1:]
+        if pages:
+            idx = torch.tensor(pages, dtype=torch.long)
+            w.index_fill_(1, idx.pin_memory().to(w.device, non_blocking=True) if w.is_cuda else idx, 0.0)
+
     # ----- remote reads (kv_store.py:484-581) -----
 
     @property
@@ -685,6 +700,7 @@ class PagedAllocationManager:
         remote = np.asarray(seq_info.page_indices[first:last + 1], dtype=np.int64)
         if remote.size != n:
             raise ValueError(f"producer lists {len(seq_info.page_indices)} pages for {seq_len} tokens")
+        self._clear_weights(state.page_indices[first:last + 1], int(ts[0]))  # the read is ordered behind it
         future = self.kv_transfer_engine.read_pages_async(seq_info.latest_kv_transfer_info, local, remote, ts, te)
         if future is not None:
             self.pending_reads[request_id].setdefault(label, []).append(future)
@@ -758,6 +774,7 @@ class PagedAllocationManager:
                 mine = pages[start:start + n]
                 start += n
                 st = self.get_state(request_id, label)
+                self._clear_weights(mine)
                 seq_len, pos = cpu_pool.reload_pages(request_id, label, self.kv_cache, mine)
                 st.page_indices, st.seq_len, st.position_id_start = mine, seq_len, pos
         cpu_pool.sync()
