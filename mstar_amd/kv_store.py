@@ -744,10 +744,12 @@ class PagedAllocationManager:
         freed = 0
         for label, st in holding:
             self.wait_for_retrieves(request_id, label)
+            cut = dict(evicted=True, dropped=st.dropped) if st.evicted else {}
             cpu_pool.offload_pages(request_id, label, self.kv_cache, st.page_indices, st.seq_len,
-                                   st.position_id_start)
+                                   st.position_id_start, **cut)
             with self._lock:
                 pages, st.page_indices, st.seq_len = st.page_indices, [], 0
+                st.evicted, st.dropped = False, 0
                 self.page_allocator.free(pages)
             freed += len(pages)
         return freed
@@ -775,6 +777,8 @@ class PagedAllocationManager:
                 start += n
                 st = self.get_state(request_id, label)
                 self._clear_weights(mine)
+                cut = getattr(held[label], "evicted", False), getattr(held[label], "dropped", 0)
                 seq_len, pos = cpu_pool.reload_pages(request_id, label, self.kv_cache, mine)
                 st.page_indices, st.seq_len, st.position_id_start = mine, seq_len, pos
+                st.evicted, st.dropped = cut
         cpu_pool.sync()

@@ -339,11 +339,14 @@ class DeviceKVTransferEngine:
 
 @dataclass
 class OffloadedState:
-    """A (request, label) held in the CPU pool (``cpu_page_pool.py:17-22``)."""
+    """A (request, label) held in the CPU pool (``cpu_page_pool.py:17-22``); ``evicted`` and ``dropped`` (extension) as in
+    ``KVRequestState``."""
 
     cpu_page_indices: list[int]
     seq_len: int
     position_id_start: int
+    evicted: bool = False
+    dropped: int = 0
 
 
 class CPUPagePool:
@@ -377,7 +380,7 @@ class CPUPagePool:
         return request_id in self.offloaded and len(self.offloaded[request_id]) > 0
 
     def offload_pages(self, request_id: str, label: str, gpu_kv_cache: torch.Tensor, gpu_page_indices: list[int],
-                      seq_len: int, position_id_start: int) -> None:
+                      seq_len: int, position_id_start: int, evicted: bool = False, dropped: int = 0) -> None:
         """GPU pages -> CPU pages, all layers, one launch (``cpu_page_pool.py:63-98``)."""
         n = len(gpu_page_indices)
         if n == 0:
@@ -393,7 +396,7 @@ class CPUPagePool:
         s.wait_stream(cur)
         copy_tokens(gpu_kv_cache, self.cpu_kv_cache, cpu_pages, gpu_page_indices, stream=s, device=dev)
         cur.wait_stream(s)
-        self.offloaded.setdefault(request_id, {})[label] = OffloadedState(cpu_pages, seq_len, position_id_start)
+        self.offloaded.setdefault(request_id, {})[label] = OffloadedState(cpu_pages, seq_len, position_id_start, evicted, dropped)
 
     def reload_pages(self, request_id: str, label: str, gpu_kv_cache: torch.Tensor,
                      gpu_page_indices: list[int]) -> tuple[int, int]:

@@ -94,3 +94,62 @@ def test_weights_given_later_are_the_pools():
     cm.kv_weights = w
     mgr.start_async_retrieve("a", "main", SequenceInfo(16, 16, "there", [0]))
     assert not bool(w[:, mgr.get_state("a", "main").page_indices].any())
+
+
+def _cut(mgr, keep):
+    st = mgr.get_state("a", "main")
+    mgr.page_allocator.free(st.page_indices[-(-keep // PS):])
+    st.dropped += st.seq_len - keep
+    st.page_indices, st.seq_len, st.evicted = st.page_indices[: -(-keep // PS)], keep, True
+
+
+@pytest.mark.parametrize("removed", [False, True])
+def test_a_cut_state_is_cut_when_it_comes_back(removed):
+    """Also to a request that was removed and added again meanwhile, and its state on the GPU is empty and whole until then."""
+    mgr, _, _ = _pool()
+    host = _HostPool()
+    mgr.alloc("a", "main", 100)
+    st = mgr.get_state("a", "main")
+    st.seq_len = st.position_id_start = 100
+    _cut(mgr, 40)
+    mgr.offload_request("a", host)
+    assert (st.seq_len, st.evicted, st.dropped) == (0, False, 0)
+    if removed:
+        mgr.remove_request("a")
+        mgr.add_request("a", ["main"])
+    mgr.reload_request("a", host)
+    st = mgr.get_state("a", "main")
+    assert (st.seq_len, st.position_id_start, st.evicted, st.dropped) == (40, 100, True, 60)
+    with pytest.raises(ValueError, match="evicted"):
+        mgr.start_async_retrieve("a", "main", SequenceInfo(110, 110, "there", list(range(8))))
+
+
+def test_a_state_filled_anew_behind_an_offload_is_whole():
+    mgr, _, _ = _pool()
+    mgr.alloc("a", "main", 100)
+    st = mgr.get_state("a", "main")
+    st.seq_len = st.position_id_start = 100
+    _cut(mgr, 40)
+    mgr.offload_request("a", _HostPool())
+    mgr.alloc("a", "main", 20)  # a prompt once more
+    st.seq_len = st.position_id_start = 20
+    mgr.start_async_retrieve("a", "main", SequenceInfo(50, 50, "there", list(range(8))))
+    assert (st.seq_len, st.evicted) == (50, False)
+
+
+def test_host_pools_of_plain_states():
+    """A pool that knows nothing of cuts holds whole states as before."""
+
+    class Plain(_HostPool):
+        def offload_pages(self, rid, label, kv, pages, seq_len, pos):
+            self.offloaded.setdefault(rid, {})[label] = type("State", (), dict(cpu_page_indices=list(range(len(pages))), seq_len=seq_len,
+                                                                               position_id_start=pos))
+
+    mgr, _, _ = _pool()
+    host = Plain()
+    mgr.alloc("a", "main", 40)
+    st = mgr.get_state("a", "main")
+    st.seq_len = st.position_id_start = 40
+    mgr.offload_request("a", host)
+    mgr.reload_request("a", host)
+    assert (st.seq_len, st.evicted, st.dropped) == (40, False, 0)
