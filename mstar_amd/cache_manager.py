@@ -726,6 +726,8 @@ class BatchedCacheManager:
         for rid in dict.fromkeys(self.request_ids):  # a request named twice is cut once
             label = self.active_labels.get(rid, "main")
             if am.get_state(rid, label).seq_len > keep:
+                if label in self._pre_planned_labels:
+                    raise ValueError(f"the next step of label {label!r} is planned already, with the pages of now")
                 am.wait_for_retrieves(rid, label)
                 cut.append(am.get_state(rid, label))
         if not cut:
