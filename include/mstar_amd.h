@@ -559,7 +559,7 @@ int mi_attention_weights_block(const mi_attention_weights_args* args);
  * left as they were, and so are shorter requests.  kept [num_layers][batch][num_kv_heads][keep] receives the places
  * that stayed, ascending, -1 behind a shorter request's tokens.  kv describes layer 0, layer_stride (in
  * kv's units) and scale_layer_stride (bytes) lead to the next one's; weights and out_weights as in
- * mi_attention_weights, weights_layer_stride elements from layer to layer.  out_weights may be weights; otherwise weights is
+ * mi_attention_weights, weights_layer_stride elements from layer to layer.  out_weights may be weights; otherwise they do not overlap, weights is
  * left as it was and every request's kept weights are written.  Pages outside [0, max_pages) weigh less than
  * any number, and what would move from or to them stays.  num_indices: elements of kv_indices.  Requests of a call share no page.  Any cache
  * type; rows 16-byte aligned. */

@@ -81,7 +81,7 @@ def evict_kv_cache(kv_cache: torch.Tensor | MXKVLayer | MXKVCache, weights: torc
     ``kv_cache``: one layer, or a pool of layers (``[num_layers, ...]`` or an ``MXKVCache``) whose ``weights`` (:func:`kv_weights`)
     have the same leading dimension.  The index tensors are those a wrapper plans with; CPU ones are
     copied to the cache's device.  Requests must not share pages.  ``out_weights``: where the kept tokens' weights are
-    written, of all requests, instead of in place; ``weights`` then stays as it was.
+    written, of all requests, instead of in place; ``weights`` then stays as it was, and they must not overlap.
 
     Returns int32 ``[(num_layers,) batch, num_kv_heads, keep]``: the places in the request that stayed,
     ascending, -1 behind those of a shorter request.
@@ -94,6 +94,8 @@ def evict_kv_cache(kv_cache: torch.Tensor | MXKVLayer | MXKVCache, weights: torc
                               or w.data_ptr() % 16):
             raise ValueError(f"{name} must be a contiguous, 16-byte aligned float32 tensor {shape} on {dev}, got {tuple(w.shape)}, "
                              f"{w.dtype} on {w.device}")
+    if out_weights is not None and 0 < abs(out_weights.data_ptr() - weights.data_ptr()) < 4 * weights.numel():
+        raise ValueError("out_weights must not overlap weights, unless it is the same tensor")
     keep, recent, sinks = int(keep), int(recent), int(sinks)
     if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
         raise ValueError(f"keep {keep} must be positive and hold recent {recent} and sinks {sinks}")

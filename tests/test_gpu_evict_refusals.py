@@ -1,10 +1,10 @@
-"""GPU: evictions that would move a plan's pages from under it are refused."""
+"""GPU: evictions that would move a plan's pages from under it, or write weights over ones still to be read, are refused."""
 
 import pytest
 import torch
 
 from mstar_amd.cache_manager import BatchedCacheManager, WorkspaceBufferManager
-from mstar_amd.eviction import kv_weights
+from mstar_amd.eviction import evict_kv_cache, kv_weights
 from mstar_amd.kv_store import KVCacheConfig, PagedAllocationManager
 
 pytestmark = pytest.mark.gpu
@@ -38,3 +38,24 @@ def test_a_step_that_is_planned_ahead(gpu):
     cm.plan_attention([1])
     run(1)
     assert cm.evict(40) == 7 - 3
+
+
+def test_out_weights_over_weights(gpu):
+    """The same tensor is in place; a part of it would be written over places still to be read."""
+    kv = torch.zeros(2, PAGES, 2, PS, HKV, D, dtype=torch.bfloat16, device=gpu)
+    flat = torch.rand(3 * PAGES * HKV * PS, device=gpu)
+    w = flat[: 2 * PAGES * HKV * PS].view(2, PAGES, HKV, PS)
+    idx = [torch.tensor(x, dtype=torch.int32, device=gpu) for x in ([0, 4], [3, 1, 2, 0], [5])]
+    was = flat.clone()
+    for at in (4, PAGES * HKV * PS):
+        other = flat[at:at + w.numel()].view(w.shape)
+        for a, b in ((w, other), (other, w)):
+            with pytest.raises(ValueError, match="overlap"):
+                evict_kv_cache(kv, a, *idx, keep=20, out_weights=b)
+    torch.cuda.synchronize()
+    assert torch.equal(flat, was)
+    one = w.clone()
+    a = evict_kv_cache(kv, one, *idx, keep=20, out_weights=one.view(one.shape))  # in place
+    b = evict_kv_cache(kv[0], w[0], *idx, keep=20, out_weights=w[1])  # beside one another
+    torch.cuda.synchronize()
+    assert torch.equal(a[0], b)
