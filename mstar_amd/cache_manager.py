@@ -430,7 +430,7 @@ class BatchedCacheManager:
         A state that :meth:`evict` has cut no longer begins as its copies do: all
         its pages are copied, and pages that the copy has beyond them go back to the
         allocator.  ``kv_weights`` are copied for every page.  States change once every
-        request's lists agree.
+        request's lists agree (with ``realloc`` the copies are emptied first).
         """
         assert self.kv_cache is not None
         am, ps_ = self.alloc_manager, self.kv_cache_config.page_size

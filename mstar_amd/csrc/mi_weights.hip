@@ -9,11 +9,11 @@
 // * Requests of at most 16 rows (qo_len x group; decode): K is what costs, so it is read once. The first
 //   launch writes the scores (group x 4 bytes a token and kv head, beside a row of K of 64 to 512 bytes) and
 //   a log-sum-exp for each run of pages; the second joins those and sums the exponentials.  256 requests over
-//   1.93M tokens, 4 heads x 128, bf16: 438 + 63 us.  K alone takes 320; any writing beside it brings reads and
+//   1.93M tokens, 4 heads x 128, bf16: 437 + 65 us.  K alone takes 320; any writing beside it brings reads and
 //   writes together to a copy's 5 TB/s (a quarter of the scores: 399).  Small batches take one launch instead.
 // * Longer ones: the products are what costs, and are done twice; a launch goes by rows with the
 //   keys streaming past (lse), one by keys with the rows streaming past (sums).  4 chunks of 512 to 2048 tokens
-//   over 22k, 28 / 4 heads x 128: 203 + 198 us, 130 GFLOP each.
+//   over 22k, 28 / 4 heads x 128: 203 + 200 us (199 to 207, 196 to 200 by machine), 130 GFLOP each.
 //
 // Every sum has one order, from the index arrays and shapes alone: the same call gives the same bits.
 // Work is found from the index arrays (unit_request): no plan is read, and any plan's workspace

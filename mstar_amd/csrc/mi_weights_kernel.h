@@ -427,8 +427,9 @@ MI_DEVICE void w_add(const WeightsParams& p, const WRequest& q, int h, int split
 // Both passes hold one side of the product in registers and stream the other through LDS in tiles
 // of 32, on the 32x32x16 MFMA: a tile's fragment serves all of a wavefront's columns.  An exponential
 // is 16 cycles of a wavefront, as long as its share of the products at head_dim 128, and each pass has one a
-// score beside an FMA and an addition.  The two take turns (MFMA busy 35-37 % of the cycles, VALU 65-67 %), so no one unit bounds them: of the 212 us of the first pass over 4 chunks and 22k
-// keys 27 go without the exponentials, 66 without seven eighths of the products, 43 without the loads.
+// score beside an FMA and an addition.  The two take turns (MFMA busy 35-37 % of the cycles, VALU 65-67 %), so no one unit bounds them: of a
+// first pass over 4 chunks and 22k keys that took 212 us (203 now) 27 went without the exponentials, 66 without seven eighths of the
+// products, 43 without the loads.
 template <typename MT>
 MI_DEVICE f32x16 mma_32x32x16(const uint4& a, const uint4& b, f32x16 c) {
   if constexpr (MT::kDtype == MI_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bitcast<bf16x8>(a), bitcast<bf16x8>(b), c, 0, 0, 0);
